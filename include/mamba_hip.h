@@ -48,8 +48,8 @@ int mcpu_check_device(void);
 const char* mcpu_version(void);
 
 /* sizeof() of an argument block ("scan", "conv", "conv_update",
- * "state_update", "ssd", "mixer_step", "norm_linear", "mamba2_step"), 0 for
- * an unknown name. A binding must compare it with its own sizeof of each
+ * "state_update", "ssd", "mixer_step", "norm_linear", "mamba2_step",
+ * "gated_scan", "gated_step"), 0 for an unknown name. A binding must compare it with its own sizeof of each
  * block it uses before its first call: the library reads a whole block,
  * whatever the caller allocated. */
 size_t mcpu_args_size(const char* name);
@@ -565,6 +565,77 @@ typedef struct mcpu_mamba2_step_args {
 size_t mcpu_mamba2_step_workspace_size(const mcpu_mamba2_step_args* a);
 /* One step. Updates conv_state and ssm_state in place and writes out. */
 int mcpu_mamba2_step(const mcpu_mamba2_step_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Gated linear recurrence.                                                  */
+/* ------------------------------------------------------------------------ */
+
+/* Per batch row, step t and channel d, in float32:
+ *   rho = sigmoid(a_gate)   iota = sigmoid(x_gate)   s = c softplus(decay_d) rho
+ *   a = exp(-s)             m = sqrt(1 - exp(-2 s))
+ *   h_t = k_t a h_{t-1} + m iota x_t        y_t = h_t, h_{-1} = initial_state or 0
+ * with k_t = 0 where seq_idx[t] != seq_idx[t-1] (t >= 1), else 1. One block for
+ * forward and backward. x, a_gate, x_gate, y and their gradients have `dtype`,
+ * shape (batch, seqlen, dim) and any element strides (not negative); everything
+ * else is float32 and contiguous. No counterpart in the reference. */
+typedef struct mcpu_gated_scan_args {
+  const void* x;
+  const void* a_gate;
+  const void* x_gate;
+  const float* decay;          /* (dim) */
+  const float* initial_state;  /* (batch, dim), optional */
+  const int32_t* seq_idx;      /* (batch, seqlen) contiguous, optional */
+  int64_t batch, seqlen, dim;
+  float c;
+  int32_t dtype;
+  int64_t x_stride[3];         /* element strides over (batch, seqlen, dim) */
+  int64_t a_stride[3];
+  int64_t i_stride[3];         /* of x_gate */
+  void* y;
+  int64_t y_stride[3];
+  float* last_state;           /* (batch, dim), optional */
+  float* ckpt;                 /* mcpu_gated_scan_ckpt_size() bytes: written by the forward when
+                                  given, read by the backward */
+  const void* dy;
+  int64_t dy_stride[3];
+  const float* dlast_state;    /* (batch, dim), optional */
+  void* dx;
+  int64_t dx_stride[3];
+  void* da_gate;
+  int64_t da_stride[3];
+  void* dx_gate;
+  int64_t di_stride[3];
+  float* ddecay;               /* (dim), summed over batch and steps in a fixed order */
+  float* dinitial_state;       /* (batch, dim), optional */
+} mcpu_gated_scan_args;
+
+/* Bytes of the states the forward keeps for the backward. */
+size_t mcpu_gated_scan_ckpt_size(const mcpu_gated_scan_args* a);
+size_t mcpu_gated_scan_fwd_workspace_size(const mcpu_gated_scan_args* a);
+int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes, void* stream);
+size_t mcpu_gated_scan_bwd_workspace_size(const mcpu_gated_scan_args* a);
+int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token per batch row: state is advanced in place and y = state. */
+typedef struct mcpu_gated_step_args {
+  float* state;                /* (state_batch, dim), any strides */
+  const void* x;               /* (batch, dim), dtype, any strides; a_gate and x_gate alike */
+  const void* a_gate;
+  const void* x_gate;
+  const float* decay;          /* (dim) contiguous */
+  void* y;                     /* (batch, dim) contiguous, dtype */
+  int64_t batch, dim, state_batch;
+  float c;
+  int32_t dtype;
+  int64_t state_stride[2];
+  int64_t x_stride[2];
+  int64_t a_stride[2];
+  int64_t i_stride[2];
+  const int32_t* state_batch_indices; /* (batch), optional: the state row of each batch row; a row
+                                         out of range is skipped and its y is zero */
+} mcpu_gated_step_args;
+
+int mcpu_gated_step(const mcpu_gated_step_args* a, void* stream);
 
 #ifdef __cplusplus
 }

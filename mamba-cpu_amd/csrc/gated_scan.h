@@ -1,0 +1,55 @@
+// Kernel parameter blocks and launch shapes of the gated linear recurrence,
+// shared by the kernels and the C-ABI layer that fills them.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace mcpu {
+
+constexpr int kGatedT = 8;      // steps per wave segment: the forward keeps the state before each
+constexpr int kGatedWaves = 4;  // waves of a workgroup, one segment each
+
+struct GatedScanParams {
+  const void* x;
+  const void* a_gate;
+  const void* x_gate;
+  const float* decay;
+  const float* init;
+  const int32_t* seq_idx;  // (batch, len) contiguous, or null
+  void* y;
+  float* last;
+  float* ckpt;  // (batch, ceil(len / kGatedT), dim): the state before each segment
+  const void* dy;
+  const float* dlast;
+  void* dx;
+  void* da_gate;
+  void* dx_gate;
+  float* ddecay;
+  float* ddecay_part;  // (batch, dim) partial sums over time
+  float* dinit;
+  int64_t batch, len, dim;
+  float c;
+  int64_t sx[3], sa[3], si[3], sy[3], sdy[3], sdx[3], sda[3], sdi[3];  // (batch, len, dim)
+};
+
+struct GatedStepParams {
+  float* state;
+  const void* x;
+  const void* a_gate;
+  const void* x_gate;
+  const float* decay;
+  void* y;
+  int64_t batch, dim;
+  float c;
+  int64_t sst[2], sx[2], sa[2], si[2];
+  const int32_t* state_idx;  // state row per batch row, or null
+  int64_t state_batch;
+};
+
+hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
+hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
+hipError_t gated_step_launch(const GatedStepParams& p, int dtype, hipStream_t st);
+
+}  // namespace mcpu

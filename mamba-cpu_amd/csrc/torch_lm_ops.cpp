@@ -1,0 +1,268 @@
+// The torch operators of a recurrent language model beside the scans of
+// torch_ops.cpp, in C++ over the C ABI of libmamba_hip.so, in the same manner:
+// registered for the CUDA dispatch key (ROCm GPU tensors) with autograd as
+// torch::autograd::Functions; argument errors raise ValueError or
+// NotImplementedError; outputs and workspaces come from torch's caching
+// allocator and launches go to the current stream, without synchronising.
+// Shape functions are registered from Python (mamba_cpu/ops/*.py).
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/autograd.h>
+#include <torch/library.h>
+
+#include <cstring>
+#include <tuple>
+
+#include "mamba_hip.h"
+#include "torch_util.h"
+
+namespace mcpu_torch {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+Tensor workspace(size_t bytes, const Tensor& like) {
+  return bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : Tensor();
+}
+void* ws_ptr(const Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
+
+// ---- gated linear recurrence -----------------------------------------------------
+
+void check_gated(const char* name, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate, const Tensor& decay,
+                 const optional<Tensor>& init, const optional<Tensor>& seq_idx) {
+  for (const optional<Tensor>& t : {opt(x), opt(a_gate), opt(x_gate), opt(decay), init, seq_idx}) check_gpu(name, t);
+  TORCH_CHECK_VALUE(x_dtype(x.scalar_type()) && a_gate.scalar_type() == x.scalar_type() &&
+                        x_gate.scalar_type() == x.scalar_type(),
+                    name, " expects x, a_gate and x_gate of one dtype among float32, bfloat16 and float16");
+  TORCH_CHECK_VALUE(x.dim() == 3 && a_gate.sizes() == x.sizes() && x_gate.sizes() == x.sizes(), name,
+                    " expects x, a_gate and x_gate of shape (batch, seqlen, dim)");
+  TORCH_CHECK_VALUE(decay.scalar_type() == at::kFloat && decay.dim() == 1 && decay.size(0) == x.size(2) &&
+                        decay.is_contiguous(),
+                    name, " expects a contiguous float32 decay of shape (dim,)");
+  TORCH_CHECK_VALUE(!has(init) || (init->scalar_type() == at::kFloat && init->dim() == 2 &&
+                                   init->size(0) == x.size(0) && init->size(1) == x.size(2) && init->is_contiguous()),
+                    name, " expects a contiguous float32 initial_state of shape (batch, dim)");
+  TORCH_CHECK_VALUE(!has(seq_idx) || (seq_idx->scalar_type() == at::kInt && seq_idx->dim() == 2 &&
+                                      seq_idx->size(0) == x.size(0) && seq_idx->size(1) == x.size(1) &&
+                                      seq_idx->is_contiguous()),
+                    name, " expects seq_idx as a contiguous int32 tensor of shape (batch, seqlen)");
+}
+
+mcpu_gated_scan_args gated_args(const Tensor& x, const Tensor& a_gate, const Tensor& x_gate, const Tensor& decay,
+                                const optional<Tensor>& init, const optional<Tensor>& seq_idx, double c) {
+  mcpu_gated_scan_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.x = x.data_ptr();
+  a.a_gate = a_gate.data_ptr();
+  a.x_gate = x_gate.data_ptr();
+  a.decay = static_cast<const float*>(decay.data_ptr());
+  a.initial_state = fptr(init);
+  a.seq_idx = has(seq_idx) ? static_cast<const int32_t*>(seq_idx->data_ptr()) : nullptr;
+  a.batch = x.size(0);
+  a.seqlen = x.size(1);
+  a.dim = x.size(2);
+  a.c = static_cast<float>(c);
+  a.dtype = dtype_tag(x.scalar_type());
+  strides3(a.x_stride, x);
+  strides3(a.a_stride, a_gate);
+  strides3(a.i_stride, x_gate);
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd(const Tensor& x, const Tensor& a_gate, const Tensor& x_gate,
+                                                  const Tensor& decay, const optional<Tensor>& init,
+                                                  const optional<Tensor>& seq_idx, double c, bool save) {
+  const char* name = "mamba_cpu::gated_scan_fwd";
+  check_gated(name, x, a_gate, x_gate, decay, init, seq_idx);
+  c10::DeviceGuard guard(x.device());
+  Tensor y = at::empty(x.sizes(), x.options());
+  Tensor last = at::empty({x.size(0), x.size(2)}, decay.options());
+  mcpu_gated_scan_args a = gated_args(x, a_gate, x_gate, decay, init, seq_idx, c);
+  const int64_t kept = save ? static_cast<int64_t>(mcpu_gated_scan_ckpt_size(&a) / sizeof(float)) : 0;
+  Tensor ckpt = at::empty({kept}, decay.options());
+  a.y = y.data_ptr();
+  strides3(a.y_stride, y);
+  a.last_state = static_cast<float*>(last.data_ptr());
+  a.ckpt = kept > 0 ? static_cast<float*>(ckpt.data_ptr()) : nullptr;
+  const size_t nws = mcpu_gated_scan_fwd_workspace_size(&a);
+  Tensor ws = workspace(nws, x);
+  check_rc(mcpu_gated_scan_fwd(&a, ws_ptr(ws), nws, stream_of(x)), name);
+  return {y, last, ckpt};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_scan_bwd(
+    const Tensor& dy, const optional<Tensor>& dlast, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate,
+    const Tensor& decay, const optional<Tensor>& init, const optional<Tensor>& seq_idx, double c,
+    const Tensor& ckpt) {
+  const char* name = "mamba_cpu::gated_scan_bwd";
+  check_gated(name, x, a_gate, x_gate, decay, init, seq_idx);
+  for (const optional<Tensor>& t : {opt(dy), dlast, opt(ckpt)}) check_gpu(name, t);
+  TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(), name,
+                    " expects dy shaped and typed like x");
+  TORCH_CHECK_VALUE(!has(dlast) || (dlast->scalar_type() == at::kFloat && dlast->dim() == 2 &&
+                                    dlast->size(0) == x.size(0) && dlast->size(1) == x.size(2) &&
+                                    dlast->is_contiguous()),
+                    name, " expects a contiguous float32 dlast_state of shape (batch, dim)");
+  c10::DeviceGuard guard(x.device());
+  mcpu_gated_scan_args a = gated_args(x, a_gate, x_gate, decay, init, seq_idx, c);
+  TORCH_CHECK_VALUE(ckpt.scalar_type() == at::kFloat && ckpt.is_contiguous() &&
+                        ckpt.numel() * sizeof(float) == mcpu_gated_scan_ckpt_size(&a),
+                    name, " expects the states that gated_scan_fwd kept");
+  Tensor dx = at::empty(x.sizes(), x.options()), da = at::empty(x.sizes(), x.options()),
+         di = at::empty(x.sizes(), x.options());
+  Tensor ddecay = at::empty(decay.sizes(), decay.options());
+  Tensor dinit = has(init) ? at::empty(init->sizes(), init->options()) : at::empty({0}, decay.options());
+  a.ckpt = static_cast<float*>(ckpt.data_ptr());
+  a.dy = dy.data_ptr();
+  strides3(a.dy_stride, dy);
+  a.dlast_state = fptr(dlast);
+  a.dx = dx.data_ptr();
+  strides3(a.dx_stride, dx);
+  a.da_gate = da.data_ptr();
+  strides3(a.da_stride, da);
+  a.dx_gate = di.data_ptr();
+  strides3(a.di_stride, di);
+  a.ddecay = static_cast<float*>(ddecay.data_ptr());
+  a.dinitial_state = has(init) ? static_cast<float*>(dinit.data_ptr()) : nullptr;
+  const size_t nws = mcpu_gated_scan_bwd_workspace_size(&a);
+  Tensor ws = workspace(nws, x);
+  check_rc(mcpu_gated_scan_bwd(&a, ws_ptr(ws), nws, stream_of(x)), name);
+  return {dx, da, di, ddecay, dinit};
+}
+
+// The states kept for the backward are an output without a gradient.
+struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate,
+                               const Tensor& decay, const optional<Tensor>& init, const optional<Tensor>& seq_idx,
+                               double c, bool save) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::gated_scan_fwd", "")
+                         .typed<decltype(gated_scan_fwd)>();
+    auto r = op.call(x, a_gate, x_gate, decay, init, seq_idx, c, save);
+    const Tensor ckpt = std::get<2>(r);
+    ctx->mark_non_differentiable({ckpt});
+    ctx->save_for_backward({x, a_gate, x_gate, decay, init.value_or(Tensor()), seq_idx.value_or(Tensor()), ckpt});
+    ctx->saved_data["c"] = c;
+    ctx->saved_data["save"] = save;
+    ctx->set_materialize_grads(false);
+    return {std::get<0>(r), std::get<1>(r), ckpt};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor& x = s[0];
+    const optional<Tensor> init = opt(s[4]), seq_idx = opt(s[5]);
+    TORCH_CHECK_VALUE(ctx->saved_data["save"].toBool(),
+                      "mamba_cpu::gated_scan_fwd kept no states (save=False), so it has no backward");
+    const Tensor dy = grads[0].defined() ? grads[0].to(x.scalar_type()) : at::zeros_like(x);
+    const optional<Tensor> dlast =
+        grads[1].defined() ? optional<Tensor>(grads[1].to(at::kFloat).contiguous()) : std::nullopt;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::gated_scan_bwd", "")
+                         .typed<decltype(gated_scan_bwd)>();
+    auto g = op.call(dy, dlast, x, s[1], s[2], s[3], init, seq_idx, ctx->saved_data["c"].toDouble(), s[6]);
+    return {std::get<0>(g), std::get<1>(g), std::get<2>(g), std::get<3>(g), has(init) ? std::get<4>(g) : Tensor(),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd_autograd(const Tensor& x, const Tensor& a_gate,
+                                                           const Tensor& x_gate, const Tensor& decay,
+                                                           const optional<Tensor>& init,
+                                                           const optional<Tensor>& seq_idx, double c, bool save) {
+  auto r = GatedScanFn::apply(x, a_gate, x_gate, decay, init, seq_idx, c, save);
+  return {r[0], r[1], r[2]};
+}
+
+Tensor gated_step(Tensor& state, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate, const Tensor& decay_in,
+                  double c, const optional<Tensor>& state_batch_indices) {
+  const char* name = "mamba_cpu::gated_step";
+  for (const optional<Tensor>& t : {opt(state), opt(x), opt(a_gate), opt(x_gate), opt(decay_in), state_batch_indices})
+    check_gpu(name, t);
+  TORCH_CHECK_VALUE(x_dtype(x.scalar_type()) && a_gate.scalar_type() == x.scalar_type() &&
+                        x_gate.scalar_type() == x.scalar_type(),
+                    name, " expects x, a_gate and x_gate of one dtype among float32, bfloat16 and float16");
+  TORCH_CHECK_VALUE(x.dim() == 2 && a_gate.sizes() == x.sizes() && x_gate.sizes() == x.sizes(), name,
+                    " expects x, a_gate and x_gate of shape (batch, dim)");
+  TORCH_CHECK_VALUE(decay_in.dim() == 1 && decay_in.size(0) == x.size(1), name, " expects decay of shape (dim,)");
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kFloat && state.dim() == 2 && state.size(1) == x.size(1) &&
+                        (has(state_batch_indices) || state.size(0) == x.size(0)),
+                    name, " expects a float32 state (batch, dim), or (rows, dim) with state_batch_indices");
+  TORCH_CHECK_VALUE(!has(state_batch_indices) ||
+                        (state_batch_indices->scalar_type() == at::kInt && state_batch_indices->dim() == 1 &&
+                         state_batch_indices->size(0) == x.size(0) && state_batch_indices->is_contiguous()),
+                    name, " expects state_batch_indices as a contiguous int32 tensor of shape (batch,)");
+  const Tensor decay = f32c(decay_in);
+  c10::DeviceGuard guard(x.device());
+  Tensor y = at::empty(x.sizes(), x.options());
+  mcpu_gated_step_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.state = static_cast<float*>(state.data_ptr());
+  a.x = x.data_ptr();
+  a.a_gate = a_gate.data_ptr();
+  a.x_gate = x_gate.data_ptr();
+  a.decay = static_cast<const float*>(decay.data_ptr());
+  a.y = y.data_ptr();
+  a.batch = x.size(0);
+  a.dim = x.size(1);
+  a.state_batch = state.size(0);
+  a.c = static_cast<float>(c);
+  a.dtype = dtype_tag(x.scalar_type());
+  for (int i = 0; i < 2; ++i) {
+    a.state_stride[i] = state.stride(i);
+    a.x_stride[i] = x.stride(i);
+    a.a_stride[i] = a_gate.stride(i);
+    a.i_stride[i] = x_gate.stride(i);
+  }
+  a.state_batch_indices =
+      has(state_batch_indices) ? static_cast<const int32_t*>(state_batch_indices->data_ptr()) : nullptr;
+  check_rc(mcpu_gated_step(&a, stream_of(x)), name);
+  return y;
+}
+
+Tensor gated_step_inplace(Tensor& state, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate,
+                          const Tensor& decay, double c, const optional<Tensor>& state_batch_indices) {
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::gated_step", "")
+                         .typed<decltype(gated_step)>();
+    y = op.call(state, x, a_gate, x_gate, decay, c, state_batch_indices);
+  }
+  state.unsafeGetTensorImpl()->bump_version();
+  return y;
+}
+
+}  // namespace
+}  // namespace mcpu_torch
+
+TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
+  m.def("gated_scan_fwd(Tensor x, Tensor a_gate, Tensor x_gate, Tensor decay, Tensor? initial_state, "
+        "Tensor? seq_idx, float c, bool save) -> (Tensor, Tensor, Tensor)");
+  m.def("gated_scan_bwd(Tensor dy, Tensor? dlast_state, Tensor x, Tensor a_gate, Tensor x_gate, Tensor decay, "
+        "Tensor? initial_state, Tensor? seq_idx, float c, Tensor ckpt) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("gated_step(Tensor(a!) state, Tensor x, Tensor a_gate, Tensor x_gate, Tensor decay, float c, "
+        "Tensor? state_batch_indices=None) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
+  using namespace mcpu_torch;
+  m.impl("gated_scan_fwd", &gated_scan_fwd);
+  m.impl("gated_scan_bwd", &gated_scan_bwd);
+  m.impl("gated_step", &gated_step);
+}
+
+TORCH_LIBRARY_IMPL(mamba_cpu, Autograd, m) {
+  using namespace mcpu_torch;
+  m.impl("gated_scan_fwd", &gated_scan_fwd_autograd);
+  // A decode step: no gradient flows through it.
+  m.impl("gated_step", torch::CppFunction::makeFallthrough());
+}
+
+TORCH_LIBRARY_IMPL(mamba_cpu, ADInplaceOrView, m) {
+  using namespace mcpu_torch;
+  m.impl("gated_step", &gated_step_inplace);
+}

@@ -151,9 +151,31 @@ class Mamba2StepArgs(ctypes.Structure):
     ]
 
 
+class GatedScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _P), ("a_gate", _P), ("x_gate", _P), ("decay", _P), ("initial_state", _P), ("seq_idx", _P),
+        ("batch", _I64), ("seqlen", _I64), ("dim", _I64), ("c", ctypes.c_float), ("dtype", _I32),
+        ("x_stride", _S3), ("a_stride", _S3), ("i_stride", _S3),
+        ("y", _P), ("y_stride", _S3), ("last_state", _P), ("ckpt", _P),
+        ("dy", _P), ("dy_stride", _S3), ("dlast_state", _P),
+        ("dx", _P), ("dx_stride", _S3), ("da_gate", _P), ("da_stride", _S3), ("dx_gate", _P), ("di_stride", _S3),
+        ("ddecay", _P), ("dinitial_state", _P),
+    ]
+
+
+class GatedStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("state", _P), ("x", _P), ("a_gate", _P), ("x_gate", _P), ("decay", _P), ("y", _P),
+        ("batch", _I64), ("dim", _I64), ("state_batch", _I64), ("c", ctypes.c_float), ("dtype", _I32),
+        ("state_stride", _S2), ("x_stride", _S2), ("a_stride", _S2), ("i_stride", _S2),
+        ("state_batch_indices", _P),
+    ]
+
+
 _BLOCKS = (("scan", ScanArgs), ("conv", ConvArgs), ("conv_update", ConvUpdateArgs),
            ("state_update", StateUpdateArgs), ("ssd", SsdArgs), ("mixer_step", MixerStepArgs),
-           ("norm_linear", NormLinearArgs), ("mamba2_step", Mamba2StepArgs))
+           ("norm_linear", NormLinearArgs), ("mamba2_step", Mamba2StepArgs),
+           ("gated_scan", GatedScanArgs), ("gated_step", GatedStepArgs))
 _ARGP = {n: ctypes.POINTER(c) for n, c in _BLOCKS}
 
 lib.mcpu_last_error.restype = ctypes.c_char_p
@@ -205,6 +227,15 @@ lib.mcpu_mamba2_step_workspace_size.argtypes = [_ARGP["mamba2_step"]]
 lib.mcpu_mamba2_step_workspace_size.restype = ctypes.c_size_t
 lib.mcpu_mamba2_step.argtypes = [_ARGP["mamba2_step"], _P, ctypes.c_size_t, _P]
 lib.mcpu_mamba2_step.restype = ctypes.c_int
+
+for _name in ("ckpt_size", "fwd_workspace_size", "bwd_workspace_size"):
+    getattr(lib, f"mcpu_gated_scan_{_name}").argtypes = [_ARGP["gated_scan"]]
+    getattr(lib, f"mcpu_gated_scan_{_name}").restype = ctypes.c_size_t
+for _name in ("fwd", "bwd"):
+    getattr(lib, f"mcpu_gated_scan_{_name}").argtypes = [_ARGP["gated_scan"], _P, ctypes.c_size_t, _P]
+    getattr(lib, f"mcpu_gated_scan_{_name}").restype = ctypes.c_int
+lib.mcpu_gated_step.argtypes = [_ARGP["gated_step"], _P]
+lib.mcpu_gated_step.restype = ctypes.c_int
 
 for _name, _cls in _BLOCKS:
     _want = lib.mcpu_args_size(_name.encode())

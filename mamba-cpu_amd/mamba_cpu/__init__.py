@@ -10,6 +10,8 @@ routes Hugging Face Mamba / FalconMamba / Jamba / Mamba-2 models on the GPU to t
 from mamba_cpu.ops import (
     causal_conv1d_fn,
     causal_conv1d_update,
+    gated_linear_scan_fn,
+    gated_linear_update,
     mamba_chunk_scan_combined,
     mamba_inner_fn,
     selective_scan_fn,
@@ -23,6 +25,8 @@ __all__ = [
     "causal_conv1d_fn",
     "causal_conv1d_ref",
     "causal_conv1d_update",
+    "gated_linear_scan_fn",
+    "gated_linear_update",
     "mamba_chunk_scan_combined",
     "mamba_inner_fn",
     "selective_scan_fn",
