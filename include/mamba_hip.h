@@ -49,7 +49,7 @@ const char* mcpu_version(void);
 
 /* sizeof() of an argument block ("scan", "conv", "conv_update",
  * "state_update", "ssd", "mixer_step", "norm_linear", "mamba2_step",
- * "gated_scan", "gated_step"), 0 for an unknown name. A binding must compare it with its own sizeof of each
+ * "gated_scan", "gated_step", "norm"), 0 for an unknown name. A binding must compare it with its own sizeof of each
  * block it uses before its first call: the library reads a whole block,
  * whatever the caller allocated. */
 size_t mcpu_args_size(const char* name);
@@ -636,6 +636,48 @@ typedef struct mcpu_gated_step_args {
 } mcpu_gated_step_args;
 
 int mcpu_gated_step(const mcpu_gated_step_args* a, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Residual norm.                                                            */
+/* ------------------------------------------------------------------------ */
+
+/* Per row, in float32: z = x + residual (residual optional),
+ *   layer norm  y = (z - mean) rstd weight + bias,  rstd = 1 / sqrt(var + eps)
+ *   RMS norm    y = z rstd weight + bias,           rstd = 1 / sqrt(mean(z^2) + eps)
+ * and res_out = z rounded to res_dtype. Backward, with zhat the normalised row
+ * and t = weight dy:
+ *   dz = rstd (t - mean(t) - zhat mean(t zhat)) + dres_out   (no mean(t) for RMS)
+ *   dx, dres = dz;  dweight = sum_rows dy zhat;  dbias = sum_rows dy
+ * x, y, dy and dx have `dtype`; residual, res_out, dres_out and dres have
+ * res_dtype, which is dtype or MCPU_F32. Rows are contiguous and a row stride
+ * apart; tensors without a stride field are contiguous. One block for both
+ * directions. No counterpart in the reference. */
+typedef struct mcpu_norm_args {
+  const void* x;
+  const void* residual;     /* optional */
+  const float* weight;      /* (dim) */
+  const float* bias;        /* (dim), optional */
+  int64_t rows, dim;
+  int64_t x_stride, res_stride, y_stride, dy_stride;  /* elements between rows */
+  float eps;
+  int32_t rms;              /* 1: RMS norm */
+  int32_t dtype, res_dtype;
+  void* y;
+  void* res_out;            /* optional */
+  float* mean;              /* (rows): written by the forward when given, read by the
+                               backward; not used by RMS norm */
+  float* rstd;              /* (rows): likewise */
+  const void* dy;
+  const void* dres_out;     /* optional */
+  void* dx;
+  void* dres;               /* optional */
+  float* dweight;
+  float* dbias;             /* required iff bias != NULL */
+} mcpu_norm_args;
+
+int mcpu_norm_fwd(const mcpu_norm_args* a, void* stream);
+size_t mcpu_norm_bwd_workspace_size(const mcpu_norm_args* a);
+int mcpu_norm_bwd(const mcpu_norm_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -58,12 +58,6 @@ GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
   return p;
 }
 
-int check_ws(const char* what, const void* ws, size_t have, size_t need) {
-  if (need > 0 && (ws == nullptr || have < need))
-    return fail(MCPU_ERR_INVALID, "%s: workspace of %zu bytes needed, got %zu", what, need, have);
-  return MCPU_OK;
-}
-
 }  // namespace
 }  // namespace mcpu
 
@@ -90,7 +84,7 @@ extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspac
   if (a->y == nullptr && a->batch * a->seqlen * a->dim > 0)
     return fail(MCPU_ERR_INVALID, "%s: y is required", what);
   if (any_negative({a->y_stride}, 3)) return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
-  if (int rc = check_ws(what, workspace, workspace_bytes, mcpu_gated_scan_fwd_workspace_size(a))) return rc;
+  if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_gated_scan_fwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   GatedScanParams p = make_gated(a);
   p.y = a->y;
@@ -120,7 +114,7 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
     return fail(MCPU_ERR_INVALID, "%s: the states the forward kept (ckpt) are required", what);
   if (any_negative({a->dy_stride, a->dx_stride, a->da_stride, a->di_stride}, 3))
     return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
-  if (int rc = check_ws(what, workspace, workspace_bytes, mcpu_gated_scan_bwd_workspace_size(a))) return rc;
+  if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_gated_scan_bwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->dim == 0) return MCPU_OK;

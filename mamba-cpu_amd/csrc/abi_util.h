@@ -22,6 +22,9 @@ inline bool valid_dtype(int dt) { return dt == MCPU_F32 || dt == MCPU_BF16 || dt
 inline int64_t dtype_size(int dt) { return dt == MCPU_F32 ? 4 : 2; }
 inline size_t align_up(size_t bytes) { return (bytes + 255) & ~size_t(255); }
 
+// MCPU_OK when a caller's workspace holds `need` bytes.
+int check_workspace(const char* what, const void* ws, size_t have, size_t need);
+
 // Fills n floats with zero on `stream`.
 int zero_f32(float* p, int64_t n, hipStream_t stream);
 

@@ -35,6 +35,12 @@ int hip_status(hipError_t e, const char* what) {
   return fail(MCPU_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
+  if (need > 0 && (ws == nullptr || have < need))
+    return fail(MCPU_ERR_INVALID, "%s: workspace of %zu bytes needed, got %zu", what, need, have);
+  return MCPU_OK;
+}
+
 int zero_f32(float* p, int64_t n, hipStream_t stream) {
   if (n <= 0) return MCPU_OK;
   int64_t blocks = (n + 255) / 256;
@@ -61,6 +67,7 @@ extern "C" size_t mcpu_args_size(const char* name) {
   if (std::strcmp(name, "mamba2_step") == 0) return sizeof(mcpu_mamba2_step_args);
   if (std::strcmp(name, "gated_scan") == 0) return sizeof(mcpu_gated_scan_args);
   if (std::strcmp(name, "gated_step") == 0) return sizeof(mcpu_gated_step_args);
+  if (std::strcmp(name, "norm") == 0) return sizeof(mcpu_norm_args);
   return 0;
 }
 

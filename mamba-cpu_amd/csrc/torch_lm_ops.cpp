@@ -236,6 +236,154 @@ Tensor gated_step_inplace(Tensor& state, const Tensor& x, const Tensor& a_gate, 
   return y;
 }
 
+// ---- residual norm -----------------------------------------------------------------
+
+// Rows the kernels take as they are: contiguous elements, any distance.
+Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
+
+void check_norm(const char* name, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
+                const optional<Tensor>& residual) {
+  for (const optional<Tensor>& t : {opt(x), opt(weight), bias, residual}) check_gpu(name, t);
+  TORCH_CHECK_VALUE(x_dtype(x.scalar_type()) && x.dim() == 2, name,
+                    " expects x (rows, dim) in float32, bfloat16 or float16");
+  for (const optional<Tensor>& t : {opt(weight), bias})
+    TORCH_CHECK_VALUE(!has(t) || (t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == x.size(1) &&
+                                  t->is_contiguous()),
+                      name, " expects contiguous float32 weight and bias of shape (dim,)");
+  TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == x.sizes() &&
+                                       (residual->scalar_type() == at::kFloat ||
+                                        residual->scalar_type() == x.scalar_type())),
+                    name, " expects residual shaped like x, in x's dtype or float32");
+}
+
+mcpu_norm_args norm_args(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
+                         const optional<Tensor>& residual, at::ScalarType res_dtype, double eps, bool rms) {
+  mcpu_norm_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.x = x.data_ptr();
+  a.residual = ptr(residual);
+  a.weight = static_cast<const float*>(weight.data_ptr());
+  a.bias = fptr(bias);
+  a.rows = x.size(0);
+  a.dim = x.size(1);
+  a.x_stride = x.stride(0);
+  a.res_stride = has(residual) ? residual->stride(0) : 0;
+  a.eps = static_cast<float>(eps);
+  a.rms = rms ? 1 : 0;
+  a.dtype = dtype_tag(x.scalar_type());
+  a.res_dtype = dtype_tag(res_dtype);
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd(const Tensor& x_in, const Tensor& weight,
+                                                    const optional<Tensor>& bias, const optional<Tensor>& res_in,
+                                                    double eps, bool rms, bool want_res, bool res_float32) {
+  const char* name = "mamba_cpu::norm_fwd";
+  check_norm(name, x_in, weight, bias, res_in);
+  c10::DeviceGuard guard(x_in.device());
+  const Tensor x = rows_of(x_in);
+  const optional<Tensor> residual = has(res_in) ? optional<Tensor>(rows_of(*res_in)) : std::nullopt;
+  const at::ScalarType rt = has(residual) ? residual->scalar_type() : (res_float32 ? at::kFloat : x.scalar_type());
+  Tensor y = at::empty(x.sizes(), x.options());
+  Tensor res = want_res ? at::empty(x.sizes(), x.options().dtype(rt)) : at::empty({0}, x.options().dtype(rt));
+  Tensor rstd = at::empty({x.size(0)}, weight.options());
+  Tensor mean = at::empty({rms ? 0 : x.size(0)}, weight.options());
+  mcpu_norm_args a = norm_args(x, weight, bias, residual, rt, eps, rms);
+  a.y = y.data_ptr();
+  a.y_stride = x.size(1);
+  a.res_out = want_res ? res.data_ptr() : nullptr;
+  a.mean = rms ? nullptr : static_cast<float*>(mean.data_ptr());
+  a.rstd = static_cast<float*>(rstd.data_ptr());
+  check_rc(mcpu_norm_fwd(&a, stream_of(x)), name);
+  return {y, res, mean, rstd};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> norm_bwd(const Tensor& dy_in, const optional<Tensor>& dres_out_in,
+                                                    const Tensor& x_in, const Tensor& weight,
+                                                    const optional<Tensor>& bias, const optional<Tensor>& res_in,
+                                                    double eps, bool rms, const Tensor& mean, const Tensor& rstd) {
+  const char* name = "mamba_cpu::norm_bwd";
+  check_norm(name, x_in, weight, bias, res_in);
+  for (const optional<Tensor>& t : {opt(dy_in), dres_out_in, opt(mean), opt(rstd)}) check_gpu(name, t);
+  TORCH_CHECK_VALUE(dy_in.sizes() == x_in.sizes() && dy_in.scalar_type() == x_in.scalar_type(), name,
+                    " expects dy shaped and typed like x");
+  TORCH_CHECK_VALUE(rstd.numel() == x_in.size(0) && (rms || mean.numel() == x_in.size(0)) &&
+                        rstd.scalar_type() == at::kFloat && mean.scalar_type() == at::kFloat &&
+                        rstd.is_contiguous() && mean.is_contiguous(),
+                    name, " expects the mean and rstd that norm_fwd returned");
+  c10::DeviceGuard guard(x_in.device());
+  const Tensor x = rows_of(x_in), dy = rows_of(dy_in);
+  const optional<Tensor> residual = has(res_in) ? optional<Tensor>(rows_of(*res_in)) : std::nullopt;
+  const at::ScalarType rt = has(residual) ? residual->scalar_type()
+                            : has(dres_out_in) ? dres_out_in->scalar_type() : x.scalar_type();
+  TORCH_CHECK_VALUE(!has(dres_out_in) || (dres_out_in->sizes() == x.sizes() && dres_out_in->scalar_type() == rt &&
+                                          (rt == at::kFloat || rt == x.scalar_type())),
+                    name, " expects dres_out shaped like x and typed like the residual");
+  const optional<Tensor> dres_out = has(dres_out_in) ? optional<Tensor>(dres_out_in->contiguous()) : std::nullopt;
+  Tensor dx = at::empty(x.sizes(), x.options());
+  Tensor dres = has(residual) ? at::empty(x.sizes(), residual->options()) : at::empty({0}, x.options());
+  Tensor dw = at::empty(weight.sizes(), weight.options());
+  Tensor db = at::empty({has(bias) ? x.size(1) : 0}, weight.options());
+  mcpu_norm_args a = norm_args(x, weight, bias, residual, rt, eps, rms);
+  a.mean = rms ? nullptr : static_cast<float*>(mean.data_ptr());
+  a.rstd = static_cast<float*>(rstd.data_ptr());
+  a.dy = dy.data_ptr();
+  a.dy_stride = dy.stride(0);
+  a.dres_out = ptr(dres_out);
+  a.dx = dx.data_ptr();
+  a.dres = has(residual) ? dres.data_ptr() : nullptr;
+  a.dweight = static_cast<float*>(dw.data_ptr());
+  a.dbias = has(bias) ? static_cast<float*>(db.data_ptr()) : nullptr;
+  const size_t nws = mcpu_norm_bwd_workspace_size(&a);
+  Tensor ws = workspace(nws, x);
+  check_rc(mcpu_norm_bwd(&a, ws_ptr(ws), nws, stream_of(x)), name);
+  return {dx, dres, dw, db};
+}
+
+struct NormFn : public torch::autograd::Function<NormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                               const optional<Tensor>& bias, const optional<Tensor>& residual, double eps, bool rms,
+                               bool want_res, bool res_float32) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::norm_fwd", "")
+                         .typed<decltype(norm_fwd)>();
+    auto r = op.call(x, weight, bias, residual, eps, rms, want_res, res_float32);
+    const Tensor mean = std::get<2>(r), rstd = std::get<3>(r);
+    ctx->mark_non_differentiable({mean, rstd});
+    ctx->save_for_backward({x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), mean, rstd});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["rms"] = rms;
+    ctx->saved_data["want_res"] = want_res;
+    ctx->set_materialize_grads(false);
+    return {std::get<0>(r), std::get<1>(r), mean, rstd};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor& x = s[0];
+    const optional<Tensor> bias = opt(s[2]), residual = opt(s[3]);
+    const Tensor dy = grads[0].defined() ? grads[0].to(x.scalar_type()) : at::zeros_like(x);
+    const optional<Tensor> dres_out =
+        ctx->saved_data["want_res"].toBool() && grads[1].defined() ? optional<Tensor>(grads[1]) : std::nullopt;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::norm_bwd", "")
+                         .typed<decltype(norm_bwd)>();
+    auto g = op.call(dy, dres_out, x, s[1], bias, residual, ctx->saved_data["eps"].toDouble(),
+                     ctx->saved_data["rms"].toBool(), s[4], s[5]);
+    return {std::get<0>(g), std::get<2>(g), has(bias) ? std::get<3>(g) : Tensor(),
+            has(residual) ? std::get<1>(g) : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd_autograd(const Tensor& x, const Tensor& weight,
+                                                             const optional<Tensor>& bias,
+                                                             const optional<Tensor>& residual, double eps, bool rms,
+                                                             bool want_res, bool res_float32) {
+  auto r = NormFn::apply(x, weight, bias, residual, eps, rms, want_res, res_float32);
+  return {r[0], r[1], r[2], r[3]};
+}
+
 }  // namespace
 }  // namespace mcpu_torch
 
@@ -246,6 +394,10 @@ TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
         "Tensor? initial_state, Tensor? seq_idx, float c, Tensor ckpt) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("gated_step(Tensor(a!) state, Tensor x, Tensor a_gate, Tensor x_gate, Tensor decay, float c, "
         "Tensor? state_batch_indices=None) -> Tensor");
+  m.def("norm_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, float eps, bool rms, bool want_residual, "
+        "bool residual_float32) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("norm_bwd(Tensor dy, Tensor? dresidual_out, Tensor x, Tensor weight, Tensor? bias, Tensor? residual, "
+        "float eps, bool rms, Tensor mean, Tensor rstd) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
@@ -253,11 +405,14 @@ TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
   m.impl("gated_scan_fwd", &gated_scan_fwd);
   m.impl("gated_scan_bwd", &gated_scan_bwd);
   m.impl("gated_step", &gated_step);
+  m.impl("norm_fwd", &norm_fwd);
+  m.impl("norm_bwd", &norm_bwd);
 }
 
 TORCH_LIBRARY_IMPL(mamba_cpu, Autograd, m) {
   using namespace mcpu_torch;
   m.impl("gated_scan_fwd", &gated_scan_fwd_autograd);
+  m.impl("norm_fwd", &norm_fwd_autograd);
   // A decode step: no gradient flows through it.
   m.impl("gated_step", torch::CppFunction::makeFallthrough());
 }

@@ -172,10 +172,20 @@ class GatedStepArgs(ctypes.Structure):
     ]
 
 
+class NormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _P), ("residual", _P), ("weight", _P), ("bias", _P), ("rows", _I64), ("dim", _I64),
+        ("x_stride", _I64), ("res_stride", _I64), ("y_stride", _I64), ("dy_stride", _I64),
+        ("eps", ctypes.c_float), ("rms", _I32), ("dtype", _I32), ("res_dtype", _I32),
+        ("y", _P), ("res_out", _P), ("mean", _P), ("rstd", _P), ("dy", _P), ("dres_out", _P), ("dx", _P),
+        ("dres", _P), ("dweight", _P), ("dbias", _P),
+    ]
+
+
 _BLOCKS = (("scan", ScanArgs), ("conv", ConvArgs), ("conv_update", ConvUpdateArgs),
            ("state_update", StateUpdateArgs), ("ssd", SsdArgs), ("mixer_step", MixerStepArgs),
            ("norm_linear", NormLinearArgs), ("mamba2_step", Mamba2StepArgs),
-           ("gated_scan", GatedScanArgs), ("gated_step", GatedStepArgs))
+           ("gated_scan", GatedScanArgs), ("gated_step", GatedStepArgs), ("norm", NormArgs))
 _ARGP = {n: ctypes.POINTER(c) for n, c in _BLOCKS}
 
 lib.mcpu_last_error.restype = ctypes.c_char_p
@@ -236,6 +246,13 @@ for _name in ("fwd", "bwd"):
     getattr(lib, f"mcpu_gated_scan_{_name}").restype = ctypes.c_int
 lib.mcpu_gated_step.argtypes = [_ARGP["gated_step"], _P]
 lib.mcpu_gated_step.restype = ctypes.c_int
+
+lib.mcpu_norm_fwd.argtypes = [_ARGP["norm"], _P]
+lib.mcpu_norm_fwd.restype = ctypes.c_int
+lib.mcpu_norm_bwd_workspace_size.argtypes = [_ARGP["norm"]]
+lib.mcpu_norm_bwd_workspace_size.restype = ctypes.c_size_t
+lib.mcpu_norm_bwd.argtypes = [_ARGP["norm"], _P, ctypes.c_size_t, _P]
+lib.mcpu_norm_bwd.restype = ctypes.c_int
 
 for _name, _cls in _BLOCKS:
     _want = lib.mcpu_args_size(_name.encode())

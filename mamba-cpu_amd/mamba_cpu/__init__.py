@@ -12,6 +12,7 @@ from mamba_cpu.ops import (
     causal_conv1d_update,
     gated_linear_scan_fn,
     gated_linear_update,
+    layer_norm_fn,
     mamba_chunk_scan_combined,
     mamba_inner_fn,
     selective_scan_fn,
@@ -27,6 +28,7 @@ __all__ = [
     "causal_conv1d_update",
     "gated_linear_scan_fn",
     "gated_linear_update",
+    "layer_norm_fn",
     "mamba_chunk_scan_combined",
     "mamba_inner_fn",
     "selective_scan_fn",

@@ -76,3 +76,29 @@ def gated_step(state, x, a_gate, x_gate, decay, c=8.0):
     state, x, a_gate, x_gate, decay = (_f64(t) for t in (state, x, a_gate, x_gate, decay))
     _, iota, _, a, m = _gates(x, a_gate, x_gate, decay, c)
     return a * state + m * iota * x
+
+
+def norm_fwd(x, weight, bias=None, residual=None, eps=1e-5, rms=False):
+    """y and z = x + residual, rows along the last axis."""
+    z = _f64(x) if residual is None else _f64(x) + _f64(residual)
+    mean = 0.0 if rms else z.mean(-1, keepdims=True)
+    var = ((z - mean) ** 2).mean(-1, keepdims=True)
+    y = (z - mean) / np.sqrt(var + eps) * _f64(weight)
+    return (y if bias is None else y + _f64(bias)), z
+
+
+def norm_bwd(x, weight, dy, bias=None, residual=None, dz_out=None, eps=1e-5, rms=False):
+    """Gradients of z (x's and the residual's), weight and bias. Through the
+    row's Jacobian: d zhat_i / d z_j = (delta_ij - [layer] 1 / n - zhat_i zhat_j / n) / std."""
+    z = _f64(x) if residual is None else _f64(x) + _f64(residual)
+    n = z.shape[-1]
+    centre = np.eye(n) if rms else np.eye(n) - 1.0 / n
+    zc = z @ centre
+    std = np.sqrt((zc ** 2).mean(-1, keepdims=True) + eps)
+    zhat = zc / std
+    t = _f64(dy) * _f64(weight)
+    dz = (t / std - zhat * (t * zhat).sum(-1, keepdims=True) / (n * std)) @ centre
+    if dz_out is not None:
+        dz = dz + _f64(dz_out)
+    flat = lambda v: v.reshape(-1, n)  # noqa: E731
+    return dz, flat(_f64(dy) * zhat).sum(0), flat(_f64(dy)).sum(0)
