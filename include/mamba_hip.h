@@ -49,7 +49,8 @@ const char* mcpu_version(void);
 
 /* sizeof() of an argument block ("scan", "conv", "conv_update",
  * "state_update", "ssd", "mixer_step", "norm_linear", "mamba2_step",
- * "gated_scan", "gated_step", "norm"), 0 for an unknown name. A binding must compare it with its own sizeof of each
+ * "gated_scan", "gated_step", "norm", "embedding", "sample"), 0 for an
+ * unknown name. A binding must compare it with its own sizeof of each
  * block it uses before its first call: the library reads a whole block,
  * whatever the caller allocated. */
 size_t mcpu_args_size(const char* name);
@@ -678,6 +679,72 @@ typedef struct mcpu_norm_args {
 int mcpu_norm_fwd(const mcpu_norm_args* a, void* stream);
 size_t mcpu_norm_bwd_workspace_size(const mcpu_norm_args* a);
 int mcpu_norm_bwd(const mcpu_norm_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Embedding.                                                                */
+/* ------------------------------------------------------------------------ */
+
+/* out_t = scale weight[ids_t];  dweight_v = scale sum_{t: ids_t = v} dout_t,
+ * summed in float32 over the tokens of v in their order and rounded once. An
+ * id outside [0, vocab) has a zero row and no gradient. weight, out, dout and
+ * dweight have `dtype`; rows are contiguous and a row stride apart; ids, out
+ * and dweight are contiguous. No counterpart in the reference. */
+typedef struct mcpu_embedding_args {
+  const void* ids;          /* (tokens) int32, or int64 when ids64 */
+  const void* weight;       /* (vocab, dim); not read by the backward */
+  int64_t tokens, vocab, dim;
+  int64_t weight_stride, dout_stride;  /* elements between rows */
+  float scale;
+  int32_t dtype;
+  int32_t ids64;
+  int32_t _pad;
+  void* out;                /* (tokens, dim) */
+  const void* dout;         /* (tokens, dim) */
+  void* dweight;            /* (vocab, dim), every row written */
+} mcpu_embedding_args;
+
+int mcpu_embedding_fwd(const mcpu_embedding_args* a, void* stream);
+size_t mcpu_embedding_bwd_workspace_size(const mcpu_embedding_args* a);
+int mcpu_embedding_bwd(const mcpu_embedding_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Token sampling.                                                           */
+/* ------------------------------------------------------------------------ */
+
+/* One token per row of logits, from random numbers the caller gives. With M
+ * the row's largest logit, T its temperature and w = exp((l - M) / T), in the
+ * order of the logits (descending, equal ones by index):
+ *   top_k > 0 keeps the first top_k;
+ *   top_p < 1 keeps a token while the mass of the kept before it is below
+ *     top_p times the mass of all kept;
+ *   min_p keeps w >= min(min_p, 1);
+ *   the first token is always kept.
+ * token = the kept one with the largest w / noise, equal ones by index: with
+ * noise from Exp(1) a draw from the kept by weight. T <= 0 takes the first
+ * token. A row whose logits are all -inf or NaN has no token: -1, logprob
+ * -inf; a NaN logit counts as -inf. logprob = log softmax(logits)[token],
+ * before temperature and cuts. Settings come as one number, or per row where
+ * the pointer is given. No counterpart in the reference. */
+typedef struct mcpu_sample_args {
+  const void* logits;       /* (rows, vocab), dtype, rows contiguous */
+  const float* noise;       /* (rows, vocab) above 0, rows contiguous; NULL allowed where the one
+                               temperature is <= 0 */
+  int64_t rows, vocab;      /* vocab at most 2^23 */
+  int64_t logits_stride, noise_stride;  /* elements between rows */
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_rows;  /* (rows), optional; likewise below */
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int32_t* top_k_rows;
+  int64_t* token;           /* (rows) */
+  float* logprob;           /* (rows), optional */
+  int32_t dtype;
+  int32_t _pad;
+} mcpu_sample_args;
+
+size_t mcpu_sample_workspace_size(const mcpu_sample_args* a);
+int mcpu_sample(const mcpu_sample_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

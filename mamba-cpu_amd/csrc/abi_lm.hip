@@ -1,5 +1,5 @@
-// C-ABI entry points of the residual norm: argument checks, workspace layout,
-// launches.
+// C-ABI entry points of the residual norm, the embedding and the token sampler:
+// argument checks, workspace layout, launches.
 #include <climits>
 #include <cstring>
 
@@ -47,6 +47,59 @@ NormParams make_norm(const mcpu_norm_args* a) {
   p.mean = a->mean;
   p.rstd = a->rstd;
   return p;
+}
+
+// ---- embedding ----------------------------------------------------------------------
+
+int check_embedding(const mcpu_embedding_args* a, const char* what) {
+  if (a == nullptr) return fail(MCPU_ERR_INVALID, "%s: null argument block", what);
+  if (a->tokens < 0 || a->vocab < 0 || a->dim < 0) return fail(MCPU_ERR_INVALID, "%s: negative size", what);
+  if (!valid_dtype(a->dtype) || (a->ids64 != 0 && a->ids64 != 1))
+    return fail(MCPU_ERR_INVALID, "%s: bad dtype %d or ids64 %d", what, a->dtype, a->ids64);
+  if (a->weight_stride < 0 || a->dout_stride < 0) return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
+  if (a->tokens > INT_MAX - 64 || a->vocab > INT_MAX - 1024 || a->dim > INT_MAX)
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: tokens, vocab and dim must fit 31 bits", what);
+  if (a->tokens > 0 && a->ids == nullptr) return fail(MCPU_ERR_INVALID, "%s: ids are required", what);
+  return MCPU_OK;
+}
+
+EmbeddingParams make_embedding(const mcpu_embedding_args* a) {
+  EmbeddingParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.ids = a->ids;
+  p.ids64 = a->ids64;
+  p.weight = a->weight;
+  p.tokens = a->tokens;
+  p.vocab = a->vocab;
+  p.dim = a->dim;
+  p.sw = a->weight_stride;
+  p.sdo = a->dout_stride;
+  p.scale = a->scale;
+  p.dtype = a->dtype;
+  return p;
+}
+
+// ---- sampling -----------------------------------------------------------------------
+
+int check_sample(const mcpu_sample_args* a, const char* what) {
+  if (a == nullptr) return fail(MCPU_ERR_INVALID, "%s: null argument block", what);
+  if (a->rows < 0 || a->vocab < 0) return fail(MCPU_ERR_INVALID, "%s: negative size", what);
+  if (!valid_dtype(a->dtype)) return fail(MCPU_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
+  if (a->logits_stride < 0 || a->noise_stride < 0) return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
+  if (a->rows > INT_MAX || a->vocab > (1 << 23))
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows of 2^23 logits", what);
+  if (a->rows > 0 && a->vocab == 0) return fail(MCPU_ERR_INVALID, "%s: no logits to choose from", what);
+  if (a->temperature_rows == nullptr && !(a->temperature == a->temperature))
+    return fail(MCPU_ERR_INVALID, "%s: temperature must be a number", what);
+  if (a->top_p_rows == nullptr && !(a->top_p >= 0.f && a->top_p <= 1.f))
+    return fail(MCPU_ERR_INVALID, "%s: top_p must lie in [0, 1]", what);
+  if (a->min_p_rows == nullptr && !(a->min_p >= 0.f && a->min_p <= 1.f))
+    return fail(MCPU_ERR_INVALID, "%s: min_p must lie in [0, 1]", what);
+  if (a->top_k_rows == nullptr && a->top_k < 0) return fail(MCPU_ERR_INVALID, "%s: top_k must not be negative", what);
+  const bool greedy = a->temperature_rows == nullptr && a->temperature <= 0.f;
+  if (a->rows > 0 && (a->logits == nullptr || a->token == nullptr || (a->noise == nullptr && !greedy)))
+    return fail(MCPU_ERR_INVALID, "%s: logits, token and noise (above temperature 0) are required", what);
+  return MCPU_OK;
 }
 
 }  // namespace
@@ -97,4 +150,77 @@ extern "C" int mcpu_norm_bwd(const mcpu_norm_args* a, void* workspace, size_t wo
   p.part = static_cast<float*>(workspace);
   p.parts = norm_bwd_parts(a->rows, a->dim);
   return hip_status(norm_bwd_launch(p, static_cast<hipStream_t>(stream)), "norm_bwd launch");
+}
+
+extern "C" int mcpu_embedding_fwd(const mcpu_embedding_args* a, void* stream) {
+  const char* what = "embedding_fwd";
+  clear_error();
+  if (int rc = check_embedding(a, what)) return rc;
+  if (a->tokens * a->dim > 0 && ((a->weight == nullptr && a->vocab > 0) || a->out == nullptr))
+    return fail(MCPU_ERR_INVALID, "%s: weight and out are required", what);
+  if (int rc = mcpu_check_device()) return rc;
+  if (a->tokens == 0 || a->dim == 0) return MCPU_OK;
+  EmbeddingParams p = make_embedding(a);
+  p.out = a->out;
+  return hip_status(embedding_fwd_launch(p, static_cast<hipStream_t>(stream)), "embedding_fwd launch");
+}
+
+extern "C" size_t mcpu_embedding_bwd_workspace_size(const mcpu_embedding_args* a) {
+  if (check_embedding(a, "embedding") != MCPU_OK) {
+    clear_error();
+    return 0;
+  }
+  return align_up(sizeof(int32_t) * a->tokens) + align_up(sizeof(int32_t) * (a->vocab + 1));
+}
+
+extern "C" int mcpu_embedding_bwd(const mcpu_embedding_args* a, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  const char* what = "embedding_bwd";
+  clear_error();
+  if (int rc = check_embedding(a, what)) return rc;
+  if ((a->tokens * a->dim > 0 && a->dout == nullptr) || (a->vocab * a->dim > 0 && a->dweight == nullptr))
+    return fail(MCPU_ERR_INVALID, "%s: dout and dweight are required", what);
+  if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_embedding_bwd_workspace_size(a))) return rc;
+  if (int rc = mcpu_check_device()) return rc;
+  if (a->vocab == 0 || a->dim == 0) return MCPU_OK;
+  EmbeddingParams p = make_embedding(a);
+  p.dout = a->dout;
+  p.dweight = a->dweight;
+  p.order = static_cast<int32_t*>(workspace);
+  p.start = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + align_up(sizeof(int32_t) * a->tokens));
+  return hip_status(embedding_bwd_launch(p, static_cast<hipStream_t>(stream)), "embedding_bwd launch");
+}
+
+extern "C" size_t mcpu_sample_workspace_size(const mcpu_sample_args* a) {
+  if (check_sample(a, "sample") != MCPU_OK) clear_error();
+  return 0;
+}
+
+extern "C" int mcpu_sample(const mcpu_sample_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "sample";
+  clear_error();
+  if (int rc = check_sample(a, what)) return rc;
+  if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_sample_workspace_size(a))) return rc;
+  if (int rc = mcpu_check_device()) return rc;
+  if (a->rows == 0) return MCPU_OK;
+  SampleParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.logits = a->logits;
+  p.noise = a->noise;
+  p.temperature = a->temperature;
+  p.top_p = a->top_p;
+  p.min_p = a->min_p;
+  p.top_k = a->top_k;
+  p.temperature_rows = a->temperature_rows;
+  p.top_p_rows = a->top_p_rows;
+  p.min_p_rows = a->min_p_rows;
+  p.top_k_rows = a->top_k_rows;
+  p.token = a->token;
+  p.logprob = a->logprob;
+  p.rows = a->rows;
+  p.vocab = a->vocab;
+  p.sl = a->logits_stride;
+  p.sn = a->noise_stride;
+  p.dtype = a->dtype;
+  return hip_status(sample_launch(p, static_cast<hipStream_t>(stream)), "sample launch");
 }

@@ -68,6 +68,8 @@ extern "C" size_t mcpu_args_size(const char* name) {
   if (std::strcmp(name, "gated_scan") == 0) return sizeof(mcpu_gated_scan_args);
   if (std::strcmp(name, "gated_step") == 0) return sizeof(mcpu_gated_step_args);
   if (std::strcmp(name, "norm") == 0) return sizeof(mcpu_norm_args);
+  if (std::strcmp(name, "embedding") == 0) return sizeof(mcpu_embedding_args);
+  if (std::strcmp(name, "sample") == 0) return sizeof(mcpu_sample_args);
   return 0;
 }
 

@@ -20,35 +20,10 @@
 // from the one the forward kept in front of every segment, in float32 (the
 // stored y may be 16 bits wide).
 #include "gated_scan.h"
-#include "mcpu_common.h"
+#include "lm_math.h"
 
 namespace mcpu {
 namespace {
-
-// exp(x) to about 1 ulp over the whole range: the rounding error of
-// x * log2(e) is carried along (v_exp_f32 alone loses |x| ulp). Clamped where
-// the result leaves the normal range, so that infinities stay exact; NaN
-// passes through.
-__device__ __forceinline__ float exp_acc(float x) {
-  x = x > 88.f ? 88.f : (x < -104.f ? -104.f : x);
-  const float t = x * kLog2e;
-  const float lo = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;  // log2(e) - float(log2(e))
-  const float e = fast_exp2(t);
-  return fmaf(e, lo * kLn2, e);
-}
-
-// sigmoid(x) and 1 - sigmoid(x) from one exponential, each to its own ulp.
-__device__ __forceinline__ float sigmoid_acc(float x, float& one_minus) {
-  const float e = exp_acc(-x);
-  const float s = fast_rcp(1.0f + e);
-  one_minus = e * s;
-  return s;
-}
-
-// c softplus(x), stable at both ends.
-__device__ __forceinline__ float softplus_acc(float x) {
-  return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x)));
-}
 
 // 1 - exp(-y) for y >= 0, given ey = exp(-y): below 1/2 its series, whose
 // first dropped term is y^9 / 9!, above it the difference, which loses less than two bits.

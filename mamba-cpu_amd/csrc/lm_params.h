@@ -36,4 +36,39 @@ int64_t norm_bwd_parts(int64_t rows, int64_t dim);
 hipError_t norm_fwd_launch(const NormParams& p, hipStream_t st);
 hipError_t norm_bwd_launch(const NormParams& p, hipStream_t st);
 
+struct EmbeddingParams {
+  const void* ids;  // (tokens) int32 or int64
+  int ids64;
+  const void* weight;  // (vocab, dim), row stride sw
+  void* out;           // (tokens, dim) contiguous
+  const void* dout;    // (tokens, dim), row stride sdo
+  void* dweight;       // (vocab, dim) contiguous
+  int32_t* order;      // token positions sorted by id, in token order within an id
+  int32_t* start;      // (vocab + 1): where each id's positions start in `order`
+  int64_t tokens, vocab, dim, sw, sdo;
+  float scale;
+  int dtype;
+};
+
+hipError_t embedding_fwd_launch(const EmbeddingParams& p, hipStream_t st);
+hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st);
+
+struct SampleParams {
+  const void* logits;  // (rows, vocab), row stride sl
+  const float* noise;  // (rows, vocab), row stride sn, or null
+  // One setting for all rows, or one per row where the pointer is given.
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int32_t* top_k_rows;
+  int64_t* token;   // (rows)
+  float* logprob;   // (rows), or null
+  int64_t rows, vocab, sl, sn;
+  int dtype;
+};
+
+hipError_t sample_launch(const SampleParams& p, hipStream_t st);
+
 }  // namespace mcpu

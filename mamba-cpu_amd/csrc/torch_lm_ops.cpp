@@ -10,6 +10,7 @@
 #include <torch/autograd.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstring>
 #include <tuple>
 
@@ -384,6 +385,144 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd_autograd(const Tensor& x, co
   return {r[0], r[1], r[2], r[3]};
 }
 
+// ---- embedding ------------------------------------------------------------------------
+
+Tensor embedding_ids(const char* name, const Tensor& ids) {
+  check_gpu(name, ids);
+  TORCH_CHECK_VALUE((ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) && ids.dim() == 1, name,
+                    " expects ids (tokens,) in int32 or int64");
+  return ids.contiguous();
+}
+
+mcpu_embedding_args embedding_args(const Tensor& ids, int64_t vocab, int64_t dim, double scale,
+                                   at::ScalarType dtype) {
+  mcpu_embedding_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.ids = ids.data_ptr();
+  a.tokens = ids.size(0);
+  a.vocab = vocab;
+  a.dim = dim;
+  a.scale = static_cast<float>(scale);
+  a.dtype = dtype_tag(dtype);
+  a.ids64 = ids.scalar_type() == at::kLong ? 1 : 0;
+  return a;
+}
+
+Tensor embedding_fwd(const Tensor& ids_in, const Tensor& weight_in, double scale) {
+  const char* name = "mamba_cpu::embedding_fwd";
+  check_gpu(name, weight_in);
+  TORCH_CHECK_VALUE(weight_in.dim() == 2 && x_dtype(weight_in.scalar_type()), name,
+                    " expects weight (vocab, dim) in float32, bfloat16 or float16");
+  c10::DeviceGuard guard(weight_in.device());
+  const Tensor ids = embedding_ids(name, ids_in), weight = rows_of(weight_in);
+  Tensor out = at::empty({ids.size(0), weight.size(1)}, weight.options());
+  mcpu_embedding_args a = embedding_args(ids, weight.size(0), weight.size(1), scale, weight.scalar_type());
+  a.weight = weight.data_ptr();
+  a.weight_stride = weight.stride(0);
+  a.out = out.data_ptr();
+  check_rc(mcpu_embedding_fwd(&a, stream_of(weight)), name);
+  return out;
+}
+
+Tensor embedding_bwd(const Tensor& dout_in, const Tensor& ids_in, int64_t vocab, double scale) {
+  const char* name = "mamba_cpu::embedding_bwd";
+  check_gpu(name, dout_in);
+  TORCH_CHECK_VALUE(dout_in.dim() == 2 && dout_in.size(0) == ids_in.size(0) && x_dtype(dout_in.scalar_type()) &&
+                        vocab >= 0,
+                    name, " expects dout (tokens, dim) in float32, bfloat16 or float16");
+  c10::DeviceGuard guard(dout_in.device());
+  const Tensor ids = embedding_ids(name, ids_in), dout = rows_of(dout_in);
+  Tensor dw = at::empty({vocab, dout.size(1)}, dout.options());
+  mcpu_embedding_args a = embedding_args(ids, vocab, dout.size(1), scale, dout.scalar_type());
+  a.dout = dout.data_ptr();
+  a.dout_stride = dout.stride(0);
+  a.dweight = dw.data_ptr();
+  const size_t nws = mcpu_embedding_bwd_workspace_size(&a);
+  Tensor ws = workspace(nws, dout);
+  check_rc(mcpu_embedding_bwd(&a, ws_ptr(ws), nws, stream_of(dout)), name);
+  return dw;
+}
+
+struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::embedding_fwd", "")
+                         .typed<decltype(embedding_fwd)>();
+    ctx->save_for_backward({ids});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    return op.call(ids, weight, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::embedding_bwd", "")
+                         .typed<decltype(embedding_bwd)>();
+    return {Tensor(), op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["vocab"].toInt(),
+                              ctx->saved_data["scale"].toDouble()),
+            Tensor()};
+  }
+};
+
+Tensor embedding_fwd_autograd(const Tensor& ids, const Tensor& weight, double scale) {
+  return EmbeddingFn::apply(ids, weight, scale);
+}
+
+// ---- sampling -------------------------------------------------------------------------
+
+const Tensor& check_setting(const char* name, const char* what, const Tensor& t, at::ScalarType dtype, int64_t rows) {
+  check_gpu(name, t);
+  TORCH_CHECK_VALUE(t.scalar_type() == dtype && t.dim() == 1 && t.size(0) == rows && t.is_contiguous(), name,
+                    " expects ", what, " per row as a contiguous ", dtype, " tensor of shape (rows,)");
+  return t;
+}
+
+std::tuple<Tensor, Tensor> sample(const Tensor& logits_in, const optional<Tensor>& noise_in, double temperature,
+                                  int64_t top_k, double top_p, double min_p,
+                                  const optional<Tensor>& temperature_rows, const optional<Tensor>& top_k_rows,
+                                  const optional<Tensor>& top_p_rows, const optional<Tensor>& min_p_rows,
+                                  bool logprobs) {
+  const char* name = "mamba_cpu::sample";
+  check_gpu(name, logits_in);
+  check_gpu(name, noise_in);
+  TORCH_CHECK_VALUE(logits_in.dim() == 2 && x_dtype(logits_in.scalar_type()), name,
+                    " expects logits (rows, vocab) in float32, bfloat16 or float16");
+  TORCH_CHECK_VALUE(!has(noise_in) || (noise_in->sizes() == logits_in.sizes() &&
+                                       noise_in->scalar_type() == at::kFloat),
+                    name, " expects float32 noise shaped like logits");
+  c10::DeviceGuard guard(logits_in.device());
+  const Tensor logits = rows_of(logits_in);
+  const optional<Tensor> noise = has(noise_in) ? optional<Tensor>(rows_of(*noise_in)) : std::nullopt;
+  const int64_t rows = logits.size(0);
+  Tensor token = at::empty({rows}, logits.options().dtype(at::kLong));
+  Tensor logprob = at::empty({logprobs ? rows : 0}, logits.options().dtype(at::kFloat));
+  mcpu_sample_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.logits = logits.data_ptr();
+  a.noise = fptr(noise);
+  a.rows = rows;
+  a.vocab = logits.size(1);
+  a.logits_stride = logits.stride(0);
+  a.noise_stride = has(noise) ? noise->stride(0) : 0;
+  a.temperature = static_cast<float>(temperature);
+  a.top_p = static_cast<float>(top_p);
+  a.min_p = static_cast<float>(min_p);
+  a.top_k = static_cast<int32_t>(std::min<int64_t>(top_k, INT32_MAX));
+  if (has(temperature_rows))
+    a.temperature_rows = fptr(check_setting(name, "temperature", *temperature_rows, at::kFloat, rows));
+  if (has(top_p_rows)) a.top_p_rows = fptr(check_setting(name, "top_p", *top_p_rows, at::kFloat, rows));
+  if (has(min_p_rows)) a.min_p_rows = fptr(check_setting(name, "min_p", *min_p_rows, at::kFloat, rows));
+  if (has(top_k_rows))
+    a.top_k_rows = static_cast<const int32_t*>(check_setting(name, "top_k", *top_k_rows, at::kInt, rows).data_ptr());
+  a.token = token.data_ptr<int64_t>();
+  a.logprob = logprobs && rows > 0 ? static_cast<float*>(logprob.data_ptr()) : nullptr;
+  a.dtype = dtype_tag(logits.scalar_type());
+  const size_t nws = mcpu_sample_workspace_size(&a);
+  Tensor ws = workspace(nws, logits);
+  check_rc(mcpu_sample(&a, ws_ptr(ws), nws, stream_of(logits)), name);
+  return {token, logprob};
+}
+
 }  // namespace
 }  // namespace mcpu_torch
 
@@ -398,6 +537,11 @@ TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
         "bool residual_float32) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("norm_bwd(Tensor dy, Tensor? dresidual_out, Tensor x, Tensor weight, Tensor? bias, Tensor? residual, "
         "float eps, bool rms, Tensor mean, Tensor rstd) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("embedding_fwd(Tensor ids, Tensor weight, float scale) -> Tensor");
+  m.def("embedding_bwd(Tensor dout, Tensor ids, int vocab, float scale) -> Tensor");
+  m.def("sample(Tensor logits, Tensor? noise, float temperature, int top_k, float top_p, float min_p, "
+        "Tensor? temperature_rows, Tensor? top_k_rows, Tensor? top_p_rows, Tensor? min_p_rows, bool logprobs) -> "
+        "(Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
@@ -407,13 +551,18 @@ TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
   m.impl("gated_step", &gated_step);
   m.impl("norm_fwd", &norm_fwd);
   m.impl("norm_bwd", &norm_bwd);
+  m.impl("embedding_fwd", &embedding_fwd);
+  m.impl("embedding_bwd", &embedding_bwd);
+  m.impl("sample", &sample);
 }
 
 TORCH_LIBRARY_IMPL(mamba_cpu, Autograd, m) {
   using namespace mcpu_torch;
   m.impl("gated_scan_fwd", &gated_scan_fwd_autograd);
   m.impl("norm_fwd", &norm_fwd_autograd);
-  // A decode step: no gradient flows through it.
+  m.impl("embedding_fwd", &embedding_fwd_autograd);
+  // No gradient flows through a decode step or a choice of tokens.
+  m.impl("sample", torch::CppFunction::makeFallthrough());
   m.impl("gated_step", torch::CppFunction::makeFallthrough());
 }
 

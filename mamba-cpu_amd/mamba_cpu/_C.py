@@ -182,10 +182,28 @@ class NormArgs(ctypes.Structure):
     ]
 
 
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [
+        ("ids", _P), ("weight", _P), ("tokens", _I64), ("vocab", _I64), ("dim", _I64),
+        ("weight_stride", _I64), ("dout_stride", _I64), ("scale", ctypes.c_float), ("dtype", _I32),
+        ("ids64", _I32), ("_pad", _I32), ("out", _P), ("dout", _P), ("dweight", _P),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", _P), ("noise", _P), ("rows", _I64), ("vocab", _I64), ("logits_stride", _I64),
+        ("noise_stride", _I64), ("temperature", ctypes.c_float), ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float), ("top_k", _I32), ("temperature_rows", _P), ("top_p_rows", _P),
+        ("min_p_rows", _P), ("top_k_rows", _P), ("token", _P), ("logprob", _P), ("dtype", _I32), ("_pad", _I32),
+    ]
+
+
 _BLOCKS = (("scan", ScanArgs), ("conv", ConvArgs), ("conv_update", ConvUpdateArgs),
            ("state_update", StateUpdateArgs), ("ssd", SsdArgs), ("mixer_step", MixerStepArgs),
            ("norm_linear", NormLinearArgs), ("mamba2_step", Mamba2StepArgs),
-           ("gated_scan", GatedScanArgs), ("gated_step", GatedStepArgs), ("norm", NormArgs))
+           ("gated_scan", GatedScanArgs), ("gated_step", GatedStepArgs), ("norm", NormArgs),
+           ("embedding", EmbeddingArgs), ("sample", SampleArgs))
 _ARGP = {n: ctypes.POINTER(c) for n, c in _BLOCKS}
 
 lib.mcpu_last_error.restype = ctypes.c_char_p
@@ -253,6 +271,17 @@ lib.mcpu_norm_bwd_workspace_size.argtypes = [_ARGP["norm"]]
 lib.mcpu_norm_bwd_workspace_size.restype = ctypes.c_size_t
 lib.mcpu_norm_bwd.argtypes = [_ARGP["norm"], _P, ctypes.c_size_t, _P]
 lib.mcpu_norm_bwd.restype = ctypes.c_int
+
+lib.mcpu_embedding_fwd.argtypes = [_ARGP["embedding"], _P]
+lib.mcpu_embedding_fwd.restype = ctypes.c_int
+lib.mcpu_embedding_bwd_workspace_size.argtypes = [_ARGP["embedding"]]
+lib.mcpu_embedding_bwd_workspace_size.restype = ctypes.c_size_t
+lib.mcpu_embedding_bwd.argtypes = [_ARGP["embedding"], _P, ctypes.c_size_t, _P]
+lib.mcpu_embedding_bwd.restype = ctypes.c_int
+lib.mcpu_sample_workspace_size.argtypes = [_ARGP["sample"]]
+lib.mcpu_sample_workspace_size.restype = ctypes.c_size_t
+lib.mcpu_sample.argtypes = [_ARGP["sample"], _P, ctypes.c_size_t, _P]
+lib.mcpu_sample.restype = ctypes.c_int
 
 for _name, _cls in _BLOCKS:
     _want = lib.mcpu_args_size(_name.encode())

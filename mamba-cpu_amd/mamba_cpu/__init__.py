@@ -10,11 +10,13 @@ routes Hugging Face Mamba / FalconMamba / Jamba / Mamba-2 models on the GPU to t
 from mamba_cpu.ops import (
     causal_conv1d_fn,
     causal_conv1d_update,
+    embedding_fn,
     gated_linear_scan_fn,
     gated_linear_update,
     layer_norm_fn,
     mamba_chunk_scan_combined,
     mamba_inner_fn,
+    sample_fn,
     selective_scan_fn,
     selective_state_update,
 )
@@ -26,11 +28,13 @@ __all__ = [
     "causal_conv1d_fn",
     "causal_conv1d_ref",
     "causal_conv1d_update",
+    "embedding_fn",
     "gated_linear_scan_fn",
     "gated_linear_update",
     "layer_norm_fn",
     "mamba_chunk_scan_combined",
     "mamba_inner_fn",
+    "sample_fn",
     "selective_scan_fn",
     "selective_scan_ref",
     "selective_state_update",

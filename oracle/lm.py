@@ -102,3 +102,56 @@ def norm_bwd(x, weight, dy, bias=None, residual=None, dz_out=None, eps=1e-5, rms
         dz = dz + _f64(dz_out)
     flat = lambda v: v.reshape(-1, n)  # noqa: E731
     return dz, flat(_f64(dy) * zhat).sum(0), flat(_f64(dy)).sum(0)
+
+
+def embedding_bwd(ids, dout, vocab, scale=1.0):
+    """Gradient of the embedding's weight; ids outside [0, vocab) have none."""
+    ids, dout = np.asarray(ids.cpu()).reshape(-1), _f64(dout)
+    dw = np.zeros((vocab, dout.shape[-1]))
+    for t, v in enumerate(ids):
+        if 0 <= v < vocab:
+            dw[v] += dout[t]
+    return dw * scale
+
+
+def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One row: the token, its logprob, how many tokens were kept, and how near
+    the choice was: the relative distance of the race's second and of a weight
+    from min_p, 0 where the token changes if the top-p edge moves by 1e-5 of
+    the mass."""
+    l = _f64(logits).reshape(-1)
+    l = np.where(np.isnan(l), -np.inf, l)
+    m = l.max() if l.size else -np.inf
+    if m == -np.inf:
+        return -1, -np.inf, 0, np.inf
+    with np.errstate(invalid="ignore"):
+        flat = np.where(l == m, 0.0, l - m)
+    logprob = lambda i: flat[i] - np.log(np.exp(flat).sum())  # noqa: E731
+    order = np.lexsort((np.arange(l.size), -l))
+    if not temperature > 0:
+        return int(order[0]), logprob(order[0]), 1, np.inf
+    w = np.exp(flat[order] / temperature)
+    n = min(top_k, l.size) if top_k > 0 else l.size
+    near, moved = np.inf, (n, n)
+    if top_p < 1:
+        before = np.concatenate([[0.0], np.cumsum(w[:n])[:-1]])
+        mass = w[:n].sum()
+        edge = float(np.float32(top_p)) * mass
+        moved = [max(1, int((before < edge + by * mass).sum())) for by in (-1e-5, 1e-5)]
+        n = max(1, int((before < edge).sum()))
+    mp = min(float(np.float32(min_p)), 1.0)
+    if mp > 0:
+        near = min(near, np.abs(w[:n] / mp - 1)[w[:n] != 1].min(initial=np.inf))
+    if moved[0] < moved[1]:
+        race = (w / _f64(noise).reshape(-1)[order])[:moved[1]]
+        race[1:][w[1:moved[1]] < mp] = -1
+        if race[:moved[0]].max() <= race[moved[0]:].max():
+            near = 0.0
+    n = max(1, int((w[:n] >= mp).sum()))
+    score = w[:n] / _f64(noise).reshape(-1)[order[:n]]
+    best = score.max()
+    ties = order[:n][score == best]
+    rest = score[score < best]
+    if rest.size and best > 0:
+        near = min(near, 1 - rest.max() / best)
+    return int(ties.min()), logprob(ties.min()), n, near
