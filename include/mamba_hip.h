@@ -685,7 +685,7 @@ int mcpu_norm_bwd(const mcpu_norm_args* a, void* workspace, size_t workspace_byt
 /* ------------------------------------------------------------------------ */
 
 /* out_t = scale weight[ids_t];  dweight_v = scale sum_{t: ids_t = v} dout_t,
- * summed in float32 over the tokens of v in their order and rounded once. An
+ * summed in float32 over the tokens of v in a fixed order and rounded once. An
  * id outside [0, vocab) has a zero row and no gradient. weight, out, dout and
  * dweight have `dtype`; rows are contiguous and a row stride apart; ids, out
  * and dweight are contiguous. No counterpart in the reference. */

@@ -170,7 +170,8 @@ extern "C" size_t mcpu_embedding_bwd_workspace_size(const mcpu_embedding_args* a
     clear_error();
     return 0;
   }
-  return align_up(sizeof(int32_t) * a->tokens) + align_up(sizeof(int32_t) * (a->vocab + 1));
+  return align_up(sizeof(int32_t) * a->tokens) + align_up(sizeof(int32_t) * (a->vocab + 1)) +
+         align_up(sizeof(float) * 2 * embedding_chunks(a->tokens) * a->dim);
 }
 
 extern "C" int mcpu_embedding_bwd(const mcpu_embedding_args* a, void* workspace, size_t workspace_bytes,
@@ -186,8 +187,12 @@ extern "C" int mcpu_embedding_bwd(const mcpu_embedding_args* a, void* workspace,
   EmbeddingParams p = make_embedding(a);
   p.dout = a->dout;
   p.dweight = a->dweight;
-  p.order = static_cast<int32_t*>(workspace);
-  p.start = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + align_up(sizeof(int32_t) * a->tokens));
+  char* ws = static_cast<char*>(workspace);
+  p.order = reinterpret_cast<int32_t*>(ws);
+  ws += align_up(sizeof(int32_t) * a->tokens);
+  p.start = reinterpret_cast<int32_t*>(ws);
+  ws += align_up(sizeof(int32_t) * (a->vocab + 1));
+  p.part = reinterpret_cast<float*>(ws);
   return hip_status(embedding_bwd_launch(p, static_cast<hipStream_t>(stream)), "embedding_bwd launch");
 }
 

@@ -2,7 +2,7 @@
 // dweight_v = scale sum_{t: id_t = v} dout_t.
 //
 // The gradient is a segmented sum over the tokens sorted by id: the sum of an
-// id runs over its tokens in their order, in float32, and is rounded once, so
+// id runs over its tokens in a fixed order, in float32, and is rounded once, so
 // the result does not depend on timing (no floating atomics). The sort needs
 // one launch: a workgroup owns a range of ids, reads every token's id and so
 // knows both how many tokens lie below its range (where its part of the order
@@ -18,12 +18,37 @@ __device__ __forceinline__ int64_t id_at(const EmbeddingParams& p, int64_t t) {
   return p.ids64 ? static_cast<const int64_t*>(p.ids)[t] : static_cast<const int32_t*>(p.ids)[t];
 }
 
+// n values (1 to 4) from element i on, as one vector where all four are there.
+template <typename T> __device__ __forceinline__ void ld_upto4(const T* row, int64_t i, int n, float (&v)[4]) {
+  if (n == 4) return ld4_elem<T>(row, i, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(row[i + e]) : 0.f;
+}
+template <typename T> __device__ __forceinline__ void st_upto4(T* row, int64_t i, int n, const float (&v)[4]) {
+  if (n == 4) return st4_elem<T>(row, i, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) row[i + e] = from_f32<T>(v[e]);
+}
+__device__ __forceinline__ int upto4(int64_t left) { return left < 4 ? static_cast<int>(left) : 4; }
+
+// One wave per token, four elements per lane.
 template <typename T> __global__ __launch_bounds__(256) void embedding_fwd_kernel(const EmbeddingParams p) {
-  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t >= p.tokens) return;
   const int64_t id = id_at(p, t);
   const bool in = id >= 0 && id < p.vocab;
-  for (int64_t i = threadIdx.x; i < p.dim; i += 256)
-    st<T>(p.out, t * p.dim + i, in ? ld<T>(p.weight, id * p.sw + i) * p.scale : 0.f);
+  const T* from = static_cast<const T*>(p.weight) + (in ? id : 0) * p.sw;
+  T* to = static_cast<T*>(p.out) + t * p.dim;
+  for (int64_t i = lane * 4; i < p.dim; i += 256) {
+    const int n = upto4(p.dim - i);
+    float v[4] = {};
+    if (in) ld_upto4<T>(from, i, n, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= p.scale;
+    st_upto4<T>(to, i, n, v);
+  }
 }
 
 constexpr int kSortWaves = 16;
@@ -96,16 +121,122 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
   }
 }
 
-// One wave per row of dweight.
-template <typename T> __global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t v = blockIdx.x * 4ll + (threadIdx.x >> 6);
+// Adds the rows of dout at the sorted positions [s0, s1), at most 64, element
+// i to i + n: the positions are read at once, one per lane, and passed on as
+// scalars, so that the rows' loads do not wait for each other.
+template <typename T>
+__device__ __forceinline__ void add_rows(const EmbeddingParams& p, int mine, int s0, int s1, int64_t i, int n,
+                                         float (&sum)[4]) {
+  const T* dout = static_cast<const T*>(p.dout);
+  int s = s0;
+  for (; s + 4 <= s1; s += 4) {
+    float v[4][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t t = __builtin_amdgcn_readlane(mine, s + k - s0);
+      ld_upto4<T>(dout + t * p.sdo, i, n, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += v[k][e];
+  }
+  for (; s < s1; ++s) {
+    const int64_t t = __builtin_amdgcn_readlane(mine, s - s0);
+    float v[4];
+    ld_upto4<T>(dout + t * p.sdo, i, n, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += v[e];
+  }
+}
+
+// dweight, in one launch of two kinds of workgroups. The first `chunks` take
+// kEmbedChunk sorted positions each and add, per id with more tokens than that
+// (a hot id), the part of its rows that lies here: the part of the id at the
+// chunk's first position goes to slot 0, that of a hot id starting later to
+// slot 1 (it runs past the chunk's end, so there is at most one). The others
+// give each wave a row of dweight: the sum of an id with few tokens, or zeros.
+// Hot rows are joined by embedding_join_kernel. Without this split one wave
+// adds the most frequent id alone: 3.5 ms of 16384 tokens' 5.1 ms.
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p, int chunks) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (static_cast<int>(blockIdx.x) < chunks) {
+    const int c0 = blockIdx.x * kEmbedChunk, valid = p.start[p.vocab];
+    const int c1 = min(c0 + kEmbedChunk, valid);
+    int s = c0;
+    while (s < c1) {
+      const int64_t id = id_at(p, p.order[s]);
+      const int end = p.start[id + 1];
+      if (end - p.start[id] > kEmbedChunk) {
+        const int s1 = min(end, c1), slot = s == c0 ? 0 : 1;
+        const int mine = lane < s1 - s ? p.order[s + lane] : 0;
+        float* part = p.part + (blockIdx.x * 2ll + slot) * p.dim;
+        for (int64_t i = (w * 64 + lane) * 4; i < p.dim; i += 1024) {
+          const int n = upto4(p.dim - i);
+          float sum[4] = {};
+          add_rows<T>(p, mine, s, s1, i, n, sum);
+          st_upto4<float>(part, i, n, sum);
+        }
+      }
+      s = end;
+    }
+    return;
+  }
+  const int64_t v = (blockIdx.x - chunks) * 4ll + w;
   if (v >= p.vocab) return;
   const int s0 = p.start[v], s1 = p.start[v + 1];
-  for (int64_t i = lane; i < p.dim; i += 64) {
-    float sum = 0.f;
-    for (int s = s0; s < s1; ++s) sum += ld<T>(p.dout, p.order[s] * p.sdo + i);
-    st<T>(p.dweight, v * p.dim + i, sum * p.scale);
+  if (s1 - s0 > kEmbedChunk) return;
+  const int mine = lane < s1 - s0 ? p.order[s0 + lane] : 0;
+  T* row = static_cast<T*>(p.dweight) + v * p.dim;
+  for (int64_t i = lane * 4; i < p.dim; i += 256) {
+    const int n = upto4(p.dim - i);
+    float sum[4] = {};
+    add_rows<T>(p, mine, s0, s1, i, n, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] *= p.scale;
+    st_upto4<T>(row, i, n, sum);
+  }
+}
+
+constexpr int kJoinWaves = 16;
+
+// The row of a hot id, by the workgroups of the chunk it starts in (256
+// elements each): its parts in every kJoinWaves-th chunk are added by one wave
+// each, then the waves' sums in order.
+template <typename T>
+__global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(const EmbeddingParams p) {
+  __shared__ float sums[kJoinWaves][256];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c0 = blockIdx.x * kEmbedChunk, valid = p.start[p.vocab];
+  if (c0 >= valid) return;
+  // The hot id that starts here is the last one of the chunk: every other id
+  // that starts here ends here.
+  const int64_t id = id_at(p, p.order[min(c0 + kEmbedChunk, valid) - 1]);
+  const int first = p.start[id], end = p.start[id + 1];
+  if (end - first <= kEmbedChunk || first < c0) return;
+  const int last = (end - 1) / kEmbedChunk;
+  const int64_t i = blockIdx.y * 256ll + lane * 4;
+  const int n = i < p.dim ? upto4(p.dim - i) : 0;
+  float sum[4] = {};
+  if (n > 0) {
+#pragma unroll 4
+    for (int64_t c = static_cast<int64_t>(blockIdx.x) + w; c <= last; c += kJoinWaves) {
+      const int slot = c == blockIdx.x && first > c0 ? 1 : 0;
+      float v[4];
+      ld_upto4<float>(p.part + (c * 2 + slot) * p.dim, i, n, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += v[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sums[w][lane * 4 + e] = sum[e];
+  __syncthreads();
+  const int64_t col = blockIdx.y * 256ll + threadIdx.x;
+  if (threadIdx.x < 256 && col < p.dim) {
+    float total = 0.f;
+    for (int v = 0; v < kJoinWaves; ++v) total += sums[v][threadIdx.x];
+    st<T>(p.dweight, id * p.dim + col, total * p.scale);
   }
 }
 
@@ -119,9 +250,15 @@ template <typename F> void by_dtype(int dtype, F&& f) {
 
 hipError_t embedding_fwd_launch(const EmbeddingParams& p, hipStream_t st) {
   by_dtype(p.dtype, [&](auto t) {
-    hipLaunchKernelGGL(embedding_fwd_kernel<decltype(t)>, dim3(static_cast<unsigned>(p.tokens)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(embedding_fwd_kernel<decltype(t)>, dim3(static_cast<unsigned>((p.tokens + 3) / 4)), dim3(256),
+                       0, st, p);
   });
   return hipGetLastError();
+}
+
+// Chunks of sorted positions, or none where no id can be hot.
+int64_t embedding_chunks(int64_t tokens) {
+  return tokens > kEmbedChunk ? (tokens + kEmbedChunk - 1) / kEmbedChunk : 0;
 }
 
 hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st) {
@@ -130,9 +267,14 @@ hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st) {
   if (range > kSortIds) range = kSortIds;
   hipLaunchKernelGGL(embedding_sort_kernel, dim3(static_cast<unsigned>((p.vocab + range - 1) / range)),
                      dim3(64 * kSortWaves), 0, st, p, static_cast<int>(range));
+  const int chunks = static_cast<int>(embedding_chunks(p.tokens));
   by_dtype(p.dtype, [&](auto t) {
-    hipLaunchKernelGGL(embedding_dw_kernel<decltype(t)>, dim3(static_cast<unsigned>((p.vocab + 3) / 4)), dim3(256), 0,
-                       st, p);
+    using T = decltype(t);
+    hipLaunchKernelGGL(embedding_dw_kernel<T>, dim3(static_cast<unsigned>(chunks + (p.vocab + 3) / 4)), dim3(256), 0,
+                       st, p, chunks);
+    if (chunks > 0)
+      hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(chunks, static_cast<unsigned>((p.dim + 255) / 256)),
+                         dim3(64 * kJoinWaves), 0, st, p);
   });
   return hipGetLastError();
 }

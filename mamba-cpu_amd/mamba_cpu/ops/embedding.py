@@ -35,7 +35,7 @@ def embedding_fn(ids, weight, scale=1.0):
     the ranks' results add up.
 
     Differentiable in weight: the gradient of a row is the float32 sum over its
-    tokens in their order, rounded once, and does not change from call to call.
+    tokens in a fixed order, rounded once, and does not change from call to call.
     """
     if weight.device.type != "cuda":
         raise ValueError(f"mamba_cpu (MI355X build) runs on ROCm GPU tensors, got device {weight.device}")
