@@ -59,6 +59,8 @@ int check_embedding(const mcpu_embedding_args* a, const char* what) {
   if (a->weight_stride < 0 || a->dout_stride < 0) return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
   if (a->tokens > INT_MAX - 64 || a->vocab > INT_MAX - 1024 || a->dim > INT_MAX)
     return fail(MCPU_ERR_UNSUPPORTED, "%s: tokens, vocab and dim must fit 31 bits", what);
+  if (embedding_chunks(a->tokens) * ((a->dim + 1023) / 1024) + a->vocab / 16 > INT_MAX - 1)
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: tokens x dim too large", what);
   if (a->tokens > 0 && a->ids == nullptr) return fail(MCPU_ERR_INVALID, "%s: ids are required", what);
   return MCPU_OK;
 }

@@ -32,7 +32,8 @@ template <typename T> __device__ __forceinline__ void st_upto4(T* row, int64_t i
 }
 __device__ __forceinline__ int upto4(int64_t left) { return left < 4 ? static_cast<int>(left) : 4; }
 
-// One wave per token, four elements per lane.
+// One wave per token, four elements per lane; the loads of up to four such
+// turns are on their way before the first store.
 template <typename T> __global__ __launch_bounds__(256) void embedding_fwd_kernel(const EmbeddingParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t t = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -41,18 +42,24 @@ template <typename T> __global__ __launch_bounds__(256) void embedding_fwd_kerne
   const bool in = id >= 0 && id < p.vocab;
   const T* from = static_cast<const T*>(p.weight) + (in ? id : 0) * p.sw;
   T* to = static_cast<T*>(p.out) + t * p.dim;
-  for (int64_t i = lane * 4; i < p.dim; i += 256) {
-    const int n = upto4(p.dim - i);
-    float v[4] = {};
-    if (in) ld_upto4<T>(from, i, n, v);
+  for (int64_t i0 = lane * 4; i0 < p.dim; i0 += 1024) {
+    float v[4][4] = {};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= p.scale;
-    st_upto4<T>(to, i, n, v);
+    for (int k = 0; k < 4; ++k)
+      if (in && i0 + k * 256 < p.dim) ld_upto4<T>(from, i0 + k * 256, upto4(p.dim - i0 - k * 256), v[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i0 + k * 256 >= p.dim) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] *= p.scale;
+      st_upto4<T>(to, i0 + k * 256, upto4(p.dim - i0 - k * 256), v[k]);
+    }
   }
 }
 
 constexpr int kSortWaves = 16;
 constexpr int kSortIds = 512;  // most ids of one workgroup's range
+constexpr int kSortBatch = 8;  // ids per lane on their way at once
 
 __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const EmbeddingParams p, int range) {
   __shared__ int count[kSortWaves][kSortIds];  // tokens of (wave, id), then where the next one goes
@@ -69,23 +76,32 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
   const int64_t t0 = w * run, t1 = t0 + run < p.tokens ? t0 + run : p.tokens;
   int under = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    for (int64_t t = t0 + lane; t - lane < t1; t += 64) {
-      const int64_t id = t < t1 ? id_at(p, t) : -1;
-      const bool in = id >= lo && id < hi;
-      const int slot = in ? static_cast<int>(id - lo) : -1;
-      if (pass == 0) under += __popcll(__ballot(id >= 0 && id < lo));
-      uint64_t left = __ballot(in);
-      while (left != 0) {
-        const int lead = __builtin_ctzll(left);
-        const int s = __builtin_amdgcn_readlane(slot, lead);
-        const uint64_t same = __ballot(slot == s);
-        int first = 0;
-        if (lane == lead) first = atomicAdd(&count[w][s], __popcll(same));
-        if (pass == 1) {
-          first = __builtin_amdgcn_readlane(first, lead);
-          if (slot == s) p.order[first + __popcll(same & ((1ull << lane) - 1))] = static_cast<int32_t>(t);
+    for (int64_t tb = t0; tb < t1; tb += 64 * kSortBatch) {
+      int64_t ids[kSortBatch];
+#pragma unroll
+      for (int k = 0; k < kSortBatch; ++k) {
+        const int64_t t = tb + k * 64 + lane;
+        ids[k] = t < t1 ? id_at(p, t) : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < kSortBatch; ++k) {
+        const bool in = ids[k] >= lo && ids[k] < hi;
+        const int slot = in ? static_cast<int>(ids[k] - lo) : -1;
+        if (pass == 0) under += __popcll(__ballot(ids[k] >= 0 && ids[k] < lo));
+        uint64_t left = __ballot(in);
+        while (left != 0) {
+          const int lead = __builtin_ctzll(left);
+          const int s = __builtin_amdgcn_readlane(slot, lead);
+          const uint64_t same = __ballot(slot == s);
+          int first = 0;
+          if (lane == lead) first = atomicAdd(&count[w][s], __popcll(same));
+          if (pass == 1) {
+            first = __builtin_amdgcn_readlane(first, lead);
+            if (slot == s)
+              p.order[first + __popcll(same & ((1ull << lane) - 1))] = static_cast<int32_t>(tb + k * 64 + lane);
+          }
+          left &= ~same;
         }
-        left &= ~same;
       }
     }
     if (pass == 1) break;
@@ -121,100 +137,93 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
   }
 }
 
-// Adds the rows of dout at the sorted positions [s0, s1), at most 64, element
-// i to i + n: the positions are read at once, one per lane, and passed on as
-// scalars, so that the rows' loads do not wait for each other.
+// dweight, in one launch of two kinds of workgroups. The first chunks x tiles
+// take kEmbedChunk sorted positions of 1024 columns each: all rows' loads are
+// on their way before the first addition, and the sums are cut where the id
+// changes. An id whose tokens all lie in the chunk is done; of one that goes on
+// before or behind it, the part here goes to the chunk's slot 0 (the id at its
+// first position) or 1 (one that starts later), and embedding_join_kernel adds
+// the parts. The other workgroups write the zeros of ids without a token, a
+// wave four rows. With a wave for each id's row instead, the most frequent ids
+// are the time: 46 us for 16384 bf16 tokens of 768 even where ids above 32
+// tokens go in chunks, @DW@ us this way.
 template <typename T>
-__device__ __forceinline__ void add_rows(const EmbeddingParams& p, int mine, int s0, int s1, int64_t i, int n,
-                                         float (&sum)[4]) {
-  const T* dout = static_cast<const T*>(p.dout);
-  int s = s0;
-  for (; s + 4 <= s1; s += 4) {
-    float v[4][4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t t = __builtin_amdgcn_readlane(mine, s + k - s0);
-      ld_upto4<T>(dout + t * p.sdo, i, n, v[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += v[k][e];
-  }
-  for (; s < s1; ++s) {
-    const int64_t t = __builtin_amdgcn_readlane(mine, s - s0);
-    float v[4];
-    ld_upto4<T>(dout + t * p.sdo, i, n, v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += v[e];
-  }
-}
-
-// dweight, in one launch of two kinds of workgroups. The first `chunks` take
-// kEmbedChunk sorted positions each and add, per id with more tokens than that
-// (a hot id), the part of its rows that lies here: the part of the id at the
-// chunk's first position goes to slot 0, that of a hot id starting later to
-// slot 1 (it runs past the chunk's end, so there is at most one). The others
-// give each wave a row of dweight: the sum of an id with few tokens, or zeros.
-// Hot rows are joined by embedding_join_kernel. Without this split one wave
-// adds the most frequent id alone: 3.5 ms of 16384 tokens' 5.1 ms.
-template <typename T>
-__global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p, int chunks) {
+__global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p, int chunks, int tiles) {
+  constexpr int kBatch = 16;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (static_cast<int>(blockIdx.x) < chunks) {
-    const int c0 = blockIdx.x * kEmbedChunk, valid = p.start[p.vocab];
-    const int c1 = min(c0 + kEmbedChunk, valid);
-    int s = c0;
-    while (s < c1) {
-      const int64_t id = id_at(p, p.order[s]);
-      const int end = p.start[id + 1];
-      if (end - p.start[id] > kEmbedChunk) {
-        const int s1 = min(end, c1), slot = s == c0 ? 0 : 1;
-        const int mine = lane < s1 - s ? p.order[s + lane] : 0;
-        float* part = p.part + (blockIdx.x * 2ll + slot) * p.dim;
-        for (int64_t i = (w * 64 + lane) * 4; i < p.dim; i += 1024) {
-          const int n = upto4(p.dim - i);
-          float sum[4] = {};
-          add_rows<T>(p, mine, s, s1, i, n, sum);
-          st_upto4<float>(part, i, n, sum);
-        }
+  if (static_cast<int>(blockIdx.x) < chunks * tiles) {
+    const int chunk = blockIdx.x / tiles, c0 = chunk * kEmbedChunk;
+    const int rows = min(kEmbedChunk, p.start[p.vocab] - c0);
+    const int64_t i = (blockIdx.x % tiles) * 1024ll + (w * 64 + lane) * 4;
+    if (rows <= 0 || i - lane * 4 >= p.dim) return;
+    const int n = i < p.dim ? upto4(p.dim - i) : 0;
+    // Lane k holds position c0 + k: its token, its id, whether its id ends here.
+    const int token = lane < rows ? p.order[c0 + lane] : 0;
+    const int id = lane < rows ? static_cast<int>(id_at(p, token)) : -1;
+    const int next = __shfl_down(id, 1);  // by every lane: a lane that sits out gives nothing
+    const uint64_t ends = __ballot(lane < rows && (lane == rows - 1 || id != next));
+    const int id0 = __builtin_amdgcn_readfirstlane(id), id1 = __builtin_amdgcn_readlane(id, rows - 1);
+    const bool before = p.start[id0] < c0, behind = p.start[id1 + 1] > c0 + rows;
+    const int head = __builtin_ctzll(ends);  // where the first id ends
+    float sum[4] = {};
+    for (int b = 0; b < rows; b += kBatch) {
+      float v[kBatch][4];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (b + k >= rows) break;
+        const int64_t t = __builtin_amdgcn_readlane(token, b + k);
+        if (n > 0) ld_upto4<T>(static_cast<const T*>(p.dout) + t * p.sdo, i, n, v[k]);
       }
-      s = end;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int at = b + k;
+        if (at >= rows) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += v[k][e];
+        if (((ends >> at) & 1) == 0) continue;
+        const bool part = (at == head && before) || (at == rows - 1 && behind);
+        if (n > 0) {
+          if (part) {
+            st_upto4<float>(p.part + (chunk * 2ll + (at == head ? 0 : 1)) * p.dim, i, n, sum);
+          } else {
+            float out[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = sum[e] * p.scale;
+            st_upto4<T>(static_cast<T*>(p.dweight) + __builtin_amdgcn_readlane(id, at) * p.dim, i, n, out);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = 0.f;
+      }
     }
     return;
   }
-  const int64_t v = (blockIdx.x - chunks) * 4ll + w;
-  if (v >= p.vocab) return;
-  const int s0 = p.start[v], s1 = p.start[v + 1];
-  if (s1 - s0 > kEmbedChunk) return;
-  const int mine = lane < s1 - s0 ? p.order[s0 + lane] : 0;
-  T* row = static_cast<T*>(p.dweight) + v * p.dim;
-  for (int64_t i = lane * 4; i < p.dim; i += 256) {
-    const int n = upto4(p.dim - i);
-    float sum[4] = {};
-    add_rows<T>(p, mine, s0, s1, i, n, sum);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] *= p.scale;
-    st_upto4<T>(row, i, n, sum);
+  const int64_t v0 = (blockIdx.x - static_cast<int64_t>(chunks) * tiles) * 16 + w * 4;
+  const int64_t at = min(v0 + lane, p.vocab);
+  const int starts = lane < 5 ? p.start[at] : 0;
+  const float zero[4] = {};
+  for (int k = 0; k < 4; ++k) {
+    if (v0 + k >= p.vocab) break;
+    if (__builtin_amdgcn_readlane(starts, k) != __builtin_amdgcn_readlane(starts, k + 1)) continue;
+    T* row = static_cast<T*>(p.dweight) + (v0 + k) * p.dim;
+    for (int64_t i = lane * 4; i < p.dim; i += 256) st_upto4<T>(row, i, upto4(p.dim - i), zero);
   }
 }
 
 constexpr int kJoinWaves = 16;
 
-// The row of a hot id, by the workgroups of the chunk it starts in (256
-// elements each): its parts in every kJoinWaves-th chunk are added by one wave
-// each, then the waves' sums in order.
+// The row of an id that goes on behind the chunk it starts in, by that chunk's
+// workgroups (256 elements each): its parts in every kJoinWaves-th chunk are
+// added by one wave each, then the waves' sums in order.
 template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(const EmbeddingParams p) {
   __shared__ float sums[kJoinWaves][256];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c0 = blockIdx.x * kEmbedChunk, valid = p.start[p.vocab];
   if (c0 >= valid) return;
-  // The hot id that starts here is the last one of the chunk: every other id
-  // that starts here ends here.
   const int64_t id = id_at(p, p.order[min(c0 + kEmbedChunk, valid) - 1]);
   const int first = p.start[id], end = p.start[id + 1];
-  if (end - first <= kEmbedChunk || first < c0) return;
+  if (first < c0 || end <= c0 + kEmbedChunk) return;
   const int last = (end - 1) / kEmbedChunk;
   const int64_t i = blockIdx.y * 256ll + lane * 4;
   const int n = i < p.dim ? upto4(p.dim - i) : 0;
@@ -256,10 +265,7 @@ hipError_t embedding_fwd_launch(const EmbeddingParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Chunks of sorted positions, or none where no id can be hot.
-int64_t embedding_chunks(int64_t tokens) {
-  return tokens > kEmbedChunk ? (tokens + kEmbedChunk - 1) / kEmbedChunk : 0;
-}
+int64_t embedding_chunks(int64_t tokens) { return (tokens + kEmbedChunk - 1) / kEmbedChunk; }
 
 hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st) {
   // 256 ranges, one per CU, or more where a range would pass the table.
@@ -268,11 +274,12 @@ hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st) {
   hipLaunchKernelGGL(embedding_sort_kernel, dim3(static_cast<unsigned>((p.vocab + range - 1) / range)),
                      dim3(64 * kSortWaves), 0, st, p, static_cast<int>(range));
   const int chunks = static_cast<int>(embedding_chunks(p.tokens));
+  const int tiles = static_cast<int>((p.dim + 1023) / 1024);
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(chunks) * tiles + (p.vocab + 15) / 16);
   by_dtype(p.dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(embedding_dw_kernel<T>, dim3(static_cast<unsigned>(chunks + (p.vocab + 3) / 4)), dim3(256), 0,
-                       st, p, chunks);
-    if (chunks > 0)
+    hipLaunchKernelGGL(embedding_dw_kernel<T>, dim3(grid), dim3(256), 0, st, p, chunks, tiles);
+    if (chunks > 1)
       hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(chunks, static_cast<unsigned>((p.dim + 255) / 256)),
                          dim3(64 * kJoinWaves), 0, st, p);
   });

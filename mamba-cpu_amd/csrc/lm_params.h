@@ -45,13 +45,13 @@ struct EmbeddingParams {
   void* dweight;       // (vocab, dim) contiguous
   int32_t* order;      // token positions sorted by id, in token order within an id
   int32_t* start;      // (vocab + 1): where each id's positions start in `order`
-  float* part;         // (chunks, 2, dim): partial sums of ids with many tokens
+  float* part;         // (chunks, 2, dim): partial sums of ids that cross a chunk's edge
   int64_t tokens, vocab, dim, sw, sdo;
   float scale;
   int dtype;
 };
 
-constexpr int kEmbedChunk = 32;  // most tokens of an id that one wave adds (at most 64: one per lane)
+constexpr int kEmbedChunk = 32;  // sorted positions per workgroup (at most 64: one per lane)
 int64_t embedding_chunks(int64_t tokens);
 hipError_t embedding_fwd_launch(const EmbeddingParams& p, hipStream_t st);
 hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st);
