@@ -68,10 +68,11 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
   const int64_t lo = blockIdx.x * int64_t{range};
   const int64_t hi = lo + range < p.vocab ? lo + range : p.vocab;
   const int n = static_cast<int>(hi - lo);
-  for (int i = threadIdx.x; i < kSortWaves * kSortIds; i += 64 * kSortWaves) (&count[0][0])[i] = 0;
+  for (int i = lane; i < n; i += 64) count[w][i] = 0;
   __syncthreads();
-  // A wave takes a run of the tokens, 64 at a time. Lanes with the same id of
-  // the range find each other by ballot, one id after the other.
+  // A wave takes a run of the tokens, 64 at a time: first it counts them, then
+  // lanes with the same id of the range find each other by ballot, one id after
+  // the other, and take their places in token order.
   const int64_t run = ((p.tokens + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int64_t t0 = w * run, t1 = t0 + run < p.tokens ? t0 + run : p.tokens;
   int under = 0;
@@ -87,7 +88,11 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
       for (int k = 0; k < kSortBatch; ++k) {
         const bool in = ids[k] >= lo && ids[k] < hi;
         const int slot = in ? static_cast<int>(ids[k] - lo) : -1;
-        if (pass == 0) under += __popcll(__ballot(ids[k] >= 0 && ids[k] < lo));
+        if (pass == 0) {
+          under += __popcll(__ballot(ids[k] >= 0 && ids[k] < lo));
+          if (in) atomicAdd(&count[w][slot], 1);
+          continue;
+        }
         uint64_t left = __ballot(in);
         while (left != 0) {
           const int lead = __builtin_ctzll(left);
@@ -95,11 +100,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
           const uint64_t same = __ballot(slot == s);
           int first = 0;
           if (lane == lead) first = atomicAdd(&count[w][s], __popcll(same));
-          if (pass == 1) {
-            first = __builtin_amdgcn_readlane(first, lead);
-            if (slot == s)
-              p.order[first + __popcll(same & ((1ull << lane) - 1))] = static_cast<int32_t>(tb + k * 64 + lane);
-          }
+          first = __builtin_amdgcn_readlane(first, lead);
+          if (slot == s)
+            p.order[first + __popcll(same & ((1ull << lane) - 1))] = static_cast<int32_t>(tb + k * 64 + lane);
           left &= ~same;
         }
       }
