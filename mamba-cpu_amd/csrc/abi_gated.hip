@@ -20,7 +20,8 @@ int check_gated(const mcpu_gated_scan_args* a, const char* what) {
   if (a == nullptr) return fail(MCPU_ERR_INVALID, "%s: null argument block", what);
   if (a->batch < 0 || a->seqlen < 0 || a->dim < 0) return fail(MCPU_ERR_INVALID, "%s: negative size", what);
   if (!valid_dtype(a->dtype)) return fail(MCPU_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
-  if (a->batch * ((a->dim + 63) / 64) > INT_MAX)
+  // The grid is at most a workgroup per 64 channels, row and time split, and rows are split only below 1024.
+  if (a->batch * ((a->dim + 63) / 64) > INT_MAX / 2)
     return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x dim too large", what);
   if ((a->decay == nullptr && a->dim > 0) ||
       ((a->x == nullptr || a->a_gate == nullptr || a->x_gate == nullptr) && a->batch * a->seqlen * a->dim > 0))
@@ -29,6 +30,42 @@ int check_gated(const mcpu_gated_scan_args* a, const char* what) {
   if (any_negative({a->x_stride, a->a_stride, a->i_stride}, 3))
     return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
   return MCPU_OK;
+}
+
+// A (batch, seqlen, dim) operand that two neighbouring 16-bit channels can be
+// moved of at once.
+bool pairs(const void* ptr, const int64_t (&s)[3]) {
+  return ptr == nullptr || (s[2] == 1 && s[0] % 2 == 0 && s[1] % 2 == 0 && reinterpret_cast<uintptr_t>(ptr) % 4 == 0);
+}
+
+// Channels per lane: two of a 16-bit type where every operand allows, so that
+// a lane moves four bytes.
+int gated_vec(const mcpu_gated_scan_args* a, bool bwd) {
+  if (a->dtype == MCPU_F32 || a->dim % 2 != 0 || !pairs(a->x, a->x_stride) || !pairs(a->a_gate, a->a_stride) ||
+      !pairs(a->x_gate, a->i_stride))
+    return 1;
+  if (!bwd) return pairs(a->y, a->y_stride) ? 2 : 1;
+  return pairs(a->dy, a->dy_stride) && pairs(a->dx, a->dx_stride) && pairs(a->da_gate, a->da_stride) &&
+                 pairs(a->dx_gate, a->di_stride)
+             ? 2
+             : 1;
+}
+
+// Time splits at most, over both widths: what the workspaces are sized for.
+int64_t most_splits(const mcpu_gated_scan_args* a) {
+  GatedScanParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.batch = a->batch;
+  p.len = a->seqlen;
+  p.dim = a->dim;
+  gated_scan_plan(p, 1);
+  const int64_t n = p.nsplit;
+  gated_scan_plan(p, 2);
+  return n > p.nsplit ? n : p.nsplit;
+}
+size_t sums_bytes(const mcpu_gated_scan_args* a) {
+  const int64_t n = most_splits(a);
+  return n > 1 ? align_up(sizeof(float2) * a->batch * n * a->dim) : 0;
 }
 
 GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
@@ -72,8 +109,11 @@ extern "C" size_t mcpu_gated_scan_ckpt_size(const mcpu_gated_scan_args* a) {
 }
 
 extern "C" size_t mcpu_gated_scan_fwd_workspace_size(const mcpu_gated_scan_args* a) {
-  if (check_gated(a, "gated_scan") != MCPU_OK) clear_error();
-  return 0;
+  if (check_gated(a, "gated_scan") != MCPU_OK) {
+    clear_error();
+    return 0;
+  }
+  return sums_bytes(a);
 }
 
 extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -89,7 +129,9 @@ extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspac
   GatedScanParams p = make_gated(a);
   p.y = a->y;
   p.last = a->last_state;
+  p.sums = static_cast<float2*>(workspace);
   if (a->batch == 0 || a->dim == 0) return MCPU_OK;
+  gated_scan_plan(p, gated_vec(a, false));
   return hip_status(gated_scan_fwd_launch(p, a->dtype, static_cast<hipStream_t>(stream)), "gated_scan_fwd launch");
 }
 
@@ -98,7 +140,7 @@ extern "C" size_t mcpu_gated_scan_bwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return align_up(sizeof(float) * a->batch * a->dim);
+  return sums_bytes(a) + align_up(sizeof(float) * a->batch * most_splits(a) * a->dim);
 }
 
 extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -127,7 +169,9 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
   p.dx_gate = a->dx_gate;
   p.ddecay = a->ddecay;
   p.dinit = a->dinitial_state;
-  p.ddecay_part = static_cast<float*>(workspace);
+  p.sums = static_cast<float2*>(workspace);
+  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(a));
+  gated_scan_plan(p, gated_vec(a, true));
   return hip_status(gated_scan_bwd_launch(p, a->dtype, st), "gated_scan_bwd launch");
 }
 

@@ -9,7 +9,8 @@
 namespace mcpu {
 
 constexpr int kGatedT = 8;      // steps per wave segment: the forward keeps the state before each
-constexpr int kGatedWaves = 4;  // waves of a workgroup, one segment each
+constexpr int kGatedWaves = 8;  // waves of a workgroup, one segment each
+constexpr int kGatedChunk = kGatedT * kGatedWaves;
 
 struct GatedScanParams {
   const void* x;
@@ -27,9 +28,12 @@ struct GatedScanParams {
   void* da_gate;
   void* dx_gate;
   float* ddecay;
-  float* ddecay_part;  // (batch, dim) partial sums over time
+  float* ddecay_part;  // (batch, nsplit, dim) partial sums over time
+  float2* sums;        // (batch, nsplit, dim): each split's step as a whole
   float* dinit;
   int64_t batch, len, dim;
+  int64_t nsplit, split_len;  // time splits, split_len steps each: whole chunks
+  int vec;                    // channels per lane
   float c;
   int64_t sx[3], sa[3], si[3], sy[3], sdy[3], sdx[3], sda[3], sdi[3];  // (batch, len, dim)
 };
@@ -48,6 +52,8 @@ struct GatedStepParams {
   int64_t state_batch;
 };
 
+// Fills in the launch shape: vec (as the operands allow) and the time splits.
+void gated_scan_plan(GatedScanParams& p, int vec);
 hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
 hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
 hipError_t gated_step_launch(const GatedStepParams& p, int dtype, hipStream_t st);
