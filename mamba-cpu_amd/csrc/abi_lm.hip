@@ -104,6 +104,29 @@ int check_sample(const mcpu_sample_args* a, const char* what) {
   return MCPU_OK;
 }
 
+SampleParams make_sample(const mcpu_sample_args* a) {
+  SampleParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.logits = a->logits;
+  p.noise = a->noise;
+  p.temperature = a->temperature;
+  p.top_p = a->top_p;
+  p.min_p = a->min_p;
+  p.top_k = a->top_k;
+  p.temperature_rows = a->temperature_rows;
+  p.top_p_rows = a->top_p_rows;
+  p.min_p_rows = a->min_p_rows;
+  p.top_k_rows = a->top_k_rows;
+  p.token = a->token;
+  p.logprob = a->logprob;
+  p.rows = a->rows;
+  p.vocab = a->vocab;
+  p.sl = a->logits_stride;
+  p.sn = a->noise_stride;
+  p.dtype = a->dtype;
+  return p;
+}
+
 }  // namespace
 }  // namespace mcpu
 
@@ -199,8 +222,11 @@ extern "C" int mcpu_embedding_bwd(const mcpu_embedding_args* a, void* workspace,
 }
 
 extern "C" size_t mcpu_sample_workspace_size(const mcpu_sample_args* a) {
-  if (check_sample(a, "sample") != MCPU_OK) clear_error();
-  return 0;
+  if (check_sample(a, "sample") != MCPU_OK) {
+    clear_error();
+    return 0;
+  }
+  return align_up(sample_workspace(make_sample(a)));
 }
 
 extern "C" int mcpu_sample(const mcpu_sample_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -210,24 +236,7 @@ extern "C" int mcpu_sample(const mcpu_sample_args* a, void* workspace, size_t wo
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_sample_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   if (a->rows == 0) return MCPU_OK;
-  SampleParams p;
-  std::memset(&p, 0, sizeof(p));
-  p.logits = a->logits;
-  p.noise = a->noise;
-  p.temperature = a->temperature;
-  p.top_p = a->top_p;
-  p.min_p = a->min_p;
-  p.top_k = a->top_k;
-  p.temperature_rows = a->temperature_rows;
-  p.top_p_rows = a->top_p_rows;
-  p.min_p_rows = a->min_p_rows;
-  p.top_k_rows = a->top_k_rows;
-  p.token = a->token;
-  p.logprob = a->logprob;
-  p.rows = a->rows;
-  p.vocab = a->vocab;
-  p.sl = a->logits_stride;
-  p.sn = a->noise_stride;
-  p.dtype = a->dtype;
+  SampleParams p = make_sample(a);
+  p.slices = workspace;
   return hip_status(sample_launch(p, static_cast<hipStream_t>(stream)), "sample launch");
 }

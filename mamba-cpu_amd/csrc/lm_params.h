@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstddef>
 #include <cstdint>
 
 namespace mcpu {
@@ -68,10 +69,14 @@ struct SampleParams {
   const int32_t* top_k_rows;
   int64_t* token;   // (rows)
   float* logprob;   // (rows), or null
+  void* slices;  // what the slices of uncut rows leave (sample_workspace bytes)
   int64_t rows, vocab, sl, sn;
   int dtype;
 };
 
+constexpr int kSampleSlice = 8192;  // logits of a slice
+int64_t sample_slices(const SampleParams& p);
+size_t sample_workspace(const SampleParams& p);
 hipError_t sample_launch(const SampleParams& p, hipStream_t st);
 
 }  // namespace mcpu

@@ -14,9 +14,8 @@
 //
 // Every cut is a prefix of the order, so it is a pair: the key (the logit as an
 // ordered integer) of its last token and the index up to which tokens of that
-// key belong. sample_row_kernel, one workgroup per row, reads the row once and
-// keeps it in registers (up to kRowRegs logits per thread; longer rows are
-// read again for every step), and finds the cuts in one of three ways:
+// key belong. sample_row_kernel, one workgroup per row, finds the cuts in one of
+// three ways:
 //  - a short list: the k-th largest of the threads' maxima is at most the k-th
 //    largest logit, so the logits from there up hold the first k and, for k up
 //    to kListK, are few more. They are sorted in LDS; all that follows is a scan
@@ -26,13 +25,14 @@
 //    the one bin that holds the cut.
 //  - radix descent over the keys, 8 bits at a time, where a list overflows:
 //    masses of equal logits, or a cut far below M.
-// Masses are added as integers (units of 2^-40 of the largest): the sums are
-// exact in any order, so LDS atomics leave the result unchanged. Where nothing
-// is cut for any row, sample_slice_kernel takes rows in slices instead, so that
-// few rows fill the chip, and sample_join_kernel compares their winners.
+// Masses are added as integers (in the list units of 2^-40 of the largest, in
+// bins units of 2^-31 of the total): the sums are exact in any order, so LDS
+// atomics leave the result unchanged. Where nothing is cut for any row,
+// sample_slice_kernel takes rows in slices instead, so that few rows fill the
+// chip, and sample_join_kernel compares their winners.
 //
-// The race runs on approximate scores first (v_exp_f32, v_rcp_f32: 8
-// instructions a logit instead of 35); what comes within 2^-13 of the best is
+// The race runs on approximate scores first (v_exp_f32, v_rcp_f32: 12
+// instructions a logit instead of 40); what comes within 2^-13 of the best is
 // scored again with the division and exponential to the last place.
 #include "lm_math.h"
 #include "lm_params.h"
@@ -65,52 +65,59 @@ __device__ __forceinline__ uint64_t mass_of(float w) {
 }
 
 struct Shared {
-  uint64_t bins[kBins];  // bins, and the radix descent's masses and counts
+  uint32_t bins[kBins];  // bins, and the radix descent's
   uint64_t list[kThreads];
   float tops[kThreads];  // each thread's largest logit
   uint64_t u64[kWaves];
   uint32_t u32[kWaves];
   float f32[kWaves];
-  uint32_t n, pick;
-  uint64_t left;
+  uint32_t n, pick, left;
+  uint64_t entry;
 };
 
-// Reductions over the workgroup, in every thread, ending behind a barrier.
-template <typename V, typename F> __device__ __forceinline__ V group_reduce(V v, V* slot, F&& join) {
+// Reductions over the WAVES waves of a workgroup, in every thread, ending
+// behind a barrier.
+template <int WAVES, typename V, typename F> __device__ __forceinline__ V group_reduce(V v, V* slot, F&& join) {
   for (int o = 32; o > 0; o >>= 1) v = join(v, __shfl_xor(v, o));
-  const int waves = blockDim.x >> 6;
   if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = slot[0];
-  for (int i = 1; i < waves; ++i) v = join(v, slot[i]);
+  V each[WAVES];
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) each[i] = slot[i];
+  v = each[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) v = join(v, each[i]);
   __syncthreads();
   return v;
 }
-__device__ __forceinline__ float group_max(float v, float* slot) {
-  return group_reduce(v, slot, [](float a, float b) { return fmaxf(a, b); });
+template <int WAVES = kWaves> __device__ __forceinline__ float group_max(float v, float* slot) {
+  return group_reduce<WAVES>(v, slot, [](float a, float b) { return fmaxf(a, b); });
 }
-__device__ __forceinline__ float group_fsum(float v, float* slot) {
-  return group_reduce(v, slot, [](float a, float b) { return a + b; });
+template <int WAVES = kWaves> __device__ __forceinline__ float group_fsum(float v, float* slot) {
+  return group_reduce<WAVES>(v, slot, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ uint64_t group_sum(uint64_t v, uint64_t* slot) {
-  return group_reduce(v, slot, [](uint64_t a, uint64_t b) { return a + b; });
+  return group_reduce<kWaves>(v, slot, [](uint64_t a, uint64_t b) { return a + b; });
 }
-__device__ __forceinline__ uint32_t group_min(uint32_t v, uint32_t* slot) {
-  return group_reduce(v, slot, [](uint32_t a, uint32_t b) { return min(a, b); });
+template <int WAVES = kWaves> __device__ __forceinline__ uint32_t group_min(uint32_t v, uint32_t* slot) {
+  return group_reduce<WAVES>(v, slot, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
 
 // Sum over the threads before this one.
-__device__ __forceinline__ uint64_t group_before(uint64_t v, uint64_t* slot) {
+template <typename V> __device__ __forceinline__ V group_before(V v, V* slot) {
   const int lane = threadIdx.x & 63;
-  uint64_t incl = v;
+  V incl = v;
   for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t up = __shfl_up(incl, o);
+    const V up = __shfl_up(incl, o);
     if (lane >= o) incl += up;
   }
   if (lane == 63) slot[threadIdx.x >> 6] = incl;
   __syncthreads();
-  uint64_t before = incl - v;
-  for (int i = 0; i < static_cast<int>(threadIdx.x >> 6); ++i) before += slot[i];
+  V each[kWaves], before = incl - v;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) each[i] = slot[i];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) before += i < static_cast<int>(threadIdx.x >> 6) ? each[i] : 0;
   __syncthreads();
   return before;
 }
@@ -167,37 +174,31 @@ template <typename T> __device__ __forceinline__ Pack<T> load_pack(const T* row,
   }
   return clean(p);
 }
-// NP packs per thread in registers, or (NP = 0) the row read again for every use.
-template <typename T, int NP> struct Row {
+// x cut to [0, 1].
+__device__ __forceinline__ float upto1(float x) { return __builtin_amdgcn_fmed3f(x, 0.f, 1.f); }
+
+// A row, read again from the cache for every use: it is there (32 rows of 50280
+// bf16 logits fill 3.2 of the 4 MB of an XCD's L2), and holding 50 logits a
+// thread in registers spilled (35 against 27 us for one float32 row).
+template <typename T> struct Row {
   const T* logits;
   int vocab;
   float top;          // the largest logit
   float ref, factor;  // weight_fast's: top (or the largest float), log2(e) / T
   float temperature;
-  mutable Pack<T> pack[NP > 0 ? NP : 1];
 
   __device__ __forceinline__ float at(int i) const { return clean(to_f32(logits[i])); }
-  __device__ __forceinline__ void load() {
-    if constexpr (NP > 0)
-#pragma unroll
-      for (int j = 0; j < NP; ++j)
-        pack[j] = load_pack(logits, min((j * kThreads + static_cast<int>(threadIdx.x)) * kPer<T>, vocab), vocab);
-  }
-  // f(index of the first, the pack) for each pack of this thread.
+  // f(index of the first, the pack) for each pack of this thread, kAhead packs
+  // on their way at once.
   template <typename F> __device__ __forceinline__ void each_pack(F&& f) const {
-    if constexpr (NP > 0) {
-      // The compiler is to forget what it knows of the values here: it would
-      // keep every use's widened logits and comparisons for the next use, in
-      // more registers than there are.
-      int first = static_cast<int>(threadIdx.x) * kPer<T>;
-      asm volatile("" : "+v"(first));
+    constexpr int kAhead = 4;
+    for (int i0 = threadIdx.x * kPer<T>; i0 < vocab; i0 += kAhead * kThreads * kPer<T>) {
+      Pack<T> p[kAhead];
 #pragma unroll
-      for (int j = 0; j < NP; ++j) {
-        asm volatile("" : "+v"(pack[j].w[0]), "+v"(pack[j].w[1]), "+v"(pack[j].w[2]), "+v"(pack[j].w[3]));
-        f(first + j * kThreads * kPer<T>, pack[j]);
-      }
-    } else {
-      for (int i = threadIdx.x * kPer<T>; i < vocab; i += kThreads * kPer<T>) f(i, load_pack(logits, i, vocab));
+      for (int j = 0; j < kAhead; ++j) p[j] = load_pack(logits, i0 + j * kThreads * kPer<T>, vocab);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * kThreads * kPer<T> < vocab) f(i0 + j * kThreads * kPer<T>, p[j]);
     }
   }
   // f(index, logit); beyond the row's end the logit is -inf.
@@ -209,27 +210,50 @@ template <typename T, int NP> struct Row {
   }
   // exp((l - M) / T); the largest logits, infinite ones too, weigh 1.
   __device__ __forceinline__ float weight(float l) const { return l == top ? 1.0f : exp_acc((l - top) / temperature); }
-  __device__ __forceinline__ float weight_fast(float l) const { return fast_exp2(fminf((l - ref) * factor, 0.f)); }
+  // Clamped to 1, for M = inf (a modifier of v_exp_f32, without an instruction).
+  __device__ __forceinline__ float weight_fast(float l) const { return upto1(fast_exp2((l - ref) * factor)); }
+  // Temperatures beyond 1e-30 and 1e30 act as those (log2(e) / T stays a number,
+  // also times 0 and infinity).
   __device__ __forceinline__ void set(float m, float t) {
     top = m;
-    temperature = t;
-    factor = kLog2e / t;
+    temperature = __builtin_amdgcn_fmed3f(t, 1e-30f, 1e30f);
+    factor = kLog2e / temperature;
     ref = fminf(m, 3.402823466e38f);
   }
 };
 
-// A prefix of the order: keys above `key`, and of `key` the indices up to `last`.
+// A prefix of the order: logits above `edge`, and of `edge` the indices up to `last`.
 struct Cut {
-  uint32_t key, last;
-  __device__ __forceinline__ bool has(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
+  float edge;
+  uint32_t last;
+  __device__ __forceinline__ bool has(float l, int i) const {
+    return l > edge || (l == edge && static_cast<uint32_t>(i) <= last);
+  }
 };
 
 // The list's n <= kThreads entries (key << 32 | ~index) in descending order,
-// thread t with entry t (0 behind the n-th): a bitonic network, whose steps
-// within a wave are lane exchanges.
+// thread t with entry t (0 behind the n-th). Short lists by counting, for each
+// entry, those above it (all are different); longer ones by a bitonic network,
+// whose steps within a wave are lane exchanges. 55 entries take 0.6 us against
+// 3 by the network, which wins from about 300 on (700: 8 us).
 __device__ __forceinline__ uint64_t sorted_entry(Shared& s, int n) {
   const int t = threadIdx.x;
   uint64_t v = t < n ? s.list[t] : 0;
+  if (n <= 256) {
+    if (t >= n && t < (n + 7) / 8 * 8) s.list[t] = 0;
+    __syncthreads();
+    int rank = 0;
+    if ((t & ~63) < n)
+      for (int i = 0; i < n; i += 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rank += s.list[i + j] > v;
+    __syncthreads();
+    if (t < n) s.list[rank] = v;
+    __syncthreads();
+    v = t < n ? s.list[t] : 0;
+    __syncthreads();
+    return v;
+  }
   for (int size = 2; size / 2 < n; size *= 2)
     for (int step = size / 2; step > 0; step /= 2) {
       uint64_t other;
@@ -248,42 +272,37 @@ __device__ __forceinline__ uint64_t sorted_entry(Shared& s, int n) {
   return v;
 }
 
-// Appends what `in` accepts of the row to the list; how many that were, of
-// which those beyond the list's end are lost.
-template <typename R, typename F> __device__ __forceinline__ int collect(const R& row, Shared& s, F&& in) {
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
-  row.each([&](int i, float l) {
-    if (i < row.vocab && in(i, l)) {
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < kThreads) s.list[at] = (static_cast<uint64_t>(key_of(l)) << 32) | (0xffffffffu - i);
-    }
-  });
-  __syncthreads();
-  const int n = static_cast<int>(s.n);
-  __syncthreads();
-  return n;
+// Appends a logit to the list; what comes behind the list's end is only counted.
+__device__ __forceinline__ void append(Shared& s, float l, int i) {
+  const uint32_t at = atomicAdd(&s.n, 1u);
+  if (at < kThreads) s.list[at] = (static_cast<uint64_t>(key_of(l)) << 32) | (0xffffffffu - i);
 }
 
 // ---- cuts -----------------------------------------------------------------------------------
 
-// The shortest prefix of `from` that holds `want` units: tokens (BY_MASS
-// false) or mass, the last token counted if any of it is wanted; want >= 1 and
-// at most what `from` holds. By radix descent over the keys.
-template <bool BY_MASS, typename R> __device__ Cut radix_cut(const R& row, const Cut& from, uint64_t want, Shared& s) {
+// What a logit counts for a cut: one token, or its mass in units of the total
+// (`unit` of them to a weight of 1, 2^31 to the whole).
+template <bool BY_MASS, typename R> __device__ __forceinline__ uint32_t units(const R& row, float l, float unit) {
+  return BY_MASS ? static_cast<uint32_t>(fmaf(row.weight_fast(l), unit, 0.5f)) : 1u;
+}
+
+// The shortest prefix of `from` that holds `want` units, the last token
+// counted if any of it is wanted; want >= 1 and at most what `from` holds. By
+// radix descent over the keys.
+template <bool BY_MASS, typename R>
+__device__ Cut radix_cut(const R& row, const Cut& from, uint32_t want, float unit, Shared& s) {
   uint32_t prefix = 0, mask = 0;  // the key's bits found so far, and which they are
   for (int shift = 24; shift >= 0; shift -= 8) {
     if (threadIdx.x < 256) s.bins[threadIdx.x] = 0;
     __syncthreads();
     row.each([&](int i, float l) {
       const uint32_t k = key_of(l);
-      if (i < row.vocab && (k & mask) == prefix && from.has(k, i))
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.bins[(k >> shift) & 255]),
-                  BY_MASS ? mass_of(row.weight_fast(l)) : 1ull);
+      if (i < row.vocab && (k & mask) == prefix && from.has(l, i))
+        atomicAdd(&s.bins[(k >> shift) & 255], units<BY_MASS>(row, l, unit));
     });
     __syncthreads();
     if (threadIdx.x == 0) {
-      uint64_t left = want;
+      uint32_t left = want;
       int bin = 255;
       for (; bin > 0 && s.bins[bin] < left; --bin) left -= s.bins[bin];
       s.pick = static_cast<uint32_t>(bin);
@@ -296,25 +315,24 @@ template <bool BY_MASS, typename R> __device__ Cut radix_cut(const R& row, const
     __syncthreads();
   }
   // `want` units of the tokens with exactly this key, by index: how many tokens
-  // that is (they weigh the same), then where the last of them lies. A wave
+  // that is (they count the same), then where the last of them lies. A wave
   // looks at a run of the row.
-  if (BY_MASS) {
-    const uint64_t each = mass_of(row.weight_fast(value_of(prefix)));
-    want = (want + each - 1) / each;  // the key's mass holds `want` >= 1, so each >= 1
-  }
+  const float edge = value_of(prefix);
+  const uint32_t each = max(units<BY_MASS>(row, edge, unit), 1u);
+  want = (want + each - 1) / each;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int run = ((row.vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int t0 = w * run, t1 = min(t0 + run, row.vocab);
   auto hits = [&](int i) {
-    const uint32_t k = key_of(i < t1 ? row.at(i) : 0.f);
-    return __ballot(i < t1 && k == prefix && from.has(k, i));
+    const float l = i < t1 ? row.at(i) : 0.f;
+    return __ballot(i < t1 && l == edge && from.has(l, i));
   };
   uint32_t mine = 0;
   for (int i = t0 + lane; i - lane < t1; i += 64) mine += __popcll(hits(i));
   if (lane == 0) s.u32[w] = mine;
   if (threadIdx.x == 0) s.pick = static_cast<uint32_t>(row.vocab - 1);
   __syncthreads();
-  uint64_t seen = 0;
+  uint32_t seen = 0;
   for (int v = 0; v < w; ++v) seen += s.u32[v];
   if (seen < want && seen + mine >= want) {  // the wave that holds the last one
     for (int i = t0 + lane; i - lane < t1; i += 64) {
@@ -327,28 +345,36 @@ template <bool BY_MASS, typename R> __device__ Cut radix_cut(const R& row, const
     }
   }
   __syncthreads();
-  const Cut cut{prefix, s.pick};
+  const Cut cut{edge, s.pick};
   __syncthreads();
   return cut;
 }
 
-// The same by bins of equal width below M: as far as the row reaches, at most
-// 24 T (where w is 4e-11); the last bin takes what lies beyond.
+// The same by bins of equal width below M: as far as the row reaches (`low`),
+// at most 24 T (where w is 4e-11); the last bin takes what lies beyond.
 template <bool BY_MASS, typename R>
-__device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from, uint64_t want, Shared& s) {
+__device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from, uint32_t want, float unit,
+                                        Shared& s) {
   const float scale = (kBins - 1) / fmaxf(fminf(24.0f * row.temperature, row.top - low), 1e-30f);
-  auto bin_of = [&](float l) { return static_cast<int>(fmaxf(fminf((row.ref - l) * scale, kBins - 1.0f), 0.f)); };
+  auto bin_of = [&](float l) {
+    return static_cast<int>(__builtin_amdgcn_fmed3f((row.ref - l) * scale, 0.f, kBins - 1.0f));
+  };
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[i] = 0;
   __syncthreads();
-  row.each([&](int i, float l) {
-    if (i < row.vocab && from.has(key_of(l), i))
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s.bins[bin_of(l)]),
-                BY_MASS ? mass_of(row.weight_fast(l)) : 1ull);
-  });
+  if (BY_MASS && from.edge == -__builtin_inff()) {  // everything; beyond the row's end the mass is 0
+    row.each([&](int, float l) { atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit)); });
+  } else {
+    row.each([&](int i, float l) {
+      if (i < row.vocab && from.has(l, i)) atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit));
+    });
+  }
   __syncthreads();
-  const uint64_t b0 = s.bins[2 * threadIdx.x], b1 = s.bins[2 * threadIdx.x + 1];
-  const uint64_t before = group_before(b0 + b1, s.u64);
-  if (threadIdx.x == 0) s.pick = kBins - 1;  // rounding may leave the sum short of `want`
+  const uint32_t b0 = s.bins[2 * threadIdx.x], b1 = s.bins[2 * threadIdx.x + 1];
+  const uint32_t before = group_before(b0 + b1, s.u32);
+  if (threadIdx.x == 0) {
+    s.pick = kBins - 1;  // rounding may leave the sum short of `want`
+    s.n = 0;
+  }
   __syncthreads();
   if (before < want && before + b0 + b1 >= want) {
     const bool second = before + b0 < want;
@@ -357,23 +383,28 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
   }
   __syncthreads();
   const int bin = static_cast<int>(s.pick);
-  const uint64_t left = s.left;
-  __syncthreads();
+  const uint32_t left = s.left;
   if (bin < kBins - 1) {
-    const int n = collect(row, s, [&](int i, float l) { return from.has(key_of(l), i) && bin_of(l) == bin; });
+    row.each([&](int i, float l) {
+      if (bin_of(l) == bin && i < row.vocab && from.has(l, i)) append(s, l, i);
+    });
+    __syncthreads();
+    const int n = static_cast<int>(s.n);
+    __syncthreads();
     if (n <= kThreads) {
       const uint64_t e = sorted_entry(s, n);
       const bool in = static_cast<int>(threadIdx.x) < n;
-      const uint64_t unit = in ? (BY_MASS ? mass_of(row.weight_fast(value_of(e >> 32))) : 1) : 0;
-      const uint64_t at = group_before(unit, s.u64);
-      if (in && at < left && at + unit >= left) s.left = e;
+      const uint32_t unit_here = in ? units<BY_MASS>(row, value_of(e >> 32), unit) : 0;
+      const uint32_t at = group_before(unit_here, s.u32);
+      if (in && at < left && at + unit_here >= left) s.entry = e;
       __syncthreads();
-      const Cut cut{static_cast<uint32_t>(s.left >> 32), 0xffffffffu - static_cast<uint32_t>(s.left)};
+      const Cut cut{value_of(s.entry >> 32), 0xffffffffu - static_cast<uint32_t>(s.entry)};
       __syncthreads();
       return cut;
     }
   }
-  return radix_cut<BY_MASS>(row, from, want, s);
+  __syncthreads();
+  return radix_cut<BY_MASS>(row, from, want, unit, s);
 }
 
 // The largest key of the threads' maxima that at least `want` of them reach,
@@ -382,7 +413,17 @@ __device__ __forceinline__ uint32_t maxima_key(const Shared& s, int want) {
   uint32_t k[kThreads / 64];
 #pragma unroll
   for (int j = 0; j < kThreads / 64; ++j) k[j] = key_of(s.tops[j * 64 + (threadIdx.x & 63)]);
-  uint32_t lo = 0, hi = 0xffffffffu;  // all reach lo; fewer than `want` reach hi
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int j = 0; j < kThreads / 64; ++j) {
+    lo = min(lo, k[j]);
+    hi = max(hi, k[j]);
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, static_cast<uint32_t>(__shfl_xor(lo, o)));
+    hi = max(hi, static_cast<uint32_t>(__shfl_xor(hi, o)));
+  }
+  hi += 1;  // all reach lo; fewer than `want` reach hi
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
     int n = 0;
@@ -392,7 +433,7 @@ __device__ __forceinline__ uint32_t maxima_key(const Shared& s, int want) {
       hi = mid;
     } else {
       lo = mid;
-      if (n <= want + want / 4 + 8) break;
+      if (n <= want + want / 16 + 4) break;
     }
   }
   return lo;
@@ -400,28 +441,113 @@ __device__ __forceinline__ uint32_t maxima_key(const Shared& s, int want) {
 
 // ---- the race ----------------------------------------------------------------------------------
 
-__device__ __forceinline__ float noise_at(const float* noise, int i) { return fmaxf(noise[i], 1.17549435e-38f); }
+constexpr float kLeastNoise = 1.17549435e-38f;
+__device__ __forceinline__ float noise_at(const float* noise, int i) { return fmaxf(noise[i], kLeastNoise); }
 
 // The workgroup's largest score and, of those who hold it, the lowest index.
+template <int WAVES = kWaves>
 __device__ __forceinline__ uint32_t winner(float score, uint32_t i, float* f32, uint32_t* u32) {
-  const float top = group_max(score, f32);
-  return group_min(score == top ? i : 0xffffffffu, u32);
+  const float top = group_max<WAVES>(score, f32);
+  return group_min<WAVES>(score == top ? i : 0xffffffffu, u32);
 }
 
-template <typename T, int NP> __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleParams p) {
+// A thread's best approximate score, where, and the second best.
+struct Best {
+  float best = -1.0f, second = -1.0f;
+  int at = 0;
+  __device__ __forceinline__ void see(float score, int i) {
+    second = __builtin_amdgcn_fmed3f(best, second, score);  // second <= best
+    at = score > best ? i : at;
+    best = fmaxf(best, score);
+  }
+};
+
+// The winner of the kept logits of a row.
+// CUT: there are cuts; otherwise every logit is kept.
+template <bool CUT, typename T>
+__device__ __forceinline__ uint32_t race(const Row<T>& row, const Cut& kept, float min_p, const float* noise,
+                                         Shared& s) {
+  constexpr int kAhead = 2, E = kPer<T>;
+  auto in = [&](float l, int i) {
+    if constexpr (!CUT) return true;
+    if (!kept.has(l, i)) return false;
+    if (!(min_p > 0.f)) return true;
+    const float w = row.weight_fast(l);
+    return w >= min_p * (2.0f - kNear) || (w >= min_p * kNear && row.weight(l) >= min_p);
+  };
+  // f(score, index) of each kept logit; logits and, where any of a pack is
+  // kept, noise of kAhead packs on their way at once.
+  auto scores = [&](auto&& f) {
+    for (int i0 = threadIdx.x * E; i0 < row.vocab; i0 += kAhead * kThreads * E) {
+      Pack<T> p[kAhead];
+      float q[kAhead][E];
+      bool keep[kAhead][E];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) p[j] = load_pack(row.logits, i0 + j * kThreads * E, row.vocab);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j * kThreads * E;
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          keep[j][e] = (!CUT || i + e < row.vocab) && in(p[j].at(e), i + e);
+          any |= keep[j][e];
+        }
+        if (any && i + E <= row.vocab) {
+#pragma unroll
+          for (int e = 0; e < E; e += 4) {
+            float q4[4];
+            ld4_elem<float>(noise, i + e, q4);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) q[j][e + x] = q4[x];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) q[j][e] = i + e < row.vocab && keep[j][e] ? noise[i + e] : 1.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (keep[j][e])
+            f(row.weight_fast(p[j].at(e)) * fast_rcp(fmaxf(q[j][e], kLeastNoise)), i0 + j * kThreads * E + e);
+    }
+  };
+  Best b;
+  scores([&](float score, int i) { b.see(score, i); });
+  const float bar = group_max(b.best, s.f32) * kNear;
+  float score = -1.0f;
+  uint32_t at = 0xffffffffu;
+  auto exactly = [&](int i) {
+    if (i >= row.vocab) return;
+    const float exact = row.weight(row.at(i)) / noise_at(noise, i);
+    if (exact > score) {
+      score = exact;
+      at = static_cast<uint32_t>(i);
+    }
+  };
+  if (b.second >= bar) {
+    scores([&](float near, int i) {
+      if (near >= bar) exactly(i);
+    });
+  } else if (b.best >= bar) {
+    exactly(b.at);
+  }
+  return winner(score, at, s.f32, s.u32);
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleParams p) {
   __shared__ Shared s;
   const int64_t r = blockIdx.x;
-  Row<T, NP> row;
+  Row<T> row;
   row.logits = static_cast<const T*>(p.logits) + r * p.sl;
   row.vocab = static_cast<int>(p.vocab);
-  // An infinite temperature would weigh -inf logits too (0 x inf).
-  float temperature = p.temperature_rows != nullptr ? p.temperature_rows[r] : p.temperature;
-  if (temperature > 1e30f) temperature = 1e30f;
+  const float temperature = p.temperature_rows != nullptr ? p.temperature_rows[r] : p.temperature;
   int k = p.top_k_rows != nullptr ? p.top_k_rows[r] : p.top_k;
   const float top_p = p.top_p_rows != nullptr ? p.top_p_rows[r] : p.top_p;
   const float min_p = fminf(p.min_p_rows != nullptr ? p.min_p_rows[r] : p.min_p, 1.0f);
   if (k >= row.vocab) k = 0;
-  row.load();
 
   const float inf = __builtin_inff();
   float m = -inf, low = inf;
@@ -439,126 +565,95 @@ template <typename T, int NP> __global__ __launch_bounds__(kThreads) void sample
     return;
   }
   const bool greedy = !(temperature > 0.f);
-  float total1 = 0.f;  // sum of exp(l - M), for the log-probability
-  row.set(m, 1.0f);
-  if (p.logprob != nullptr) {
-    row.each([&](int, float l) { total1 += row.weight_fast(l); });
-    total1 = group_fsum(total1, s.f32);
-  }
-
+  const bool few = !greedy && k > 0 && k <= kListK;
+  const bool by_p = !greedy && top_p < 1.0f;
+  const bool list = few || (by_p && k == 0);
+  row.set(m, greedy ? 1.0f : temperature);
+  // One more look at the row: the sums of exp(l - M), for the log-probability,
+  // and of the weights, where top-p is asked without top-k; the lowest index of
+  // M for T <= 0; the short list.
+  const bool sum1 = p.logprob != nullptr, sum_t = by_p && k == 0;
+  const float from = row.vocab <= kThreads ? -inf : list ? value_of(maxima_key(s, few ? k : kTryK)) : inf;
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  float total1 = 0.f, total = 0.f;
   uint32_t token = 0xffffffffu;
-  if (greedy) {
-    row.each([&](int i, float l) {
-      if (l == m) token = min(token, static_cast<uint32_t>(i));
+  if (sum1 || list || greedy) {
+    // What is looked for is rare: a pack's largest logit says whether it is there.
+    const bool one = row.temperature == 1.0f, both = sum_t && !one;
+    const float look = greedy ? m : from;
+    row.each_pack([&](int i, const Pack<T>& q) {
+      float high = -inf;
+#pragma unroll
+      for (int e = 0; e < kPer<T>; ++e) high = fmaxf(high, q.at(e));
+      if (high >= look) {
+        for (int e = 0; e < kPer<T>; ++e) {
+          const float l = q.at(e);
+          if (l >= look && i + e < row.vocab) {
+            if (greedy) token = min(token, static_cast<uint32_t>(i + e));
+            else append(s, l, i + e);
+          }
+        }
+      }
+      if (sum1) {
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) total1 += upto1(fast_exp2((q.at(e) - row.ref) * kLog2e));
+      }
+      if (both) {
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) total += row.weight_fast(q.at(e));
+      }
     });
+    if (sum1) total1 = group_fsum(total1, s.f32);
+    if (sum_t && one && !sum1) row.each([&](int, float l) { total += row.weight_fast(l); });
+    if (sum_t) total = one && sum1 ? total1 : group_fsum(total, s.f32);
+    __syncthreads();
+  }
+  if (greedy) {
     token = group_min(token, s.u32);
   } else {
-    row.set(m, temperature);
     const float* noise = p.noise + r * p.sn;
-    const bool few = k > 0 && k <= kListK;
-    float total = 0.f;  // mass of all, where top-p is asked without top-k
-    if (top_p < 1.0f && k == 0) {
-      if (temperature == 1.0f && p.logprob != nullptr) {
-        total = total1;
-      } else {
-        row.each([&](int, float l) { total += row.weight_fast(l); });
-        total = group_fsum(total, s.f32);
-      }
-    }
     const float part = fmaxf(top_p, 0.f);
-    if (few || (top_p < 1.0f && k == 0)) {
-      // The short list.
-      const float from = row.vocab <= kThreads ? -inf : value_of(maxima_key(s, few ? k : kTryK));
-      const int n = collect(row, s, [&](int, float l) { return l >= from; });
-      if (n <= kThreads) {
-        const bool in = static_cast<int>(threadIdx.x) < n;
-        bool holds = few;
-        if (!few) {
-          const uint64_t e = in ? s.list[threadIdx.x] : 0;
-          holds = row.vocab <= kThreads ||
-                  static_cast<float>(group_sum(in ? mass_of(row.weight(value_of(e >> 32))) : 0, s.u64)) >
-                      part * total * kMassUnit * kNear;
+    const int n = static_cast<int>(s.n);
+    __syncthreads();
+    if (list && n <= kThreads) {
+      const bool in = static_cast<int>(threadIdx.x) < n;
+      bool holds = few || row.vocab <= kThreads;
+      if (!holds) {
+        const float w = in ? row.weight_fast(value_of(s.list[threadIdx.x] >> 32)) : 0.f;
+        holds = group_fsum(w, s.f32) > part * total * (2.0f - kNear);
+      }
+      if (holds) {
+        const uint64_t e = sorted_entry(s, n);
+        const float w = in ? row.weight(value_of(e >> 32)) : 0.f;
+        const uint32_t i = 0xffffffffu - static_cast<uint32_t>(e);
+        bool keep = in && (!few || static_cast<int>(threadIdx.x) < k);
+        if (by_p) {
+          const uint64_t mass = keep ? mass_of(w) : 0;
+          const uint64_t all = few ? group_sum(mass, s.u64) : static_cast<uint64_t>(total * kMassUnit);
+          const double want = ceil(static_cast<double>(part) * static_cast<double>(all));
+          keep = group_before(mass, s.u64) < static_cast<uint64_t>(want) && keep;
         }
-        if (holds) {
-          const uint64_t e = sorted_entry(s, n);
-          const float w = in ? row.weight(value_of(e >> 32)) : 0.f;
-          const uint32_t i = 0xffffffffu - static_cast<uint32_t>(e);
-          bool keep = in && (!few || static_cast<int>(threadIdx.x) < k);
-          if (top_p < 1.0f) {
-            const uint64_t mass = keep ? mass_of(w) : 0;
-            const uint64_t all = few ? group_sum(mass, s.u64) : static_cast<uint64_t>(total * kMassUnit);
-            const double want = ceil(static_cast<double>(part) * static_cast<double>(all));
-            keep = group_before(mass, s.u64) < static_cast<uint64_t>(want) && keep;
-          }
-          keep = (keep && w >= min_p) || threadIdx.x == 0;
-          token = winner(keep ? w / noise_at(noise, static_cast<int>(i)) : -1.0f, i, s.f32, s.u32);
-        }
+        keep = (keep && w >= min_p) || threadIdx.x == 0;
+        token = winner(keep ? w / noise_at(noise, static_cast<int>(i)) : -1.0f, i, s.f32, s.u32);
       }
     }
     if (token == 0xffffffffu) {
-      Cut kept{key_of(-inf), static_cast<uint32_t>(row.vocab - 1)};  // everything
-      low = -group_max(-low, s.f32);
+      Cut kept{-inf, static_cast<uint32_t>(row.vocab - 1)};  // everything
+      if (k > 0 || by_p) low = -group_max(-low, s.f32);
       if (k > 0) {
-        kept = find_cut<false>(row, low, kept, static_cast<uint64_t>(k), s);
-        if (top_p < 1.0f) {
-          row.each([&](int i, float l) { total += i < row.vocab && kept.has(key_of(l), i) ? row.weight_fast(l) : 0.f; });
+        kept = find_cut<false>(row, low, kept, static_cast<uint32_t>(k), 1.0f, s);
+        if (by_p) {
+          row.each([&](int i, float l) { total += i < row.vocab && kept.has(l, i) ? row.weight_fast(l) : 0.f; });
           total = group_fsum(total, s.f32);
         }
       }
-      if (top_p < 1.0f) {
-        const double want = ceil(static_cast<double>(part) * static_cast<double>(total) * kMassUnit);
-        kept = find_cut<true>(row, low, kept, want < 1.0 ? 1 : static_cast<uint64_t>(want), s);
+      if (by_p) {
+        const float want = ceilf(part * 0x1p31f);
+        kept = find_cut<true>(row, low, kept, want < 1.0f ? 1 : static_cast<uint32_t>(want), 0x1p31f / total, s);
       }
-      // The race over the row. `edge` is the cut's logit.
-      const float edge = value_of(kept.key);
-      auto scores = [&](auto&& f) {
-        row.each_pack([&](int i, const Pack<T>& q) {
-          bool any = false;
-          float l[kPer<T>];
-          bool in[kPer<T>];
-#pragma unroll
-          for (int e = 0; e < kPer<T>; ++e) {
-            l[e] = q.at(e);
-            in[e] = l[e] > edge || (l[e] == edge && static_cast<uint32_t>(i + e) <= kept.last);
-            if (in[e] && min_p > 0.f) {
-              const float w = row.weight_fast(l[e]);
-              in[e] = w >= min_p * (2.0f - kNear) || (w >= min_p * kNear && row.weight(l[e]) >= min_p);
-            }
-            any |= in[e];
-          }
-          if (!any) return;
-          if (i + kPer<T> <= row.vocab) {
-#pragma unroll
-            for (int h = 0; h < kPer<T>; h += 4) {
-              float q4[4];
-              ld4_elem<float>(noise, i + h, q4);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (in[h + e]) f(i + h + e, l[h + e], fmaxf(q4[e], 1.17549435e-38f));
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < kPer<T>; ++e)
-              if (in[e] && i + e < row.vocab) f(i + e, l[e], noise_at(noise, i + e));
-          }
-        });
-      };
-      float best = -1.0f;
-      scores([&](int, float l, float q) { best = fmaxf(best, row.weight_fast(l) * fast_rcp(q)); });
-      const float bar = group_max(best, s.f32) * kNear;
-      float score = -1.0f;
-      uint32_t at = 0xffffffffu;
-      if (best >= bar) {
-        scores([&](int i, float l, float q) {
-          if (row.weight_fast(l) * fast_rcp(q) < bar) return;
-          const float exact = row.weight(l) / q;
-          if (exact > score) {
-            score = exact;
-            at = static_cast<uint32_t>(i);
-          }
-        });
-      }
-      token = winner(score, at, s.f32, s.u32);
+      token = k > 0 || by_p || min_p > 0.f ? race<true>(row, kept, min_p, noise, s)
+                                           : race<false>(row, kept, min_p, noise, s);
     }
   }
   if (threadIdx.x == 0) {
@@ -570,20 +665,171 @@ template <typename T, int NP> __global__ __launch_bounds__(kThreads) void sample
   }
 }
 
+// ---- rows that nothing cuts, in slices -----------------------------------------------------------
+
+constexpr int kSliceThreads = 512, kSliceMost = 64;  // threads, and slices of a row
+
+// What a slice leaves for its row.
+struct Slice {
+  float top, sum;  // the largest logit; the sum of exp(l - top)
+  uint32_t at;     // its winner, or for T <= 0 the lowest index of `top`
+};
+
+// The slice's packs of logits, and of noise, all on their way at once.
+template <typename T, bool GREEDY>
+__global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const SampleParams p, int slices) {
+  constexpr int E = kPer<T>, NP = kSampleSlice / (kSliceThreads * E);
+  __shared__ float f32[kSliceThreads / 64];
+  __shared__ uint32_t u32[kSliceThreads / 64];
+  const int64_t r = blockIdx.x / slices;
+  const int first = static_cast<int>(blockIdx.x % slices) * kSampleSlice + static_cast<int>(threadIdx.x) * E;
+  Row<T> row;
+  row.logits = static_cast<const T*>(p.logits) + r * p.sl;
+  row.vocab = static_cast<int>(p.vocab);
+  const float* noise = p.noise + r * p.sn;
+  Pack<T> l[NP];
+  float q[GREEDY ? 1 : NP][E];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int i = first + j * kSliceThreads * E;
+    l[j] = load_pack(row.logits, i, row.vocab);
+    if constexpr (!GREEDY) {
+      if (i + E <= row.vocab) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          float q4[4];
+          ld4_elem<float>(noise, i + e, q4);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) q[j][e + x] = q4[x];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[j][e] = i + e < row.vocab ? noise[i + e] : 1.0f;
+      }
+    }
+  }
+  const float inf = __builtin_inff();
+  float m = -inf;
+#pragma unroll
+  for (int j = 0; j < NP; ++j)
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, l[j].at(e));
+  m = group_max<kSliceThreads / 64>(m, f32);
+  row.set(m, GREEDY ? 1.0f : p.temperature);
+  float sum = 0.f, score = -1.0f;
+  uint32_t at = 0xffffffffu;
+  Best b;
+#pragma unroll
+  for (int j = 0; j < NP; ++j)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float v = l[j].at(e);
+      const int i = first + j * kSliceThreads * E + e;
+      sum += upto1(fast_exp2((v - row.ref) * kLog2e));
+      if constexpr (GREEDY) at = v == m ? min(at, static_cast<uint32_t>(i)) : at;
+      else b.see(row.weight_fast(v) * fast_rcp(fmaxf(q[j][e], kLeastNoise)), i);
+    }
+  sum = group_fsum<kSliceThreads / 64>(sum, f32);
+  if constexpr (GREEDY) {
+    at = group_min<kSliceThreads / 64>(at, u32);
+  } else {
+    const float bar = group_max<kSliceThreads / 64>(b.best, f32) * kNear;
+    auto exactly = [&](int i) {
+      if (i >= row.vocab) return;
+      const float exact = row.weight(row.at(i)) / noise_at(noise, i);
+      if (exact > score) {
+        score = exact;
+        at = static_cast<uint32_t>(i);
+      }
+    };
+    if (b.second >= bar) {
+      for (int j = 0; j < NP; ++j)
+        for (int e = 0; e < E; ++e) exactly(first + j * kSliceThreads * E + e);
+    } else if (b.best >= bar) {
+      exactly(b.at);
+    }
+    at = winner<kSliceThreads / 64>(score, at, f32, u32);
+  }
+  if (threadIdx.x == 0) static_cast<Slice*>(p.slices)[blockIdx.x] = Slice{m, m == -inf ? 0.f : sum, at};
+}
+
+// A row's token from its slices' winners, one lane each.
+template <typename T, bool GREEDY>
+__global__ __launch_bounds__(64) void sample_join_kernel(const SampleParams p, int slices) {
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float inf = __builtin_inff();
+  const Slice mine = lane < slices ? static_cast<const Slice*>(p.slices)[r * slices + lane] : Slice{-inf, 0.f, 0u};
+  float m = mine.top;
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (m == -inf) {
+    if (lane == 0) {
+      p.token[r] = -1;
+      if (p.logprob != nullptr) p.logprob[r] = -inf;
+    }
+    return;
+  }
+  Row<T> row;
+  row.logits = static_cast<const T*>(p.logits) + r * p.sl;
+  row.vocab = static_cast<int>(p.vocab);
+  row.set(m, GREEDY ? 1.0f : p.temperature);
+  // Slices without a logit above -inf, or with none near M, lose or have no winner.
+  const bool in = lane < slices && mine.top > -inf && mine.at < static_cast<uint32_t>(row.vocab);
+  float score = -1.0f, sum = 0.f;
+  if (in) {
+    if constexpr (GREEDY) score = mine.top == m ? 1.0f : 0.f;
+    else score = row.weight(row.at(static_cast<int>(mine.at))) / noise_at(p.noise + r * p.sn, static_cast<int>(mine.at));
+    sum = mine.sum * (mine.top == m ? 1.0f : exp_acc(mine.top - m));
+  }
+  float best = score;
+  for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+  uint32_t token = in && score == best ? mine.at : 0xffffffffu;
+  for (int o = 32; o > 0; o >>= 1) token = min(token, static_cast<uint32_t>(__shfl_xor(token, o)));
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) {
+    p.token[r] = static_cast<int64_t>(token);
+    if (p.logprob != nullptr && token < static_cast<uint32_t>(row.vocab)) {
+      const float l = row.at(static_cast<int>(token));
+      p.logprob[r] = (l == m ? 0.f : l - m) - logf(sum);
+    }
+  }
+}
+
+template <typename T> void launch(const SampleParams& p, hipStream_t st) {
+  const int64_t slices = sample_slices(p);
+  if (slices == 0) {
+    hipLaunchKernelGGL(sample_row_kernel<T>, dim3(static_cast<unsigned>(p.rows)), dim3(kThreads), 0, st, p);
+    return;
+  }
+  const dim3 grid(static_cast<unsigned>(p.rows * slices)), rows(static_cast<unsigned>(p.rows));
+  if (p.temperature > 0.f) {
+    hipLaunchKernelGGL((sample_slice_kernel<T, false>), grid, dim3(kSliceThreads), 0, st, p, static_cast<int>(slices));
+    hipLaunchKernelGGL((sample_join_kernel<T, false>), rows, dim3(64), 0, st, p, static_cast<int>(slices));
+  } else {
+    hipLaunchKernelGGL((sample_slice_kernel<T, true>), grid, dim3(kSliceThreads), 0, st, p, static_cast<int>(slices));
+    hipLaunchKernelGGL((sample_join_kernel<T, true>), rows, dim3(64), 0, st, p, static_cast<int>(slices));
+  }
+}
+
 }  // namespace
 
+// Slices of a row (0: none, the row kernel): where one setting holds for all
+// rows and cuts nothing, and a row has at most a lane's worth of slices. A row
+// of one slice needs no second launch: 8 x 1000 take 9 us with one, 12 with two.
+int64_t sample_slices(const SampleParams& p) {
+  const bool rows_alike = p.temperature_rows == nullptr && p.top_k_rows == nullptr && p.top_p_rows == nullptr &&
+                          p.min_p_rows == nullptr;
+  const bool greedy = p.temperature <= 0.f;
+  const bool uncut = greedy || ((p.top_k == 0 || p.top_k >= p.vocab) && p.top_p >= 1.0f && p.min_p <= 0.f);
+  const int64_t n = (p.vocab + kSampleSlice - 1) / kSampleSlice;
+  return rows_alike && uncut && n > 1 && n <= kSliceMost && p.rows * n <= INT32_MAX ? n : 0;
+}
+size_t sample_workspace(const SampleParams& p) { return sizeof(Slice) * p.rows * sample_slices(p); }
+
 hipError_t sample_launch(const SampleParams& p, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(p.rows)), block(kThreads);
-  auto by_size = [&](auto t) {
-    using T = decltype(t);
-    constexpr int kFull = 64 / kPer<T>, kSmall = 16 / kPer<T>;  // packs of 64 and 16 logits per thread
-    if (p.vocab <= 16 * kThreads) hipLaunchKernelGGL((sample_row_kernel<T, kSmall>), grid, block, 0, st, p);
-    else if (p.vocab <= 64 * kThreads) hipLaunchKernelGGL((sample_row_kernel<T, kFull>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((sample_row_kernel<T, 0>), grid, block, 0, st, p);
-  };
-  if (p.dtype == MCPU_F32) by_size(float{});
-  else if (p.dtype == MCPU_BF16) by_size(bf16{});
-  else by_size(f16{});
+  if (p.dtype == MCPU_F32) launch<float>(p, st);
+  else if (p.dtype == MCPU_BF16) launch<bf16>(p, st);
+  else launch<f16>(p, st);
   return hipGetLastError();
 }
 
