@@ -20,16 +20,16 @@
 //    largest logit, so the logits from there up hold the first k and, for k up
 //    to kListK, are few more. They are sorted in LDS; all that follows is a scan
 //    over the list. Without top-k the kTryK-th maximum is tried: where the list
-//    holds p of the mass it holds every token that top-p keeps.
+//    holds p of the mass it holds every token that top-p keeps. Min-p's own
+//    lowest logit, M + T log(min_p), does as well.
 //  - bins: counts or masses of kBins equal steps below M, and the sorted list of
 //    the one bin that holds the cut.
 //  - radix descent over the keys, 8 bits at a time, where a list overflows:
 //    masses of equal logits, or a cut far below M.
-// Masses are added as integers (in the list units of 2^-40 of the largest, in
-// bins units of 2^-31 of the total): the sums are exact in any order, so LDS
-// atomics leave the result unchanged. Where nothing is cut for any row,
-// sample_slice_kernel takes rows in slices instead, so that few rows fill the
-// chip, and sample_join_kernel compares their winners.
+// Masses in bins are added as integers, in units of 2^-31 of the total: the sums
+// are exact in any order, so LDS atomics leave the result unchanged. Where
+// nothing is cut for any row, sample_slice_kernel takes rows in slices instead,
+// so that few rows fill the chip, and sample_join_kernel compares their winners.
 //
 // The race runs on approximate scores first (v_exp_f32, v_rcp_f32: 12
 // instructions a logit instead of 40); what comes within 2^-13 of the best is
@@ -42,7 +42,6 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr float kMassUnit = 1099511627776.0f;  // 2^40
 constexpr float kNear = 1.0f - 0x1p-13f;
 constexpr int kBins = 2048;
 constexpr int kListK = 512;  // up to here the list holds about 1.4 k logits of its kThreads
@@ -57,18 +56,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key >> 31) != 0 ? 0x80000000u : 0xffffffffu));
 }
 
-// w * 2^40 rounded down, from its two halves (w <= 1, so both are exact).
-__device__ __forceinline__ uint64_t mass_of(float w) {
-  const float hi = truncf(w * 256.0f);
-  const float lo = (w * 256.0f - hi) * 4294967296.0f;
-  return (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo);
-}
-
 struct Shared {
   uint32_t bins[kBins];  // bins, and the radix descent's
   uint64_t list[kThreads];
   float tops[kThreads];  // each thread's largest logit
-  uint64_t u64[kWaves];
   uint32_t u32[kWaves];
   float f32[kWaves];
   uint32_t n, pick, left;
@@ -95,9 +86,6 @@ template <int WAVES = kWaves> __device__ __forceinline__ float group_max(float v
 }
 template <int WAVES = kWaves> __device__ __forceinline__ float group_fsum(float v, float* slot) {
   return group_reduce<WAVES>(v, slot, [](float a, float b) { return a + b; });
-}
-__device__ __forceinline__ uint64_t group_sum(uint64_t v, uint64_t* slot) {
-  return group_reduce<kWaves>(v, slot, [](uint64_t a, uint64_t b) { return a + b; });
 }
 template <int WAVES = kWaves> __device__ __forceinline__ uint32_t group_min(uint32_t v, uint32_t* slot) {
   return group_reduce<WAVES>(v, slot, [](uint32_t a, uint32_t b) { return min(a, b); });
@@ -181,6 +169,7 @@ __device__ __forceinline__ float upto1(float x) { return __builtin_amdgcn_fmed3f
 // bf16 logits fill 3.2 of the 4 MB of an XCD's L2), and holding 50 logits a
 // thread in registers spilled (35 against 27 us for one float32 row).
 template <typename T> struct Row {
+  static constexpr int kE = kPer<T>;
   const T* logits;
   int vocab;
   float top;          // the largest logit
@@ -231,6 +220,22 @@ struct Cut {
   }
 };
 
+// The value of lane ^ STEP, by DPP moves: xor 4 is half a row mirrored (xor 7)
+// and quads reversed (xor 3), xor 8 a row turned by half.
+template <int STEP> __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  auto half = [](int x) {
+    constexpr int kRowRor8 = 0x128;
+    if constexpr (STEP == 1) return __builtin_amdgcn_mov_dpp(x, kQuadXor1, 0xf, 0xf, true);
+    else if constexpr (STEP == 2) return __builtin_amdgcn_mov_dpp(x, kQuadXor2, 0xf, 0xf, true);
+    else if constexpr (STEP == 4)
+      return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(x, kQuadXor3, 0xf, 0xf, true), kRowHalfMirror, 0xf, 0xf,
+                                      true);
+    else return __builtin_amdgcn_mov_dpp(x, kRowRor8, 0xf, 0xf, true);
+  };
+  const uint32_t lo = half(static_cast<int>(v)), hi = half(static_cast<int>(v >> 32));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
 // The list's n <= kThreads entries (key << 32 | ~index) in descending order,
 // thread t with entry t (0 behind the n-th). Short lists by counting, for each
 // entry, those above it (all are different); longer ones by a bitonic network,
@@ -254,20 +259,23 @@ __device__ __forceinline__ uint64_t sorted_entry(Shared& s, int n) {
     __syncthreads();
     return v;
   }
-  for (int size = 2; size / 2 < n; size *= 2)
-    for (int step = size / 2; step > 0; step /= 2) {
-      uint64_t other;
-      if (step < 64) {
-        other = __shfl_xor(v, step);
-      } else {
-        __syncthreads();
-        s.list[t] = v;
-        __syncthreads();
-        other = s.list[t ^ step];
-      }
+  for (int size = 2; size / 2 < n; size *= 2) {
+    auto keep = [&](uint64_t other, int step) {
       const bool first = (t & step) == 0, down = (t & size) == 0;
       v = (v > other) == (first == down) ? v : other;
+    };
+    for (int step = size / 2; step >= 64; step /= 2) {
+      __syncthreads();
+      s.list[t] = v;
+      __syncthreads();
+      keep(s.list[t ^ step], step);
     }
+    for (int step = min(size / 2, 32); step >= 16; step /= 2) keep(__shfl_xor(v, step), step);
+    if (size > 8) keep(lane_xor<8>(v), 8);
+    if (size > 4) keep(lane_xor<4>(v), 4);
+    if (size > 2) keep(lane_xor<2>(v), 2);
+    keep(lane_xor<1>(v), 1);
+  }
   __syncthreads();
   return v;
 }
@@ -385,8 +393,20 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
   const int bin = static_cast<int>(s.pick);
   const uint32_t left = s.left;
   if (bin < kBins - 1) {
-    row.each([&](int i, float l) {
-      if (bin_of(l) == bin && i < row.vocab && from.has(l, i)) append(s, l, i);
+    // Logits near the bin's range first (two comparisons), then the bin itself:
+    // half a bin and four roundings of M wide of it, and bin 0 has no upper end.
+    const float slack = 0.5f / scale + 4.8e-7f * fabsf(row.ref);
+    const float high = bin == 0 ? __builtin_inff() : row.ref - bin / scale + slack;
+    const float least = row.ref - (bin + 1) / scale - slack;
+    row.each_pack([&](int i, const auto& q) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < R::kE; ++e) any |= q.at(e) <= high && q.at(e) >= least;
+      if (!any) return;
+      for (int e = 0; e < R::kE; ++e) {
+        const float l = q.at(e);
+        if (bin_of(l) == bin && i + e < row.vocab && from.has(l, i + e)) append(s, l, i + e);
+      }
     });
     __syncthreads();
     const int n = static_cast<int>(s.n);
@@ -408,41 +428,64 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
 }
 
 // The largest key of the threads' maxima that at least `want` of them reach,
-// or one a little lower: bisection, by every wave for itself.
-__device__ __forceinline__ uint32_t maxima_key(const Shared& s, int want) {
-  uint32_t k[kThreads / 64];
+// or one a little lower: bisection by the first wave, the others wait.
+__device__ __forceinline__ uint32_t maxima_key(Shared& s, int want) {
+  if (threadIdx.x < 64) {
+    uint32_t k[kThreads / 64];
 #pragma unroll
-  for (int j = 0; j < kThreads / 64; ++j) k[j] = key_of(s.tops[j * 64 + (threadIdx.x & 63)]);
-  uint32_t lo = 0xffffffffu, hi = 0;
+    for (int j = 0; j < kThreads / 64; ++j) k[j] = key_of(s.tops[j * 64 + threadIdx.x]);
+    uint32_t lo = 0xffffffffu, hi = 0;
 #pragma unroll
-  for (int j = 0; j < kThreads / 64; ++j) {
-    lo = min(lo, k[j]);
-    hi = max(hi, k[j]);
-  }
-  for (int o = 32; o > 0; o >>= 1) {
-    lo = min(lo, static_cast<uint32_t>(__shfl_xor(lo, o)));
-    hi = max(hi, static_cast<uint32_t>(__shfl_xor(hi, o)));
-  }
-  hi += 1;  // all reach lo; fewer than `want` reach hi
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < kThreads / 64; ++j) n += __popcll(__ballot(k[j] >= mid));
-    if (n < want) {
-      hi = mid;
-    } else {
-      lo = mid;
-      if (n <= want + want / 16 + 4) break;
+    for (int j = 0; j < kThreads / 64; ++j) {
+      lo = min(lo, k[j]);
+      hi = max(hi, k[j]);
     }
+    for (int o = 32; o > 0; o >>= 1) {
+      lo = min(lo, static_cast<uint32_t>(__shfl_xor(lo, o)));
+      hi = max(hi, static_cast<uint32_t>(__shfl_xor(hi, o)));
+    }
+    hi += 1;  // all reach lo; fewer than `want` reach hi
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < kThreads / 64; ++j) n += __popcll(__ballot(k[j] >= mid));
+      if (n < want) {
+        hi = mid;
+      } else {
+        lo = mid;
+        if (n <= want + want / 16 + 4) break;
+      }
+    }
+    if (threadIdx.x == 0) s.pick = lo;
   }
-  return lo;
+  __syncthreads();
+  const uint32_t key = s.pick;
+  __syncthreads();
+  return key;
 }
 
 // ---- the race ----------------------------------------------------------------------------------
 
 constexpr float kLeastNoise = 1.17549435e-38f;
 __device__ __forceinline__ float noise_at(const float* noise, int i) { return fmaxf(noise[i], kLeastNoise); }
+
+// E values of noise from i on; beyond the row's end 1.
+template <int E>
+__device__ __forceinline__ void load_noise(const float* noise, int i, int vocab, float (&q)[E]) {
+  if (i + E <= vocab) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      float q4[4];
+      ld4_elem<float>(noise, i + e, q4);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) q[e + x] = q4[x];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] = i + e < vocab ? noise[i + e] : 1.0f;
+  }
+}
 
 // The workgroup's largest score and, of those who hold it, the lowest index.
 template <int WAVES = kWaves>
@@ -475,43 +518,25 @@ __device__ __forceinline__ uint32_t race(const Row<T>& row, const Cut& kept, flo
     const float w = row.weight_fast(l);
     return w >= min_p * (2.0f - kNear) || (w >= min_p * kNear && row.weight(l) >= min_p);
   };
-  // f(score, index) of each kept logit; logits and, where any of a pack is
-  // kept, noise of kAhead packs on their way at once.
+  // f(score, index) of each logit, -1 for one that is not kept; logits and noise
+  // of kAhead packs on their way at once.
   auto scores = [&](auto&& f) {
     for (int i0 = threadIdx.x * E; i0 < row.vocab; i0 += kAhead * kThreads * E) {
       Pack<T> p[kAhead];
       float q[kAhead][E];
-      bool keep[kAhead][E];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) p[j] = load_pack(row.logits, i0 + j * kThreads * E, row.vocab);
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int i = i0 + j * kThreads * E;
-        bool any = false;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          keep[j][e] = (!CUT || i + e < row.vocab) && in(p[j].at(e), i + e);
-          any |= keep[j][e];
-        }
-        if (any && i + E <= row.vocab) {
-#pragma unroll
-          for (int e = 0; e < E; e += 4) {
-            float q4[4];
-            ld4_elem<float>(noise, i + e, q4);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) q[j][e + x] = q4[x];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) q[j][e] = i + e < row.vocab && keep[j][e] ? noise[i + e] : 1.0f;
-        }
-      }
+      for (int j = 0; j < kAhead; ++j) load_noise<E>(noise, i0 + j * kThreads * E, row.vocab, q[j]);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (keep[j][e])
-            f(row.weight_fast(p[j].at(e)) * fast_rcp(fmaxf(q[j][e], kLeastNoise)), i0 + j * kThreads * E + e);
+        for (int e = 0; e < E; ++e) {
+          const int i = i0 + j * kThreads * E + e;
+          const float l = p[j].at(e);
+          const float score = row.weight_fast(l) * fast_rcp(fmaxf(q[j][e], kLeastNoise));
+          f(!CUT || (i < row.vocab && in(l, i)) ? score : -1.0f, i);
+        }
     }
   };
   Best b;
@@ -567,13 +592,25 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
   const bool greedy = !(temperature > 0.f);
   const bool few = !greedy && k > 0 && k <= kListK;
   const bool by_p = !greedy && top_p < 1.0f;
-  const bool list = few || (by_p && k == 0);
+  const bool by_min = !greedy && !few && k == 0 && min_p > 0.f;
+  const bool list = few || by_min || (by_p && k == 0);
   row.set(m, greedy ? 1.0f : temperature);
   // One more look at the row: the sums of exp(l - M), for the log-probability,
   // and of the weights, where top-p is asked without top-k; the lowest index of
   // M for T <= 0; the short list.
   const bool sum1 = p.logprob != nullptr, sum_t = by_p && k == 0;
-  const float from = row.vocab <= kThreads ? -inf : list ? value_of(maxima_key(s, few ? k : kTryK)) : inf;
+  // The list's lowest logit: without top-k not below min-p's, with half a
+  // percent of the weight and four roundings of M to spare.
+  float from = inf;
+  bool least = false;  // the list is min-p's
+  if (list && row.vocab > kThreads) {
+    if (few || by_p) from = value_of(maxima_key(s, few ? k : kTryK));
+    const float by = by_min ? row.ref + row.temperature * (logf(min_p) - 0.005f) - 4.8e-7f * fabsf(row.ref) : -inf;
+    least = by_min && (!by_p || by >= from);
+    if (least) from = by;
+  } else if (list) {
+    from = -inf;
+  }
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   float total1 = 0.f, total = 0.f;
@@ -618,7 +655,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
     __syncthreads();
     if (list && n <= kThreads) {
       const bool in = static_cast<int>(threadIdx.x) < n;
-      bool holds = few || row.vocab <= kThreads;
+      bool holds = few || least || row.vocab <= kThreads;
       if (!holds) {
         const float w = in ? row.weight_fast(value_of(s.list[threadIdx.x] >> 32)) : 0.f;
         holds = group_fsum(w, s.f32) > part * total * (2.0f - kNear);
@@ -628,11 +665,10 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
         const float w = in ? row.weight(value_of(e >> 32)) : 0.f;
         const uint32_t i = 0xffffffffu - static_cast<uint32_t>(e);
         bool keep = in && (!few || static_cast<int>(threadIdx.x) < k);
-        if (by_p) {
-          const uint64_t mass = keep ? mass_of(w) : 0;
-          const uint64_t all = few ? group_sum(mass, s.u64) : static_cast<uint64_t>(total * kMassUnit);
-          const double want = ceil(static_cast<double>(part) * static_cast<double>(all));
-          keep = group_before(mass, s.u64) < static_cast<uint64_t>(want) && keep;
+        if (by_p) {  // sums in the list's order, which is always the same
+          const float mass = keep ? w : 0.f;
+          const float all = few ? group_fsum(mass, s.f32) : total;
+          keep = group_before(mass, s.f32) < part * all && keep;
         }
         keep = (keep && w >= min_p) || threadIdx.x == 0;
         token = winner(keep ? w / noise_at(noise, static_cast<int>(i)) : -1.0f, i, s.f32, s.u32);
@@ -693,20 +729,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   for (int j = 0; j < NP; ++j) {
     const int i = first + j * kSliceThreads * E;
     l[j] = load_pack(row.logits, i, row.vocab);
-    if constexpr (!GREEDY) {
-      if (i + E <= row.vocab) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          float q4[4];
-          ld4_elem<float>(noise, i + e, q4);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) q[j][e + x] = q4[x];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) q[j][e] = i + e < row.vocab ? noise[i + e] : 1.0f;
-      }
-    }
+    if constexpr (!GREEDY) load_noise<E>(noise, i, row.vocab, q[j]);
   }
   const float inf = __builtin_inff();
   float m = -inf;
