@@ -668,6 +668,8 @@ typedef struct mcpu_norm_args {
   float* mean;              /* (rows): written by the forward when given, read by the
                                backward; not used by RMS norm */
   float* rstd;              /* (rows): likewise */
+  const float* z;           /* (rows, dim), optional, backward: x + residual (a float32 res_out);
+                               x and residual are then not read */
   const void* dy;
   const void* dres_out;     /* optional */
   void* dx;

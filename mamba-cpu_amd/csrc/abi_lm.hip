@@ -20,8 +20,8 @@ int check_norm(const mcpu_norm_args* a, const char* what) {
   if (!(a->eps >= 0.f)) return fail(MCPU_ERR_INVALID, "%s: eps must not be negative", what);
   if (a->rows > INT_MAX || a->dim > (int64_t{1} << 24))
     return fail(MCPU_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows of 2^24 elements", what);
-  if ((a->weight == nullptr && a->dim > 0) || (a->x == nullptr && a->rows * a->dim > 0))
-    return fail(MCPU_ERR_INVALID, "%s: x and weight are required", what);
+  if ((a->weight == nullptr && a->dim > 0) || (a->x == nullptr && a->z == nullptr && a->rows * a->dim > 0))
+    return fail(MCPU_ERR_INVALID, "%s: x (or z) and weight are required", what);
   if (a->x_stride < 0 || a->res_stride < 0 || a->y_stride < 0 || a->dy_stride < 0)
     return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
   return MCPU_OK;
@@ -136,7 +136,8 @@ extern "C" int mcpu_norm_fwd(const mcpu_norm_args* a, void* stream) {
   const char* what = "norm_fwd";
   clear_error();
   if (int rc = check_norm(a, what)) return rc;
-  if (a->y == nullptr && a->rows * a->dim > 0) return fail(MCPU_ERR_INVALID, "%s: y is required", what);
+  if ((a->y == nullptr || a->x == nullptr) && a->rows * a->dim > 0)
+    return fail(MCPU_ERR_INVALID, "%s: x and y are required", what);
   if (int rc = mcpu_check_device()) return rc;
   if (a->rows == 0 || a->dim == 0) return MCPU_OK;
   NormParams p = make_norm(a);
@@ -166,6 +167,7 @@ extern "C" int mcpu_norm_bwd(const mcpu_norm_args* a, void* workspace, size_t wo
   if (int rc = mcpu_check_device()) return rc;
   if (a->dim == 0) return MCPU_OK;
   NormParams p = make_norm(a);
+  p.z = a->z;
   p.dy = a->dy;
   p.dres_out = a->dres_out;
   p.dx = a->dx;

@@ -9,7 +9,7 @@
 // starts) and its own tokens; nothing passes between workgroups. An id outside
 // the vocabulary has a zero row and no gradient.
 #include "lm_params.h"
-#include "mcpu_common.h"
+#include "lm_math.h"
 
 namespace mcpu {
 namespace {
@@ -17,20 +17,6 @@ namespace {
 __device__ __forceinline__ int64_t id_at(const EmbeddingParams& p, int64_t t) {
   return p.ids64 ? static_cast<const int64_t*>(p.ids)[t] : static_cast<const int32_t*>(p.ids)[t];
 }
-
-// n values (1 to 4) from element i on, as one vector where all four are there.
-template <typename T> __device__ __forceinline__ void ld_upto4(const T* row, int64_t i, int n, float (&v)[4]) {
-  if (n == 4) return ld4_elem<T>(row, i, v);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(row[i + e]) : 0.f;
-}
-template <typename T> __device__ __forceinline__ void st_upto4(T* row, int64_t i, int n, const float (&v)[4]) {
-  if (n == 4) return st4_elem<T>(row, i, v);
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (e < n) row[i + e] = from_f32<T>(v[e]);
-}
-__device__ __forceinline__ int upto4(int64_t left) { return left < 4 ? static_cast<int>(left) : 4; }
 
 // One wave per token, four elements per lane; the loads of up to four such
 // turns are on their way before the first store.

@@ -1,5 +1,6 @@
 // Scalar functions to about one unit in the last place of float32, for the
-// kernels whose results are compared at that accuracy.
+// kernels whose results are compared at that accuracy, and rows of any length
+// in vectors of four elements.
 #pragma once
 
 #include "mcpu_common.h"
@@ -27,5 +28,21 @@ __device__ __forceinline__ float sigmoid_acc(float x, float& one_minus) {
 
 // softplus(x), stable at both ends.
 __device__ __forceinline__ float softplus_acc(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+
+// ---- four elements of a row, or what is left of it -----------------------------------
+
+// n values (1 to 4) from element i on, as one vector where all four are there.
+template <typename T> __device__ __forceinline__ void ld_upto4(const T* row, int64_t i, int n, float (&v)[4]) {
+  if (n == 4) return ld4_elem<T>(row, i, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(row[i + e]) : 0.f;
+}
+template <typename T> __device__ __forceinline__ void st_upto4(T* row, int64_t i, int n, const float (&v)[4]) {
+  if (n == 4) return st4_elem<T>(row, i, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) row[i + e] = from_f32<T>(v[e]);
+}
+__device__ __forceinline__ int upto4(int64_t left) { return left < 4 ? static_cast<int>(left) : 4; }
 
 }  // namespace mcpu

@@ -12,6 +12,7 @@ namespace mcpu {
 struct NormParams {
   const void* x;         // (rows, dim), row stride sx
   const void* residual;  // (rows, dim), row stride sres, or null
+  const float* z;     // backward: x + residual, contiguous, instead of the two; or null
   const float* weight;
   const float* bias;  // or null
   void* y;            // (rows, dim), row stride sy
@@ -24,7 +25,7 @@ struct NormParams {
   void* dres;            // contiguous, or null
   float* dweight;
   float* dbias;  // or null
-  float* part;   // (parts, 1 or 2, dim): dweight and dbias partials
+  float* part;   // (parts, 1 or, with dbias, 2, dim): dweight and dbias partials
   int64_t rows, dim, parts;
   int64_t sx, sres, sy, sdy;
   float eps;
@@ -32,6 +33,8 @@ struct NormParams {
   int x_dtype, res_dtype;
 };
 
+constexpr int64_t kNormWave = 1536;  // longest row of one wave
+constexpr int64_t kNormMost = 8192;  // longest row held in registers
 // Workgroups of the backward: each leaves one partial of dweight and dbias.
 int64_t norm_bwd_parts(int64_t rows, int64_t dim);
 hipError_t norm_fwd_launch(const NormParams& p, hipStream_t st);

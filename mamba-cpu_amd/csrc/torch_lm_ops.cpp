@@ -28,6 +28,13 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 }
 void* ws_ptr(const Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
 
+bool any_grad(std::initializer_list<optional<Tensor>> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const optional<Tensor>& t : tensors)
+    if (has(t) && t->requires_grad()) return true;
+  return false;
+}
+
 // ---- gated linear recurrence -----------------------------------------------------
 
 void check_gated(const char* name, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate, const Tensor& decay,
@@ -173,6 +180,13 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd_autograd(const Tensor& x, cons
                                                            const Tensor& x_gate, const Tensor& decay,
                                                            const optional<Tensor>& init,
                                                            const optional<Tensor>& seq_idx, double c, bool save) {
+  if (!any_grad({opt(x), opt(a_gate), opt(x_gate), opt(decay), init})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::gated_scan_fwd", "")
+                         .typed<decltype(gated_scan_fwd)>();
+    return op.call(x, a_gate, x_gate, decay, init, seq_idx, c, save);
+  }
   auto r = GatedScanFn::apply(x, a_gate, x_gate, decay, init, seq_idx, c, save);
   return {r[0], r[1], r[2]};
 }
@@ -241,57 +255,59 @@ Tensor gated_step_inplace(Tensor& state, const Tensor& x, const Tensor& a_gate, 
 
 // Rows the kernels take as they are: contiguous elements, any distance.
 Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
+// The same of a tensor of any dimensions, rows along the last.
+Tensor as_rows(const Tensor& t) {
+  const int64_t dim = t.size(-1);
+  return rows_of(t.dim() == 2 ? t : t.reshape({dim > 0 ? t.numel() / dim : 0, dim}));
+}
+optional<Tensor> as_rows(const optional<Tensor>& t) { return has(t) ? optional<Tensor>(as_rows(*t)) : std::nullopt; }
 
-void check_norm(const char* name, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
-                const optional<Tensor>& residual) {
-  for (const optional<Tensor>& t : {opt(x), opt(weight), bias, residual}) check_gpu(name, t);
-  TORCH_CHECK_VALUE(x_dtype(x.scalar_type()) && x.dim() == 2, name,
-                    " expects x (rows, dim) in float32, bfloat16 or float16");
+void check_norm(const char* name, const Tensor& like, const Tensor& weight, const optional<Tensor>& bias,
+                double eps) {
+  for (const optional<Tensor>& t : {opt(like), opt(weight), bias}) check_gpu(name, t);
+  TORCH_CHECK_VALUE(x_dtype(like.scalar_type()) && like.dim() >= 1, name,
+                    " expects x (..., dim) in float32, bfloat16 or float16");
   for (const optional<Tensor>& t : {opt(weight), bias})
-    TORCH_CHECK_VALUE(!has(t) || (t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == x.size(1) &&
-                                  t->is_contiguous()),
-                      name, " expects contiguous float32 weight and bias of shape (dim,)");
+    TORCH_CHECK_VALUE(!has(t) || (t->dim() == 1 && t->size(0) == like.size(-1) && t->is_floating_point()), name,
+                      " expects weight and bias of shape (dim,) = (", like.size(-1), ",)");
+  TORCH_CHECK_VALUE(eps >= 0, name, ": eps must not be negative, got ", eps);
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd(const Tensor& x, const Tensor& weight_in,
+                                                    const optional<Tensor>& bias_in, const optional<Tensor>& residual,
+                                                    double eps, bool rms, bool want_res, bool res_float32) {
+  const char* name = "mamba_cpu::norm_fwd";
+  check_norm(name, x, weight_in, bias_in, eps);
+  check_gpu(name, residual);
   TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == x.sizes() &&
                                        (residual->scalar_type() == at::kFloat ||
                                         residual->scalar_type() == x.scalar_type())),
                     name, " expects residual shaped like x, in x's dtype or float32");
-}
-
-mcpu_norm_args norm_args(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
-                         const optional<Tensor>& residual, at::ScalarType res_dtype, double eps, bool rms) {
+  c10::DeviceGuard guard(x.device());
+  const Tensor xr = as_rows(x), weight = f32c(weight_in);
+  const optional<Tensor> rr = as_rows(residual), bias = f32c(bias_in);
+  const at::ScalarType rt = has(rr) ? rr->scalar_type() : (res_float32 ? at::kFloat : x.scalar_type());
+  const int64_t rows = xr.size(0);
+  Tensor y = at::empty(x.sizes(), x.options());
+  Tensor res = want_res ? at::empty(x.sizes(), x.options().dtype(rt)) : at::empty({0}, x.options().dtype(rt));
+  Tensor rstd = at::empty({rows}, weight.options());
+  Tensor mean = at::empty({rms ? 0 : rows}, weight.options());
   mcpu_norm_args a;
   std::memset(&a, 0, sizeof(a));
-  a.x = x.data_ptr();
-  a.residual = ptr(residual);
+  a.x = xr.data_ptr();
+  a.residual = ptr(rr);
   a.weight = static_cast<const float*>(weight.data_ptr());
   a.bias = fptr(bias);
-  a.rows = x.size(0);
-  a.dim = x.size(1);
-  a.x_stride = x.stride(0);
-  a.res_stride = has(residual) ? residual->stride(0) : 0;
+  a.rows = rows;
+  a.dim = xr.size(1);
+  a.x_stride = xr.stride(0);
+  a.res_stride = has(rr) ? rr->stride(0) : 0;
+  a.y_stride = xr.size(1);
   a.eps = static_cast<float>(eps);
   a.rms = rms ? 1 : 0;
   a.dtype = dtype_tag(x.scalar_type());
-  a.res_dtype = dtype_tag(res_dtype);
-  return a;
-}
-
-std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd(const Tensor& x_in, const Tensor& weight,
-                                                    const optional<Tensor>& bias, const optional<Tensor>& res_in,
-                                                    double eps, bool rms, bool want_res, bool res_float32) {
-  const char* name = "mamba_cpu::norm_fwd";
-  check_norm(name, x_in, weight, bias, res_in);
-  c10::DeviceGuard guard(x_in.device());
-  const Tensor x = rows_of(x_in);
-  const optional<Tensor> residual = has(res_in) ? optional<Tensor>(rows_of(*res_in)) : std::nullopt;
-  const at::ScalarType rt = has(residual) ? residual->scalar_type() : (res_float32 ? at::kFloat : x.scalar_type());
-  Tensor y = at::empty(x.sizes(), x.options());
-  Tensor res = want_res ? at::empty(x.sizes(), x.options().dtype(rt)) : at::empty({0}, x.options().dtype(rt));
-  Tensor rstd = at::empty({x.size(0)}, weight.options());
-  Tensor mean = at::empty({rms ? 0 : x.size(0)}, weight.options());
-  mcpu_norm_args a = norm_args(x, weight, bias, residual, rt, eps, rms);
+  a.res_dtype = dtype_tag(rt);
   a.y = y.data_ptr();
-  a.y_stride = x.size(1);
   a.res_out = want_res ? res.data_ptr() : nullptr;
   a.mean = rms ? nullptr : static_cast<float*>(mean.data_ptr());
   a.rstd = static_cast<float*>(rstd.data_ptr());
@@ -299,81 +315,119 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd(const Tensor& x_in, const Te
   return {y, res, mean, rstd};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> norm_bwd(const Tensor& dy_in, const optional<Tensor>& dres_out_in,
-                                                    const Tensor& x_in, const Tensor& weight,
-                                                    const optional<Tensor>& bias, const optional<Tensor>& res_in,
-                                                    double eps, bool rms, const Tensor& mean, const Tensor& rstd) {
+// The gradients from z (a float32 residual that norm_fwd returned) or from x
+// and residual. `res_kind`: 0 without a residual, 1 one of x's dtype, 2 float32.
+std::tuple<Tensor, Tensor, Tensor, Tensor> norm_bwd(const Tensor& dy, const optional<Tensor>& dres_out,
+                                                    const optional<Tensor>& x, const optional<Tensor>& residual,
+                                                    const optional<Tensor>& z, const Tensor& weight_in, bool has_bias,
+                                                    int64_t res_kind, double eps, bool rms, const Tensor& mean,
+                                                    const Tensor& rstd) {
   const char* name = "mamba_cpu::norm_bwd";
-  check_norm(name, x_in, weight, bias, res_in);
-  for (const optional<Tensor>& t : {opt(dy_in), dres_out_in, opt(mean), opt(rstd)}) check_gpu(name, t);
-  TORCH_CHECK_VALUE(dy_in.sizes() == x_in.sizes() && dy_in.scalar_type() == x_in.scalar_type(), name,
+  check_norm(name, dy, weight_in, std::nullopt, eps);
+  for (const optional<Tensor>& t : {dres_out, x, residual, z, opt(mean), opt(rstd)}) check_gpu(name, t);
+  const at::ScalarType xt = dy.scalar_type();
+  TORCH_CHECK_VALUE(has(x) != has(z), name, " expects either x or z");
+  TORCH_CHECK_VALUE(!has(x) || (x->sizes() == dy.sizes() && x->scalar_type() == xt), name,
                     " expects dy shaped and typed like x");
-  TORCH_CHECK_VALUE(rstd.numel() == x_in.size(0) && (rms || mean.numel() == x_in.size(0)) &&
-                        rstd.scalar_type() == at::kFloat && mean.scalar_type() == at::kFloat &&
-                        rstd.is_contiguous() && mean.is_contiguous(),
+  TORCH_CHECK_VALUE(!has(z) || (z->sizes() == dy.sizes() && z->scalar_type() == at::kFloat && z->is_contiguous()),
+                    name, " expects z as norm_fwd returned it in float32");
+  const at::ScalarType rt = res_kind == 2 || (res_kind == 0 && has(dres_out) && dres_out->scalar_type() == at::kFloat)
+                                ? at::kFloat
+                                : xt;
+  TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == dy.sizes() && residual->scalar_type() == rt &&
+                                       res_kind > 0),
+                    name, " expects residual shaped like x, of the type that residual_kind says");
+  TORCH_CHECK_VALUE(!has(dres_out) || (dres_out->sizes() == dy.sizes() && dres_out->scalar_type() == rt), name,
+                    " expects dresidual_out shaped like x and typed like the residual");
+  const Tensor g = as_rows(dy);
+  const int64_t rows = g.size(0), dim = g.size(1);
+  TORCH_CHECK_VALUE(rstd.numel() == rows && (rms || mean.numel() == rows) && rstd.scalar_type() == at::kFloat &&
+                        mean.scalar_type() == at::kFloat && rstd.is_contiguous() && mean.is_contiguous(),
                     name, " expects the mean and rstd that norm_fwd returned");
-  c10::DeviceGuard guard(x_in.device());
-  const Tensor x = rows_of(x_in), dy = rows_of(dy_in);
-  const optional<Tensor> residual = has(res_in) ? optional<Tensor>(rows_of(*res_in)) : std::nullopt;
-  const at::ScalarType rt = has(residual) ? residual->scalar_type()
-                            : has(dres_out_in) ? dres_out_in->scalar_type() : x.scalar_type();
-  TORCH_CHECK_VALUE(!has(dres_out_in) || (dres_out_in->sizes() == x.sizes() && dres_out_in->scalar_type() == rt &&
-                                          (rt == at::kFloat || rt == x.scalar_type())),
-                    name, " expects dres_out shaped like x and typed like the residual");
-  const optional<Tensor> dres_out = has(dres_out_in) ? optional<Tensor>(dres_out_in->contiguous()) : std::nullopt;
-  Tensor dx = at::empty(x.sizes(), x.options());
-  Tensor dres = has(residual) ? at::empty(x.sizes(), residual->options()) : at::empty({0}, x.options());
-  Tensor dw = at::empty(weight.sizes(), weight.options());
-  Tensor db = at::empty({has(bias) ? x.size(1) : 0}, weight.options());
-  mcpu_norm_args a = norm_args(x, weight, bias, residual, rt, eps, rms);
+  c10::DeviceGuard guard(dy.device());
+  const Tensor weight = f32c(weight_in);
+  const optional<Tensor> xr = as_rows(x), rr = as_rows(residual);
+  const optional<Tensor> dr = has(dres_out) ? optional<Tensor>(dres_out->contiguous()) : std::nullopt;
+  Tensor dx = at::empty(dy.sizes(), dy.options());
+  Tensor dres = res_kind > 0 ? at::empty(dy.sizes(), dy.options().dtype(rt)) : at::empty({0}, dy.options());
+  Tensor dw = at::empty({dim}, weight.options());
+  Tensor db = at::empty({has_bias ? dim : 0}, weight.options());
+  mcpu_norm_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.x = ptr(xr);
+  a.residual = ptr(rr);
+  a.z = fptr(z);
+  a.weight = static_cast<const float*>(weight.data_ptr());
+  a.bias = has_bias ? a.weight : nullptr;  // only whether there is one
+  a.rows = rows;
+  a.dim = dim;
+  a.x_stride = has(xr) ? xr->stride(0) : 0;
+  a.res_stride = has(rr) ? rr->stride(0) : 0;
+  a.eps = static_cast<float>(eps);
+  a.rms = rms ? 1 : 0;
+  a.dtype = dtype_tag(xt);
+  a.res_dtype = dtype_tag(rt);
   a.mean = rms ? nullptr : static_cast<float*>(mean.data_ptr());
   a.rstd = static_cast<float*>(rstd.data_ptr());
-  a.dy = dy.data_ptr();
-  a.dy_stride = dy.stride(0);
-  a.dres_out = ptr(dres_out);
+  a.dy = g.data_ptr();
+  a.dy_stride = g.stride(0);
+  a.dres_out = ptr(dr);
   a.dx = dx.data_ptr();
-  a.dres = has(residual) ? dres.data_ptr() : nullptr;
+  a.dres = res_kind > 0 ? dres.data_ptr() : nullptr;
   a.dweight = static_cast<float*>(dw.data_ptr());
-  a.dbias = has(bias) ? static_cast<float*>(db.data_ptr()) : nullptr;
+  a.dbias = has_bias ? static_cast<float*>(db.data_ptr()) : nullptr;
   const size_t nws = mcpu_norm_bwd_workspace_size(&a);
-  Tensor ws = workspace(nws, x);
-  check_rc(mcpu_norm_bwd(&a, ws_ptr(ws), nws, stream_of(x)), name);
+  Tensor ws = workspace(nws, dy);
+  check_rc(mcpu_norm_bwd(&a, ws_ptr(ws), nws, stream_of(dy)), name);
   return {dx, dres, dw, db};
 }
 
+auto norm_fwd_below() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("mamba_cpu::norm_fwd", "")
+                       .typed<decltype(norm_fwd)>();
+  return op;
+}
+
+// Keeps the summed residual where it is returned in float32, x and residual
+// where it is not.
 struct NormFn : public torch::autograd::Function<NormFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
                                const optional<Tensor>& bias, const optional<Tensor>& residual, double eps, bool rms,
                                bool want_res, bool res_float32) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("mamba_cpu::norm_fwd", "")
-                         .typed<decltype(norm_fwd)>();
-    auto r = op.call(x, weight, bias, residual, eps, rms, want_res, res_float32);
-    const Tensor mean = std::get<2>(r), rstd = std::get<3>(r);
+    auto r = norm_fwd_below().call(x, weight, bias, residual, eps, rms, want_res, res_float32);
+    const Tensor res = std::get<1>(r), mean = std::get<2>(r), rstd = std::get<3>(r);
+    const bool keep_z = want_res && res.scalar_type() == at::kFloat;
     ctx->mark_non_differentiable({mean, rstd});
-    ctx->save_for_backward({x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), mean, rstd});
+    ctx->save_for_backward({weight, keep_z ? Tensor() : x, keep_z ? Tensor() : residual.value_or(Tensor()),
+                            keep_z ? res : Tensor(), mean, rstd});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["rms"] = rms;
     ctx->saved_data["want_res"] = want_res;
+    ctx->saved_data["bias"] = has(bias);
+    ctx->saved_data["kind"] = static_cast<int64_t>(!has(residual) ? 0 : residual->scalar_type() == at::kFloat ? 2 : 1);
+    ctx->saved_data["dtype"] = static_cast<int64_t>(x.scalar_type());
     ctx->set_materialize_grads(false);
-    return {std::get<0>(r), std::get<1>(r), mean, rstd};
+    return {std::get<0>(r), res, mean, rstd};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor& x = s[0];
-    const optional<Tensor> bias = opt(s[2]), residual = opt(s[3]);
-    const Tensor dy = grads[0].defined() ? grads[0].to(x.scalar_type()) : at::zeros_like(x);
+    const at::ScalarType xt = static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt());
+    const Tensor& like = s[1].defined() ? s[1] : s[3];
+    const Tensor dy = grads[0].defined() ? grads[0].to(xt) : at::zeros(like.sizes(), like.options().dtype(xt));
     const optional<Tensor> dres_out =
         ctx->saved_data["want_res"].toBool() && grads[1].defined() ? optional<Tensor>(grads[1]) : std::nullopt;
+    const int64_t kind = ctx->saved_data["kind"].toInt();
+    const bool bias = ctx->saved_data["bias"].toBool();
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("mamba_cpu::norm_bwd", "")
                          .typed<decltype(norm_bwd)>();
-    auto g = op.call(dy, dres_out, x, s[1], bias, residual, ctx->saved_data["eps"].toDouble(),
-                     ctx->saved_data["rms"].toBool(), s[4], s[5]);
-    return {std::get<0>(g), std::get<2>(g), has(bias) ? std::get<3>(g) : Tensor(),
-            has(residual) ? std::get<1>(g) : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    auto g = op.call(dy, dres_out, opt(s[1]), opt(s[2]), opt(s[3]), s[0], bias, kind,
+                     ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool(), s[4], s[5]);
+    return {std::get<0>(g), std::get<2>(g).to(s[0].scalar_type()), bias ? std::get<3>(g) : Tensor(),
+            kind > 0 ? std::get<1>(g) : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -381,6 +435,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm_fwd_autograd(const Tensor& x, co
                                                              const optional<Tensor>& bias,
                                                              const optional<Tensor>& residual, double eps, bool rms,
                                                              bool want_res, bool res_float32) {
+  if (!any_grad({opt(x), opt(weight), bias, residual})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return norm_fwd_below().call(x, weight, bias, residual, eps, rms, want_res, res_float32);
+  }
   auto r = NormFn::apply(x, weight, bias, residual, eps, rms, want_res, res_float32);
   return {r[0], r[1], r[2], r[3]};
 }
@@ -465,6 +523,13 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
 };
 
 Tensor embedding_fwd_autograd(const Tensor& ids, const Tensor& weight, double scale) {
+  if (!any_grad({opt(weight)})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::embedding_fwd", "")
+                         .typed<decltype(embedding_fwd)>();
+    return op.call(ids, weight, scale);
+  }
   return EmbeddingFn::apply(ids, weight, scale);
 }
 
@@ -535,8 +600,9 @@ TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
         "Tensor? state_batch_indices=None) -> Tensor");
   m.def("norm_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, float eps, bool rms, bool want_residual, "
         "bool residual_float32) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("norm_bwd(Tensor dy, Tensor? dresidual_out, Tensor x, Tensor weight, Tensor? bias, Tensor? residual, "
-        "float eps, bool rms, Tensor mean, Tensor rstd) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("norm_bwd(Tensor dy, Tensor? dresidual_out, Tensor? x, Tensor? residual, Tensor? z, Tensor weight, "
+        "bool has_bias, int residual_kind, float eps, bool rms, Tensor mean, Tensor rstd) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
   m.def("embedding_fwd(Tensor ids, Tensor weight, float scale) -> Tensor");
   m.def("embedding_bwd(Tensor dout, Tensor ids, int vocab, float scale) -> Tensor");
   m.def("sample(Tensor logits, Tensor? noise, float temperature, int top_k, float top_p, float min_p, "

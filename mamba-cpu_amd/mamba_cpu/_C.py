@@ -177,8 +177,8 @@ class NormArgs(ctypes.Structure):
         ("x", _P), ("residual", _P), ("weight", _P), ("bias", _P), ("rows", _I64), ("dim", _I64),
         ("x_stride", _I64), ("res_stride", _I64), ("y_stride", _I64), ("dy_stride", _I64),
         ("eps", ctypes.c_float), ("rms", _I32), ("dtype", _I32), ("res_dtype", _I32),
-        ("y", _P), ("res_out", _P), ("mean", _P), ("rstd", _P), ("dy", _P), ("dres_out", _P), ("dx", _P),
-        ("dres", _P), ("dweight", _P), ("dbias", _P),
+        ("y", _P), ("res_out", _P), ("mean", _P), ("rstd", _P), ("z", _P), ("dy", _P), ("dres_out", _P),
+        ("dx", _P), ("dres", _P), ("dweight", _P), ("dbias", _P),
     ]
 
 

@@ -20,16 +20,19 @@ _X_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 @torch.library.register_fake("mamba_cpu::norm_fwd")
 def _(x, weight, bias, residual, eps, rms, want_residual, residual_float32):
-    rows = x.shape[0]
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
     rdt = residual.dtype if residual is not None else torch.float32 if residual_float32 else x.dtype
+    f32 = dict(dtype=torch.float32)
     return (x.new_empty(x.shape), x.new_empty(x.shape if want_residual else (0,), dtype=rdt),
-            weight.new_empty(0 if rms else rows), weight.new_empty(rows))
+            weight.new_empty(0 if rms else rows, **f32), weight.new_empty(rows, **f32))
 
 
 @torch.library.register_fake("mamba_cpu::norm_bwd")
-def _(dy, dresidual_out, x, weight, bias, residual, eps, rms, mean, rstd):
-    return (x.new_empty(x.shape), x.new_empty(0) if residual is None else residual.new_empty(x.shape),
-            weight.new_empty(weight.shape), weight.new_empty(weight.shape if bias is not None else (0,)))
+def _(dy, dresidual_out, x, residual, z, weight, has_bias, residual_kind, eps, rms, mean, rstd):
+    rdt = torch.float32 if residual_kind == 2 else dy.dtype
+    f32 = dict(dtype=torch.float32)
+    return (dy.new_empty(dy.shape), dy.new_empty(dy.shape if residual_kind else (0,), dtype=rdt),
+            weight.new_empty(weight.shape, **f32), weight.new_empty(weight.shape if has_bias else (0,), **f32))
 
 
 def layer_norm_fn(x, weight, bias=None, residual=None, eps=1e-5, prenorm=False, residual_in_fp32=False,
@@ -46,28 +49,19 @@ def layer_norm_fn(x, weight, bias=None, residual=None, eps=1e-5, prenorm=False, 
     """
     if x.device.type != "cuda":
         raise ValueError(f"mamba_cpu (MI355X build) runs on ROCm GPU tensors, got device {x.device}")
-    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
-        raise ValueError(f"layer_norm_fn expects x (..., dim) and weight (dim,), got {tuple(x.shape)} and "
-                         f"{tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape:
-        raise ValueError(f"bias must have weight's shape {tuple(weight.shape)}, got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-    dim, in_dtype, res = x.shape[-1], x.dtype, residual
-    rows = x.numel() // dim if dim else 0
-    xr = (x if in_dtype in _X_DTYPES else x.float()).reshape(rows, dim)
-    if res is not None:
-        res = (res if res.dtype == xr.dtype else res.float()).reshape(rows, dim)
-    wide = residual_in_fp32 and xr.dtype != torch.float32
+    in_dtype, res = x.dtype, residual
+    if in_dtype not in _X_DTYPES:
+        x = x.float()
+    if res is not None and res.dtype != x.dtype and res.dtype != torch.float32:
+        res = res.float()
+    wide = residual_in_fp32 and x.dtype != torch.float32
     want = prenorm and (res is not None or wide)
-    y, z, _, _ = torch.ops.mamba_cpu.norm_fwd(
-        xr, weight.float().contiguous(), None if bias is None else bias.float().contiguous(), res, float(eps),
-        bool(is_rms_norm), want, bool(wide))
-    y = y.view(x.shape).to(in_dtype)
+    # The operator takes any leading dimensions and casts the parameters
+    # itself: the common call is one dispatch.
+    y, z, _, _ = torch.ops.mamba_cpu.norm_fwd(x, weight, bias, res, eps, is_rms_norm, want, wide)
+    y = y.to(in_dtype)
     if not prenorm:
         return y
     if not want:
         return y, x
-    return y, z.view(x.shape).to(z.dtype if residual is None else residual.dtype)
+    return y, z if residual is None else z.to(residual.dtype)
