@@ -16,19 +16,34 @@ bool any_negative(std::initializer_list<const int64_t*> strides, int n) {
   return false;
 }
 
+int64_t chunks_of(const mcpu_gated_scan_args* a) { return (a->seqlen + kGatedChunk - 1) / kGatedChunk; }
+
+// The kernels reach an element by 32-bit byte offsets from a segment's first step.
+bool in_reach(const mcpu_gated_scan_args* a, std::initializer_list<const int64_t*> strides) {
+  constexpr int64_t kReach = int64_t{1} << 32;
+  for (const int64_t* s : strides)
+    if (s[2] >= kReach / (dtype_size(a->dtype) * (a->dim > 0 ? a->dim : 1)) ||
+        s[1] >= kReach / (dtype_size(a->dtype) * kGatedT))
+      return false;
+  return true;
+}
+
 int check_gated(const mcpu_gated_scan_args* a, const char* what) {
   if (a == nullptr) return fail(MCPU_ERR_INVALID, "%s: null argument block", what);
   if (a->batch < 0 || a->seqlen < 0 || a->dim < 0) return fail(MCPU_ERR_INVALID, "%s: negative size", what);
   if (!valid_dtype(a->dtype)) return fail(MCPU_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
-  // The grid is at most a workgroup per 64 channels, row and time split, and rows are split only below 1024.
-  if (a->batch * ((a->dim + 63) / 64) > INT_MAX / 2)
-    return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x dim too large", what);
+  const int64_t tiles = (a->dim + 63) / 64;
+  if (a->batch > INT_MAX || a->seqlen > (int64_t{1} << 40) || tiles > INT_MAX ||
+      (tiles > 0 && a->batch > 0 && chunks_of(a) > INT_MAX / (tiles * a->batch)))
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x seqlen x dim too large", what);
   if ((a->decay == nullptr && a->dim > 0) ||
       ((a->x == nullptr || a->a_gate == nullptr || a->x_gate == nullptr) && a->batch * a->seqlen * a->dim > 0))
     return fail(MCPU_ERR_INVALID, "%s: x, a_gate, x_gate and decay are required", what);
   if (!(a->c >= 0.f)) return fail(MCPU_ERR_INVALID, "%s: c must not be negative", what);
   if (any_negative({a->x_stride, a->a_stride, a->i_stride}, 3))
     return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
+  if (!in_reach(a, {a->x_stride, a->a_stride, a->i_stride}))
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: a row's steps or channels lie too far apart", what);
   return MCPU_OK;
 }
 
@@ -38,34 +53,28 @@ bool pairs(const void* ptr, const int64_t (&s)[3]) {
   return ptr == nullptr || (s[2] == 1 && s[0] % 2 == 0 && s[1] % 2 == 0 && reinterpret_cast<uintptr_t>(ptr) % 4 == 0);
 }
 
-// Channels per lane: two of a 16-bit type where every operand allows, so that
-// a lane moves four bytes.
-int gated_vec(const mcpu_gated_scan_args* a, bool bwd) {
-  if (a->dtype == MCPU_F32 || a->dim % 2 != 0 || !pairs(a->x, a->x_stride) || !pairs(a->a_gate, a->a_stride) ||
-      !pairs(a->x_gate, a->i_stride))
-    return 1;
-  if (!bwd) return pairs(a->y, a->y_stride) ? 2 : 1;
-  return pairs(a->dy, a->dy_stride) && pairs(a->dx, a->dx_stride) && pairs(a->da_gate, a->da_stride) &&
-                 pairs(a->dx_gate, a->di_stride)
+// Channels per lane of the forward: two of a 16-bit type where every operand
+// allows, so that a lane moves four bytes. The backward holds five numbers a
+// step and channel between its two halves: with two channels a lane it spills
+// at two workgroups a CU (165 against 124 us for 8 x 2048 x 1536).
+int gated_vec(const mcpu_gated_scan_args* a) {
+  return a->dtype != MCPU_F32 && a->dim % 2 == 0 && pairs(a->x, a->x_stride) && pairs(a->a_gate, a->a_stride) &&
+                 pairs(a->x_gate, a->i_stride) && pairs(a->y, a->y_stride)
              ? 2
              : 1;
 }
 
-// Time splits at most, over both widths: what the workspaces are sized for.
-int64_t most_splits(const mcpu_gated_scan_args* a) {
-  GatedScanParams p;
-  std::memset(&p, 0, sizeof(p));
-  p.batch = a->batch;
-  p.len = a->seqlen;
-  p.dim = a->dim;
-  gated_scan_plan(p, 1);
-  const int64_t n = p.nsplit;
-  gated_scan_plan(p, 2);
-  return n > p.nsplit ? n : p.nsplit;
+// The tickets and records of a call of more than one chunk.
+size_t ticket_bytes(const mcpu_gated_scan_args* a) {
+  return align_up(sizeof(uint32_t) * a->batch * ((a->dim + 63) / 64));
 }
-size_t sums_bytes(const mcpu_gated_scan_args* a) {
-  const int64_t n = most_splits(a);
-  return n > 1 ? align_up(sizeof(float2) * a->batch * n * a->dim) : 0;
+size_t record_bytes(const mcpu_gated_scan_args* a) {
+  return chunks_of(a) > 1 ? ticket_bytes(a) + align_up(sizeof(uint64_t) * a->batch * chunks_of(a) * a->dim) : 0;
+}
+int clear_records(GatedScanParams& p, const mcpu_gated_scan_args* a, void* workspace, hipStream_t st) {
+  p.tickets = static_cast<uint32_t*>(workspace);
+  p.records = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + ticket_bytes(a));
+  return zero_f32(static_cast<float*>(workspace), static_cast<int64_t>(record_bytes(a) / sizeof(float)), st);
 }
 
 GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
@@ -81,6 +90,7 @@ GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
   p.len = a->seqlen;
   p.dim = a->dim;
   p.c = a->c;
+  p.chunks = chunks_of(a);
   p.ckpt = a->ckpt;
   for (int i = 0; i < 3; ++i) {
     p.sx[i] = a->x_stride[i];
@@ -113,7 +123,7 @@ extern "C" size_t mcpu_gated_scan_fwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return sums_bytes(a);
+  return record_bytes(a);
 }
 
 extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -124,15 +134,23 @@ extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspac
   if (a->y == nullptr && a->batch * a->seqlen * a->dim > 0)
     return fail(MCPU_ERR_INVALID, "%s: y is required", what);
   if (any_negative({a->y_stride}, 3)) return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
+  if (!in_reach(a, {a->y_stride}))
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: a row's steps or channels lie too far apart", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_gated_scan_fwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   GatedScanParams p = make_gated(a);
   p.y = a->y;
   p.last = a->last_state;
-  p.sums = static_cast<float2*>(workspace);
   if (a->batch == 0 || a->dim == 0) return MCPU_OK;
-  gated_scan_plan(p, gated_vec(a, false));
-  return hip_status(gated_scan_fwd_launch(p, a->dtype, static_cast<hipStream_t>(stream)), "gated_scan_fwd launch");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a->seqlen == 0)
+    return a->last_state == nullptr
+               ? MCPU_OK
+               : hip_status(gated_edge_launch(a->initial_state, a->last_state, a->batch * a->dim, st), what);
+  p.vec = gated_vec(a);
+  if (p.chunks > 1)
+    if (int rc = clear_records(p, a, workspace, st)) return rc;
+  return hip_status(gated_scan_fwd_launch(p, a->dtype, st), "gated_scan_fwd launch");
 }
 
 extern "C" size_t mcpu_gated_scan_bwd_workspace_size(const mcpu_gated_scan_args* a) {
@@ -140,7 +158,7 @@ extern "C" size_t mcpu_gated_scan_bwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return sums_bytes(a) + align_up(sizeof(float) * a->batch * most_splits(a) * a->dim);
+  return record_bytes(a) + align_up(sizeof(float) * a->batch * chunks_of(a) * a->dim);
 }
 
 extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -156,11 +174,18 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
     return fail(MCPU_ERR_INVALID, "%s: the states the forward kept (ckpt) are required", what);
   if (any_negative({a->dy_stride, a->dx_stride, a->da_stride, a->di_stride}, 3))
     return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
+  if (!in_reach(a, {a->dy_stride, a->dx_stride, a->da_stride, a->di_stride}))
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: a row's steps or channels lie too far apart", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_gated_scan_bwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->dim == 0) return MCPU_OK;
-  if (a->batch == 0) return zero_f32(a->ddecay, a->dim, st);
+  if (a->batch == 0 || a->seqlen == 0) {
+    if (int rc = zero_f32(a->ddecay, a->dim, st)) return rc;
+    return a->batch == 0 || a->dinitial_state == nullptr
+               ? MCPU_OK
+               : hip_status(gated_edge_launch(a->dlast_state, a->dinitial_state, a->batch * a->dim, st), what);
+  }
   GatedScanParams p = make_gated(a);
   p.dy = a->dy;
   p.dlast = a->dlast_state;
@@ -169,9 +194,9 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
   p.dx_gate = a->dx_gate;
   p.ddecay = a->ddecay;
   p.dinit = a->dinitial_state;
-  p.sums = static_cast<float2*>(workspace);
-  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(a));
-  gated_scan_plan(p, gated_vec(a, true));
+  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + record_bytes(a));
+  if (p.chunks > 1)
+    if (int rc = clear_records(p, a, workspace, st)) return rc;
   return hip_status(gated_scan_bwd_launch(p, a->dtype, st), "gated_scan_bwd launch");
 }
 

@@ -10,7 +10,7 @@ namespace mcpu {
 
 constexpr int kGatedT = 8;      // steps per wave segment: the forward keeps the state before each
 constexpr int kGatedWaves = 8;  // waves of a workgroup, one segment each
-constexpr int kGatedChunk = kGatedT * kGatedWaves;
+constexpr int kGatedChunk = kGatedT * kGatedWaves;  // steps of a workgroup
 
 struct GatedScanParams {
   const void* x;
@@ -28,12 +28,15 @@ struct GatedScanParams {
   void* da_gate;
   void* dx_gate;
   float* ddecay;
-  float* ddecay_part;  // (batch, nsplit, dim) partial sums over time
-  float2* sums;        // (batch, nsplit, dim): each split's step as a whole
+  float* ddecay_part;  // (batch, chunks, dim) partial sums over time
+  // Zeroed before the launch, with more than one chunk: the tickets handed out
+  // for each tile of each row, and (batch, chunks, dim) what a chunk has published.
+  uint32_t* tickets;
+  uint64_t* records;
   float* dinit;
   int64_t batch, len, dim;
-  int64_t nsplit, split_len;  // time splits, split_len steps each: whole chunks
-  int vec;                    // channels per lane
+  int64_t chunks;
+  int vec;  // channels per lane
   float c;
   int64_t sx[3], sa[3], si[3], sy[3], sdy[3], sdx[3], sda[3], sdi[3];  // (batch, len, dim)
 };
@@ -52,10 +55,9 @@ struct GatedStepParams {
   int64_t state_batch;
 };
 
-// Fills in the launch shape: vec (as the operands allow) and the time splits.
-void gated_scan_plan(GatedScanParams& p, int vec);
 hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
 hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
+hipError_t gated_edge_launch(const float* from, float* to, int64_t n, hipStream_t st);
 hipError_t gated_step_launch(const GatedStepParams& p, int dtype, hipStream_t st);
 
 }  // namespace mcpu

@@ -9,15 +9,25 @@
 // The step h -> a h + b composes as (P, S): h -> P h + S, so time is split: a
 // wave takes kGatedT consecutive steps of its channels in registers and forms
 // their (P, S), the workgroup's waves exchange theirs through LDS, and each
-// wave then knows the state in front of its segment. A lane holds `vec`
-// neighbouring channels (4 bytes where the operands allow), so that a wave
-// reads 256 bytes of a row at once.
+// wave then knows the state in front of its segment, given the one in front of
+// the workgroup's chunk. A lane holds `vec` neighbouring channels (4 bytes where
+// the operands allow), so that a wave reads 256 bytes of a row at once.
 //
-// Where the channels alone do not fill the chip, a row's steps are split over
-// workgroups too: a first launch forms the (P, S) of every split but the last,
-// the second starts each split from the composition of those before it. It
-// reads the inputs twice; a single launch of few workgroups is slower (the
-// rule and both sides: gated_scan_plan).
+// A workgroup takes one chunk of 64 steps of 64 vec channels, so that every
+// length fills the chip and every input is read once. The state in front of a
+// chunk comes from the chunks before it: a workgroup publishes its (P, S) as
+// soon as it has them (its inputs stay in registers), then looks back, a
+// predecessor per wave, until nothing older matters: a predecessor that knows the state behind its chunk has published that, as
+// (0, h), in the place of its (P, S). Its own (0, h) is published before its
+// outputs are written.
+// Every wait ends: the chunks of a row's tile are taken by ticket, in the order
+// of time, so the chunks a workgroup waits for have been taken by workgroups
+// that run or have ended, and a workgroup publishes its (P, S) before it waits.
+// Records pass between workgroups as single 64-bit words, written by agent-scope
+// atomic stores and polled by agent-scope atomic loads; a word carries all that
+// is read, and either of a chunk's two is right, so no fence is needed. Two launches, the first for
+// each split's (P, S), read the inputs twice: forward + backward of
+// 8 x 2048 x 1536 bf16 took 221 us that way, @GLS1@ us this way.
 //
 // Backward, with g_t = dL/dh_t:  g_t = dy_t + k_{t+1} a_{t+1} g_{t+1},
 //   dx = g m iota          dx_gate = dx x (1 - iota)
@@ -96,371 +106,406 @@ __device__ __forceinline__ float input_share(float s, float a) {
 
 struct Place {
   int lane, w;
-  int64_t b, split, d;  // first channel of the lane
-  int64_t t0, t1;       // steps of the split
+  int64_t b, chunk, d;  // d: first channel of the lane
+  int64_t t0;           // first step of the chunk
+  int64_t ts;           // first step of the wave's segment
+  int n;                // steps of the segment
   bool live;
-  int64_t dd;           // d, or 0 for lanes beyond the last channel
+  int64_t dd;           // d, or the tile's first channel for lanes beyond the last
 };
-template <int VC> __device__ __forceinline__ Place place(const GatedScanParams& p, int64_t splits) {
+// Which chunk of its row's tile the workgroup takes: the next one in the order of
+// time, from the last on with LAST_FIRST. A counter for each tile: 3072
+// workgroups at one counter wait 1.4 us each, with a burst of 5 at the start.
+template <int VC, bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
+  __shared__ uint32_t ticket;
   Place q;
   q.lane = threadIdx.x & 63;
   q.w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tiles = (p.dim + 64 * VC - 1) / (64 * VC);
-  const int64_t row = blockIdx.x / tiles;
-  q.b = row / splits;
-  q.split = row % splits;
-  q.d = ((blockIdx.x % tiles) * 64 + q.lane) * VC;
+  const uint32_t tiles = static_cast<uint32_t>((p.dim + 64 * VC - 1) / (64 * VC));
+  const uint32_t rows = tiles * static_cast<uint32_t>(p.batch), row = blockIdx.x % rows;
+  uint32_t t = 0;
+  if (p.chunks > 1) {
+    if (threadIdx.x == 0) ticket = atomicAdd(p.tickets + row, 1u);
+    __syncthreads();
+    t = __builtin_amdgcn_readfirstlane(ticket);
+  }
+  q.chunk = LAST_FIRST ? p.chunks - 1 - t : t;
+  q.b = row / tiles;
+  const int64_t first = row % tiles * 64ll * VC;
+  q.d = first + q.lane * VC;
   q.live = q.d < p.dim;
-  q.dd = q.live ? q.d : 0;
-  q.t0 = q.split * p.split_len;
-  q.t1 = q.t0 + p.split_len < p.len ? q.t0 + p.split_len : p.len;
+  q.dd = q.live ? q.d : first;
+  q.t0 = q.chunk * kGatedChunk;
+  q.ts = q.t0 + q.w * TS;
+  const int64_t left = p.len - q.ts;
+  q.n = left < 0 ? 0 : left < TS ? static_cast<int>(left) : TS;
   return q;
 }
 
+// The wave's segment of an operand: a scalar base, the lane's byte offset, and
+// a scalar offset per step. Steps behind the row's end read its last one.
 template <typename T, int VC> struct Column {
-  const char* base;
-  int64_t step;
-  __device__ __forceinline__ Column(const void* ptr, const int64_t (&s)[3], const Place& q)
-      : base(static_cast<const char*>(ptr) + (q.b * s[0] + q.dd * s[2]) * static_cast<int64_t>(sizeof(T))),
-        step(s[1] * static_cast<int64_t>(sizeof(T))) {}
-  __device__ __forceinline__ Word<T, VC> load(int64_t t) const {
-    return *reinterpret_cast<const Word<T, VC>*>(base + t * step);
+  __amdgpu_buffer_rsrc_t rsrc;
+  uint32_t lane, step;
+  __device__ __forceinline__ Column(const void* ptr, const int64_t (&s)[3], const GatedScanParams& p, const Place& q)
+      : rsrc(wave_rsrc(static_cast<const char*>(ptr) +
+                       (q.b * s[0] + (q.n > 0 ? q.ts : p.len - 1) * s[1]) * static_cast<int64_t>(sizeof(T)))),
+        lane(static_cast<uint32_t>(q.dd * s[2] * static_cast<int64_t>(sizeof(T)))),
+        step(static_cast<uint32_t>(s[1] * static_cast<int64_t>(sizeof(T)))) {}
+  __device__ __forceinline__ Word<T, VC> load(const Place& q, int i) const {
+    const int at = i < q.n ? i : q.n > 0 ? q.n - 1 : 0;
+    if constexpr (sizeof(T) * VC == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, lane, at * step, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b16(rsrc, lane, at * step, 0);
   }
-  __device__ __forceinline__ void store(int64_t t, const float (&v)[VC]) const {
-    *reinterpret_cast<Word<T, VC>*>(const_cast<char*>(base) + t * step) = narrow<T, VC>(v);
+  __device__ __forceinline__ void store(int i, const float (&v)[VC]) const {
+    if constexpr (sizeof(T) * VC == 4)
+      __builtin_amdgcn_raw_buffer_store_b32(narrow<T, VC>(v), rsrc, lane, i * step, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b16(narrow<T, VC>(v), rsrc, lane, i * step, 0);
   }
 };
 
 // Bit i: step ts + i starts another sequence than the step before it.
-__device__ __forceinline__ uint64_t starts(const GatedScanParams& p, const Place& q, int64_t ts) {
-  if (p.seq_idx == nullptr) return 0;
-  const int64_t t = ts + q.lane;
+__device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place& q) {
+  const int64_t t = q.ts + q.lane;
   const int32_t* ids = p.seq_idx + q.b * p.len;
   bool s = false;
   if (q.lane < TS && t > 0 && t < p.len) s = ids[t] != ids[t - 1];
-  return __ballot(s);
+  return static_cast<uint32_t>(__ballot(s));
+}
+
+// ---- steps and what is published of them --------------------------------------------------
+
+// P h + S; nothing of h where P is 0, a NaN or an infinity neither.
+__device__ __forceinline__ float after(float P, float S, float h) { return P == 0.f ? S : fmaf(P, h, S); }
+
+// A record is (P, S) with every bit flipped, so that zeroed memory, the flipped
+// all-ones NaN pair, means none yet; a NaN is published as another one.
+__device__ __forceinline__ uint32_t plain(float x) { return x == x ? __builtin_bit_cast(uint32_t, x) : 0x7fc00000u; }
+__device__ __forceinline__ void publish(uint64_t* at, float P, float S) {
+  const uint64_t v = ~(static_cast<uint64_t>(plain(P)) << 32 | plain(S));
+  __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+constexpr int kWindows = 4;  // windows of W chunks that are kept
+template <int VC> struct Exchange {
+  float2 agg[W][64 * VC];                // the segments' (P, S)
+  float2 win[kWindows + 2][W][64 * VC];  // what the waves found of W neighbouring chunks; two for those further back
+};
+
+// The state that enters the wave's segment, from the segments' (P, S) and
+// `edge`, the state that enters the row's first chunk (in the direction of the
+// scan: DIR 1 forward, -1 backward). `out` is the state behind the chunk.
+template <int VC, int DIR>
+__device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Place& q, Exchange<VC>& x,
+                                            const float (&P)[VC], const float (&S)[VC], const float (&edge)[VC],
+                                            float (&in)[VC], float (&out)[VC]) {
+#pragma unroll
+  for (int v = 0; v < VC; ++v) x.agg[q.w][v * 64 + q.lane] = make_float2(P[v], S[v]);
+  __syncthreads();
+  // The segments before this one, and the whole chunk.
+  float mineP[VC], mineS[VC], allP[VC], allS[VC];
+#pragma unroll
+  for (int v = 0; v < VC; ++v) {
+    allP[v] = 1.f;
+    allS[v] = 0.f;
+#pragma unroll
+    for (int o = 0; o < W; ++o) {
+      const int seg = DIR > 0 ? o : W - 1 - o;
+      if (seg == q.w) {
+        mineP[v] = allP[v];
+        mineS[v] = allS[v];
+      }
+      const float2 s = x.agg[seg][v * 64 + q.lane];
+      allS[v] = after(s.x, s.y, allS[v]);
+      allP[v] *= s.x;
+    }
+  }
+  const int64_t first = DIR > 0 ? 0 : p.chunks - 1;
+  const int64_t back = DIR * (q.chunk - first);  // chunks before this one
+  uint64_t* const rec = p.records + q.b * p.chunks * p.dim + q.dd;
+  float state[VC];
+#pragma unroll
+  for (int v = 0; v < VC; ++v) state[v] = edge[v];
+  if (back > 0) {
+    if (q.w == 0 && q.live) {
+#pragma unroll
+      for (int v = 0; v < VC; ++v) publish(rec + q.chunk * p.dim + v, allP[v], allS[v]);
+    }
+    auto slot = [](int64_t win) { return win < kWindows ? static_cast<int>(win) : kWindows + static_cast<int>(win & 1); };
+    // This wave's chunk of a window, as published.
+    auto fetch = [&](int64_t win) {
+      const int64_t away = win * W + q.w + 1;  // how far back the chunk is
+      float pP[VC], pS[VC];
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {  // in front of the row's first chunk: the edge, then nothing
+        pP[v] = away == back + 1 ? 0.f : 1.f;
+        pS[v] = away == back + 1 ? edge[v] : 0.f;
+      }
+      if (away <= back) {
+        const uint64_t* at = rec + (q.chunk - DIR * away) * p.dim;
+        for (;;) {
+          bool have = true;
+#pragma unroll
+          for (int v = 0; v < VC; ++v) {
+            const uint64_t word = peek(at + v), r = ~word;
+            have &= word != 0;
+            pP[v] = __builtin_bit_cast(float, static_cast<uint32_t>(r >> 32));
+            pS[v] = __builtin_bit_cast(float, static_cast<uint32_t>(r));
+          }
+          if (__ballot(!have) == 0) break;
+          __builtin_amdgcn_s_sleep(1);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < VC; ++v) x.win[slot(win)][q.w][v * 64 + q.lane] = make_float2(pP[v], pS[v]);
+      __syncthreads();
+    };
+    // Back until every channel has met a chunk that does not depend on older ones.
+    bool known[VC] = {};
+    int64_t win = 0;
+    for (;; ++win) {
+      fetch(win);
+      bool all = true;
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+#pragma unroll
+        for (int o = 0; o < W; ++o) known[v] |= x.win[slot(win)][o][v * 64 + q.lane].x == 0.f;
+        all &= known[v];
+      }
+      // All waves read the same values, so all leave together.
+      if (__ballot(!all) == 0 || (win + 1) * W > back) break;
+    }
+    // Then forward again, one chunk after the other: the state behind chunk j is
+    // always after(P_j, S_j, the state in front of it), whether another
+    // workgroup formed it or this one, so that the result does not depend on
+    // what had been published when. Windows further back than those kept are
+    // read again, except the last.
+#pragma unroll
+    for (int v = 0; v < VC; ++v) state[v] = 0.f;
+    for (int64_t w = win; w >= 0; --w) {
+      if (w >= kWindows && w < win) fetch(w);
+#pragma unroll
+      for (int v = 0; v < VC; ++v)
+#pragma unroll
+        for (int o = W - 1; o >= 0; --o) {
+          const float2 s = x.win[slot(w)][o][v * 64 + q.lane];
+          state[v] = after(s.x, s.y, state[v]);
+        }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VC; ++v) {
+    in[v] = after(mineP[v], mineS[v], state[v]);
+    out[v] = after(allP[v], allS[v], state[v]);
+  }
+  if (p.chunks > 1 && back < p.chunks - 1 && q.w == 0 && q.live) {
+#pragma unroll
+    for (int v = 0; v < VC; ++v) publish(rec + q.chunk * p.dim + v, 0.f, out[v]);
+  }
 }
 
 // ---- forward -----------------------------------------------------------------------------
-// SUM: the split's (P, S) only, for the splits that others start from.
+// SEQ: packed sequences.
 
-template <typename T, int VC, bool SUM>
+template <typename T, int VC, bool SEQ>
 __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams p) {
-  const Place q = place<VC>(p, SUM ? p.nsplit - 1 : p.nsplit);
-  const Column<T, VC> x(p.x, p.sx, q), ag(p.a_gate, p.sa, q), ig(p.x_gate, p.si, q), y(p.y, p.sy, q);
-  const int64_t nseg = (p.len + TS - 1) / TS;
-  __shared__ float2 agg[2][W][64 * VC];
-  float csp[VC], carry[VC], run[VC];  // run: the product of the decays so far (SUM)
+  __shared__ Exchange<VC> exchange;
+  const Place q = place<VC, false>(p);
+  const Column<T, VC> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), y(p.y, p.sy, p, q);
+  Word<T, VC> rx[TS], ra[TS], ri[TS];
+#pragma unroll
+  for (int i = 0; i < TS; ++i) {
+    ra[i] = ag.load(q, i);
+    ri[i] = ig.load(q, i);
+    rx[i] = x.load(q, i);
+  }
+  const uint32_t cut = SEQ ? starts(p, q) : 0;
+  float csp[VC], edge[VC], P[VC], S[VC], a[TS][VC], u[TS][VC];
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
     csp[v] = p.c * softplus_acc(p.decay[q.dd + v]);
-    carry[v] = SUM || p.init == nullptr ? 0.f : p.init[q.b * p.dim + q.dd + v];
-    run[v] = 1.f;
+    edge[v] = p.init == nullptr ? 0.f : p.init[q.b * p.dim + q.dd + v];
+    P[v] = 1.f;
+    S[v] = 0.f;
   }
-  if constexpr (!SUM) {
-    for (int64_t sp = 0; sp < q.split; ++sp)
 #pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        const float2 s = p.sums[(q.b * p.nsplit + sp) * p.dim + q.dd + v];
-        carry[v] = fmaf(s.x, carry[v], s.y);
-      }
-  }
-  Word<T, VC> rx[TS], ra[TS], ri[TS];
-  auto fetch = [&](int64_t ts) {
-#pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      const int64_t t = ts + i < q.t1 ? ts + i : q.t1 - 1;
-      ra[i] = ag.load(t);
-      ri[i] = ig.load(t);
-      rx[i] = x.load(t);
-    }
-  };
-  int buf = 0;
-  if (q.t0 < q.t1) fetch(q.t0 + q.w * TS);
-  for (int64_t t0 = q.t0; t0 < q.t1; t0 += kGatedChunk, buf ^= 1) {
-    const int64_t ts = t0 + q.w * TS;
-    const int n = static_cast<int>(q.t1 - ts < 0 ? 0 : q.t1 - ts < TS ? q.t1 - ts : TS);
-    const uint64_t cut = starts(p, q, ts);
-    float a[TS][VC], u[TS][VC], P[VC], S[VC];
+  for (int i = 0; i < TS; ++i) {
+    float fx[VC], fa[VC], fi[VC];
+    widen<T, VC>(rx[i], fx);
+    widen<T, VC>(ra[i], fa);
+    widen<T, VC>(ri[i], fi);
+    const bool restart = SEQ && ((cut >> i) & 1) != 0;
 #pragma unroll
     for (int v = 0; v < VC; ++v) {
-      P[v] = 1.f;
-      S[v] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      float fx[VC], fa[VC], fi[VC];
-      widen<T, VC>(rx[i], fx);
-      widen<T, VC>(ra[i], fa);
-      widen<T, VC>(ri[i], fi);
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        float e;
-        const float s = csp[v] * gate(fa[v], e);
-        const float dec = fast_exp(-s);
-        const float m = __builtin_amdgcn_sqrtf(input_share(s, dec));
-        a[i][v] = i < n ? (((cut >> i) & 1) != 0 ? 0.f : dec) : 1.f;
-        u[i][v] = i < n ? m * gate(fi[v], e) * fx[v] : 0.f;
-        S[v] = fmaf(a[i][v], S[v], u[i][v]);
-        P[v] *= a[i][v];
-      }
-    }
-    if (t0 + kGatedChunk < q.t1) fetch(ts + kGatedChunk);
-#pragma unroll
-    for (int v = 0; v < VC; ++v) agg[buf][q.w][v * 64 + q.lane] = make_float2(P[v], S[v]);
-    __syncthreads();
-    float h[VC];
-#pragma unroll
-    for (int v = 0; v < VC; ++v) h[v] = carry[v];
-#pragma unroll
-    for (int o = 0; o < W; ++o)
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        if (o == q.w) h[v] = carry[v];
-        const float2 s = agg[buf][o][v * 64 + q.lane];
-        carry[v] = fmaf(s.x, carry[v], s.y);
-        if constexpr (SUM) run[v] *= s.x;
-      }
-    if constexpr (!SUM) {
-      if (q.live && n > 0) {
-        if (p.ckpt != nullptr) {
-          float* to = p.ckpt + (q.b * nseg + ts / TS) * p.dim + q.d;
-#pragma unroll
-          for (int v = 0; v < VC; ++v) to[v] = h[v];
-        }
-#pragma unroll
-        for (int i = 0; i < TS; ++i) {
-#pragma unroll
-          for (int v = 0; v < VC; ++v) h[v] = fmaf(a[i][v], h[v], u[i][v]);
-          if (i < n) y.store(ts + i, h);
-        }
-      }
+      float e;
+      const float s = csp[v] * gate(fa[v], e);
+      const float dec = fast_exp(-s);
+      const float m = __builtin_amdgcn_sqrtf(input_share(s, dec));
+      a[i][v] = i < q.n ? (restart ? 0.f : dec) : 1.f;
+      u[i][v] = i < q.n ? m * gate(fi[v], e) * fx[v] : 0.f;
+      S[v] = restart ? u[i][v] : fmaf(a[i][v], S[v], u[i][v]);
+      P[v] *= a[i][v];
     }
   }
-  if (q.live && q.w == 0) {
+  float h[VC], out[VC];
+  scan_chunks<VC, 1>(p, q, exchange, P, S, edge, h, out);
+  if (!q.live) return;
+  if (q.w == 0 && q.chunk == p.chunks - 1 && p.last != nullptr)
 #pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      if constexpr (SUM) p.sums[(q.b * p.nsplit + q.split) * p.dim + q.d + v] = make_float2(run[v], carry[v]);
-      else if (p.last != nullptr && q.split == p.nsplit - 1) p.last[q.b * p.dim + q.d + v] = carry[v];
-    }
+    for (int v = 0; v < VC; ++v) p.last[q.b * p.dim + q.d + v] = out[v];
+  if (q.n <= 0) return;
+  if (p.ckpt != nullptr) {
+    float* to = p.ckpt + (q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.d;
+#pragma unroll
+    for (int v = 0; v < VC; ++v) to[v] = h[v];
+  }
+#pragma unroll
+  for (int i = 0; i < TS; ++i) {
+    const bool restart = SEQ && ((cut >> i) & 1) != 0;
+#pragma unroll
+    for (int v = 0; v < VC; ++v) h[v] = restart ? u[i][v] : fmaf(a[i][v], h[v], u[i][v]);
+    if (i < q.n) y.store(i, h);
   }
 }
 
 // ---- backward ----------------------------------------------------------------------------
 
-// (P, S) of the gradient's step over a split, from its last step to its first,
-// for every split but the first. Its S is what leaves the split to the left
-// when nothing enters from the right.
-template <typename T, int VC>
-__global__ __launch_bounds__(64 * W) void gated_bwd_sum_kernel(const GatedScanParams p) {
-  Place q = place<VC>(p, p.nsplit - 1);
-  q.split += 1;
-  q.t0 = q.split * p.split_len;
-  q.t1 = q.t0 + p.split_len < p.len ? q.t0 + p.split_len : p.len;
-  const Column<T, VC> ag(p.a_gate, p.sa, q), dy(p.dy, p.sdy, q);
-  __shared__ float2 agg[2][W][64 * VC];
-  float csp[VC], carry[VC], run[VC];
-#pragma unroll
-  for (int v = 0; v < VC; ++v) {
-    csp[v] = p.c * softplus_acc(p.decay[q.dd + v]);
-    carry[v] = 0.f;
-    run[v] = 1.f;
-  }
-  int buf = 0;
-  const int64_t chunks = (q.t1 - q.t0 + kGatedChunk - 1) / kGatedChunk;
-  for (int64_t ch = chunks - 1; ch >= 0; --ch, buf ^= 1) {
-    const int64_t ts = q.t0 + ch * kGatedChunk + q.w * TS;
-    const int n = static_cast<int>(q.t1 - ts < 0 ? 0 : q.t1 - ts < TS ? q.t1 - ts : TS);
-    const uint64_t cut = starts(p, q, ts);
-    Word<T, VC> ra[TS], rd[TS];
-#pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      const int64_t t = ts + i < q.t1 ? ts + i : q.t1 - 1;
-      ra[i] = ag.load(t);
-      rd[i] = dy.load(t);
-    }
-    float P[VC], S[VC];
-#pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      P[v] = 1.f;
-      S[v] = 0.f;
-    }
-#pragma unroll
-    for (int i = TS - 1; i >= 0; --i) {
-      float fa[VC], fd[VC];
-      widen<T, VC>(ra[i], fa);
-      widen<T, VC>(rd[i], fd);
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        float e;
-        const float dec = fast_exp(-csp[v] * gate(fa[v], e));
-        const float ka = i < n ? (((cut >> i) & 1) != 0 ? 0.f : dec) : 1.f;
-        S[v] = ka * (S[v] + (i < n ? fd[v] : 0.f));
-        P[v] *= ka;
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < VC; ++v) agg[buf][q.w][v * 64 + q.lane] = make_float2(P[v], S[v]);
-    __syncthreads();
-#pragma unroll
-    for (int o = W - 1; o >= 0; --o)
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        const float2 s = agg[buf][o][v * 64 + q.lane];
-        carry[v] = fmaf(s.x, carry[v], s.y);
-        run[v] *= s.x;
-      }
-  }
-  if (q.live && q.w == 0)
-#pragma unroll
-    for (int v = 0; v < VC; ++v)
-      p.sums[(q.b * p.nsplit + q.split) * p.dim + q.d + v] = make_float2(run[v], carry[v]);
-}
-
-template <typename T, int VC>
+template <typename T, bool SEQ>
 __global__ __launch_bounds__(64 * W) void gated_bwd_kernel(const GatedScanParams p) {
-  // 1 - rho and 1 - iota to their own ulp are kept for float32 gradients; a
-  // 16-bit one does not show the difference to 1 minus the sigmoid.
   constexpr bool EXACT = sizeof(T) == 4;
-  const Place q = place<VC>(p, p.nsplit);
-  const Column<T, VC> x(p.x, p.sx, q), ag(p.a_gate, p.sa, q), ig(p.x_gate, p.si, q), dy(p.dy, p.sdy, q);
-  const Column<T, VC> dx(p.dx, p.sdx, q), da(p.da_gate, p.sda, q), di(p.dx_gate, p.sdi, q);
-  const int64_t nseg = (p.len + TS - 1) / TS;
-  __shared__ float2 agg[2][W][64 * VC];
-  float csp[VC], carry[VC], acc[VC];  // acc: this lane's sum of e rho
+  constexpr int VC = 1;
+  __shared__ Exchange<VC> exchange;
+  const Place q = place<VC, true>(p);
+  const Column<T, VC> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), dy(p.dy, p.sdy, p, q);
+  Word<T, VC> rx[TS], ra[TS], ri[TS], rd[TS];
+#pragma unroll
+  for (int i = 0; i < TS; ++i) {
+    ra[i] = ag.load(q, i);
+    rd[i] = dy.load(q, i);
+    ri[i] = ig.load(q, i);
+    rx[i] = x.load(q, i);
+  }
+  const uint32_t cut = SEQ ? starts(p, q) : 0;
+  float csp[VC], edge[VC], P[VC], S[VC], h[VC];
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
+    h[v] = q.n > 0 ? p.ckpt[(q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.dd + v] : 0.f;
     csp[v] = p.c * softplus_acc(p.decay[q.dd + v]);
-    carry[v] = p.dlast == nullptr ? 0.f : p.dlast[q.b * p.dim + q.dd + v];
-    acc[v] = 0.f;
+    edge[v] = p.dlast == nullptr ? 0.f : p.dlast[q.b * p.dim + q.dd + v];
+    P[v] = 1.f;
+    S[v] = 0.f;
   }
-  for (int64_t sp = p.nsplit - 1; sp > q.split; --sp)
+  // What a step's gradients are per unit of g: dx, dx_gate, da_gate, e rho; and k a.
+  float gx[TS][VC], gi[TS][VC], ga[TS][VC], gd[TS][VC], ka[TS][VC];
+#pragma unroll
+  for (int i = 0; i < TS; ++i) {
+    float fx[VC], fa[VC], fi[VC];
+    widen<T, VC>(rx[i], fx);
+    widen<T, VC>(ra[i], fa);
+    widen<T, VC>(ri[i], fi);
+    const bool restart = SEQ && ((cut >> i) & 1) != 0;
 #pragma unroll
     for (int v = 0; v < VC; ++v) {
-      const float2 s = p.sums[(q.b * p.nsplit + sp) * p.dim + q.dd + v];
-      carry[v] = fmaf(s.x, carry[v], s.y);
-    }
-  int buf = 0;
-  const int64_t chunks = q.t1 > q.t0 ? (q.t1 - q.t0 + kGatedChunk - 1) / kGatedChunk : 0;
-  for (int64_t ch = chunks - 1; ch >= 0; --ch, buf ^= 1) {
-    const int64_t ts = q.t0 + ch * kGatedChunk + q.w * TS;
-    const int n = static_cast<int>(q.t1 - ts < 0 ? 0 : q.t1 - ts < TS ? q.t1 - ts : TS);
-    const uint64_t cut = starts(p, q, ts);
-    Word<T, VC> rx[TS], ra[TS], ri[TS], rd[TS];
-    float h[VC];
-#pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      const int64_t t = ts + i < q.t1 ? ts + i : q.t1 - 1;
-      ra[i] = ag.load(t);
-      ri[i] = ig.load(t);
-      rx[i] = x.load(t);
-      rd[i] = dy.load(t);
-    }
-#pragma unroll
-    for (int v = 0; v < VC; ++v) h[v] = n > 0 ? p.ckpt[(q.b * nseg + ts / TS) * p.dim + q.dd + v] : 0.f;
-    float rho[TS][VC], iota[TS][VC], share[TS][VC], ka[TS][VC], kah[TS][VC];
-    float nrho[EXACT ? TS : 1][VC], niota[EXACT ? TS : 1][VC];
-    float P[VC], S[VC];
-#pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      P[v] = 1.f;
-      S[v] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      float fx[VC], fa[VC], fi[VC];
-      widen<T, VC>(rx[i], fx);
-      widen<T, VC>(ra[i], fa);
-      widen<T, VC>(ri[i], fi);
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        float ea, ei;
-        rho[i][v] = gate(fa[v], ea);
-        iota[i][v] = gate(fi[v], ei);
-        if constexpr (EXACT) {
-          nrho[i][v] = rest(ea, rho[i][v]);
-          niota[i][v] = rest(ei, iota[i][v]);
-        }
-        const float s = csp[v] * rho[i][v];
-        const float dec = fast_exp(-s);
-        share[i][v] = input_share(s, dec);
-        ka[i][v] = i < n ? (((cut >> i) & 1) != 0 ? 0.f : dec) : 1.f;
-        kah[i][v] = ka[i][v] * h[v];
-        h[v] = fmaf(__builtin_amdgcn_sqrtf(share[i][v]) * iota[i][v], fx[v], kah[i][v]);
-        P[v] *= ka[i][v];
-      }
-    }
-#pragma unroll
-    for (int i = TS - 1; i >= 0; --i) {
-      float fd[VC];
-      widen<T, VC>(rd[i], fd);
-#pragma unroll
-      for (int v = 0; v < VC; ++v) S[v] = ka[i][v] * (S[v] + (i < n ? fd[v] : 0.f));
-    }
-#pragma unroll
-    for (int v = 0; v < VC; ++v) agg[buf][q.w][v * 64 + q.lane] = make_float2(P[v], S[v]);
-    __syncthreads();
-    float G[VC];
-#pragma unroll
-    for (int v = 0; v < VC; ++v) G[v] = carry[v];
-#pragma unroll
-    for (int o = W - 1; o >= 0; --o)
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        if (o == q.w) G[v] = carry[v];
-        const float2 s = agg[buf][o][v * 64 + q.lane];
-        carry[v] = fmaf(s.x, carry[v], s.y);
-      }
-#pragma unroll
-    for (int i = TS - 1; i >= 0; --i) {
-      if (i >= n) continue;
-      float fx[VC], fd[VC], ox[VC], oa[VC], oi[VC];
-      widen<T, VC>(rx[i], fx);
-      widen<T, VC>(rd[i], fd);
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        const float g = fd[v] + G[v];
-        // 1 / m, cut above what the smallest normal q gives: a closed gate
-        // (q = 0) has m = 0, and a^2 s / m = 0, which is its limit.
-        const float inv = fminf(__builtin_amdgcn_rsqf(share[i][v]), 1e19f);
-        const float gi = g * iota[i][v];
-        ox[v] = gi * (share[i][v] * inv);
-        oi[v] = ox[v] * fx[v] * (EXACT ? niota[EXACT ? i : 0][v] : 1.0f - iota[i][v]);
-        const float e = fmaf(gi * fx[v], (1.0f - share[i][v]) * inv, -g * kah[i][v]);
-        oa[v] = e * (csp[v] * rho[i][v]) * (EXACT ? nrho[EXACT ? i : 0][v] : 1.0f - rho[i][v]);
-        acc[v] = fmaf(e, rho[i][v], acc[v]);
-        G[v] = ka[i][v] * g;
-      }
-      if (q.live) {
-        dx.store(ts + i, ox);
-        di.store(ts + i, oi);
-        da.store(ts + i, oa);
-      }
+      float ea, ei;
+      const float rho = gate(fa[v], ea), iota = gate(fi[v], ei);
+      // 1 minus a sigmoid to its own ulp for float32 gradients; a 16-bit one
+      // does not show the difference.
+      const float nrho = EXACT ? rest(ea, rho) : 1.0f - rho, niota = EXACT ? rest(ei, iota) : 1.0f - iota;
+      const float s = csp[v] * rho;
+      const float dec = fast_exp(-s);
+      const float share = input_share(s, dec);
+      // 1 / m, cut above what the smallest normal share gives: a closed gate
+      // (share = 0) has m = 0, and a^2 s / m = 0, which is its limit.
+      const float inv = fminf(__builtin_amdgcn_rsqf(share), 1e19f);
+      ka[i][v] = i < q.n ? (restart ? 0.f : dec) : 1.f;
+      const float kah = restart ? 0.f : ka[i][v] * h[v];
+      gx[i][v] = iota * (share * inv);
+      const float u = gx[i][v] * fx[v];
+      gi[i][v] = u * niota;
+      const float e = fmaf(iota * fx[v], (1.0f - share) * inv, -kah);
+      ga[i][v] = e * s * nrho;
+      gd[i][v] = e * rho;
+      h[v] = kah + u;
+      P[v] *= ka[i][v];
+      // These five are to be formed here: moved down to their use, their
+      // operands would be kept instead, in 239 registers, two waves a SIMD.
+      asm volatile("" : "+v"(gx[i][v]), "+v"(gi[i][v]), "+v"(ga[i][v]), "+v"(gd[i][v]), "+v"(ka[i][v]));
     }
   }
-  if (q.live && q.w == 0 && q.split == 0 && p.dinit != nullptr)
 #pragma unroll
-    for (int v = 0; v < VC; ++v) p.dinit[q.b * p.dim + q.d + v] = carry[v];
+  for (int i = TS - 1; i >= 0; --i) {
+    float fd[VC];
+    widen<T, VC>(rd[i], fd);
+    const bool restart = SEQ && ((cut >> i) & 1) != 0;
+#pragma unroll
+    for (int v = 0; v < VC; ++v) S[v] = restart ? 0.f : ka[i][v] * (S[v] + (i < q.n ? fd[v] : 0.f));
+  }
+  float G[VC], out[VC], acc[VC] = {};  // acc: this lane's sum of e rho
+  scan_chunks<VC, -1>(p, q, exchange, P, S, edge, G, out);
+  if (q.live && q.w == 0 && q.chunk == 0 && p.dinit != nullptr)
+#pragma unroll
+    for (int v = 0; v < VC; ++v) p.dinit[q.b * p.dim + q.d + v] = out[v];
+  const Column<T, VC> dx(p.dx, p.sdx, p, q), da(p.da_gate, p.sda, p, q), di(p.dx_gate, p.sdi, p, q);
+#pragma unroll
+  for (int i = TS - 1; i >= 0; --i) {
+    if (i >= q.n) continue;
+    float fd[VC], ox[VC], oa[VC], oi[VC];
+    widen<T, VC>(rd[i], fd);
+    const bool restart = SEQ && ((cut >> i) & 1) != 0;
+#pragma unroll
+    for (int v = 0; v < VC; ++v) {
+      const float g = fd[v] + G[v];
+      ox[v] = g * gx[i][v];
+      oi[v] = g * gi[i][v];
+      oa[v] = g * ga[i][v];
+      acc[v] = fmaf(g, gd[i][v], acc[v]);
+      G[v] = restart ? 0.f : ka[i][v] * g;
+    }
+    if (q.live) {
+      dx.store(i, ox);
+      di.store(i, oi);
+      da.store(i, oa);
+    }
+  }
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < VC; ++v) agg[0][q.w][v * 64 + q.lane].x = acc[v];
+  for (int v = 0; v < VC; ++v) exchange.agg[q.w][v * 64 + q.lane].x = acc[v];
   __syncthreads();
   if (q.w == 0 && q.live)
 #pragma unroll
     for (int v = 0; v < VC; ++v) {
       float sum = 0.f, e;
-      for (int o = 0; o < W; ++o) sum += agg[0][o][v * 64 + q.lane].x;
-      p.ddecay_part[(q.b * p.nsplit + q.split) * p.dim + q.d + v] = sum * p.c * gate(p.decay[q.d + v], e);
+      for (int o = 0; o < W; ++o) sum += exchange.agg[o][v * 64 + q.lane].x;
+      p.ddecay_part[(q.b * p.chunks + q.chunk) * p.dim + q.d + v] = sum * p.c * gate(p.decay[q.d + v], e);
     }
 }
 
-// ddecay: the partial sums of the batch rows and splits, added in order.
-__global__ __launch_bounds__(64) void gated_ddecay_kernel(const GatedScanParams p) {
-  const int64_t d = blockIdx.x * 64ll + threadIdx.x;
-  if (d >= p.dim) return;
+constexpr int kReduceWaves = 16;
+
+// No steps: the state that enters leaves.
+__global__ __launch_bounds__(256) void gated_edge_kernel(const float* from, float* to, int64_t n) {
+  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+  if (i < n) to[i] = from == nullptr ? 0.f : from[i];
+}
+
+// ddecay: every kReduceWaves-th partial sum by one wave, then the waves' in order.
+__global__ __launch_bounds__(64 * kReduceWaves) void gated_ddecay_kernel(const GatedScanParams p) {
+  __shared__ float sums[kReduceWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t d = blockIdx.x * 64ll + lane;
   float sum = 0.f;
+  if (d < p.dim) {
 #pragma unroll 8
-  for (int64_t k = 0; k < p.batch * p.nsplit; ++k) sum += p.ddecay_part[k * p.dim + d];
+    for (int64_t k = wave; k < p.batch * p.chunks; k += kReduceWaves) sum += p.ddecay_part[k * p.dim + d];
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (wave > 0 || d >= p.dim) return;
+  for (int v = 1; v < kReduceWaves; ++v) sum += sums[v][lane];
   p.ddecay[d] = sum;
 }
 
@@ -492,58 +537,38 @@ template <typename F> void by_dtype(int dtype, F&& f) {
   else f(f16{});
 }
 
-template <typename T, int VC> void launch_fwd(const GatedScanParams& p, hipStream_t st) {
-  const int64_t tiles = (p.dim + 64 * VC - 1) / (64 * VC);
-  if (p.nsplit > 1)
-    hipLaunchKernelGGL((gated_fwd_kernel<T, VC, true>), dim3(static_cast<unsigned>(tiles * p.batch * (p.nsplit - 1))),
-                       dim3(64 * W), 0, st, p);
-  hipLaunchKernelGGL((gated_fwd_kernel<T, VC, false>), dim3(static_cast<unsigned>(tiles * p.batch * p.nsplit)),
-                     dim3(64 * W), 0, st, p);
-}
-
-template <typename T, int VC> void launch_bwd(const GatedScanParams& p, hipStream_t st) {
-  const int64_t tiles = (p.dim + 64 * VC - 1) / (64 * VC);
-  if (p.nsplit > 1)
-    hipLaunchKernelGGL((gated_bwd_sum_kernel<T, VC>), dim3(static_cast<unsigned>(tiles * p.batch * (p.nsplit - 1))),
-                       dim3(64 * W), 0, st, p);
-  hipLaunchKernelGGL((gated_bwd_kernel<T, VC>), dim3(static_cast<unsigned>(tiles * p.batch * p.nsplit)), dim3(64 * W),
-                     0, st, p);
-}
-
 }  // namespace
 
-void gated_scan_plan(GatedScanParams& p, int vec) {
-  p.vec = vec;
-  const int64_t wgs = (p.dim + 64 * vec - 1) / (64 * vec) * p.batch;
-  const int64_t chunks = (p.len + kGatedChunk - 1) / kGatedChunk;
-  int64_t n = wgs >= 400 || wgs < 1 ? 1 : (1024 + wgs - 1) / wgs;
-  if (n > chunks) n = chunks;
-  if (n < 1) n = 1;
-  const int64_t per = (chunks + n - 1) / n;  // chunks per split
-  p.split_len = (per < 1 ? 1 : per) * kGatedChunk;
-  p.nsplit = chunks < 1 ? 1 : (chunks + per - 1) / per;
+hipError_t gated_edge_launch(const float* from, float* to, int64_t n, hipStream_t st) {
+  hipLaunchKernelGGL(gated_edge_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, from, to, n);
+  return hipGetLastError();
 }
 
 hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
-  by_dtype(dtype, [&](auto t) {
+  auto launch = [&](auto t, auto vc) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2) {
-      if (p.vec == 2) return launch_fwd<T, 2>(p, st);
-    }
-    launch_fwd<T, 1>(p, st);
-  });
+    constexpr int VC = decltype(vc)::value;
+    const dim3 grid(static_cast<unsigned>((p.dim + 64 * VC - 1) / (64 * VC) * p.batch * p.chunks)), block(64 * W);
+    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, VC, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gated_fwd_kernel<T, VC, false>), grid, block, 0, st, p);
+  };
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  if (dtype == MCPU_F32) launch(float{}, one);
+  else if (dtype == MCPU_BF16) p.vec == 2 ? launch(bf16{}, two) : launch(bf16{}, one);
+  else p.vec == 2 ? launch(f16{}, two) : launch(f16{}, one);
   return hipGetLastError();
 }
 
 hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2) {
-      if (p.vec == 2) return launch_bwd<T, 2>(p, st);
-    }
-    launch_bwd<T, 1>(p, st);
+    const dim3 grid(static_cast<unsigned>((p.dim + 63) / 64 * p.batch * p.chunks)), block(64 * W);
+    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), grid, block, 0, st, p);
   });
-  hipLaunchKernelGGL(gated_ddecay_kernel, dim3(static_cast<unsigned>((p.dim + 63) / 64)), dim3(64), 0, st, p);
+  hipLaunchKernelGGL(gated_ddecay_kernel, dim3(static_cast<unsigned>((p.dim + 63) / 64)), dim3(64 * kReduceWaves), 0,
+                     st, p);
   return hipGetLastError();
 }
 

@@ -57,6 +57,13 @@ void check_gated(const char* name, const Tensor& x, const Tensor& a_gate, const 
                     name, " expects seq_idx as a contiguous int32 tensor of shape (batch, seqlen)");
 }
 
+// A (batch, seqlen, dim) operand within the kernels' reach (32-bit byte offsets
+// over a row's channels and eight of its steps), copied where it is not.
+Tensor in_reach(const Tensor& t) {
+  const int64_t reach = (int64_t{1} << 32) / t.element_size();
+  return t.stride(2) < reach / std::max<int64_t>(t.size(2), 1) && t.stride(1) < reach / 8 ? t : t.contiguous();
+}
+
 mcpu_gated_scan_args gated_args(const Tensor& x, const Tensor& a_gate, const Tensor& x_gate, const Tensor& decay,
                                 const optional<Tensor>& init, const optional<Tensor>& seq_idx, double c) {
   mcpu_gated_scan_args a;
@@ -78,12 +85,13 @@ mcpu_gated_scan_args gated_args(const Tensor& x, const Tensor& a_gate, const Ten
   return a;
 }
 
-std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd(const Tensor& x, const Tensor& a_gate, const Tensor& x_gate,
+std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd(const Tensor& x_in, const Tensor& a_in, const Tensor& i_in,
                                                   const Tensor& decay, const optional<Tensor>& init,
                                                   const optional<Tensor>& seq_idx, double c, bool save) {
   const char* name = "mamba_cpu::gated_scan_fwd";
-  check_gated(name, x, a_gate, x_gate, decay, init, seq_idx);
-  c10::DeviceGuard guard(x.device());
+  check_gated(name, x_in, a_in, i_in, decay, init, seq_idx);
+  c10::DeviceGuard guard(x_in.device());
+  const Tensor x = in_reach(x_in), a_gate = in_reach(a_in), x_gate = in_reach(i_in);
   Tensor y = at::empty(x.sizes(), x.options());
   Tensor last = at::empty({x.size(0), x.size(2)}, decay.options());
   mcpu_gated_scan_args a = gated_args(x, a_gate, x_gate, decay, init, seq_idx, c);
@@ -100,14 +108,16 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd(const Tensor& x, const Tensor&
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_scan_bwd(
-    const Tensor& dy, const optional<Tensor>& dlast, const Tensor& x, const Tensor& a_gate, const Tensor& x_gate,
+    const Tensor& dy_in, const optional<Tensor>& dlast, const Tensor& x_in, const Tensor& a_in, const Tensor& i_in,
     const Tensor& decay, const optional<Tensor>& init, const optional<Tensor>& seq_idx, double c,
     const Tensor& ckpt) {
   const char* name = "mamba_cpu::gated_scan_bwd";
-  check_gated(name, x, a_gate, x_gate, decay, init, seq_idx);
-  for (const optional<Tensor>& t : {opt(dy), dlast, opt(ckpt)}) check_gpu(name, t);
-  TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(), name,
+  check_gated(name, x_in, a_in, i_in, decay, init, seq_idx);
+  for (const optional<Tensor>& t : {opt(dy_in), dlast, opt(ckpt)}) check_gpu(name, t);
+  const Tensor x = in_reach(x_in), a_gate = in_reach(a_in), x_gate = in_reach(i_in);
+  TORCH_CHECK_VALUE(dy_in.sizes() == x.sizes() && dy_in.scalar_type() == x.scalar_type(), name,
                     " expects dy shaped and typed like x");
+  const Tensor dy = in_reach(dy_in);
   TORCH_CHECK_VALUE(!has(dlast) || (dlast->scalar_type() == at::kFloat && dlast->dim() == 2 &&
                                     dlast->size(0) == x.size(0) && dlast->size(1) == x.size(2) &&
                                     dlast->is_contiguous()),
