@@ -17,17 +17,24 @@
 // length fills the chip and every input is read once. The state in front of a
 // chunk comes from the chunks before it: a workgroup publishes its (P, S) as
 // soon as it has them (its inputs stay in registers), then looks back, a
-// predecessor per wave, until nothing older matters: a predecessor that knows the state behind its chunk has published that, as
-// (0, h), in the place of its (P, S). Its own (0, h) is published before its
-// outputs are written.
+// predecessor per wave, until nothing older matters: a predecessor that knows
+// the state behind its chunk has published that, as (0, h), in the place of its
+// (P, S). Its own (0, h) is published before its outputs are written.
 // Every wait ends: the chunks of a row's tile are taken by ticket, in the order
 // of time, so the chunks a workgroup waits for have been taken by workgroups
 // that run or have ended, and a workgroup publishes its (P, S) before it waits.
 // Records pass between workgroups as single 64-bit words, written by agent-scope
 // atomic stores and polled by agent-scope atomic loads; a word carries all that
-// is read, and either of a chunk's two is right, so no fence is needed. Two launches, the first for
-// each split's (P, S), read the inputs twice: forward + backward of
-// 8 x 2048 x 1536 bf16 took 221 us that way, @GLS1@ us this way.
+// is read, and either of a chunk's two is right, so no fence is needed.
+//
+// Bound: the inputs and outputs once, 8 x 2048 x 1536 bf16 201 MB forward and
+// 352 MB backward. Measured there: forward 74 us (2.7 TB/s), backward 104 us
+// (3.4 TB/s), 175 us a training step with its clears and the decay's sum; 221 us
+// by two launches each, the first for every split's (P, S), whose inputs are
+// read twice. What is left is the chain of a tile, the time from a chunk's
+// inputs to its (0, h), which the workgroups in flight behind it wait for.
+// Workgroups that stay and take chunk after chunk, with the next one's inputs
+// requested ahead, lengthen that chain (105 and 167 us).
 //
 // Backward, with g_t = dL/dh_t:  g_t = dy_t + k_{t+1} a_{t+1} g_{t+1},
 //   dx = g m iota          dx_gate = dx x (1 - iota)
@@ -114,8 +121,8 @@ struct Place {
   int64_t dd;           // d, or the tile's first channel for lanes beyond the last
 };
 // Which chunk of its row's tile the workgroup takes: the next one in the order of
-// time, from the last on with LAST_FIRST. A counter for each tile: 3072
-// workgroups at one counter wait 1.4 us each, with a burst of 5 at the start.
+// time, from the last on with LAST_FIRST. A counter for each tile: when thousands
+// of workgroups share one, each waits 1.4 us for it, 5 us at the start.
 template <int VC, bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
   __shared__ uint32_t ticket;
   Place q;
@@ -375,9 +382,9 @@ __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams
 // ---- backward ----------------------------------------------------------------------------
 
 template <typename T, bool SEQ>
-__global__ __launch_bounds__(64 * W) void gated_bwd_kernel(const GatedScanParams p) {
+__global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanParams p) {
   constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int VC = 1;
+  constexpr int VC = 1;  // with two channels a lane, half as many waves fit
   __shared__ Exchange<VC> exchange;
   const Place q = place<VC, true>(p);
   const Column<T, VC> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), dy(p.dy, p.sdy, p, q);
@@ -433,17 +440,31 @@ __global__ __launch_bounds__(64 * W) void gated_bwd_kernel(const GatedScanParams
       P[v] *= ka[i][v];
       // These five are to be formed here: moved down to their use, their
       // operands would be kept instead, in 239 registers, two waves a SIMD.
+      // 80 (the launch bound) leave room for three workgroups a CU: 104 us
+      // against 120 for two, at 8 x 2048 x 1536 bf16.
       asm volatile("" : "+v"(gx[i][v]), "+v"(gi[i][v]), "+v"(ga[i][v]), "+v"(gd[i][v]), "+v"(ka[i][v]));
     }
+    __builtin_amdgcn_sched_barrier(0);  // one step after the other: registers
   }
+  // 16-bit dy waits two to a register.
+  constexpr int PACK = sizeof(T) * VC == 2 ? 2 : 1;
+  uint32_t kept[TS / PACK];
+#pragma unroll
+  for (int i = 0; i < TS; i += PACK) {
+    if constexpr (PACK == 2) kept[i / 2] = rd[i] | static_cast<uint32_t>(rd[i + 1]) << 16;
+    else kept[i] = rd[i];
+  }
+  auto dy_at = [&](int i) { return static_cast<Word<T, VC>>(kept[i / PACK] >> (PACK == 2 && i % 2 == 1 ? 16 : 0)); };
 #pragma unroll
   for (int i = TS - 1; i >= 0; --i) {
     float fd[VC];
-    widen<T, VC>(rd[i], fd);
+    widen<T, VC>(dy_at(i), fd);
     const bool restart = SEQ && ((cut >> i) & 1) != 0;
 #pragma unroll
     for (int v = 0; v < VC; ++v) S[v] = restart ? 0.f : ka[i][v] * (S[v] + (i < q.n ? fd[v] : 0.f));
   }
+#pragma unroll
+  for (int i = 0; i < TS / PACK; ++i) asm volatile("" : "+v"(kept[i]));  // and is not kept widened
   float G[VC], out[VC], acc[VC] = {};  // acc: this lane's sum of e rho
   scan_chunks<VC, -1>(p, q, exchange, P, S, edge, G, out);
   if (q.live && q.w == 0 && q.chunk == 0 && p.dinit != nullptr)
@@ -454,7 +475,7 @@ __global__ __launch_bounds__(64 * W) void gated_bwd_kernel(const GatedScanParams
   for (int i = TS - 1; i >= 0; --i) {
     if (i >= q.n) continue;
     float fd[VC], ox[VC], oa[VC], oi[VC];
-    widen<T, VC>(rd[i], fd);
+    widen<T, VC>(dy_at(i), fd);
     const bool restart = SEQ && ((cut >> i) & 1) != 0;
 #pragma unroll
     for (int v = 0; v < VC; ++v) {
