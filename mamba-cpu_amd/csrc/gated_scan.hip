@@ -183,8 +183,12 @@ __device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place
 
 // ---- steps and what is published of them --------------------------------------------------
 
-// P h + S; nothing of h where P is 0, a NaN or an infinity neither.
+// P is 0 where a sequence starts among the steps, and only there: products of
+// decays are held above 0, so that a NaN or an infinity stays in the state of
+// its sequence however much decays, and never enters the next one's.
+constexpr float kFaint = 1.17549435e-38f;  // the smallest normal number
 __device__ __forceinline__ float after(float P, float S, float h) { return P == 0.f ? S : fmaf(P, h, S); }
+__device__ __forceinline__ float join(float P, float Q) { return fmaxf(P * Q, fminf(fminf(P, Q), kFaint)); }
 
 // A record is (P, S) with every bit flipped, so that zeroed memory, the flipped
 // all-ones NaN pair, means none yet; a NaN is published as another one.
@@ -228,7 +232,7 @@ __device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Plac
       }
       const float2 s = x.agg[seg][v * 64 + q.lane];
       allS[v] = after(s.x, s.y, allS[v]);
-      allP[v] *= s.x;
+      allP[v] = join(allP[v], s.x);
     }
   }
   const int64_t first = DIR > 0 ? 0 : p.chunks - 1;
@@ -358,6 +362,9 @@ __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams
       P[v] *= a[i][v];
     }
   }
+  // (a NaN in P is one in S, too)
+#pragma unroll
+  for (int v = 0; v < VC; ++v) P[v] = cut != 0 ? 0.f : fmaxf(P[v], kFaint);
   float h[VC], out[VC];
   scan_chunks<VC, 1>(p, q, exchange, P, S, edge, h, out);
   if (!q.live) return;
@@ -465,6 +472,8 @@ __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanPar
   }
 #pragma unroll
   for (int i = 0; i < TS / PACK; ++i) asm volatile("" : "+v"(kept[i]));  // and is not kept widened
+#pragma unroll
+  for (int v = 0; v < VC; ++v) P[v] = cut != 0 ? 0.f : fmaxf(P[v], kFaint);
   float G[VC], out[VC], acc[VC] = {};  // acc: this lane's sum of e rho
   scan_chunks<VC, -1>(p, q, exchange, P, S, edge, G, out);
   if (q.live && q.w == 0 && q.chunk == 0 && p.dinit != nullptr)
