@@ -96,17 +96,16 @@ __device__ __forceinline__ float gate(float x, float& e) {
 __device__ __forceinline__ float rest(float e, float sigmoid) { return fminf(e, 3e38f) * sigmoid; }
 
 // q = 1 - exp(-2 s) for s >= 0, given a = exp(-s): below 2 s = 1/2 by a
-// polynomial of (1 - exp(-y)) / y (degree 5, fitted to 1.3e-9), above it by
-// the difference, which loses little more than a bit.
+// polynomial of (1 - exp(-y)) / y, y = 2 s (degree 5, fitted to 1.3e-9; here in
+// powers of s), above it by the difference, which loses little more than a bit.
 __device__ __forceinline__ float input_share(float s, float a) {
-  const float y = 2.0f * s;
-  float q = -0.001124026020988822f;
-  q = fmaf(q, y, 0.008190391585230827f);
-  q = fmaf(q, y, -0.04163041338324547f);
-  q = fmaf(q, y, 0.16666248440742493f);
-  q = fmaf(q, y, -0.4999998211860657f);
-  q = fmaf(q, y, 1.0f);
-  return y < 0.5f ? q * y : fmaf(-a, a, 1.0f);
+  float q = -64 * 0.001124026020988822f;
+  q = fmaf(q, s, 32 * 0.008190391585230827f);
+  q = fmaf(q, s, -16 * 0.04163041338324547f);
+  q = fmaf(q, s, 8 * 0.16666248440742493f);
+  q = fmaf(q, s, -4 * 0.4999998211860657f);
+  q = fmaf(q, s, 2.0f);
+  return s < 0.25f ? q * s : fmaf(-a, a, 1.0f);
 }
 
 // ---- a workgroup's place ------------------------------------------------------------------
@@ -349,20 +348,43 @@ __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams
     widen<T, VC>(rx[i], fx);
     widen<T, VC>(ra[i], fa);
     widen<T, VC>(ri[i], fi);
-    const bool restart = SEQ && ((cut >> i) & 1) != 0;
 #pragma unroll
     for (int v = 0; v < VC; ++v) {
       float e;
       const float s = csp[v] * gate(fa[v], e);
-      const float dec = fast_exp(-s);
-      const float m = __builtin_amdgcn_sqrtf(input_share(s, dec));
-      a[i][v] = i < q.n ? (restart ? 0.f : dec) : 1.f;
-      u[i][v] = i < q.n ? m * gate(fi[v], e) * fx[v] : 0.f;
-      S[v] = restart ? u[i][v] : fmaf(a[i][v], S[v], u[i][v]);
-      P[v] *= a[i][v];
+      a[i][v] = fast_exp(-s);
+      u[i][v] = __builtin_amdgcn_sqrtf(input_share(s, a[i][v])) * gate(fi[v], e) * fx[v];
     }
   }
+  // What few segments need is done behind branches that a wave takes as one.
+  if (q.n < TS) {
+#pragma unroll
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        a[i][v] = i < q.n ? a[i][v] : 1.f;
+        u[i][v] = i < q.n ? u[i][v] : 0.f;
+      }
+  }
+  // h[v] through the segment, with each(i) behind step i.
+  auto walk = [&](float (&h)[VC], auto&& each) {
+    auto steps = [&](auto packed) {
+#pragma unroll
+      for (int i = 0; i < TS; ++i) {
+        const bool restart = packed.value && ((cut >> i) & 1) != 0;
+#pragma unroll
+        for (int v = 0; v < VC; ++v) h[v] = restart ? u[i][v] : fmaf(a[i][v], h[v], u[i][v]);
+        each(i);
+      }
+    };
+    if (SEQ && cut != 0) steps(std::true_type{});
+    else steps(std::false_type{});
+  };
   // (a NaN in P is one in S, too)
+  walk(S, [&](int i) {
+#pragma unroll
+    for (int v = 0; v < VC; ++v) P[v] *= a[i][v];
+  });
 #pragma unroll
   for (int v = 0; v < VC; ++v) P[v] = cut != 0 ? 0.f : fmaxf(P[v], kFaint);
   float h[VC], out[VC];
@@ -377,13 +399,9 @@ __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams
 #pragma unroll
     for (int v = 0; v < VC; ++v) to[v] = h[v];
   }
-#pragma unroll
-  for (int i = 0; i < TS; ++i) {
-    const bool restart = SEQ && ((cut >> i) & 1) != 0;
-#pragma unroll
-    for (int v = 0; v < VC; ++v) h[v] = restart ? u[i][v] : fmaf(a[i][v], h[v], u[i][v]);
+  walk(h, [&](int i) {
     if (i < q.n) y.store(i, h);
-  }
+  });
 }
 
 // ---- backward ----------------------------------------------------------------------------
@@ -426,25 +444,23 @@ __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanPar
     for (int v = 0; v < VC; ++v) {
       float ea, ei;
       const float rho = gate(fa[v], ea), iota = gate(fi[v], ei);
-      // 1 minus a sigmoid to its own ulp for float32 gradients; a 16-bit one
-      // does not show the difference.
-      const float nrho = EXACT ? rest(ea, rho) : 1.0f - rho, niota = EXACT ? rest(ei, iota) : 1.0f - iota;
       const float s = csp[v] * rho;
       const float dec = fast_exp(-s);
       const float share = input_share(s, dec);
       // 1 / m, cut above what the smallest normal share gives: a closed gate
       // (share = 0) has m = 0, and a^2 s / m = 0, which is its limit.
       const float inv = fminf(__builtin_amdgcn_rsqf(share), 1e19f);
-      ka[i][v] = i < q.n ? (restart ? 0.f : dec) : 1.f;
+      ka[i][v] = restart ? 0.f : dec;
       const float kah = restart ? 0.f : ka[i][v] * h[v];
       gx[i][v] = iota * (share * inv);
       const float u = gx[i][v] * fx[v];
-      gi[i][v] = u * niota;
       const float e = fmaf(iota * fx[v], (1.0f - share) * inv, -kah);
-      ga[i][v] = e * s * nrho;
       gd[i][v] = e * rho;
+      // 1 minus a sigmoid to its own ulp for float32 gradients; a 16-bit one
+      // does not show the difference.
+      gi[i][v] = EXACT ? u * rest(ei, iota) : fmaf(-u, iota, u);
+      ga[i][v] = EXACT ? e * s * rest(ea, rho) : gd[i][v] * (csp[v] - s);
       h[v] = kah + u;
-      P[v] *= ka[i][v];
       // These five are to be formed here: moved down to their use, their
       // operands would be kept instead, in 239 registers, two waves a SIMD.
       // 80 (the launch bound) leave room for three workgroups a CU: 104 us
@@ -462,14 +478,22 @@ __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanPar
     else kept[i] = rd[i];
   }
   auto dy_at = [&](int i) { return static_cast<Word<T, VC>>(kept[i / PACK] >> (PACK == 2 && i % 2 == 1 ? 16 : 0)); };
+  auto bridge = [&](auto full) {
 #pragma unroll
-  for (int i = TS - 1; i >= 0; --i) {
-    float fd[VC];
-    widen<T, VC>(dy_at(i), fd);
-    const bool restart = SEQ && ((cut >> i) & 1) != 0;
+    for (int i = TS - 1; i >= 0; --i) {
+      float fd[VC];
+      widen<T, VC>(dy_at(i), fd);
+      const bool restart = SEQ && ((cut >> i) & 1) != 0, in = full.value || i < q.n;
 #pragma unroll
-    for (int v = 0; v < VC; ++v) S[v] = restart ? 0.f : ka[i][v] * (S[v] + (i < q.n ? fd[v] : 0.f));
-  }
+      for (int v = 0; v < VC; ++v) {
+        ka[i][v] = in ? ka[i][v] : 1.f;
+        S[v] = restart ? 0.f : ka[i][v] * (S[v] + (in ? fd[v] : 0.f));
+        P[v] *= ka[i][v];
+      }
+    }
+  };
+  if (q.n < TS) bridge(std::false_type{});
+  else bridge(std::true_type{});
 #pragma unroll
   for (int i = 0; i < TS / PACK; ++i) asm volatile("" : "+v"(kept[i]));  // and is not kept widened
 #pragma unroll

@@ -26,8 +26,14 @@ __device__ __forceinline__ float sigmoid_acc(float x, float& one_minus) {
   return s;
 }
 
-// softplus(x), stable at both ends.
-__device__ __forceinline__ float softplus_acc(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+// softplus(x), stable at both ends: log(1 + e) by v_log_f32 of u = 1 + e as
+// rounded, times e / (u - 1), which takes the rounding back (Kahan's log1p); 20
+// instructions where expf and log1pf take 100.
+__device__ __forceinline__ float softplus_acc(float x) {
+  const float e = exp_acc(-fabsf(x)), u = 1.0f + e;
+  const float l = __builtin_amdgcn_logf(u) * kLn2 * (e * fast_rcp(u - 1.0f));
+  return fmaxf(x, 0.f) + (u == 1.0f ? e : l);
+}
 
 // ---- four elements of a row, or what is left of it -----------------------------------
 
