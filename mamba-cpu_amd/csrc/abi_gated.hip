@@ -16,14 +16,14 @@ bool any_negative(std::initializer_list<const int64_t*> strides, int n) {
   return false;
 }
 
-int64_t chunks_of(const mcpu_gated_scan_args* a) { return (a->seqlen + kGatedChunk - 1) / kGatedChunk; }
+int64_t chunks_of(const mcpu_gated_scan_args* a, int steps) { return (a->seqlen + steps - 1) / steps; }
 
 // The kernels reach an element by 32-bit byte offsets from a segment's first step.
 bool in_reach(const mcpu_gated_scan_args* a, std::initializer_list<const int64_t*> strides) {
   constexpr int64_t kReach = int64_t{1} << 32;
   for (const int64_t* s : strides)
     if (s[2] >= kReach / (dtype_size(a->dtype) * (a->dim > 0 ? a->dim : 1)) ||
-        s[1] >= kReach / (dtype_size(a->dtype) * kGatedT))
+        s[1] >= kReach / (dtype_size(a->dtype) * kGatedFwdT))
       return false;
   return true;
 }
@@ -34,7 +34,7 @@ int check_gated(const mcpu_gated_scan_args* a, const char* what) {
   if (!valid_dtype(a->dtype)) return fail(MCPU_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
   const int64_t tiles = (a->dim + 63) / 64;
   if (a->batch > INT_MAX || a->seqlen > (int64_t{1} << 40) || tiles > INT_MAX ||
-      (tiles > 0 && a->batch > 0 && chunks_of(a) > INT_MAX / (tiles * a->batch)))
+      (tiles > 0 && a->batch > 0 && chunks_of(a, kGatedChunk) > INT_MAX / (tiles * a->batch)))
     return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x seqlen x dim too large", what);
   if ((a->decay == nullptr && a->dim > 0) ||
       ((a->x == nullptr || a->a_gate == nullptr || a->x_gate == nullptr) && a->batch * a->seqlen * a->dim > 0))
@@ -47,37 +47,21 @@ int check_gated(const mcpu_gated_scan_args* a, const char* what) {
   return MCPU_OK;
 }
 
-// A (batch, seqlen, dim) operand that two neighbouring 16-bit channels can be
-// moved of at once.
-bool pairs(const void* ptr, const int64_t (&s)[3]) {
-  return ptr == nullptr || (s[2] == 1 && s[0] % 2 == 0 && s[1] % 2 == 0 && reinterpret_cast<uintptr_t>(ptr) % 4 == 0);
-}
-
-// Channels per lane of the forward: two of a 16-bit type where every operand
-// allows, so that a lane moves four bytes. The backward holds five numbers a
-// step and channel between its two halves: with two channels a lane it spills
-// at two workgroups a CU (165 against 124 us for 8 x 2048 x 1536).
-int gated_vec(const mcpu_gated_scan_args* a) {
-  return a->dtype != MCPU_F32 && a->dim % 2 == 0 && pairs(a->x, a->x_stride) && pairs(a->a_gate, a->a_stride) &&
-                 pairs(a->x_gate, a->i_stride) && pairs(a->y, a->y_stride)
-             ? 2
-             : 1;
-}
-
 // The tickets and records of a call of more than one chunk.
 size_t ticket_bytes(const mcpu_gated_scan_args* a) {
   return align_up(sizeof(uint32_t) * a->batch * ((a->dim + 63) / 64));
 }
-size_t record_bytes(const mcpu_gated_scan_args* a) {
-  return chunks_of(a) > 1 ? ticket_bytes(a) + align_up(sizeof(uint64_t) * a->batch * chunks_of(a) * a->dim) : 0;
+size_t record_bytes(const mcpu_gated_scan_args* a, int64_t chunks) {
+  return chunks > 1 ? ticket_bytes(a) + align_up(sizeof(uint64_t) * a->batch * chunks * a->dim) : 0;
 }
 int clear_records(GatedScanParams& p, const mcpu_gated_scan_args* a, void* workspace, hipStream_t st) {
+  if (p.chunks == 1) return MCPU_OK;
   p.tickets = static_cast<uint32_t*>(workspace);
   p.records = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + ticket_bytes(a));
-  return zero_f32(static_cast<float*>(workspace), static_cast<int64_t>(record_bytes(a) / sizeof(float)), st);
+  return zero_f32(static_cast<float*>(workspace), static_cast<int64_t>(record_bytes(a, p.chunks) / sizeof(float)), st);
 }
 
-GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
+GatedScanParams make_gated(const mcpu_gated_scan_args* a, int steps) {
   GatedScanParams p;
   std::memset(&p, 0, sizeof(p));
   p.x = a->x;
@@ -90,7 +74,7 @@ GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
   p.len = a->seqlen;
   p.dim = a->dim;
   p.c = a->c;
-  p.chunks = chunks_of(a);
+  p.chunks = chunks_of(a, steps);
   p.ckpt = a->ckpt;
   for (int i = 0; i < 3; ++i) {
     p.sx[i] = a->x_stride[i];
@@ -123,7 +107,7 @@ extern "C" size_t mcpu_gated_scan_fwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return record_bytes(a);
+  return record_bytes(a, chunks_of(a, kGatedFwdChunk));
 }
 
 extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -138,7 +122,7 @@ extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspac
     return fail(MCPU_ERR_UNSUPPORTED, "%s: a row's steps or channels lie too far apart", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_gated_scan_fwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
-  GatedScanParams p = make_gated(a);
+  GatedScanParams p = make_gated(a, kGatedFwdChunk);
   p.y = a->y;
   p.last = a->last_state;
   if (a->batch == 0 || a->dim == 0) return MCPU_OK;
@@ -147,9 +131,7 @@ extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspac
     return a->last_state == nullptr
                ? MCPU_OK
                : hip_status(gated_edge_launch(a->initial_state, a->last_state, a->batch * a->dim, st), what);
-  p.vec = gated_vec(a);
-  if (p.chunks > 1)
-    if (int rc = clear_records(p, a, workspace, st)) return rc;
+  if (int rc = clear_records(p, a, workspace, st)) return rc;
   return hip_status(gated_scan_fwd_launch(p, a->dtype, st), "gated_scan_fwd launch");
 }
 
@@ -158,7 +140,8 @@ extern "C" size_t mcpu_gated_scan_bwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return record_bytes(a) + align_up(sizeof(float) * a->batch * chunks_of(a) * a->dim);
+  const int64_t chunks = chunks_of(a, kGatedChunk);
+  return record_bytes(a, chunks) + align_up(sizeof(float) * a->batch * chunks * a->dim);
 }
 
 extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -186,7 +169,7 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
                ? MCPU_OK
                : hip_status(gated_edge_launch(a->dlast_state, a->dinitial_state, a->batch * a->dim, st), what);
   }
-  GatedScanParams p = make_gated(a);
+  GatedScanParams p = make_gated(a, kGatedChunk);
   p.dy = a->dy;
   p.dlast = a->dlast_state;
   p.dx = a->dx;
@@ -194,9 +177,8 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
   p.dx_gate = a->dx_gate;
   p.ddecay = a->ddecay;
   p.dinit = a->dinitial_state;
-  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + record_bytes(a));
-  if (p.chunks > 1)
-    if (int rc = clear_records(p, a, workspace, st)) return rc;
+  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + record_bytes(a, p.chunks));
+  if (int rc = clear_records(p, a, workspace, st)) return rc;
   return hip_status(gated_scan_bwd_launch(p, a->dtype, st), "gated_scan_bwd launch");
 }
 

@@ -8,9 +8,13 @@
 
 namespace mcpu {
 
-constexpr int kGatedT = 8;      // steps per wave segment: the forward keeps the state before each
-constexpr int kGatedWaves = 8;  // waves of a workgroup, one segment each
-constexpr int kGatedChunk = kGatedT * kGatedWaves;  // steps of a workgroup
+constexpr int kGatedWaves = 8;  // waves of a workgroup, one segment of a chunk each
+// Steps of a segment. The forward keeps the state before every kGatedT steps for
+// the backward, which holds five numbers a step between its two halves.
+constexpr int kGatedT = 8;
+constexpr int kGatedFwdT = 16;
+constexpr int kGatedChunk = kGatedT * kGatedWaves;
+constexpr int kGatedFwdChunk = kGatedFwdT * kGatedWaves;
 
 struct GatedScanParams {
   const void* x;
@@ -21,7 +25,7 @@ struct GatedScanParams {
   const int32_t* seq_idx;  // (batch, len) contiguous, or null
   void* y;
   float* last;
-  float* ckpt;  // (batch, ceil(len / kGatedT), dim): the state before each segment
+  float* ckpt;  // (batch, ceil(len / kGatedT), dim)
   const void* dy;
   const float* dlast;
   void* dx;
@@ -35,8 +39,7 @@ struct GatedScanParams {
   uint64_t* records;
   float* dinit;
   int64_t batch, len, dim;
-  int64_t chunks;
-  int vec;  // channels per lane
+  int64_t chunks;  // of the direction's steps
   float c;
   int64_t sx[3], sa[3], si[3], sy[3], sdy[3], sdx[3], sda[3], sdi[3];  // (batch, len, dim)
 };

@@ -49,37 +49,7 @@
 namespace mcpu {
 namespace {
 
-constexpr int TS = kGatedT, W = kGatedWaves;
-
-// ---- VC neighbouring channels of a row -------------------------------------------------
-
-template <int BYTES> struct WordOf;
-template <> struct WordOf<2> { using type = uint16_t; };
-template <> struct WordOf<4> { using type = uint32_t; };
-template <> struct WordOf<8> { using type = uint2; };
-template <typename T, int VC> using Word = typename WordOf<sizeof(T) * VC>::type;
-
-template <typename T, int VC> __device__ __forceinline__ void widen(Word<T, VC> r, float (&v)[VC]) {
-  if constexpr (sizeof(T) == 4 && VC == 1) {
-    v[0] = __builtin_bit_cast(float, r);
-  } else if constexpr (VC == 1) {
-    v[0] = to_f32(__builtin_bit_cast(T, r));
-  } else {
-    static_assert(sizeof(T) == 2 && VC == 2);
-    v[0] = to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(r)));
-    v[1] = to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(r >> 16)));
-  }
-}
-template <typename T, int VC> __device__ __forceinline__ Word<T, VC> narrow(const float (&v)[VC]) {
-  if constexpr (VC == 1) {
-    return __builtin_bit_cast(Word<T, VC>, from_f32<T>(v[0]));
-  } else if constexpr (std::is_same_v<T, bf16>) {
-    return pack_bf16x2(v[0], v[1]);
-  } else {
-    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from_f32<T>(v[0]))) |
-           static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from_f32<T>(v[1]))) << 16;
-  }
-}
+constexpr int W = kGatedWaves;
 
 // ---- gates -----------------------------------------------------------------------------
 // The exponentials are v_exp_f32's: for a gate x it is off by |x| 2^-24 at
@@ -112,8 +82,7 @@ __device__ __forceinline__ float input_share(float s, float a) {
 
 struct Place {
   int lane, w;
-  int64_t b, chunk, d;  // d: first channel of the lane
-  int64_t t0;           // first step of the chunk
+  int64_t b, chunk, d;  // d: the lane's channel
   int64_t ts;           // first step of the wave's segment
   int n;                // steps of the segment
   bool live;
@@ -122,12 +91,12 @@ struct Place {
 // Which chunk of its row's tile the workgroup takes: the next one in the order of
 // time, from the last on with LAST_FIRST. A counter for each tile: when thousands
 // of workgroups share one, each waits 1.4 us for it, 5 us at the start.
-template <int VC, bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
+template <int TS, bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
   __shared__ uint32_t ticket;
   Place q;
   q.lane = threadIdx.x & 63;
   q.w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tiles = static_cast<uint32_t>((p.dim + 64 * VC - 1) / (64 * VC));
+  const uint32_t tiles = static_cast<uint32_t>((p.dim + 63) / 64);
   const uint32_t rows = tiles * static_cast<uint32_t>(p.batch), row = blockIdx.x % rows;
   uint32_t t = 0;
   if (p.chunks > 1) {
@@ -137,12 +106,11 @@ template <int VC, bool LAST_FIRST> __device__ __forceinline__ Place place(const 
   }
   q.chunk = LAST_FIRST ? p.chunks - 1 - t : t;
   q.b = row / tiles;
-  const int64_t first = row % tiles * 64ll * VC;
-  q.d = first + q.lane * VC;
+  const int64_t first = row % tiles * 64ll;
+  q.d = first + q.lane;
   q.live = q.d < p.dim;
   q.dd = q.live ? q.d : first;
-  q.t0 = q.chunk * kGatedChunk;
-  q.ts = q.t0 + q.w * TS;
+  q.ts = (q.chunk * W + q.w) * TS;
   const int64_t left = p.len - q.ts;
   q.n = left < 0 ? 0 : left < TS ? static_cast<int>(left) : TS;
   return q;
@@ -150,7 +118,7 @@ template <int VC, bool LAST_FIRST> __device__ __forceinline__ Place place(const 
 
 // The wave's segment of an operand: a scalar base, the lane's byte offset, and
 // a scalar offset per step. Steps behind the row's end read its last one.
-template <typename T, int VC> struct Column {
+template <typename T> struct Column {
   __amdgpu_buffer_rsrc_t rsrc;
   uint32_t lane, step;
   __device__ __forceinline__ Column(const void* ptr, const int64_t (&s)[3], const GatedScanParams& p, const Place& q)
@@ -158,21 +126,26 @@ template <typename T, int VC> struct Column {
                        (q.b * s[0] + (q.n > 0 ? q.ts : p.len - 1) * s[1]) * static_cast<int64_t>(sizeof(T)))),
         lane(static_cast<uint32_t>(q.dd * s[2] * static_cast<int64_t>(sizeof(T)))),
         step(static_cast<uint32_t>(s[1] * static_cast<int64_t>(sizeof(T)))) {}
-  __device__ __forceinline__ Word<T, VC> load(const Place& q, int i) const {
+  // The bits, to be widened where they are used: that is where the wave waits.
+  __device__ __forceinline__ uint32_t load(const Place& q, int i) const {
     const int at = i < q.n ? i : q.n > 0 ? q.n - 1 : 0;
-    if constexpr (sizeof(T) * VC == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, lane, at * step, 0);
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, lane, at * step, 0);
     else return __builtin_amdgcn_raw_buffer_load_b16(rsrc, lane, at * step, 0);
   }
-  __device__ __forceinline__ void store(int i, const float (&v)[VC]) const {
-    if constexpr (sizeof(T) * VC == 4)
-      __builtin_amdgcn_raw_buffer_store_b32(narrow<T, VC>(v), rsrc, lane, i * step, 0);
+  __device__ __forceinline__ void store(int i, float v) const {
+    if constexpr (sizeof(T) == 4)
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rsrc, lane, i * step, 0);
     else
-      __builtin_amdgcn_raw_buffer_store_b16(narrow<T, VC>(v), rsrc, lane, i * step, 0);
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<T>(v)), rsrc, lane, i * step, 0);
   }
 };
+template <typename T> __device__ __forceinline__ float widen(uint32_t bits) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, bits);
+  else return to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(bits)));
+}
 
 // Bit i: step ts + i starts another sequence than the step before it.
-__device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place& q) {
+template <int TS> __device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place& q) {
   const int64_t t = q.ts + q.lane;
   const int32_t* ids = p.seq_idx + q.b * p.len;
   bool s = false;
@@ -186,7 +159,7 @@ __device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place
 // decays are held above 0, so that a NaN or an infinity stays in the state of
 // its sequence however much decays, and never enters the next one's.
 constexpr float kFaint = 1.17549435e-38f;  // the smallest normal number
-__device__ __forceinline__ float after(float P, float S, float h) { return P == 0.f ? S : fmaf(P, h, S); }
+__device__ __forceinline__ float after(float2 s, float h) { return s.x == 0.f ? s.y : fmaf(s.x, h, s.y); }
 __device__ __forceinline__ float join(float P, float Q) { return fmaxf(P * Q, fminf(fminf(P, Q), kFaint)); }
 
 // A record is (P, S) with every bit flipped, so that zeroed memory, the flipped
@@ -201,206 +174,144 @@ __device__ __forceinline__ uint64_t peek(const uint64_t* at) {
 }
 
 constexpr int kWindows = 4;  // windows of W chunks that are kept
-template <int VC> struct Exchange {
-  float2 agg[W][64 * VC];                // the segments' (P, S)
-  float2 win[kWindows + 2][W][64 * VC];  // what the waves found of W neighbouring chunks; two for those further back
+struct Exchange {
+  float2 agg[W][64];                // the segments' (P, S)
+  float2 win[kWindows + 2][W][64];  // what the waves found of W neighbouring chunks; two for those further back
 };
 
 // The state that enters the wave's segment, from the segments' (P, S) and
 // `edge`, the state that enters the row's first chunk (in the direction of the
 // scan: DIR 1 forward, -1 backward). `out` is the state behind the chunk.
-template <int VC, int DIR>
-__device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Place& q, Exchange<VC>& x,
-                                            const float (&P)[VC], const float (&S)[VC], const float (&edge)[VC],
-                                            float (&in)[VC], float (&out)[VC]) {
-#pragma unroll
-  for (int v = 0; v < VC; ++v) x.agg[q.w][v * 64 + q.lane] = make_float2(P[v], S[v]);
+template <int DIR>
+__device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Place& q, Exchange& x, float P, float S,
+                                            float edge, float& in, float& out) {
+  x.agg[q.w][q.lane] = make_float2(P, S);
   __syncthreads();
   // The segments before this one, and the whole chunk.
-  float mineP[VC], mineS[VC], allP[VC], allS[VC];
+  float2 mine, all = make_float2(1.f, 0.f);
 #pragma unroll
-  for (int v = 0; v < VC; ++v) {
-    allP[v] = 1.f;
-    allS[v] = 0.f;
-#pragma unroll
-    for (int o = 0; o < W; ++o) {
-      const int seg = DIR > 0 ? o : W - 1 - o;
-      if (seg == q.w) {
-        mineP[v] = allP[v];
-        mineS[v] = allS[v];
-      }
-      const float2 s = x.agg[seg][v * 64 + q.lane];
-      allS[v] = after(s.x, s.y, allS[v]);
-      allP[v] = join(allP[v], s.x);
-    }
+  for (int o = 0; o < W; ++o) {
+    const int seg = DIR > 0 ? o : W - 1 - o;
+    if (seg == q.w) mine = all;
+    const float2 s = x.agg[seg][q.lane];
+    all = make_float2(join(all.x, s.x), after(s, all.y));
   }
   const int64_t first = DIR > 0 ? 0 : p.chunks - 1;
   const int64_t back = DIR * (q.chunk - first);  // chunks before this one
   uint64_t* const rec = p.records + q.b * p.chunks * p.dim + q.dd;
-  float state[VC];
-#pragma unroll
-  for (int v = 0; v < VC; ++v) state[v] = edge[v];
+  float state = edge;
   if (back > 0) {
-    if (q.w == 0 && q.live) {
-#pragma unroll
-      for (int v = 0; v < VC; ++v) publish(rec + q.chunk * p.dim + v, allP[v], allS[v]);
-    }
-    auto slot = [](int64_t win) { return win < kWindows ? static_cast<int>(win) : kWindows + static_cast<int>(win & 1); };
+    if (q.w == 0 && q.live) publish(rec + q.chunk * p.dim, all.x, all.y);
+    auto slot = [](int64_t win) {
+      return win < kWindows ? static_cast<int>(win) : kWindows + static_cast<int>(win & 1);
+    };
     // This wave's chunk of a window, as published.
     auto fetch = [&](int64_t win) {
       const int64_t away = win * W + q.w + 1;  // how far back the chunk is
-      float pP[VC], pS[VC];
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {  // in front of the row's first chunk: the edge, then nothing
-        pP[v] = away == back + 1 ? 0.f : 1.f;
-        pS[v] = away == back + 1 ? edge[v] : 0.f;
-      }
+      // In front of the row's first chunk: the edge, then nothing.
+      float2 s = away == back + 1 ? make_float2(0.f, edge) : make_float2(1.f, 0.f);
       if (away <= back) {
         const uint64_t* at = rec + (q.chunk - DIR * away) * p.dim;
-        for (;;) {
-          bool have = true;
-#pragma unroll
-          for (int v = 0; v < VC; ++v) {
-            const uint64_t word = peek(at + v), r = ~word;
-            have &= word != 0;
-            pP[v] = __builtin_bit_cast(float, static_cast<uint32_t>(r >> 32));
-            pS[v] = __builtin_bit_cast(float, static_cast<uint32_t>(r));
-          }
-          if (__ballot(!have) == 0) break;
+        uint64_t word = peek(at);
+        while (__ballot(word == 0) != 0) {
           __builtin_amdgcn_s_sleep(1);
+          word = peek(at);
         }
+        s.x = __builtin_bit_cast(float, ~static_cast<uint32_t>(word >> 32));
+        s.y = __builtin_bit_cast(float, ~static_cast<uint32_t>(word));
       }
-#pragma unroll
-      for (int v = 0; v < VC; ++v) x.win[slot(win)][q.w][v * 64 + q.lane] = make_float2(pP[v], pS[v]);
+      x.win[slot(win)][q.w][q.lane] = s;
       __syncthreads();
     };
     // Back until every channel has met a chunk that does not depend on older ones.
-    bool known[VC] = {};
+    bool known = false;
     int64_t win = 0;
     for (;; ++win) {
       fetch(win);
-      bool all = true;
 #pragma unroll
-      for (int v = 0; v < VC; ++v) {
-#pragma unroll
-        for (int o = 0; o < W; ++o) known[v] |= x.win[slot(win)][o][v * 64 + q.lane].x == 0.f;
-        all &= known[v];
-      }
+      for (int o = 0; o < W; ++o) known |= x.win[slot(win)][o][q.lane].x == 0.f;
       // All waves read the same values, so all leave together.
-      if (__ballot(!all) == 0 || (win + 1) * W > back) break;
+      if (__ballot(!known) == 0 || (win + 1) * W > back) break;
     }
     // Then forward again, one chunk after the other: the state behind chunk j is
-    // always after(P_j, S_j, the state in front of it), whether another
+    // always after((P, S)_j, the state in front of it), whether another
     // workgroup formed it or this one, so that the result does not depend on
     // what had been published when. Windows further back than those kept are
     // read again, except the last.
-#pragma unroll
-    for (int v = 0; v < VC; ++v) state[v] = 0.f;
+    state = 0.f;
     for (int64_t w = win; w >= 0; --w) {
       if (w >= kWindows && w < win) fetch(w);
 #pragma unroll
-      for (int v = 0; v < VC; ++v)
-#pragma unroll
-        for (int o = W - 1; o >= 0; --o) {
-          const float2 s = x.win[slot(w)][o][v * 64 + q.lane];
-          state[v] = after(s.x, s.y, state[v]);
-        }
+      for (int o = W - 1; o >= 0; --o) state = after(x.win[slot(w)][o][q.lane], state);
     }
   }
-#pragma unroll
-  for (int v = 0; v < VC; ++v) {
-    in[v] = after(mineP[v], mineS[v], state[v]);
-    out[v] = after(allP[v], allS[v], state[v]);
-  }
-  if (p.chunks > 1 && back < p.chunks - 1 && q.w == 0 && q.live) {
-#pragma unroll
-    for (int v = 0; v < VC; ++v) publish(rec + q.chunk * p.dim + v, 0.f, out[v]);
-  }
+  in = after(mine, state);
+  out = after(all, state);
+  if (back < p.chunks - 1 && q.w == 0 && q.live) publish(rec + q.chunk * p.dim, 0.f, out);
 }
 
 // ---- forward -----------------------------------------------------------------------------
 // SEQ: packed sequences.
 
-template <typename T, int VC, bool SEQ>
-__global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams p) {
-  __shared__ Exchange<VC> exchange;
-  const Place q = place<VC, false>(p);
-  const Column<T, VC> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), y(p.y, p.sy, p, q);
-  Word<T, VC> rx[TS], ra[TS], ri[TS];
+template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams p) {
+  constexpr int TS = kGatedFwdT;
+  __shared__ Exchange exchange;
+  const Place q = place<TS, false>(p);
+  const Column<T> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), y(p.y, p.sy, p, q);
+  uint32_t rx[TS], ra[TS], ri[TS];
 #pragma unroll
   for (int i = 0; i < TS; ++i) {
     ra[i] = ag.load(q, i);
     ri[i] = ig.load(q, i);
     rx[i] = x.load(q, i);
   }
-  const uint32_t cut = SEQ ? starts(p, q) : 0;
-  float csp[VC], edge[VC], P[VC], S[VC], a[TS][VC], u[TS][VC];
-#pragma unroll
-  for (int v = 0; v < VC; ++v) {
-    csp[v] = p.c * softplus_acc(p.decay[q.dd + v]);
-    edge[v] = p.init == nullptr ? 0.f : p.init[q.b * p.dim + q.dd + v];
-    P[v] = 1.f;
-    S[v] = 0.f;
-  }
+  const uint32_t cut = SEQ ? starts<TS>(p, q) : 0;
+  const float csp = p.c * softplus_acc(p.decay[q.dd]);
+  const float edge = p.init == nullptr ? 0.f : p.init[q.b * p.dim + q.dd];
+  float a[TS], u[TS], P = 1.f, S = 0.f;
 #pragma unroll
   for (int i = 0; i < TS; ++i) {
-    float fx[VC], fa[VC], fi[VC];
-    widen<T, VC>(rx[i], fx);
-    widen<T, VC>(ra[i], fa);
-    widen<T, VC>(ri[i], fi);
-#pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      float e;
-      const float s = csp[v] * gate(fa[v], e);
-      a[i][v] = fast_exp(-s);
-      u[i][v] = __builtin_amdgcn_sqrtf(input_share(s, a[i][v])) * gate(fi[v], e) * fx[v];
-    }
+    float e;
+    const float s = csp * gate(widen<T>(ra[i]), e);
+    a[i] = fast_exp(-s);
+    u[i] = __builtin_amdgcn_sqrtf(input_share(s, a[i])) * gate(widen<T>(ri[i]), e) * widen<T>(rx[i]);
   }
   // What few segments need is done behind branches that a wave takes as one.
   if (q.n < TS) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i)
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        a[i][v] = i < q.n ? a[i][v] : 1.f;
-        u[i][v] = i < q.n ? u[i][v] : 0.f;
-      }
+    for (int i = 0; i < TS; ++i) {
+      a[i] = i < q.n ? a[i] : 1.f;
+      u[i] = i < q.n ? u[i] : 0.f;
+    }
   }
-  // h[v] through the segment, with each(i) behind step i.
-  auto walk = [&](float (&h)[VC], auto&& each) {
+  // h through the segment, with each(i) behind step i.
+  auto walk = [&](float& h, auto&& each) {
     auto steps = [&](auto packed) {
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
-        const bool restart = packed.value && ((cut >> i) & 1) != 0;
-#pragma unroll
-        for (int v = 0; v < VC; ++v) h[v] = restart ? u[i][v] : fmaf(a[i][v], h[v], u[i][v]);
+        h = packed.value && ((cut >> i) & 1) != 0 ? u[i] : fmaf(a[i], h, u[i]);
         each(i);
       }
     };
     if (SEQ && cut != 0) steps(std::true_type{});
     else steps(std::false_type{});
   };
-  // (a NaN in P is one in S, too)
-  walk(S, [&](int i) {
-#pragma unroll
-    for (int v = 0; v < VC; ++v) P[v] *= a[i][v];
-  });
-#pragma unroll
-  for (int v = 0; v < VC; ++v) P[v] = cut != 0 ? 0.f : fmaxf(P[v], kFaint);
-  float h[VC], out[VC];
-  scan_chunks<VC, 1>(p, q, exchange, P, S, edge, h, out);
+  walk(S, [&](int i) { P *= a[i]; });
+  P = cut != 0 ? 0.f : fmaxf(P, kFaint);  // a NaN in P is one in S, too
+  float h, out;
+  scan_chunks<1>(p, q, exchange, P, S, edge, h, out);
   if (!q.live) return;
-  if (q.w == 0 && q.chunk == p.chunks - 1 && p.last != nullptr)
-#pragma unroll
-    for (int v = 0; v < VC; ++v) p.last[q.b * p.dim + q.d + v] = out[v];
+  if (q.w == 0 && q.chunk == p.chunks - 1 && p.last != nullptr) p.last[q.b * p.dim + q.d] = out;
   if (q.n <= 0) return;
-  if (p.ckpt != nullptr) {
-    float* to = p.ckpt + (q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.d;
-#pragma unroll
-    for (int v = 0; v < VC; ++v) to[v] = h[v];
-  }
+  // The state before every kGatedT steps is kept for the backward.
+  float* const keep = p.ckpt + (q.b * ((p.len + kGatedT - 1) / kGatedT) + q.ts / kGatedT) * p.dim + q.d;
+  auto kept = [&](int i) {
+    if (i < q.n && i % kGatedT == 0 && p.ckpt != nullptr) keep[i / kGatedT * p.dim] = h;
+  };
+  kept(0);
   walk(h, [&](int i) {
     if (i < q.n) y.store(i, h);
+    kept(i + 1);
   });
 }
 
@@ -408,12 +319,12 @@ __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams
 
 template <typename T, bool SEQ>
 __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanParams p) {
+  constexpr int TS = kGatedT;
   constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int VC = 1;  // with two channels a lane, half as many waves fit
-  __shared__ Exchange<VC> exchange;
-  const Place q = place<VC, true>(p);
-  const Column<T, VC> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), dy(p.dy, p.sdy, p, q);
-  Word<T, VC> rx[TS], ra[TS], ri[TS], rd[TS];
+  __shared__ Exchange exchange;
+  const Place q = place<TS, true>(p);
+  const Column<T> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), dy(p.dy, p.sdy, p, q);
+  uint32_t rx[TS], ra[TS], ri[TS], rd[TS];
 #pragma unroll
   for (int i = 0; i < TS; ++i) {
     ra[i] = ag.load(q, i);
@@ -421,121 +332,91 @@ __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanPar
     ri[i] = ig.load(q, i);
     rx[i] = x.load(q, i);
   }
-  const uint32_t cut = SEQ ? starts(p, q) : 0;
-  float csp[VC], edge[VC], P[VC], S[VC], h[VC];
-#pragma unroll
-  for (int v = 0; v < VC; ++v) {
-    h[v] = q.n > 0 ? p.ckpt[(q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.dd + v] : 0.f;
-    csp[v] = p.c * softplus_acc(p.decay[q.dd + v]);
-    edge[v] = p.dlast == nullptr ? 0.f : p.dlast[q.b * p.dim + q.dd + v];
-    P[v] = 1.f;
-    S[v] = 0.f;
-  }
+  const uint32_t cut = SEQ ? starts<TS>(p, q) : 0;
+  float h = q.n > 0 ? p.ckpt[(q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.dd] : 0.f;
+  const float csp = p.c * softplus_acc(p.decay[q.dd]);
+  const float edge = p.dlast == nullptr ? 0.f : p.dlast[q.b * p.dim + q.dd];
   // What a step's gradients are per unit of g: dx, dx_gate, da_gate, e rho; and k a.
-  float gx[TS][VC], gi[TS][VC], ga[TS][VC], gd[TS][VC], ka[TS][VC];
+  float gx[TS], gi[TS], ga[TS], gd[TS], ka[TS];
 #pragma unroll
   for (int i = 0; i < TS; ++i) {
-    float fx[VC], fa[VC], fi[VC];
-    widen<T, VC>(rx[i], fx);
-    widen<T, VC>(ra[i], fa);
-    widen<T, VC>(ri[i], fi);
     const bool restart = SEQ && ((cut >> i) & 1) != 0;
-#pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      float ea, ei;
-      const float rho = gate(fa[v], ea), iota = gate(fi[v], ei);
-      const float s = csp[v] * rho;
-      const float dec = fast_exp(-s);
-      const float share = input_share(s, dec);
-      // 1 / m, cut above what the smallest normal share gives: a closed gate
-      // (share = 0) has m = 0, and a^2 s / m = 0, which is its limit.
-      const float inv = fminf(__builtin_amdgcn_rsqf(share), 1e19f);
-      ka[i][v] = restart ? 0.f : dec;
-      const float kah = restart ? 0.f : ka[i][v] * h[v];
-      gx[i][v] = iota * (share * inv);
-      const float u = gx[i][v] * fx[v];
-      const float e = fmaf(iota * fx[v], (1.0f - share) * inv, -kah);
-      gd[i][v] = e * rho;
-      // 1 minus a sigmoid to its own ulp for float32 gradients; a 16-bit one
-      // does not show the difference.
-      gi[i][v] = EXACT ? u * rest(ei, iota) : fmaf(-u, iota, u);
-      ga[i][v] = EXACT ? e * s * rest(ea, rho) : gd[i][v] * (csp[v] - s);
-      h[v] = kah + u;
-      // These five are to be formed here: moved down to their use, their
-      // operands would be kept instead, in 239 registers, two waves a SIMD.
-      // 80 (the launch bound) leave room for three workgroups a CU: 104 us
-      // against 120 for two, at 8 x 2048 x 1536 bf16.
-      asm volatile("" : "+v"(gx[i][v]), "+v"(gi[i][v]), "+v"(ga[i][v]), "+v"(gd[i][v]), "+v"(ka[i][v]));
-    }
+    const float fx = widen<T>(rx[i]);
+    float ea, ei;
+    const float rho = gate(widen<T>(ra[i]), ea), iota = gate(widen<T>(ri[i]), ei);
+    const float s = csp * rho;
+    const float dec = fast_exp(-s);
+    const float share = input_share(s, dec);
+    // 1 / m, cut above what the smallest normal share gives: a closed gate
+    // (share = 0) has m = 0, and a^2 s / m = 0, which is its limit.
+    const float inv = fminf(__builtin_amdgcn_rsqf(share), 1e19f);
+    ka[i] = restart ? 0.f : dec;
+    const float kah = restart ? 0.f : dec * h;
+    gx[i] = iota * (share * inv);
+    const float u = gx[i] * fx;
+    const float e = fmaf(iota * fx, (1.0f - share) * inv, -kah);
+    gd[i] = e * rho;
+    // 1 minus a sigmoid to its own ulp for float32 gradients; a 16-bit one
+    // does not show the difference.
+    gi[i] = EXACT ? u * rest(ei, iota) : fmaf(-u, iota, u);
+    ga[i] = EXACT ? e * s * rest(ea, rho) : gd[i] * (csp - s);
+    h = kah + u;
+    // These five are to be formed here: moved down to their use, their
+    // operands would be kept instead, in 239 registers, two waves a SIMD.
+    // 80 (the launch bound) leave room for three workgroups a CU: 104 us
+    // against 120 for two, at 8 x 2048 x 1536 bf16.
+    asm volatile("" : "+v"(gx[i]), "+v"(gi[i]), "+v"(ga[i]), "+v"(gd[i]), "+v"(ka[i]));
     __builtin_amdgcn_sched_barrier(0);  // one step after the other: registers
   }
   // 16-bit dy waits two to a register.
-  constexpr int PACK = sizeof(T) * VC == 2 ? 2 : 1;
+  constexpr int PACK = sizeof(T) == 2 ? 2 : 1;
   uint32_t kept[TS / PACK];
 #pragma unroll
   for (int i = 0; i < TS; i += PACK) {
-    if constexpr (PACK == 2) kept[i / 2] = rd[i] | static_cast<uint32_t>(rd[i + 1]) << 16;
+    if constexpr (PACK == 2) kept[i / 2] = rd[i] | rd[i + 1] << 16;
     else kept[i] = rd[i];
   }
-  auto dy_at = [&](int i) { return static_cast<Word<T, VC>>(kept[i / PACK] >> (PACK == 2 && i % 2 == 1 ? 16 : 0)); };
+  auto dy_at = [&](int i) { return widen<T>(kept[i / PACK] >> (PACK == 2 && i % 2 == 1 ? 16 : 0)); };
+  float P = 1.f, S = 0.f;
   auto bridge = [&](auto full) {
 #pragma unroll
     for (int i = TS - 1; i >= 0; --i) {
-      float fd[VC];
-      widen<T, VC>(dy_at(i), fd);
       const bool restart = SEQ && ((cut >> i) & 1) != 0, in = full.value || i < q.n;
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        ka[i][v] = in ? ka[i][v] : 1.f;
-        S[v] = restart ? 0.f : ka[i][v] * (S[v] + (in ? fd[v] : 0.f));
-        P[v] *= ka[i][v];
-      }
+      ka[i] = in ? ka[i] : 1.f;
+      S = restart ? 0.f : ka[i] * (S + (in ? dy_at(i) : 0.f));
+      P *= ka[i];
     }
   };
   if (q.n < TS) bridge(std::false_type{});
   else bridge(std::true_type{});
+  P = cut != 0 ? 0.f : fmaxf(P, kFaint);
 #pragma unroll
   for (int i = 0; i < TS / PACK; ++i) asm volatile("" : "+v"(kept[i]));  // and is not kept widened
-#pragma unroll
-  for (int v = 0; v < VC; ++v) P[v] = cut != 0 ? 0.f : fmaxf(P[v], kFaint);
-  float G[VC], out[VC], acc[VC] = {};  // acc: this lane's sum of e rho
-  scan_chunks<VC, -1>(p, q, exchange, P, S, edge, G, out);
-  if (q.live && q.w == 0 && q.chunk == 0 && p.dinit != nullptr)
-#pragma unroll
-    for (int v = 0; v < VC; ++v) p.dinit[q.b * p.dim + q.d + v] = out[v];
-  const Column<T, VC> dx(p.dx, p.sdx, p, q), da(p.da_gate, p.sda, p, q), di(p.dx_gate, p.sdi, p, q);
+  float G, out, acc = 0.f;  // acc: this lane's sum of e rho
+  scan_chunks<-1>(p, q, exchange, P, S, edge, G, out);
+  if (q.live && q.w == 0 && q.chunk == 0 && p.dinit != nullptr) p.dinit[q.b * p.dim + q.d] = out;
+  const Column<T> dx(p.dx, p.sdx, p, q), da(p.da_gate, p.sda, p, q), di(p.dx_gate, p.sdi, p, q);
 #pragma unroll
   for (int i = TS - 1; i >= 0; --i) {
     if (i >= q.n) continue;
-    float fd[VC], ox[VC], oa[VC], oi[VC];
-    widen<T, VC>(dy_at(i), fd);
-    const bool restart = SEQ && ((cut >> i) & 1) != 0;
-#pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      const float g = fd[v] + G[v];
-      ox[v] = g * gx[i][v];
-      oi[v] = g * gi[i][v];
-      oa[v] = g * ga[i][v];
-      acc[v] = fmaf(g, gd[i][v], acc[v]);
-      G[v] = restart ? 0.f : ka[i][v] * g;
-    }
+    const float g = dy_at(i) + G;
+    acc = fmaf(g, gd[i], acc);
+    G = SEQ && ((cut >> i) & 1) != 0 ? 0.f : ka[i] * g;
     if (q.live) {
-      dx.store(i, ox);
-      di.store(i, oi);
-      da.store(i, oa);
+      dx.store(i, g * gx[i]);
+      di.store(i, g * gi[i]);
+      da.store(i, g * ga[i]);
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int v = 0; v < VC; ++v) exchange.agg[q.w][v * 64 + q.lane].x = acc[v];
+  exchange.agg[q.w][q.lane].x = acc;
   __syncthreads();
-  if (q.w == 0 && q.live)
+  if (q.w == 0 && q.live) {
+    float sum = 0.f, e;
 #pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      float sum = 0.f, e;
-      for (int o = 0; o < W; ++o) sum += exchange.agg[o][v * 64 + q.lane].x;
-      p.ddecay_part[(q.b * p.chunks + q.chunk) * p.dim + q.d + v] = sum * p.c * gate(p.decay[q.d + v], e);
-    }
+    for (int o = 0; o < W; ++o) sum += exchange.agg[o][q.lane].x;
+    p.ddecay_part[(q.b * p.chunks + q.chunk) * p.dim + q.d] = sum * p.c * gate(p.decay[q.d], e);
+  }
 }
 
 constexpr int kReduceWaves = 16;
@@ -598,28 +479,25 @@ hipError_t gated_edge_launch(const float* from, float* to, int64_t n, hipStream_
   return hipGetLastError();
 }
 
+// A workgroup for each chunk of 64 channels.
+static dim3 gated_grid(const GatedScanParams& p) {
+  return dim3(static_cast<unsigned>((p.dim + 63) / 64 * p.batch * p.chunks));
+}
+
 hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
-  auto launch = [&](auto t, auto vc) {
+  by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int VC = decltype(vc)::value;
-    const dim3 grid(static_cast<unsigned>((p.dim + 64 * VC - 1) / (64 * VC) * p.batch * p.chunks)), block(64 * W);
-    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, VC, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((gated_fwd_kernel<T, VC, false>), grid, block, 0, st, p);
-  };
-  constexpr std::integral_constant<int, 1> one;
-  constexpr std::integral_constant<int, 2> two;
-  if (dtype == MCPU_F32) launch(float{}, one);
-  else if (dtype == MCPU_BF16) p.vec == 2 ? launch(bf16{}, two) : launch(bf16{}, one);
-  else p.vec == 2 ? launch(f16{}, two) : launch(f16{}, one);
+    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, true>), gated_grid(p), dim3(64 * W), 0, st, p);
+    else hipLaunchKernelGGL((gated_fwd_kernel<T, false>), gated_grid(p), dim3(64 * W), 0, st, p);
+  });
   return hipGetLastError();
 }
 
 hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid(static_cast<unsigned>((p.dim + 63) / 64 * p.batch * p.chunks)), block(64 * W);
-    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), grid, block, 0, st, p);
+    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), gated_grid(p), dim3(64 * W), 0, st, p);
+    else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), gated_grid(p), dim3(64 * W), 0, st, p);
   });
   hipLaunchKernelGGL(gated_ddecay_kernel, dim3(static_cast<unsigned>((p.dim + 63) / 64)), dim3(64 * kReduceWaves), 0,
                      st, p);
