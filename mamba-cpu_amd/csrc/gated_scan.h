@@ -9,12 +9,8 @@
 namespace mcpu {
 
 constexpr int kGatedWaves = 8;  // waves of a workgroup, one segment of a chunk each
-// Steps of a segment. The forward keeps the state before every kGatedT steps for
-// the backward, which holds five numbers a step between its two halves.
-constexpr int kGatedT = 8;
-constexpr int kGatedFwdT = 16;
-constexpr int kGatedChunk = kGatedT * kGatedWaves;
-constexpr int kGatedFwdChunk = kGatedFwdT * kGatedWaves;
+constexpr int kGatedT = 16;     // steps of a segment: the forward keeps the state before each
+constexpr int kGatedChunk = kGatedT * kGatedWaves;  // steps of a workgroup
 
 struct GatedScanParams {
   const void* x;
@@ -39,7 +35,7 @@ struct GatedScanParams {
   uint64_t* records;
   float* dinit;
   int64_t batch, len, dim;
-  int64_t chunks;  // of the direction's steps
+  int64_t chunks;
   float c;
   int64_t sx[3], sa[3], si[3], sy[3], sdy[3], sdx[3], sda[3], sdi[3];  // (batch, len, dim)
 };

@@ -7,19 +7,18 @@
 //
 // with k_t = 0 at the first step of another sequence of a packed row, else 1.
 // The step h -> a h + b composes as (P, S): h -> P h + S, so time is split: a
-// wave takes kGatedT consecutive steps of its channels in registers and forms
-// their (P, S), the workgroup's waves exchange theirs through LDS, and each
+// wave takes kGatedT = 16 consecutive steps of 64 channels in registers and forms
+// their (P, S), the workgroup's 8 waves exchange theirs through LDS, and each
 // wave then knows the state in front of its segment, given the one in front of
-// the workgroup's chunk. A lane holds `vec` neighbouring channels (4 bytes where
-// the operands allow), so that a wave reads 256 bytes of a row at once.
+// the workgroup's chunk.
 //
-// A workgroup takes one chunk of 64 steps of 64 vec channels, so that every
-// length fills the chip and every input is read once. The state in front of a
-// chunk comes from the chunks before it: a workgroup publishes its (P, S) as
-// soon as it has them (its inputs stay in registers), then looks back, a
-// predecessor per wave, until nothing older matters: a predecessor that knows
-// the state behind its chunk has published that, as (0, h), in the place of its
-// (P, S). Its own (0, h) is published before its outputs are written.
+// A workgroup takes one chunk of 128 steps of 64 channels, so that every length
+// fills the chip and every input is read once. The state in front of a chunk
+// comes from the chunks before it: a workgroup publishes its (P, S) as soon as
+// it has them (its inputs stay in registers), then looks back, a predecessor per
+// wave, until nothing older matters: a predecessor that knows the state behind
+// its chunk has published that, as (0, h), in the place of its (P, S). Its own
+// (0, h) is published before its outputs are written.
 // Every wait ends: the chunks of a row's tile are taken by ticket, in the order
 // of time, so the chunks a workgroup waits for have been taken by workgroups
 // that run or have ended, and a workgroup publishes its (P, S) before it waits.
@@ -27,14 +26,19 @@
 // atomic stores and polled by agent-scope atomic loads; a word carries all that
 // is read, and either of a chunk's two is right, so no fence is needed.
 //
-// Bound: the inputs and outputs once, 8 x 2048 x 1536 bf16 201 MB forward and
-// 352 MB backward. Measured there: forward 74 us (2.7 TB/s), backward 104 us
-// (3.4 TB/s), 175 us a training step with its clears and the decay's sum; 221 us
-// by two launches each, the first for every split's (P, S), whose inputs are
-// read twice. What is left is the chain of a tile, the time from a chunk's
-// inputs to its (0, h), which the workgroups in flight behind it wait for.
-// Workgroups that stay and take chunk after chunk, with the next one's inputs
-// requested ahead, lengthen that chain (105 and 167 us).
+// Bound: the inputs and outputs once, for 8 x 2048 x 1536 bf16 201 MB forward
+// and 352 MB backward, and vector issue: 50 and 85 instructions a step and
+// channel, 0.6 to 0.7 of the cycles. Measured there: forward 57 us (3.5 TB/s),
+// backward 98 us (3.6 TB/s), a training step with its clears and the decay's sum
+// 156 us. Other splits, for the same step:
+//   two launches a direction, the first for every split's (P, S)   221 us
+//   8 steps a wave: twice the chunks, each with its exchange and
+//   look back, which are 20 instructions a step then               166 us
+//   workgroups that stay and take chunk after chunk, the next one's
+//   inputs requested ahead: the chain of a tile gets longer        276 us
+// What is left is that chain, the time from a chunk's inputs to its (0, h), and
+// that loads, arithmetic and the wait of one workgroup overlap with only two (in
+// the backward) or three others' on a CU.
 //
 // Backward, with g_t = dL/dh_t:  g_t = dy_t + k_{t+1} a_{t+1} g_{t+1},
 //   dx = g m iota          dx_gate = dx x (1 - iota)
@@ -49,7 +53,7 @@
 namespace mcpu {
 namespace {
 
-constexpr int W = kGatedWaves;
+constexpr int TS = kGatedT, W = kGatedWaves;
 
 // ---- gates -----------------------------------------------------------------------------
 // The exponentials are v_exp_f32's: for a gate x it is off by |x| 2^-24 at
@@ -91,7 +95,7 @@ struct Place {
 // Which chunk of its row's tile the workgroup takes: the next one in the order of
 // time, from the last on with LAST_FIRST. A counter for each tile: when thousands
 // of workgroups share one, each waits 1.4 us for it, 5 us at the start.
-template <int TS, bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
+template <bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
   __shared__ uint32_t ticket;
   Place q;
   q.lane = threadIdx.x & 63;
@@ -145,7 +149,7 @@ template <typename T> __device__ __forceinline__ float widen(uint32_t bits) {
 }
 
 // Bit i: step ts + i starts another sequence than the step before it.
-template <int TS> __device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place& q) {
+__device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place& q) {
   const int64_t t = q.ts + q.lane;
   const int32_t* ids = p.seq_idx + q.b * p.len;
   bool s = false;
@@ -254,9 +258,8 @@ __device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Plac
 // SEQ: packed sequences.
 
 template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams p) {
-  constexpr int TS = kGatedFwdT;
   __shared__ Exchange exchange;
-  const Place q = place<TS, false>(p);
+  const Place q = place<false>(p);
   const Column<T> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), y(p.y, p.sy, p, q);
   uint32_t rx[TS], ra[TS], ri[TS];
 #pragma unroll
@@ -265,7 +268,7 @@ template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_
     ri[i] = ig.load(q, i);
     rx[i] = x.load(q, i);
   }
-  const uint32_t cut = SEQ ? starts<TS>(p, q) : 0;
+  const uint32_t cut = SEQ ? starts(p, q) : 0;
   const float csp = p.c * softplus_acc(p.decay[q.dd]);
   const float edge = p.init == nullptr ? 0.f : p.init[q.b * p.dim + q.dd];
   float a[TS], u[TS], P = 1.f, S = 0.f;
@@ -303,26 +306,19 @@ template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_
   if (!q.live) return;
   if (q.w == 0 && q.chunk == p.chunks - 1 && p.last != nullptr) p.last[q.b * p.dim + q.d] = out;
   if (q.n <= 0) return;
-  // The state before every kGatedT steps is kept for the backward.
-  float* const keep = p.ckpt + (q.b * ((p.len + kGatedT - 1) / kGatedT) + q.ts / kGatedT) * p.dim + q.d;
-  auto kept = [&](int i) {
-    if (i < q.n && i % kGatedT == 0 && p.ckpt != nullptr) keep[i / kGatedT * p.dim] = h;
-  };
-  kept(0);
+  if (p.ckpt != nullptr) p.ckpt[(q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.d] = h;
   walk(h, [&](int i) {
     if (i < q.n) y.store(i, h);
-    kept(i + 1);
   });
 }
 
 // ---- backward ----------------------------------------------------------------------------
 
 template <typename T, bool SEQ>
-__global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanParams p) {
-  constexpr int TS = kGatedT;
+__global__ __launch_bounds__(64 * W, 4) void gated_bwd_kernel(const GatedScanParams p) {
   constexpr bool EXACT = sizeof(T) == 4;
   __shared__ Exchange exchange;
-  const Place q = place<TS, true>(p);
+  const Place q = place<true>(p);
   const Column<T> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), dy(p.dy, p.sdy, p, q);
   uint32_t rx[TS], ra[TS], ri[TS], rd[TS];
 #pragma unroll
@@ -332,7 +328,7 @@ __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanPar
     ri[i] = ig.load(q, i);
     rx[i] = x.load(q, i);
   }
-  const uint32_t cut = SEQ ? starts<TS>(p, q) : 0;
+  const uint32_t cut = SEQ ? starts(p, q) : 0;
   float h = q.n > 0 ? p.ckpt[(q.b * ((p.len + TS - 1) / TS) + q.ts / TS) * p.dim + q.dd] : 0.f;
   const float csp = p.c * softplus_acc(p.decay[q.dd]);
   const float edge = p.dlast == nullptr ? 0.f : p.dlast[q.b * p.dim + q.dd];
@@ -362,11 +358,9 @@ __global__ __launch_bounds__(64 * W, 6) void gated_bwd_kernel(const GatedScanPar
     ga[i] = EXACT ? e * s * rest(ea, rho) : gd[i] * (csp - s);
     h = kah + u;
     // These five are to be formed here: moved down to their use, their
-    // operands would be kept instead, in 239 registers, two waves a SIMD.
-    // 80 (the launch bound) leave room for three workgroups a CU: 104 us
-    // against 120 for two, at 8 x 2048 x 1536 bf16.
+    // operands would be kept instead, in twice the registers. 128 (the launch
+    // bound) leave room for two workgroups a CU.
     asm volatile("" : "+v"(gx[i]), "+v"(gi[i]), "+v"(ga[i]), "+v"(gd[i]), "+v"(ka[i]));
-    __builtin_amdgcn_sched_barrier(0);  // one step after the other: registers
   }
   // 16-bit dy waits two to a register.
   constexpr int PACK = sizeof(T) == 2 ? 2 : 1;

@@ -17,7 +17,7 @@ import torch
 from mamba_cpu import _C  # noqa: F401  (loads the operator library)
 
 _X_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-_SEG = 8  # steps between the states the forward keeps
+_SEG = 16  # steps between the states the forward keeps
 
 
 # mamba_cpu::gated_scan_fwd (autograd through mamba_cpu::gated_scan_bwd) and
