@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
 // the parts. The other workgroups write the zeros of ids without a token, a
 // wave four rows. With a wave for each id's row instead, the most frequent ids
 // are the time: 46 us for 16384 bf16 tokens of 768 even where ids above 32
-// tokens go in chunks, @DW@ us this way.
+// tokens go in chunks, 27 us this way.
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p, int chunks, int tiles) {
   constexpr int kBatch = 16;

@@ -27,8 +27,8 @@
 // is read, and either of a chunk's two is right, so no fence is needed.
 //
 // Bound: the inputs and outputs once, for 8 x 2048 x 1536 bf16 201 MB forward
-// and 352 MB backward, and vector issue: 50 and 85 instructions a step and
-// channel, 0.6 to 0.7 of the cycles. Measured there: forward 57 us (3.5 TB/s),
+// and 352 MB backward, and vector issue: 43 and 68 instructions a step and
+// channel, 0.56 to 0.66 of the cycles. Measured there: forward 57 us (3.5 TB/s),
 // backward 98 us (3.6 TB/s), a training step with its clears and the decay's sum
 // 156 us. Other splits, for the same step:
 //   two launches a direction, the first for every split's (P, S)   221 us

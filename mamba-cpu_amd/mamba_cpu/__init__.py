@@ -5,6 +5,9 @@ libmamba_hip.so; they take ROCm GPU tensors. `mamba_chunk_scan_combined` is
 Mamba-2's SSD scan (mamba_ssm's function of that name) over the same library. `mamba_inner_fn` is the fused
 Mamba-1 mixer over them (transformers' training path). `mamba_cpu.hf.patch_transformers()`
 routes Hugging Face Mamba / FalconMamba / Jamba / Mamba-2 models on the GPU to them.
+
+Beside the scans: the gated linear recurrence (`gated_linear_scan_fn`, `gated_linear_update`),
+`layer_norm_fn`, `embedding_fn` and `sample_fn`, which `mamba_cpu.recurrent_lm` puts together.
 """
 
 from mamba_cpu.ops import (

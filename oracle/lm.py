@@ -1,6 +1,6 @@
-"""Float64 numpy restatements of the operators beside the scans: the gated
-linear recurrence, step by step as its definition reads. Test infrastructure
-only.
+"""Float64 numpy restatements of the operators beside the scans, as their
+definitions read: the gated linear recurrence step by step, the residual norm,
+the embedding's gradient, token sampling. Test infrastructure only.
 """
 
 import numpy as np
