@@ -31,9 +31,12 @@
 // nothing is cut for any row, sample_slice_kernel takes rows in slices instead,
 // so that few rows fill the chip, and sample_join_kernel compares their winners.
 //
-// The race runs on approximate scores first (v_exp_f32, v_rcp_f32: 12
-// instructions a logit instead of 40); what comes within 2^-13 of the best is
-// scored again with the division and exponential to the last place.
+// The race runs on approximate logarithms of the scores first, 9 instructions a
+// logit, of which a pack's largest is kept; what comes near the best is scored
+// again with the division and exponential to the last place. A pass over a row
+// is bound by its instructions on one CU: 50280 logits take 0.35 us for each. So
+// NaN are cleaned only in rows that have any, and what few logits need is worked
+// off in loops over bits.
 #include "lm_math.h"
 #include "lm_params.h"
 
@@ -62,6 +65,7 @@ struct Shared {
   float tops[kThreads];  // each thread's largest logit
   uint32_t u32[kWaves];
   float f32[kWaves];
+  uint32_t odd[kWaves];
   uint32_t n, pick, left;
   uint64_t entry;
 };
@@ -124,6 +128,22 @@ template <typename T> struct Pack {
     if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[e]);
     else return to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2)))));
   }
+  // The same for an e that is not a constant.
+  __device__ __forceinline__ float pick(int e) const {
+    const int j = sizeof(T) == 4 ? e : e / 2;
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+    const uint32_t word = j < 2 ? (j == 0 ? w0 : w1) : (j == 2 ? w2 : w3);
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, word);
+    else return to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(word >> (16 * (e % 2)))));
+  }
+  // Bit e: whether f holds for element e. For what is rare: the bits are then
+  // worked off in a loop, where code for each element would crowd out the passes.
+  template <typename F> __device__ __forceinline__ uint32_t which(F&& f) const {
+    uint32_t hits = 0;
+#pragma unroll
+    for (int e = 0; e < kPer<T>; ++e) hits |= f(at(e)) ? 1u << e : 0u;
+    return hits;
+  }
 };
 // NaN counts as -inf.
 __device__ __forceinline__ float clean(float l) { return l == l ? l : -__builtin_inff(); }
@@ -146,7 +166,7 @@ template <typename T> __device__ __forceinline__ Pack<T> load_pack(const T* row,
     p.w[1] = q.y;
     p.w[2] = q.z;
     p.w[3] = q.w;
-    return clean(p);
+    return p;
   }
   // The row's end: -inf beyond it.
   const uint32_t low = sizeof(T) == 4 ? 0xff800000u : kLowest<T> | kLowest<T> << 16;
@@ -160,7 +180,7 @@ template <typename T> __device__ __forceinline__ Pack<T> load_pack(const T* row,
       p.w[e / 2] = e % 2 == 0 ? (p.w[e / 2] & 0xffff0000u) | b : (p.w[e / 2] & 0xffffu) | (b << 16);
     }
   }
-  return clean(p);
+  return p;
 }
 // x cut to [0, 1].
 __device__ __forceinline__ float upto1(float x) { return __builtin_amdgcn_fmed3f(x, 0.f, 1.f); }
@@ -172,6 +192,7 @@ template <typename T> struct Row {
   static constexpr int kE = kPer<T>;
   const T* logits;
   int vocab;
+  bool odd;           // there are NaN in it
   float top;          // the largest logit
   float ref, factor;  // weight_fast's: top (or the largest float), log2(e) / T
   float temperature;
@@ -185,6 +206,10 @@ template <typename T> struct Row {
       Pack<T> p[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) p[j] = load_pack(logits, i0 + j * kThreads * kPer<T>, vocab);
+      if (odd) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) p[j] = clean(p[j]);
+      }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
         if (i0 + j * kThreads * kPer<T> < vocab) f(i0 + j * kThreads * kPer<T>, p[j]);
@@ -200,7 +225,9 @@ template <typename T> struct Row {
   // exp((l - M) / T); the largest logits, infinite ones too, weigh 1.
   __device__ __forceinline__ float weight(float l) const { return l == top ? 1.0f : exp_acc((l - top) / temperature); }
   // Clamped to 1, for M = inf (a modifier of v_exp_f32, without an instruction).
-  __device__ __forceinline__ float weight_fast(float l) const { return upto1(fast_exp2((l - ref) * factor)); }
+  __device__ __forceinline__ float weight_fast(float l) const { return upto1(fast_exp2(steps(l))); }
+  // log2 of the weight; of an infinite M itself infinity.
+  __device__ __forceinline__ float steps(float l) const { return (l - ref) * factor; }
   // Temperatures beyond 1e-30 and 1e30 act as those (log2(e) / T stays a number,
   // also times 0 and infinity).
   __device__ __forceinline__ void set(float m, float t) {
@@ -215,6 +242,7 @@ template <typename T> struct Row {
 struct Cut {
   float edge;
   uint32_t last;
+  // Not what lies beyond the row's end: it is -inf, and `last` lies in the row.
   __device__ __forceinline__ bool has(float l, int i) const {
     return l > edge || (l == edge && static_cast<uint32_t>(i) <= last);
   }
@@ -305,7 +333,7 @@ __device__ Cut radix_cut(const R& row, const Cut& from, uint32_t want, float uni
     __syncthreads();
     row.each([&](int i, float l) {
       const uint32_t k = key_of(l);
-      if (i < row.vocab && (k & mask) == prefix && from.has(l, i))
+      if ((k & mask) == prefix && from.has(l, i))
         atomicAdd(&s.bins[(k >> shift) & 255], units<BY_MASS>(row, l, unit));
     });
     __syncthreads();
@@ -365,7 +393,7 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
                                         Shared& s) {
   const float scale = (kBins - 1) / fmaxf(fminf(24.0f * row.temperature, row.top - low), 1e-30f);
   auto bin_of = [&](float l) {
-    return static_cast<int>(__builtin_amdgcn_fmed3f((row.ref - l) * scale, 0.f, kBins - 1.0f));
+    return static_cast<int>(__builtin_amdgcn_fmed3f((l - row.ref) * -scale, 0.f, kBins - 1.0f));
   };
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[i] = 0;
   __syncthreads();
@@ -373,7 +401,7 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
     row.each([&](int, float l) { atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit)); });
   } else {
     row.each([&](int i, float l) {
-      if (i < row.vocab && from.has(l, i)) atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit));
+      if (from.has(l, i)) atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit));
     });
   }
   __syncthreads();
@@ -403,9 +431,10 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
 #pragma unroll
       for (int e = 0; e < R::kE; ++e) any |= q.at(e) <= high && q.at(e) >= least;
       if (!any) return;
-      for (int e = 0; e < R::kE; ++e) {
-        const float l = q.at(e);
-        if (bin_of(l) == bin && i + e < row.vocab && from.has(l, i + e)) append(s, l, i + e);
+      for (uint32_t hits = q.which([&](float l) { return l <= high && l >= least; }); hits != 0; hits &= hits - 1) {
+        const int e = __builtin_ctz(hits);
+        const float l = q.pick(e);
+        if (bin_of(l) == bin && from.has(l, i + e)) append(s, l, i + e);
       }
     });
     __syncthreads();
@@ -494,9 +523,17 @@ __device__ __forceinline__ uint32_t winner(float score, uint32_t i, float* f32, 
   return group_min<WAVES>(score == top ? i : 0xffffffffu, u32);
 }
 
-// A thread's best approximate score, where, and the second best.
+// Scores are compared as log2(w / noise) first. Both logarithms are off by less
+// than 150 x 2^-22, so whatever may be the winner lies within kNearLog, log2 of
+// 1 / kNear, of the best.
+constexpr float kNearLog = 1.7611e-4f;
+template <typename R> __device__ __forceinline__ float fast_score(const R& row, float l, float noise) {
+  return row.steps(l) - __builtin_amdgcn_logf(fmaxf(noise, kLeastNoise));
+}
+
+// A thread's best pack by its largest fast score, where, and the second best.
 struct Best {
-  float best = -1.0f, second = -1.0f;
+  float best = -__builtin_inff(), second = -__builtin_inff();
   int at = 0;
   __device__ __forceinline__ void see(float score, int i) {
     second = __builtin_amdgcn_fmed3f(best, second, score);  // second <= best
@@ -511,53 +548,91 @@ template <bool CUT, typename T>
 __device__ __forceinline__ uint32_t race(const Row<T>& row, const Cut& kept, float min_p, const float* noise,
                                          Shared& s) {
   constexpr int kAhead = 2, E = kPer<T>;
-  auto in = [&](float l, int i) {
-    if constexpr (!CUT) return true;
-    if (!kept.has(l, i)) return false;
-    if (!(min_p > 0.f)) return true;
-    const float w = row.weight_fast(l);
-    return w >= min_p * (2.0f - kNear) || (w >= min_p * kNear && row.weight(l) >= min_p);
-  };
-  // f(score, index) of each logit, -1 for one that is not kept; logits and noise
-  // of kAhead packs on their way at once.
-  auto scores = [&](auto&& f) {
-    for (int i0 = threadIdx.x * E; i0 < row.vocab; i0 += kAhead * kThreads * E) {
-      Pack<T> p[kAhead];
-      float q[kAhead][E];
+  const float inf = __builtin_inff();
+  const float above = value_of(key_of(kept.edge) + 1);  // the next logit above the edge; NaN above infinity
+  const float least = __builtin_amdgcn_logf(min_p);
+  // The fast scores of a pack, -inf for a logit that is not kept.
+  auto scores = [&](int i, const Pack<T>& p, const float (&q)[E], float (&score)[E]) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) p[j] = load_pack(row.logits, i0 + j * kThreads * E, row.vocab);
+    for (int e = 0; e < E; ++e) score[e] = fast_score(row, p.at(e), q[e]);
+    if constexpr (CUT) {
+      const int last = static_cast<int>(kept.last);
+      if (i <= last && last < i + E - 1) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) load_noise<E>(noise, i0 + j * kThreads * E, row.vocab, q[j]);
+        for (int e = 0; e < E; ++e) score[e] = p.at(e) >= (i + e <= last ? kept.edge : above) ? score[e] : -inf;
+      } else {
+        const float edge = i <= last ? kept.edge : above;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
+        for (int e = 0; e < E; ++e) score[e] = p.at(e) >= edge ? score[e] : -inf;
+      }
+      if (min_p > 0.f) {
+        // What lies too near min-p to tell is left to the weight itself.
+        uint32_t hits = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int i = i0 + j * kThreads * E + e;
-          const float l = p[j].at(e);
-          const float score = row.weight_fast(l) * fast_rcp(fmaxf(q[j][e], kLeastNoise));
-          f(!CUT || (i < row.vocab && in(l, i)) ? score : -1.0f, i);
+          const float x = row.steps(p.at(e)) - least;
+          score[e] = x >= -kNearLog ? score[e] : -inf;
+          hits |= x >= -kNearLog && x <= kNearLog ? 1u << e : 0u;
         }
+        for (; hits != 0; hits &= hits - 1) {
+          const int at = __builtin_ctz(hits);
+          if (row.weight(p.pick(at)) >= min_p) continue;
+#pragma unroll
+          for (int e = 0; e < E; ++e) score[e] = e == at ? -inf : score[e];
+        }
+      }
     }
+  };
+  auto load = [&](int i, Pack<T>& p, float (&q)[E]) {
+    p = load_pack(row.logits, i, row.vocab);
+    load_noise<E>(noise, i, row.vocab, q);
   };
   Best b;
-  scores([&](float score, int i) { b.see(score, i); });
-  const float bar = group_max(b.best, s.f32) * kNear;
+  for (int i0 = threadIdx.x * E; i0 < row.vocab; i0 += kAhead * kThreads * E) {
+    Pack<T> p[kAhead];
+    float q[kAhead][E];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) load(i0 + j * kThreads * E, p[j], q[j]);
+    if (row.odd) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) p[j] = clean(p[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      float score[E], most = -inf;
+      scores(i0 + j * kThreads * E, p[j], q[j], score);
+#pragma unroll
+      for (int e = 0; e < E; ++e) most = __builtin_elementwise_maximum(most, score[e]);
+      b.see(most, i0 + j * kThreads * E);
+    }
+  }
+  const float bar = group_max(b.best, s.f32) - kNearLog;
   float score = -1.0f;
   uint32_t at = 0xffffffffu;
-  auto exactly = [&](int i) {
-    if (i >= row.vocab) return;
-    const float exact = row.weight(row.at(i)) / noise_at(noise, i);
-    if (exact > score) {
-      score = exact;
-      at = static_cast<uint32_t>(i);
+  if (b.best >= bar) {
+    // The near ones of the best pack, or of all where another comes near it too.
+    const bool all = b.second >= bar;
+    for (int i = all ? static_cast<int>(threadIdx.x) * E : b.at; i < row.vocab; i += kThreads * E) {
+      Pack<T> p;
+      float q[E], fast[E];
+      load(i, p, q);
+      if (row.odd) p = clean(p);
+      scores(i, p, q, fast);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) hits |= fast[e] >= bar ? 1u << e : 0u;
+      for (; hits != 0; hits &= hits - 1) {
+        const int w = i + __builtin_ctz(hits);
+        const float l = row.at(min(w, row.vocab - 1));
+        if (w >= row.vocab || (CUT && (!kept.has(l, w) || !(row.weight(l) >= min_p)))) continue;
+        const float exact = row.weight(l) / noise_at(noise, w);
+        if (exact > score) {
+          score = exact;
+          at = static_cast<uint32_t>(w);
+        }
+      }
+      if (!all) break;
     }
-  };
-  if (b.second >= bar) {
-    scores([&](float near, int i) {
-      if (near >= bar) exactly(i);
-    });
-  } else if (b.best >= bar) {
-    exactly(b.at);
   }
   return winner(score, at, s.f32, s.u32);
 }
@@ -576,12 +651,28 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
 
   const float inf = __builtin_inff();
   float m = -inf, low = inf;
-  row.each([&](int, float l) {
-    m = fmaxf(m, l);
-    low = fminf(low, l == -inf ? inf : l);
-  });
+  // By v_maximum3_f32 and v_minimum3_f32, half an instruction a logit; a NaN
+  // comes through, and the thread looks again.
+  auto range = [&](bool clean_first) {
+    m = -inf;
+    low = inf;
+    row.odd = clean_first;
+    row.each_pack([&](int i, const Pack<T>& q) {
+#pragma unroll
+      for (int e = 0; e < kPer<T>; ++e) {
+        m = __builtin_elementwise_maximum(m, q.at(e));
+        low = __builtin_elementwise_minimum(low, i + kPer<T> <= row.vocab || i + e < row.vocab ? q.at(e) : inf);
+      }
+    });
+  };
+  range(false);
+  const bool bad = m != m;
+  if (bad) range(true);
+  if ((threadIdx.x & 63) == 0) s.odd[threadIdx.x >> 6] = 0;
+  if (bad) s.odd[threadIdx.x >> 6] = 1;
   s.tops[threadIdx.x] = m;
   m = group_max(m, s.f32);
+  row.odd = __ballot(s.odd[threadIdx.x & (kWaves - 1)] != 0) != 0;
   if (m == -inf) {
     if (threadIdx.x == 0) {
       p.token[r] = -1;
@@ -622,15 +713,15 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
     row.each_pack([&](int i, const Pack<T>& q) {
       float high = -inf;
 #pragma unroll
-      for (int e = 0; e < kPer<T>; ++e) high = fmaxf(high, q.at(e));
+      for (int e = 0; e < kPer<T>; ++e) high = __builtin_elementwise_maximum(high, q.at(e));
       if (high >= look) {
-        for (int e = 0; e < kPer<T>; ++e) {
-          const float l = q.at(e);
-          if (l >= look && i + e < row.vocab) {
-            if (greedy) token = min(token, static_cast<uint32_t>(i + e));
-            else append(s, l, i + e);
-          }
+        uint32_t hits = q.which([&](float l) { return l >= look; });
+        if (i + kPer<T> > row.vocab) hits &= (1u << (row.vocab - i)) - 1;
+        if (greedy) {
+          if (hits != 0) token = min(token, static_cast<uint32_t>(i + __builtin_ctz(hits)));
+          hits = 0;
         }
+        for (; hits != 0; hits &= hits - 1) append(s, q.pick(__builtin_ctz(hits)), i + __builtin_ctz(hits));
       }
       if (sum1) {
 #pragma unroll
@@ -680,7 +771,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
       if (k > 0) {
         kept = find_cut<false>(row, low, kept, static_cast<uint32_t>(k), 1.0f, s);
         if (by_p) {
-          row.each([&](int i, float l) { total += i < row.vocab && kept.has(l, i) ? row.weight_fast(l) : 0.f; });
+          row.each([&](int i, float l) { total += kept.has(l, i) ? row.weight_fast(l) : 0.f; });
           total = group_fsum(total, s.f32);
         }
       }
@@ -733,43 +824,56 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   }
   const float inf = __builtin_inff();
   float m = -inf;
+  auto top = [&] {
+    m = -inf;
 #pragma unroll
-  for (int j = 0; j < NP; ++j)
+    for (int j = 0; j < NP; ++j)
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, l[j].at(e));
+      for (int e = 0; e < E; ++e) m = __builtin_elementwise_maximum(m, l[j].at(e));
+  };
+  top();
+  if (__ballot(m != m) != 0) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) l[j] = clean(l[j]);
+    top();
+  }
   m = group_max<kSliceThreads / 64>(m, f32);
   row.set(m, GREEDY ? 1.0f : p.temperature);
   float sum = 0.f, score = -1.0f;
   uint32_t at = 0xffffffffu;
   Best b;
 #pragma unroll
-  for (int j = 0; j < NP; ++j)
+  for (int j = 0; j < NP; ++j) {
+    const int i = first + j * kSliceThreads * E;
+    float most = -inf;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float v = l[j].at(e);
-      const int i = first + j * kSliceThreads * E + e;
       sum += upto1(fast_exp2((v - row.ref) * kLog2e));
-      if constexpr (GREEDY) at = v == m ? min(at, static_cast<uint32_t>(i)) : at;
-      else b.see(row.weight_fast(v) * fast_rcp(fmaxf(q[j][e], kLeastNoise)), i);
+      if constexpr (GREEDY) at = v == m ? min(at, static_cast<uint32_t>(i + e)) : at;
+      else most = __builtin_elementwise_maximum(most, fast_score(row, v, q[j][e]));
     }
+    if constexpr (!GREEDY) b.see(most, i);
+  }
   sum = group_fsum<kSliceThreads / 64>(sum, f32);
   if constexpr (GREEDY) {
     at = group_min<kSliceThreads / 64>(at, u32);
   } else {
-    const float bar = group_max<kSliceThreads / 64>(b.best, f32) * kNear;
-    auto exactly = [&](int i) {
-      if (i >= row.vocab) return;
-      const float exact = row.weight(row.at(i)) / noise_at(noise, i);
-      if (exact > score) {
-        score = exact;
-        at = static_cast<uint32_t>(i);
+    const float bar = group_max<kSliceThreads / 64>(b.best, f32) - kNearLog;
+    // The best pack's logits, or all the thread's where another comes near it.
+    if (b.best >= bar) {
+      const bool all = b.second >= bar;
+      const int most = all ? NP * E : E;
+#pragma unroll 1
+      for (int n = 0; n < most; ++n) {
+        const int i = (all ? first + n / E * kSliceThreads * E : b.at) + n % E;
+        if (i >= row.vocab) continue;
+        const float exact = row.weight(row.at(i)) / noise_at(noise, i);
+        if (exact > score) {
+          score = exact;
+          at = static_cast<uint32_t>(i);
+        }
       }
-    };
-    if (b.second >= bar) {
-      for (int j = 0; j < NP; ++j)
-        for (int e = 0; e < E; ++e) exactly(first + j * kSliceThreads * E + e);
-    } else if (b.best >= bar) {
-      exactly(b.at);
     }
     at = winner<kSliceThreads / 64>(score, at, f32, u32);
   }
