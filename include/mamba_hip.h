@@ -577,8 +577,8 @@ int mcpu_mamba2_step(const mcpu_mamba2_step_args* a, void* workspace, size_t wor
  *   h_t = k_t a h_{t-1} + m iota x_t        y_t = h_t, h_{-1} = initial_state or 0
  * with k_t = 0 where seq_idx[t] != seq_idx[t-1] (t >= 1), else 1. One block for
  * forward and backward. x, a_gate, x_gate, y and their gradients have `dtype`,
- * shape (batch, seqlen, dim) and any element strides (not negative; the channels
- * of a step, and 16 steps of a channel, within 4 GiB, else MCPU_ERR_UNSUPPORTED);
+ * shape (batch, seqlen, dim) and any element strides (not negative; 16 steps of a
+ * row's channels within 4 GiB, else MCPU_ERR_UNSUPPORTED);
  * everything else is float32 and contiguous. No counterpart in the reference. */
 typedef struct mcpu_gated_scan_args {
   const void* x;

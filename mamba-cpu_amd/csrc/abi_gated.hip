@@ -18,13 +18,13 @@ bool any_negative(std::initializer_list<const int64_t*> strides, int n) {
 
 int64_t chunks_of(const mcpu_gated_scan_args* a) { return (a->seqlen + kGatedChunk - 1) / kGatedChunk; }
 
-// The kernels reach an element by 32-bit byte offsets from a segment's first step.
+// The kernels reach an element by 32-bit byte offsets, of its channel and its
+// step, from a segment's first step; the sum stays below 2^32, where buffer
+// accesses end.
 bool in_reach(const mcpu_gated_scan_args* a, std::initializer_list<const int64_t*> strides) {
-  constexpr int64_t kReach = int64_t{1} << 32;
+  const int64_t reach = (int64_t{1} << 32) / dtype_size(a->dtype), dim = a->dim > 0 ? a->dim : 1;
   for (const int64_t* s : strides)
-    if (s[2] >= kReach / (dtype_size(a->dtype) * (a->dim > 0 ? a->dim : 1)) ||
-        s[1] >= kReach / (dtype_size(a->dtype) * kGatedT))
-      return false;
+    if (s[2] >= reach / dim || s[1] >= reach / kGatedT || dim * s[2] + kGatedT * s[1] >= reach) return false;
   return true;
 }
 

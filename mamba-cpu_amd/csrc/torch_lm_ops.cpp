@@ -57,11 +57,12 @@ void check_gated(const char* name, const Tensor& x, const Tensor& a_gate, const 
                     name, " expects seq_idx as a contiguous int32 tensor of shape (batch, seqlen)");
 }
 
-// A (batch, seqlen, dim) operand within the kernels' reach (32-bit byte offsets
-// over a row's channels and eight of its steps), copied where it is not.
+// A (batch, seqlen, dim) operand within the kernels' reach (a row's channels over
+// 16 steps within 4 GiB), copied where it is not.
 Tensor in_reach(const Tensor& t) {
-  const int64_t reach = (int64_t{1} << 32) / t.element_size();
-  return t.stride(2) < reach / std::max<int64_t>(t.size(2), 1) && t.stride(1) < reach / 8 ? t : t.contiguous();
+  const int64_t reach = (int64_t{1} << 32) / t.element_size(), dim = std::max<int64_t>(t.size(2), 1);
+  const bool in = t.stride(2) < reach / dim && t.stride(1) < reach / 16 && dim * t.stride(2) + 16 * t.stride(1) < reach;
+  return in ? t : t.contiguous();
 }
 
 mcpu_gated_scan_args gated_args(const Tensor& x, const Tensor& a_gate, const Tensor& x_gate, const Tensor& decay,

@@ -344,3 +344,45 @@ def test_recurrence_past_4_gib(room):
         got, ref = got[:, -tail + skip:].detach().float(), ref[:, skip:].detach().float()
         assert ((got - ref).abs() <= 2e-5 * ref.abs().max() + 2.0 ** -7 * ref.abs()).all(), name
     assert torch.equal(y[:, 5000], y[:, 500_000]) and y[0, 5000, 0] > 0  # settled
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [130_000_000, 140_000_000, 270_000_000])
+def test_recurrence_steps_far_apart(room, step):
+    """16 steps of 2-byte elements on both sides of 4 GiB, and 8 steps beyond it."""
+    from mamba_cpu import gated_linear_scan_fn
+
+    l, d = 20, 70
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, a, i, dy = (torch.randn(1, l, d, device=DEV, generator=g).bfloat16() for _ in range(4))
+    decay = torch.randn(d, device=DEV, generator=g)
+    store = torch.empty((l - 1) * step + d, device=DEV, dtype=torch.bfloat16)
+
+    def run(x, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, a, i)]
+        y = gated_linear_scan_fn(*leaves, decay)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = run(x, dy)
+    far = store.as_strided((1, l, d), (0, step, 1))
+    far.copy_(x)
+    got = run(far, dy)
+    far.copy_(dy)
+    got += run(x, far)
+    for have, ref in zip(got, want + want):
+        assert torch.equal(have, ref)
+
+
+def test_abi_refuses_steps_too_far_apart():
+    from mamba_cpu import _C
+
+    a = _C.GatedScanArgs()
+    a.x = a.a_gate = a.x_gate = a.decay = a.y = 16  # placeholders: never dereferenced
+    a.batch, a.seqlen, a.dim, a.c, a.dtype = 1, 20, 70, 8.0, _C.MCPU_BF16
+    for s in (a.x_stride, a.a_stride, a.i_stride, a.y_stride):
+        s[:] = (1400, 70, 1)
+    assert _C.lib.mcpu_gated_scan_ckpt_size(ctypes.byref(a)) == 4 * 2 * 70
+    for far in ((0, 2 ** 27, 1), (0, 1, 2 ** 31 // 70 + 1), (0, 2 ** 26, 2 ** 30 // 70 + 1), (0, 2 ** 62, 2 ** 62)):
+        a.x_stride[:] = far
+        rc = _C.lib.mcpu_gated_scan_fwd(ctypes.byref(a), None, 0, None)
+        assert rc == _C.MCPU_ERR_UNSUPPORTED and "far apart" in _C.lib.mcpu_last_error().decode(), far
