@@ -16,7 +16,9 @@ bool any_negative(std::initializer_list<const int64_t*> strides, int n) {
   return false;
 }
 
-int64_t chunks_of(const mcpu_gated_scan_args* a) { return (a->seqlen + kGatedChunk - 1) / kGatedChunk; }
+int64_t chunks_of(const mcpu_gated_scan_args* a, int waves) {
+  return (a->seqlen + waves * kGatedT - 1) / (waves * kGatedT);
+}
 
 // The kernels reach an element by 32-bit byte offsets, of its channel and its
 // step, from a segment's first step; the sum stays below 2^32, where buffer
@@ -34,7 +36,7 @@ int check_gated(const mcpu_gated_scan_args* a, const char* what) {
   if (!valid_dtype(a->dtype)) return fail(MCPU_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
   const int64_t tiles = (a->dim + 63) / 64;
   if (a->batch > INT_MAX || a->seqlen > (int64_t{1} << 40) || tiles > INT_MAX ||
-      (tiles > 0 && a->batch > 0 && chunks_of(a) > INT_MAX / (tiles * a->batch)))
+      (tiles > 0 && a->batch > 0 && chunks_of(a, kGatedBwdWaves) > INT_MAX / (tiles * a->batch)))
     return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x seqlen x dim too large", what);
   if ((a->decay == nullptr && a->dim > 0) ||
       ((a->x == nullptr || a->a_gate == nullptr || a->x_gate == nullptr) && a->batch * a->seqlen * a->dim > 0))
@@ -51,17 +53,17 @@ int check_gated(const mcpu_gated_scan_args* a, const char* what) {
 size_t ticket_bytes(const mcpu_gated_scan_args* a) {
   return align_up(sizeof(uint32_t) * a->batch * ((a->dim + 63) / 64));
 }
-size_t record_bytes(const mcpu_gated_scan_args* a) {
-  return chunks_of(a) > 1 ? ticket_bytes(a) + align_up(sizeof(uint64_t) * a->batch * chunks_of(a) * a->dim) : 0;
+size_t record_bytes(const mcpu_gated_scan_args* a, int64_t chunks) {
+  return chunks > 1 ? ticket_bytes(a) + align_up(sizeof(uint64_t) * a->batch * chunks * a->dim) : 0;
 }
 int clear_records(GatedScanParams& p, const mcpu_gated_scan_args* a, void* workspace, hipStream_t st) {
   if (p.chunks == 1) return MCPU_OK;
   p.tickets = static_cast<uint32_t*>(workspace);
   p.records = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + ticket_bytes(a));
-  return zero_f32(static_cast<float*>(workspace), static_cast<int64_t>(record_bytes(a) / sizeof(float)), st);
+  return zero_f32(static_cast<float*>(workspace), static_cast<int64_t>(record_bytes(a, p.chunks) / sizeof(float)), st);
 }
 
-GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
+GatedScanParams make_gated(const mcpu_gated_scan_args* a, int waves) {
   GatedScanParams p;
   std::memset(&p, 0, sizeof(p));
   p.x = a->x;
@@ -74,7 +76,7 @@ GatedScanParams make_gated(const mcpu_gated_scan_args* a) {
   p.len = a->seqlen;
   p.dim = a->dim;
   p.c = a->c;
-  p.chunks = chunks_of(a);
+  p.chunks = chunks_of(a, waves);
   p.ckpt = a->ckpt;
   for (int i = 0; i < 3; ++i) {
     p.sx[i] = a->x_stride[i];
@@ -107,7 +109,7 @@ extern "C" size_t mcpu_gated_scan_fwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return record_bytes(a);
+  return record_bytes(a, chunks_of(a, kGatedFwdWaves));
 }
 
 extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -122,7 +124,7 @@ extern "C" int mcpu_gated_scan_fwd(const mcpu_gated_scan_args* a, void* workspac
     return fail(MCPU_ERR_UNSUPPORTED, "%s: a row's steps or channels lie too far apart", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_gated_scan_fwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
-  GatedScanParams p = make_gated(a);
+  GatedScanParams p = make_gated(a, kGatedFwdWaves);
   p.y = a->y;
   p.last = a->last_state;
   if (a->batch == 0 || a->dim == 0) return MCPU_OK;
@@ -140,7 +142,8 @@ extern "C" size_t mcpu_gated_scan_bwd_workspace_size(const mcpu_gated_scan_args*
     clear_error();
     return 0;
   }
-  return record_bytes(a) + align_up(sizeof(float) * a->batch * chunks_of(a) * a->dim);
+  const int64_t chunks = chunks_of(a, kGatedBwdWaves);
+  return record_bytes(a, chunks) + align_up(sizeof(float) * a->batch * chunks * a->dim);
 }
 
 extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -168,7 +171,7 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
                ? MCPU_OK
                : hip_status(gated_edge_launch(a->dlast_state, a->dinitial_state, a->batch * a->dim, st), what);
   }
-  GatedScanParams p = make_gated(a);
+  GatedScanParams p = make_gated(a, kGatedBwdWaves);
   p.dy = a->dy;
   p.dlast = a->dlast_state;
   p.dx = a->dx;
@@ -176,7 +179,7 @@ extern "C" int mcpu_gated_scan_bwd(const mcpu_gated_scan_args* a, void* workspac
   p.dx_gate = a->dx_gate;
   p.ddecay = a->ddecay;
   p.dinit = a->dinitial_state;
-  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + record_bytes(a));
+  p.ddecay_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + record_bytes(a, p.chunks));
   if (int rc = clear_records(p, a, workspace, st)) return rc;
   return hip_status(gated_scan_bwd_launch(p, a->dtype, st), "gated_scan_bwd launch");
 }

@@ -8,12 +8,12 @@
 // with k_t = 0 at the first step of another sequence of a packed row, else 1.
 // The step h -> a h + b composes as (P, S): h -> P h + S, so time is split: a
 // wave takes kGatedT = 16 consecutive steps of 64 channels in registers and forms
-// their (P, S), the workgroup's 8 waves exchange theirs through LDS, and each
+// their (P, S), the workgroup's waves exchange theirs through LDS, and each
 // wave then knows the state in front of its segment, given the one in front of
 // the workgroup's chunk.
 //
-// A workgroup takes one chunk of 128 steps of 64 channels, so that every length
-// fills the chip and every input is read once. The state in front of a chunk
+// A workgroup takes one chunk (128 steps forward, 64 backward) of 64 channels, so
+// that every length fills the chip and every input is read once. The state in front of a chunk
 // comes from the chunks before it: a workgroup publishes its (P, S) as soon as
 // it has them (its inputs stay in registers), then looks back, a predecessor per
 // wave, until nothing older matters: a predecessor that knows the state behind
@@ -28,17 +28,17 @@
 //
 // Bound: the inputs and outputs once, for 8 x 2048 x 1536 bf16 201 MB forward
 // and 352 MB backward, and vector issue: 43 and 68 instructions a step and
-// channel, 0.56 to 0.66 of the cycles. Measured there: forward 57 us (3.5 TB/s),
-// backward 98 us (3.6 TB/s), a training step with its clears and the decay's sum
-// 156 us. Other splits, for the same step:
+// channel. Measured there: forward 57 us (3.5 TB/s), backward 87 us (4.0 TB/s), a
+// training step with its clears and the decay's sum 149 us. Other splits, for the
+// same step:
 //   two launches a direction, the first for every split's (P, S)   221 us
-//   8 steps a wave: twice the chunks, each with its exchange and
+//   8 steps a wave: twice the segments, each with its exchange and
 //   look back, which are 20 instructions a step then               166 us
 //   workgroups that stay and take chunk after chunk, the next one's
 //   inputs requested ahead: the chain of a tile gets longer        276 us
 // What is left is that chain, the time from a chunk's inputs to its (0, h), and
-// that loads, arithmetic and the wait of one workgroup overlap with only two (in
-// the backward) or three others' on a CU.
+// that loads, arithmetic and the wait of one workgroup overlap with only three
+// others' on a CU.
 //
 // Backward, with g_t = dL/dh_t:  g_t = dy_t + k_{t+1} a_{t+1} g_{t+1},
 //   dx = g m iota          dx_gate = dx x (1 - iota)
@@ -53,7 +53,7 @@
 namespace mcpu {
 namespace {
 
-constexpr int TS = kGatedT, W = kGatedWaves;
+constexpr int TS = kGatedT;
 
 // ---- gates -----------------------------------------------------------------------------
 // The exponentials are v_exp_f32's: for a gate x it is off by |x| 2^-24 at
@@ -95,7 +95,7 @@ struct Place {
 // Which chunk of its row's tile the workgroup takes: the next one in the order of
 // time, from the last on with LAST_FIRST. A counter for each tile: when thousands
 // of workgroups share one, each waits 1.4 us for it, 5 us at the start.
-template <bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
+template <int W, bool LAST_FIRST> __device__ __forceinline__ Place place(const GatedScanParams& p) {
   __shared__ uint32_t ticket;
   Place q;
   q.lane = threadIdx.x & 63;
@@ -178,7 +178,7 @@ __device__ __forceinline__ uint64_t peek(const uint64_t* at) {
 }
 
 constexpr int kWindows = 4;  // windows of W chunks that are kept
-struct Exchange {
+template <int W> struct Exchange {
   float2 agg[W][64];                // the segments' (P, S)
   float2 win[kWindows + 2][W][64];  // what the waves found of W neighbouring chunks; two for those further back
 };
@@ -186,8 +186,8 @@ struct Exchange {
 // The state that enters the wave's segment, from the segments' (P, S) and
 // `edge`, the state that enters the row's first chunk (in the direction of the
 // scan: DIR 1 forward, -1 backward). `out` is the state behind the chunk.
-template <int DIR>
-__device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Place& q, Exchange& x, float P, float S,
+template <int W, int DIR>
+__device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Place& q, Exchange<W>& x, float P, float S,
                                             float edge, float& in, float& out) {
   x.agg[q.w][q.lane] = make_float2(P, S);
   __syncthreads();
@@ -257,9 +257,11 @@ __device__ __forceinline__ void scan_chunks(const GatedScanParams& p, const Plac
 // ---- forward -----------------------------------------------------------------------------
 // SEQ: packed sequences.
 
-template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_fwd_kernel(const GatedScanParams p) {
-  __shared__ Exchange exchange;
-  const Place q = place<false>(p);
+template <typename T, bool SEQ>
+__global__ __launch_bounds__(64 * kGatedFwdWaves) void gated_fwd_kernel(const GatedScanParams p) {
+  constexpr int W = kGatedFwdWaves;
+  __shared__ Exchange<W> exchange;
+  const Place q = place<W, false>(p);
   const Column<T> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), y(p.y, p.sy, p, q);
   uint32_t rx[TS], ra[TS], ri[TS];
 #pragma unroll
@@ -302,7 +304,7 @@ template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_
   walk(S, [&](int i) { P *= a[i]; });
   P = cut != 0 ? 0.f : fmaxf(P, kFaint);  // a NaN in P is one in S, too
   float h, out;
-  scan_chunks<1>(p, q, exchange, P, S, edge, h, out);
+  scan_chunks<W, 1>(p, q, exchange, P, S, edge, h, out);
   if (!q.live) return;
   if (q.w == 0 && q.chunk == p.chunks - 1 && p.last != nullptr) p.last[q.b * p.dim + q.d] = out;
   if (q.n <= 0) return;
@@ -315,10 +317,11 @@ template <typename T, bool SEQ> __global__ __launch_bounds__(64 * W) void gated_
 // ---- backward ----------------------------------------------------------------------------
 
 template <typename T, bool SEQ>
-__global__ __launch_bounds__(64 * W, 4) void gated_bwd_kernel(const GatedScanParams p) {
+__global__ __launch_bounds__(64 * kGatedBwdWaves, 4) void gated_bwd_kernel(const GatedScanParams p) {
+  constexpr int W = kGatedBwdWaves;
   constexpr bool EXACT = sizeof(T) == 4;
-  __shared__ Exchange exchange;
-  const Place q = place<true>(p);
+  __shared__ Exchange<W> exchange;
+  const Place q = place<W, true>(p);
   const Column<T> x(p.x, p.sx, p, q), ag(p.a_gate, p.sa, p, q), ig(p.x_gate, p.si, p, q), dy(p.dy, p.sdy, p, q);
   uint32_t rx[TS], ra[TS], ri[TS], rd[TS];
 #pragma unroll
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(64 * W, 4) void gated_bwd_kernel(const GatedScanPar
     h = kah + u;
     // These five are to be formed here: moved down to their use, their
     // operands would be kept instead, in twice the registers. 128 (the launch
-    // bound) leave room for two workgroups a CU.
+    // bound) leave room for four workgroups a CU.
     asm volatile("" : "+v"(gx[i]), "+v"(gi[i]), "+v"(ga[i]), "+v"(gd[i]), "+v"(ka[i]));
   }
   // 16-bit dy waits two to a register.
@@ -387,7 +390,7 @@ __global__ __launch_bounds__(64 * W, 4) void gated_bwd_kernel(const GatedScanPar
 #pragma unroll
   for (int i = 0; i < TS / PACK; ++i) asm volatile("" : "+v"(kept[i]));  // and is not kept widened
   float G, out, acc = 0.f;  // acc: this lane's sum of e rho
-  scan_chunks<-1>(p, q, exchange, P, S, edge, G, out);
+  scan_chunks<W, -1>(p, q, exchange, P, S, edge, G, out);
   if (q.live && q.w == 0 && q.chunk == 0 && p.dinit != nullptr) p.dinit[q.b * p.dim + q.d] = out;
   const Column<T> dx(p.dx, p.sdx, p, q), da(p.da_gate, p.sda, p, q), di(p.dx_gate, p.sdi, p, q);
 #pragma unroll
@@ -481,8 +484,9 @@ static dim3 gated_grid(const GatedScanParams& p) {
 hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, true>), gated_grid(p), dim3(64 * W), 0, st, p);
-    else hipLaunchKernelGGL((gated_fwd_kernel<T, false>), gated_grid(p), dim3(64 * W), 0, st, p);
+    const dim3 grid = gated_grid(p), block(64 * kGatedFwdWaves);
+    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gated_fwd_kernel<T, false>), grid, block, 0, st, p);
   });
   return hipGetLastError();
 }
@@ -490,8 +494,9 @@ hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_
 hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), gated_grid(p), dim3(64 * W), 0, st, p);
-    else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), gated_grid(p), dim3(64 * W), 0, st, p);
+    const dim3 grid = gated_grid(p), block(64 * kGatedBwdWaves);
+    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), grid, block, 0, st, p);
   });
   hipLaunchKernelGGL(gated_ddecay_kernel, dim3(static_cast<unsigned>((p.dim + 63) / 64)), dim3(64 * kReduceWaves), 0,
                      st, p);
