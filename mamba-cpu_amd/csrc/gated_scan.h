@@ -9,7 +9,7 @@
 namespace mcpu {
 
 constexpr int kGatedT = 16;  // steps of a wave's segment: the forward keeps the state before each
-// Waves of a workgroup, which takes one chunk of a segment each. The backward
+// Waves of a workgroup, with one segment of its chunk each. The backward
 // holds twice the registers: with 4 waves four of its workgroups share a CU
 // instead of two (87 against 98 us for 8 x 2048 x 1536 bf16, 158 against 161 for
 // 16384 x 2560). The forward has three or more either way, and longer chunks

@@ -27,9 +27,9 @@
 // is read, and either of a chunk's two is right, so no fence is needed.
 //
 // Bound: the inputs and outputs once, for 8 x 2048 x 1536 bf16 201 MB forward
-// and 352 MB backward, and vector issue: 43 and 68 instructions a step and
+// and 352 MB backward, and vector issue: 43 and 65 instructions a step and
 // channel. Measured there: forward 57 us (3.5 TB/s), backward 87 us (4.0 TB/s), a
-// training step with its clears and the decay's sum 149 us. Other splits, for the
+// training step with its clears and the decay's sum 148 us. Other splits, for the
 // same step:
 //   two launches a direction, the first for every split's (P, S)   221 us
 //   8 steps a wave: twice the segments, each with its exchange and
