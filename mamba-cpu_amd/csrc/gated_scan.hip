@@ -13,12 +13,12 @@
 // the workgroup's chunk.
 //
 // A workgroup takes one chunk (128 steps forward, 64 backward) of 64 channels, so
-// that every length fills the chip and every input is read once. The state in front of a chunk
-// comes from the chunks before it: a workgroup publishes its (P, S) as soon as
-// it has them (its inputs stay in registers), then looks back, a predecessor per
-// wave, until nothing older matters: a predecessor that knows the state behind
-// its chunk has published that, as (0, h), in the place of its (P, S). Its own
-// (0, h) is published before its outputs are written.
+// that every length fills the chip and every input is read once. The state in
+// front of a chunk comes from the chunks before it: a workgroup publishes its
+// (P, S) as soon as it has them (its inputs stay in registers), then looks back,
+// a predecessor per wave, until nothing older matters: a predecessor that knows
+// the state behind its chunk has published that, as (0, h), in the place of its
+// (P, S). Its own (0, h) is published before its outputs are written.
 // Every wait ends: the chunks of a row's tile are taken by ticket, in the order
 // of time, so the chunks a workgroup waits for have been taken by workgroups
 // that run or have ended, and a workgroup publishes its (P, S) before it waits.
