@@ -45,7 +45,7 @@ template <typename T> __global__ __launch_bounds__(256) void embedding_fwd_kerne
 
 constexpr int kSortWaves = 16;
 constexpr int kSortIds = 512;  // most ids of one workgroup's range
-constexpr int kSortBatch = 8;  // ids per lane on their way at once
+constexpr int kSortBatch = 16;  // ids per lane on their way at once
 
 __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const EmbeddingParams p, int range) {
   __shared__ int count[kSortWaves][kSortIds];  // tokens of (wave, id), then where the next one goes
@@ -62,32 +62,38 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_sort_kernel(const E
   const int64_t run = ((p.tokens + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int64_t t0 = w * run, t1 = t0 + run < p.tokens ? t0 + run : p.tokens;
   int under = 0;
+  int slot[kSortBatch];  // the id's place in the range; -1 not in it, -2 below it
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t tb = t0; tb < t1; tb += 64 * kSortBatch) {
-      int64_t ids[kSortBatch];
+      // A run of one batch is read once.
+      if (pass == 0 || run > 64 * kSortBatch) {
+        int64_t ids[kSortBatch];
 #pragma unroll
-      for (int k = 0; k < kSortBatch; ++k) {
-        const int64_t t = tb + k * 64 + lane;
-        ids[k] = t < t1 ? id_at(p, t) : -1;
+        for (int k = 0; k < kSortBatch; ++k) {
+          const int64_t t = tb + k * 64 + lane;
+          ids[k] = t < t1 ? id_at(p, t) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k)
+          slot[k] = ids[k] >= lo ? (ids[k] < hi ? static_cast<int>(ids[k] - lo) : -1) : ids[k] >= 0 ? -2 : -1;
       }
 #pragma unroll
       for (int k = 0; k < kSortBatch; ++k) {
-        const bool in = ids[k] >= lo && ids[k] < hi;
-        const int slot = in ? static_cast<int>(ids[k] - lo) : -1;
+        if (tb + k * 64 >= t1) break;
         if (pass == 0) {
-          under += __popcll(__ballot(ids[k] >= 0 && ids[k] < lo));
-          if (in) atomicAdd(&count[w][slot], 1);
+          under += __popcll(__ballot(slot[k] == -2));
+          if (slot[k] >= 0) atomicAdd(&count[w][slot[k]], 1);
           continue;
         }
-        uint64_t left = __ballot(in);
+        uint64_t left = __ballot(slot[k] >= 0);
         while (left != 0) {
           const int lead = __builtin_ctzll(left);
-          const int s = __builtin_amdgcn_readlane(slot, lead);
-          const uint64_t same = __ballot(slot == s);
+          const int s = __builtin_amdgcn_readlane(slot[k], lead);
+          const uint64_t same = __ballot(slot[k] == s);
           int first = 0;
           if (lane == lead) first = atomicAdd(&count[w][s], __popcll(same));
           first = __builtin_amdgcn_readlane(first, lead);
-          if (slot == s)
+          if (slot[k] == s)
             p.order[first + __popcll(same & ((1ull << lane) - 1))] = static_cast<int32_t>(tb + k * 64 + lane);
           left &= ~same;
         }
