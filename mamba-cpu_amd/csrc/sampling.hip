@@ -25,9 +25,12 @@
 //  - bins: counts or masses of kBins equal steps below M, and the sorted list of
 //    the one bin that holds the cut.
 //  - radix descent over the keys, 8 bits at a time, where a list overflows:
-//    masses of equal logits, or a cut far below M.
-// Masses in bins are added as integers, in units of 2^-31 of the total: the sums
-// are exact in any order, so LDS atomics leave the result unchanged. Where
+//    masses of equal logits, or a cut far below M; and for top-p near 1.
+// Masses are added as integers: the sums are exact in any order, so LDS atomics
+// leave the result unchanged. Bins count in units of 2^-31 of the total, each
+// logit to the nearest: the cut is off by at most vocab / 2 units, which is allowed
+// up to 1/16 of what top-p cuts off (and 2^-13 of the total). Beyond that, the
+// radix descent counts in 64 bits. Where
 // nothing is cut for any row, sample_slice_kernel takes rows in slices instead,
 // so that few rows fill the chip, and sample_join_kernel compares their winners.
 //
@@ -322,40 +325,53 @@ template <bool BY_MASS, typename R> __device__ __forceinline__ uint32_t units(co
   return BY_MASS ? static_cast<uint32_t>(fmaf(row.weight_fast(l), unit, 0.5f)) : 1u;
 }
 
-// The shortest prefix of `from` that holds `want` units, the last token
-// counted if any of it is wanted; want >= 1 and at most what `from` holds. By
-// radix descent over the keys.
+// The shortest prefix of `from` that holds what is wanted, the last token
+// counted if any of it is: BY_MASS the fraction `part` of its mass, else `count`
+// tokens (at least 1 and at most what `from` holds). By radix descent over the
+// keys. Masses are integers of 2^(62 - bits of vocab) to a weight of 1, so that a
+// row's sum fits 63 bits; what is wanted is taken from their own sum, so that it
+// is there to be found.
 template <bool BY_MASS, typename R>
-__device__ Cut radix_cut(const R& row, const Cut& from, uint32_t want, float unit, Shared& s) {
+__device__ Cut radix_cut(const R& row, const Cut& from, uint32_t count, float part, Shared& s) {
+  auto* const bins = reinterpret_cast<unsigned long long*>(s.bins);
+  const float one = ldexpf(1.0f, 30 + __builtin_clz(row.vocab));
+  auto units = [&](float l) -> uint64_t { return BY_MASS ? static_cast<uint64_t>(row.weight_fast(l) * one) : 1u; };
   uint32_t prefix = 0, mask = 0;  // the key's bits found so far, and which they are
+  uint64_t left = count;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) s.bins[threadIdx.x] = 0;
+    if (threadIdx.x < 256) bins[threadIdx.x] = 0;
     __syncthreads();
     row.each([&](int i, float l) {
       const uint32_t k = key_of(l);
-      if ((k & mask) == prefix && from.has(l, i))
-        atomicAdd(&s.bins[(k >> shift) & 255], units<BY_MASS>(row, l, unit));
+      if ((k & mask) == prefix && from.has(l, i)) atomicAdd(&bins[(k >> shift) & 255], units(l));
     });
     __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t left = want;
-      int bin = 255;
-      for (; bin > 0 && s.bins[bin] < left; --bin) left -= s.bins[bin];
-      s.pick = static_cast<uint32_t>(bin);
-      s.left = left;
+    // Thread t has bin 255 - t, of the largest keys first.
+    const uint64_t mine = threadIdx.x < 256 ? bins[255 - threadIdx.x] : 0;
+    const uint64_t before = group_before(mine, s.list);
+    if (BY_MASS && shift == 24) {
+      if (threadIdx.x == kThreads - 1) s.entry = before + mine;  // the whole, at least the largest logit's
+      __syncthreads();
+      const double want = ceil(static_cast<double>(part) * static_cast<double>(s.entry));
+      left = want < 1.0 ? 1 : min(static_cast<uint64_t>(want), s.entry);
+      __syncthreads();
+    }
+    if (before < left && before + mine >= left) {
+      s.pick = 255 - threadIdx.x;
+      s.entry = left - before;
     }
     __syncthreads();
     prefix |= s.pick << shift;
     mask |= 255u << shift;
-    want = s.left;
+    left = s.entry;
     __syncthreads();
   }
-  // `want` units of the tokens with exactly this key, by index: how many tokens
+  // What is left of the tokens with exactly this key, by index: how many tokens
   // that is (they count the same), then where the last of them lies. A wave
   // looks at a run of the row.
   const float edge = value_of(prefix);
-  const uint32_t each = max(units<BY_MASS>(row, edge, unit), 1u);
-  want = (want + each - 1) / each;
+  const uint64_t each = max(units(edge), uint64_t{1});
+  const uint32_t want = static_cast<uint32_t>((left + each - 1) / each);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int run = ((row.vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int t0 = w * run, t1 = min(t0 + run, row.vocab);
@@ -387,10 +403,11 @@ __device__ Cut radix_cut(const R& row, const Cut& from, uint32_t want, float uni
 }
 
 // The same by bins of equal width below M: as far as the row reaches (`low`),
-// at most 24 T (where w is 4e-11); the last bin takes what lies beyond.
+// at most 24 T (where w is 4e-11); the last bin takes what lies beyond. `want` is
+// in units. False where that bin holds the cut, or the cut's bin too many logits.
 template <bool BY_MASS, typename R>
-__device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from, uint32_t want, float unit,
-                                        Shared& s) {
+__device__ __forceinline__ bool bins_cut(const R& row, float low, const Cut& from, uint32_t want, float unit, Shared& s,
+                                         Cut& cut) {
   const float scale = (kBins - 1) / fmaxf(fminf(24.0f * row.temperature, row.top - low), 1e-30f);
   auto bin_of = [&](float l) {
     return static_cast<int>(__builtin_amdgcn_fmed3f((l - row.ref) * -scale, 0.f, kBins - 1.0f));
@@ -447,13 +464,24 @@ __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from
       const uint32_t at = group_before(unit_here, s.u32);
       if (in && at < left && at + unit_here >= left) s.entry = e;
       __syncthreads();
-      const Cut cut{value_of(s.entry >> 32), 0xffffffffu - static_cast<uint32_t>(s.entry)};
+      cut = Cut{value_of(s.entry >> 32), 0xffffffffu - static_cast<uint32_t>(s.entry)};
       __syncthreads();
-      return cut;
+      return true;
     }
   }
   __syncthreads();
-  return radix_cut<BY_MASS>(row, from, want, unit, s);
+  return false;
+}
+
+// `total`: the mass of `from`.
+template <bool BY_MASS, typename R>
+__device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from, uint32_t count, float part,
+                                        float total, Shared& s) {
+  Cut cut;
+  const bool bins = !BY_MASS || row.vocab * 0x1p-28f <= fminf(1.0f - part, 0x1p-9f);  // 16 vocab / 2 units
+  const uint32_t want = BY_MASS ? static_cast<uint32_t>(fmaxf(ceilf(part * 0x1p31f), 1.0f)) : count;
+  if (bins && bins_cut<BY_MASS>(row, low, from, want, BY_MASS ? 0x1p31f / total : 1.0f, s, cut)) return cut;
+  return radix_cut<BY_MASS>(row, from, count, part, s);
 }
 
 // The largest key of the threads' maxima that at least `want` of them reach,
@@ -769,18 +797,19 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
       Cut kept{-inf, static_cast<uint32_t>(row.vocab - 1)};  // everything
       if (k > 0 || by_p) low = -group_max(-low, s.f32);
       if (k > 0) {
-        kept = find_cut<false>(row, low, kept, static_cast<uint32_t>(k), 1.0f, s);
+        kept = find_cut<false>(row, low, kept, static_cast<uint32_t>(k), 0.f, 0.f, s);
         if (by_p) {
           row.each([&](int i, float l) { total += kept.has(l, i) ? row.weight_fast(l) : 0.f; });
           total = group_fsum(total, s.f32);
         }
       }
-      if (by_p) {
-        const float want = ceilf(part * 0x1p31f);
-        kept = find_cut<true>(row, low, kept, want < 1.0f ? 1 : static_cast<uint32_t>(want), 0x1p31f / total, s);
-      }
+      if (by_p) kept = find_cut<true>(row, low, kept, 0, part, total, s);
       token = k > 0 || by_p || min_p > 0.f ? race<true>(row, kept, min_p, noise, s)
                                            : race<false>(row, kept, min_p, noise, s);
+      if (token == 0xffffffffu) {  // no score is a number (an infinite logit over infinite noise): the first token
+        row.each([&](int i, float l) { token = l == m ? min(token, static_cast<uint32_t>(i)) : token; });
+        token = group_min(token, s.u32);
+      }
     }
   }
   if (threadIdx.x == 0) {
