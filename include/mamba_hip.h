@@ -739,7 +739,7 @@ typedef struct mcpu_sample_args {
   const float* temperature_rows;  /* (rows), optional; likewise below */
   const float* top_p_rows;
   const float* min_p_rows;
-  const int32_t* top_k_rows;
+  const int32_t* top_k_rows;      /* 0 or below: off */
   int64_t* token;           /* (rows) */
   float* logprob;           /* (rows), optional */
   int32_t dtype;

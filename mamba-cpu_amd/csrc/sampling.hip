@@ -675,7 +675,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
   int k = p.top_k_rows != nullptr ? p.top_k_rows[r] : p.top_k;
   const float top_p = p.top_p_rows != nullptr ? p.top_p_rows[r] : p.top_p;
   const float min_p = fminf(p.min_p_rows != nullptr ? p.min_p_rows[r] : p.min_p, 1.0f);
-  if (k >= row.vocab) k = 0;
+  if (k < 0 || k >= row.vocab) k = 0;  // off
 
   const float inf = __builtin_inff();
   float m = -inf, low = inf;

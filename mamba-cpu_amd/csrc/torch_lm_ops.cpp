@@ -583,7 +583,7 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits_in, const optional<Tensor
   a.temperature = static_cast<float>(temperature);
   a.top_p = static_cast<float>(top_p);
   a.min_p = static_cast<float>(min_p);
-  a.top_k = static_cast<int32_t>(std::min<int64_t>(top_k, INT32_MAX));
+  a.top_k = static_cast<int32_t>(std::clamp<int64_t>(top_k, -1, INT32_MAX));  // -1: refused
   if (has(temperature_rows))
     a.temperature_rows = fptr(check_setting(name, "temperature", *temperature_rows, at::kFloat, rows));
   if (has(top_p_rows)) a.top_p_rows = fptr(check_setting(name, "top_p", *top_p_rows, at::kFloat, rows));

@@ -22,13 +22,26 @@ def _(logits, noise, temperature, top_k, top_p, min_p, temperature_rows, top_k_r
             logits.new_empty(rows if logprobs else 0, dtype=torch.float32))
 
 
-def _setting(name, value, dtype, rows, device, off):
+# Each setting's type where it is given per row, and what it is where it is off.
+SETTINGS = {"temperature": (torch.float32, 1.0), "top_k": (torch.int32, 0), "top_p": (torch.float32, 1.0),
+            "min_p": (torch.float32, 0.0)}
+
+
+def setting_rows(name, value, device):
+    """A setting given per row, as the kernel reads it."""
+    dtype = SETTINGS[name][0]
+    if dtype == torch.int32 and value.dtype == torch.int64:
+        value = value.clamp(0, 2 ** 31 - 1)  # below 0 is off, as 0 is
+    return value.to(device=device, dtype=dtype).contiguous()
+
+
+def _setting(name, value, rows, device):
     """(number, per-row tensor or None) of a setting given either way."""
     if not isinstance(value, torch.Tensor):
         return value, None
     if value.shape != (rows,):
         raise ValueError(f"{name} must be a number or a tensor of shape ({rows},), got {tuple(value.shape)}")
-    return off, value.to(device=device, dtype=dtype).contiguous()
+    return SETTINGS[name][1], setting_rows(name, value, device)
 
 
 def sample_fn(logits, noise=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logprobs=False):
@@ -37,8 +50,8 @@ def sample_fn(logits, noise=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
         torch.empty(batch, vocab, device=...).exponential_(); above 0. May be
         None where temperature is the number 0.
     temperature, top_k, top_p, min_p: numbers, or tensors of shape (batch,)
-        with one setting for each row. top_k 0, top_p 1 and min_p 0 are off;
-        temperature 0 takes the largest logit.
+        with one setting for each row. top_k 0 (per row also below 0), top_p 1
+        and min_p 0 are off; temperature 0 takes the largest logit.
     Returns tokens: (batch,) int64 [, logprobs: (batch,) float32, the
     log-softmax of the logits (before temperature and cuts) at the token].
 
@@ -55,10 +68,10 @@ def sample_fn(logits, noise=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     if logits.dim() != 2:
         raise ValueError(f"logits must be (batch, vocab), got {tuple(logits.shape)}")
     rows, dev = logits.shape[0], logits.device
-    t, t_rows = _setting("temperature", temperature, torch.float32, rows, dev, 1.0)
-    k, k_rows = _setting("top_k", top_k, torch.int32, rows, dev, 0)
-    p, p_rows = _setting("top_p", top_p, torch.float32, rows, dev, 1.0)
-    m, m_rows = _setting("min_p", min_p, torch.float32, rows, dev, 0.0)
+    t, t_rows = _setting("temperature", temperature, rows, dev)
+    k, k_rows = _setting("top_k", top_k, rows, dev)
+    p, p_rows = _setting("top_p", top_p, rows, dev)
+    m, m_rows = _setting("min_p", min_p, rows, dev)
     if logits.dtype not in _DTYPES:
         logits = logits.float()
     token, logprob = torch.ops.mamba_cpu.sample(logits, noise, float(t), int(k), float(p), float(m), t_rows, k_rows,

@@ -33,6 +33,7 @@ from mamba_cpu.ops import (
     layer_norm_fn,
     sample_fn,
 )
+from mamba_cpu.ops.sampling import setting_rows
 
 
 class RecurrentBlock(nn.Module):
@@ -133,10 +134,8 @@ def generate(model, prompt, max_new_tokens, temperature=1.0, top_k=0, top_p=1.0,
         return prompt.long()
     batch, vocab = prompt.shape[0], model.embedding.shape[0]
     # Settings given per row are put where the kernel reads them before the capture.
-    as_read = {"temperature": torch.float32, "top_k": torch.int32, "top_p": torch.float32, "min_p": torch.float32}
     settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
-    settings = {k: v.to(dev, as_read[k]).contiguous() if isinstance(v, torch.Tensor) else v
-                for k, v in settings.items()}
+    settings = {k: setting_rows(k, v, dev) if isinstance(v, torch.Tensor) else v for k, v in settings.items()}
     cache = model.new_cache(batch)
     new = torch.empty(batch, max_new_tokens, dtype=torch.long, device=dev)
     noise = torch.empty(batch, vocab, device=dev).exponential_(generator=generator)
