@@ -208,6 +208,7 @@ extern "C" int mcpu_embedding_bwd(const mcpu_embedding_args* a, void* workspace,
   if (int rc = check_embedding(a, what)) return rc;
   if ((a->tokens * a->dim > 0 && a->dout == nullptr) || (a->vocab * a->dim > 0 && a->dweight == nullptr))
     return fail(MCPU_ERR_INVALID, "%s: dout and dweight are required", what);
+  if (a->dim > 65535 * 256) return fail(MCPU_ERR_UNSUPPORTED, "%s: at most 65535 x 256 columns", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_embedding_bwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   if (a->vocab == 0 || a->dim == 0) return MCPU_OK;

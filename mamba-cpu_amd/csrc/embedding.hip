@@ -8,6 +8,7 @@
 // knows both how many tokens lie below its range (where its part of the order
 // starts) and its own tokens; nothing passes between workgroups. An id outside
 // the vocabulary has a zero row and no gradient.
+#include "launch.h"
 #include "lm_params.h"
 #include "lm_math.h"
 
@@ -22,7 +23,7 @@ __device__ __forceinline__ int64_t id_at(const EmbeddingParams& p, int64_t t) {
 // turns are on their way before the first store.
 template <typename T> __global__ __launch_bounds__(256) void embedding_fwd_kernel(const EmbeddingParams p) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= p.tokens) return;
   const int64_t id = id_at(p, t);
   const bool in = id >= 0 && id < p.vocab;
@@ -146,10 +147,11 @@ template <typename T>
 __global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p, int chunks, int tiles) {
   constexpr int kBatch = 16;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (static_cast<int>(blockIdx.x) < chunks * tiles) {
-    const int chunk = blockIdx.x / tiles, c0 = chunk * kEmbedChunk;
+  const int group = static_cast<int>(p.first + blockIdx.x);
+  if (group < chunks * tiles) {
+    const int chunk = group / tiles, c0 = chunk * kEmbedChunk;
     const int rows = min(kEmbedChunk, p.start[p.vocab] - c0);
-    const int64_t i = (blockIdx.x % tiles) * 1024ll + (w * 64 + lane) * 4;
+    const int64_t i = (group % tiles) * 1024ll + (w * 64 + lane) * 4;
     if (rows <= 0 || i - lane * 4 >= p.dim) return;
     const int n = i < p.dim ? upto4(p.dim - i) : 0;
     // Lane k holds position c0 + k: its token, its id, whether its id ends here.
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams
     }
     return;
   }
-  const int64_t v0 = (blockIdx.x - static_cast<int64_t>(chunks) * tiles) * 16 + w * 4;
+  const int64_t v0 = (group - chunks * tiles) * 16ll + w * 4;
   const int64_t at = min(v0 + lane, p.vocab);
   const int starts = lane < 5 ? p.start[at] : 0;
   const float zero[4] = {};
@@ -214,7 +216,7 @@ template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(const EmbeddingParams p) {
   __shared__ float sums[kJoinWaves][256];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c0 = blockIdx.x * kEmbedChunk, valid = p.start[p.vocab];
+  const int chunk = static_cast<int>(p.first + blockIdx.x), c0 = chunk * kEmbedChunk, valid = p.start[p.vocab];
   if (c0 >= valid) return;
   const int64_t id = id_at(p, p.order[min(c0 + kEmbedChunk, valid) - 1]);
   const int first = p.start[id], end = p.start[id + 1];
@@ -225,8 +227,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join_kernel(const E
   float sum[4] = {};
   if (n > 0) {
 #pragma unroll 4
-    for (int64_t c = static_cast<int64_t>(blockIdx.x) + w; c <= last; c += kJoinWaves) {
-      const int slot = c == blockIdx.x && first > c0 ? 1 : 0;
+    for (int64_t c = static_cast<int64_t>(chunk) + w; c <= last; c += kJoinWaves) {
+      const int slot = c == chunk && first > c0 ? 1 : 0;
       float v[4];
       ld_upto4<float>(p.part + (c * 2 + slot) * p.dim, i, n, v);
 #pragma unroll
@@ -252,17 +254,19 @@ template <typename F> void by_dtype(int dtype, F&& f) {
 
 }  // namespace
 
-hipError_t embedding_fwd_launch(const EmbeddingParams& p, hipStream_t st) {
+hipError_t embedding_fwd_launch(EmbeddingParams p, hipStream_t st) {
   by_dtype(p.dtype, [&](auto t) {
-    hipLaunchKernelGGL(embedding_fwd_kernel<decltype(t)>, dim3(static_cast<unsigned>((p.tokens + 3) / 4)), dim3(256),
-                       0, st, p);
+    launch_all((p.tokens + 3) / 4, 256, [&](int64_t first, unsigned groups) {
+      p.first = first;
+      hipLaunchKernelGGL(embedding_fwd_kernel<decltype(t)>, dim3(groups), dim3(256), 0, st, p);
+    });
   });
   return hipGetLastError();
 }
 
 int64_t embedding_chunks(int64_t tokens) { return (tokens + kEmbedChunk - 1) / kEmbedChunk; }
 
-hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st) {
+hipError_t embedding_bwd_launch(EmbeddingParams p, hipStream_t st) {
   // 256 ranges, one per CU, or more where a range would pass the table.
   int64_t range = (p.vocab + 255) / 256;
   if (range > kSortIds) range = kSortIds;
@@ -270,13 +274,18 @@ hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st) {
                      dim3(64 * kSortWaves), 0, st, p, static_cast<int>(range));
   const int chunks = static_cast<int>(embedding_chunks(p.tokens));
   const int tiles = static_cast<int>((p.dim + 1023) / 1024);
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(chunks) * tiles + (p.vocab + 15) / 16);
   by_dtype(p.dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(embedding_dw_kernel<T>, dim3(grid), dim3(256), 0, st, p, chunks, tiles);
+    launch_all(static_cast<int64_t>(chunks) * tiles + (p.vocab + 15) / 16, 256, [&](int64_t first, unsigned groups) {
+      p.first = first;
+      hipLaunchKernelGGL(embedding_dw_kernel<T>, dim3(groups), dim3(256), 0, st, p, chunks, tiles);
+    });
     if (chunks > 1)
-      hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(chunks, static_cast<unsigned>((p.dim + 255) / 256)),
-                         dim3(64 * kJoinWaves), 0, st, p);
+      launch_all(chunks, 64 * kJoinWaves, [&](int64_t first, unsigned groups) {
+        p.first = first;
+        hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(groups, static_cast<unsigned>((p.dim + 255) / 256)),
+                           dim3(64 * kJoinWaves), 0, st, p);
+      });
   });
   return hipGetLastError();
 }

@@ -40,6 +40,7 @@ struct GatedScanParams {
   float* dinit;
   int64_t batch, len, dim;
   int64_t chunks;
+  int64_t first;  // this launch's first workgroup
   float c;
   int64_t sx[3], sa[3], si[3], sy[3], sdy[3], sdx[3], sda[3], sdi[3];  // (batch, len, dim)
 };
@@ -52,15 +53,16 @@ struct GatedStepParams {
   const float* decay;
   void* y;
   int64_t batch, dim;
+  int64_t first;  // this launch's first workgroup
   float c;
   int64_t sst[2], sx[2], sa[2], si[2];
   const int32_t* state_idx;  // state row per batch row, or null
   int64_t state_batch;
 };
 
-hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
-hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st);
+hipError_t gated_scan_fwd_launch(GatedScanParams p, int dtype, hipStream_t st);
+hipError_t gated_scan_bwd_launch(GatedScanParams p, int dtype, hipStream_t st);
 hipError_t gated_edge_launch(const float* from, float* to, int64_t n, hipStream_t st);
-hipError_t gated_step_launch(const GatedStepParams& p, int dtype, hipStream_t st);
+hipError_t gated_step_launch(GatedStepParams p, int dtype, hipStream_t st);
 
 }  // namespace mcpu

@@ -48,6 +48,7 @@
 // from the one the forward kept in front of every segment, in float32 (the
 // stored y may be 16 bits wide).
 #include "gated_scan.h"
+#include "launch.h"
 #include "lm_math.h"
 
 namespace mcpu {
@@ -101,7 +102,7 @@ template <int W, bool LAST_FIRST> __device__ __forceinline__ Place place(const G
   q.lane = threadIdx.x & 63;
   q.w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = static_cast<uint32_t>((p.dim + 63) / 64);
-  const uint32_t rows = tiles * static_cast<uint32_t>(p.batch), row = blockIdx.x % rows;
+  const uint32_t rows = tiles * static_cast<uint32_t>(p.batch), row = (static_cast<uint32_t>(p.first) + blockIdx.x) % rows;
   uint32_t t = 0;
   if (p.chunks > 1) {
     if (threadIdx.x == 0) ticket = atomicAdd(p.tickets + row, 1u);
@@ -419,8 +420,8 @@ __global__ __launch_bounds__(64 * kGatedBwdWaves, 4) void gated_bwd_kernel(const
 constexpr int kReduceWaves = 16;
 
 // No steps: the state that enters leaves.
-__global__ __launch_bounds__(256) void gated_edge_kernel(const float* from, float* to, int64_t n) {
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+__global__ __launch_bounds__(256) void gated_edge_kernel(const float* from, float* to, int64_t n, int64_t first) {
+  const int64_t i = (first + blockIdx.x) * 256 + threadIdx.x;
   if (i < n) to[i] = from == nullptr ? 0.f : from[i];
 }
 
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(256) void gated_edge_kernel(const float* from, floa
 __global__ __launch_bounds__(64 * kReduceWaves) void gated_ddecay_kernel(const GatedScanParams p) {
   __shared__ float sums[kReduceWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t d = blockIdx.x * 64ll + lane;
+  const int64_t d = (p.first + blockIdx.x) * 64 + lane;
   float sum = 0.f;
   if (d < p.dim) {
 #pragma unroll 8
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(64 * kReduceWaves) void gated_ddecay_kernel(const G
 // One token: state (rows, dim) float32 in place.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_step_kernel(const GatedStepParams p) {
-  const int64_t n = blockIdx.x * 256ll + threadIdx.x;
+  const int64_t n = (p.first + blockIdx.x) * 256 + threadIdx.x;
   if (n >= p.batch * p.dim) return;
   const int64_t b = n / p.dim, d = n % p.dim;
   const int64_t row = p.state_idx == nullptr ? b : p.state_idx[b];
@@ -472,41 +473,51 @@ template <typename F> void by_dtype(int dtype, F&& f) {
 }  // namespace
 
 hipError_t gated_edge_launch(const float* from, float* to, int64_t n, hipStream_t st) {
-  hipLaunchKernelGGL(gated_edge_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, from, to, n);
+  launch_all((n + 255) / 256, 256, [&](int64_t first, unsigned groups) {
+    hipLaunchKernelGGL(gated_edge_kernel, dim3(groups), dim3(256), 0, st, from, to, n, first);
+  });
   return hipGetLastError();
 }
 
 // A workgroup for each chunk of 64 channels.
-static dim3 gated_grid(const GatedScanParams& p) {
-  return dim3(static_cast<unsigned>((p.dim + 63) / 64 * p.batch * p.chunks));
-}
+static int64_t gated_groups(const GatedScanParams& p) { return (p.dim + 63) / 64 * p.batch * p.chunks; }
 
-hipError_t gated_scan_fwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
+hipError_t gated_scan_fwd_launch(GatedScanParams p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid = gated_grid(p), block(64 * kGatedFwdWaves);
-    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((gated_fwd_kernel<T, false>), grid, block, 0, st, p);
+    const dim3 block(64 * kGatedFwdWaves);
+    launch_all(gated_groups(p), block.x, [&](int64_t first, unsigned groups) {
+      p.first = first;
+      if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_fwd_kernel<T, true>), dim3(groups), block, 0, st, p);
+      else hipLaunchKernelGGL((gated_fwd_kernel<T, false>), dim3(groups), block, 0, st, p);
+    });
   });
   return hipGetLastError();
 }
 
-hipError_t gated_scan_bwd_launch(const GatedScanParams& p, int dtype, hipStream_t st) {
+hipError_t gated_scan_bwd_launch(GatedScanParams p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid = gated_grid(p), block(64 * kGatedBwdWaves);
-    if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), grid, block, 0, st, p);
+    const dim3 block(64 * kGatedBwdWaves);
+    launch_all(gated_groups(p), block.x, [&](int64_t first, unsigned groups) {
+      p.first = first;
+      if (p.seq_idx != nullptr) hipLaunchKernelGGL((gated_bwd_kernel<T, true>), dim3(groups), block, 0, st, p);
+      else hipLaunchKernelGGL((gated_bwd_kernel<T, false>), dim3(groups), block, 0, st, p);
+    });
   });
-  hipLaunchKernelGGL(gated_ddecay_kernel, dim3(static_cast<unsigned>((p.dim + 63) / 64)), dim3(64 * kReduceWaves), 0,
-                     st, p);
+  launch_all((p.dim + 63) / 64, 64 * kReduceWaves, [&](int64_t first, unsigned groups) {
+    p.first = first;
+    hipLaunchKernelGGL(gated_ddecay_kernel, dim3(groups), dim3(64 * kReduceWaves), 0, st, p);
+  });
   return hipGetLastError();
 }
 
-hipError_t gated_step_launch(const GatedStepParams& p, int dtype, hipStream_t st) {
-  const unsigned grid = static_cast<unsigned>((p.batch * p.dim + 255) / 256);
+hipError_t gated_step_launch(GatedStepParams p, int dtype, hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
-    hipLaunchKernelGGL(gated_step_kernel<decltype(t)>, dim3(grid), dim3(256), 0, st, p);
+    launch_all((p.batch * p.dim + 255) / 256, 256, [&](int64_t first, unsigned groups) {
+      p.first = first;
+      hipLaunchKernelGGL(gated_step_kernel<decltype(t)>, dim3(groups), dim3(256), 0, st, p);
+    });
   });
   return hipGetLastError();
 }

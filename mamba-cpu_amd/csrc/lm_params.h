@@ -27,6 +27,7 @@ struct NormParams {
   float* dbias;  // or null
   float* part;   // (parts, 1 or, with dbias, 2, dim): dweight and dbias partials
   int64_t rows, dim, parts;
+  int64_t first;  // this launch's first workgroup
   int64_t sx, sres, sy, sdy;
   float eps;
   int rms;
@@ -37,8 +38,8 @@ constexpr int64_t kNormWave = 1536;  // longest row of one wave
 constexpr int64_t kNormMost = 8192;  // longest row held in registers
 // Workgroups of the backward: each leaves one partial of dweight and dbias.
 int64_t norm_bwd_parts(int64_t rows, int64_t dim);
-hipError_t norm_fwd_launch(const NormParams& p, hipStream_t st);
-hipError_t norm_bwd_launch(const NormParams& p, hipStream_t st);
+hipError_t norm_fwd_launch(NormParams p, hipStream_t st);
+hipError_t norm_bwd_launch(NormParams p, hipStream_t st);
 
 struct EmbeddingParams {
   const void* ids;  // (tokens) int32 or int64
@@ -51,14 +52,15 @@ struct EmbeddingParams {
   int32_t* start;      // (vocab + 1): where each id's positions start in `order`
   float* part;         // (chunks, 2, dim): partial sums of ids that cross a chunk's edge
   int64_t tokens, vocab, dim, sw, sdo;
+  int64_t first;  // this launch's first workgroup
   float scale;
   int dtype;
 };
 
 constexpr int kEmbedChunk = 32;  // sorted positions per workgroup (at most 64: one per lane)
 int64_t embedding_chunks(int64_t tokens);
-hipError_t embedding_fwd_launch(const EmbeddingParams& p, hipStream_t st);
-hipError_t embedding_bwd_launch(const EmbeddingParams& p, hipStream_t st);
+hipError_t embedding_fwd_launch(EmbeddingParams p, hipStream_t st);
+hipError_t embedding_bwd_launch(EmbeddingParams p, hipStream_t st);
 
 struct SampleParams {
   const void* logits;  // (rows, vocab), row stride sl
@@ -74,12 +76,13 @@ struct SampleParams {
   float* logprob;   // (rows), or null
   void* slices;  // what the slices of uncut rows leave (sample_workspace bytes)
   int64_t rows, vocab, sl, sn;
+  int64_t first;  // this launch's first workgroup
   int dtype;
 };
 
 constexpr int kSampleSlice = 8192;  // logits of a slice
 int64_t sample_slices(const SampleParams& p);
 size_t sample_workspace(const SampleParams& p);
-hipError_t sample_launch(const SampleParams& p, hipStream_t st);
+hipError_t sample_launch(SampleParams p, hipStream_t st);
 
 }  // namespace mcpu

@@ -21,6 +21,7 @@
 //
 // Every sum is float32 in a fixed order. t is rounded before mean(t) is taken
 // from it (no contraction), so that what cancels cancels exactly.
+#include "launch.h"
 #include "lm_params.h"
 #include "lm_math.h"
 
@@ -68,7 +69,8 @@ __device__ __forceinline__ void load_z4(const NormParams& p, int64_t row, int64_
 template <typename T, typename R, int W, int NV>
 __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const NormParams p) {
   __shared__ float slots[3][kGroupWaves];
-  const int64_t row = W == 1 ? blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+  const int64_t group = p.first + blockIdx.x;
+  const int64_t row = W == 1 ? group * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : group;
   if (row >= p.rows) return;
   const float inv = 1.0f / static_cast<float>(p.dim);
   float z[NV][4] = {};
@@ -251,7 +253,7 @@ __device__ __forceinline__ float load_z(const NormParams& p, int64_t row, int64_
 
 template <typename T, typename R> __global__ __launch_bounds__(kThreads) void norm_wide_fwd_kernel(const NormParams p) {
   __shared__ float slots[2][kThreads / 64];
-  const int64_t row = blockIdx.x;
+  const int64_t row = p.first + blockIdx.x;
   float sum = 0.f;
   if (!p.rms)
     for (int64_t i = threadIdx.x; i < p.dim; i += kThreads) sum += load_z<T, R>(p, row, i);
@@ -276,7 +278,7 @@ template <typename T, typename R> __global__ __launch_bounds__(kThreads) void no
 
 template <typename T, typename R> __global__ __launch_bounds__(kThreads) void norm_wide_dx_kernel(const NormParams p) {
   __shared__ float slots[2][kThreads / 64];
-  const int64_t row = blockIdx.x;
+  const int64_t row = p.first + blockIdx.x;
   const float mean = p.rms ? 0.f : p.mean[row], rstd = p.rstd[row];
   float s1 = 0.f, s2 = 0.f;
   for (int64_t i = threadIdx.x; i < p.dim; i += kThreads) {
@@ -346,31 +348,38 @@ int64_t norm_bwd_parts(int64_t rows, int64_t dim) {
   return groups < 1 ? 1 : groups < most ? groups : most;
 }
 
-hipError_t norm_fwd_launch(const NormParams& p, hipStream_t st) {
+hipError_t norm_fwd_launch(NormParams p, hipStream_t st) {
   by_dtypes(p, [&](auto t, auto r) {
     using T = decltype(t);
     using R = decltype(r);
     if (p.dim > kNormMost) {
-      hipLaunchKernelGGL((norm_wide_fwd_kernel<T, R>), dim3(static_cast<unsigned>(p.rows)), dim3(kThreads), 0, st, p);
+      launch_all(p.rows, kThreads, [&](int64_t first, unsigned groups) {
+        p.first = first;
+        hipLaunchKernelGGL((norm_wide_fwd_kernel<T, R>), dim3(groups), dim3(kThreads), 0, st, p);
+      });
       return;
     }
     by_dim(p.dim, [&](auto w, auto nv) {
       constexpr int W = decltype(w)::value, NV = decltype(nv)::value;
-      hipLaunchKernelGGL((norm_fwd_kernel<T, R, W, NV>), dim3(static_cast<unsigned>((p.rows * W + 3) / 4)),
-                         dim3(kThreads), 0, st, p);
+      launch_all((p.rows * W + 3) / 4, kThreads, [&](int64_t first, unsigned groups) {
+        p.first = first;
+        hipLaunchKernelGGL((norm_fwd_kernel<T, R, W, NV>), dim3(groups), dim3(kThreads), 0, st, p);
+      });
     });
   });
   return hipGetLastError();
 }
 
-hipError_t norm_bwd_launch(const NormParams& p, hipStream_t st) {
+hipError_t norm_bwd_launch(NormParams p, hipStream_t st) {
   const unsigned kinds = p.dbias != nullptr ? 2 : 1;
   by_dtypes(p, [&](auto t, auto r) {
     using T = decltype(t);
     using R = decltype(r);
     if (p.dim > kNormMost) {
-      if (p.rows > 0)
-        hipLaunchKernelGGL((norm_wide_dx_kernel<T, R>), dim3(static_cast<unsigned>(p.rows)), dim3(kThreads), 0, st, p);
+      launch_all(p.rows, kThreads, [&](int64_t first, unsigned groups) {
+        p.first = first;
+        hipLaunchKernelGGL((norm_wide_dx_kernel<T, R>), dim3(groups), dim3(kThreads), 0, st, p);
+      });
       hipLaunchKernelGGL((norm_wide_dw_kernel<T, R>),
                          dim3(static_cast<unsigned>((p.dim + kThreads - 1) / kThreads), static_cast<unsigned>(p.parts)),
                          dim3(kThreads), 0, st, p);

@@ -40,6 +40,7 @@
 // is bound by its instructions on one CU: 50280 logits take 0.35 us for each. So
 // NaN are cleaned only in rows that have any, and what few logits need is worked
 // off in loops over bits.
+#include "launch.h"
 #include "lm_math.h"
 #include "lm_params.h"
 
@@ -667,7 +668,7 @@ __device__ __forceinline__ uint32_t race(const Row<T>& row, const Cut& kept, flo
 
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleParams p) {
   __shared__ Shared s;
-  const int64_t r = blockIdx.x;
+  const int64_t r = p.first + blockIdx.x;
   Row<T> row;
   row.logits = static_cast<const T*>(p.logits) + r * p.sl;
   row.vocab = static_cast<int>(p.vocab);
@@ -837,8 +838,9 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   constexpr int E = kPer<T>, NP = kSampleSlice / (kSliceThreads * E);
   __shared__ float f32[kSliceThreads / 64];
   __shared__ uint32_t u32[kSliceThreads / 64];
-  const int64_t r = blockIdx.x / slices;
-  const int first = static_cast<int>(blockIdx.x % slices) * kSampleSlice + static_cast<int>(threadIdx.x) * E;
+  const int group = static_cast<int>(p.first + blockIdx.x);
+  const int64_t r = group / slices;
+  const int first = group % slices * kSampleSlice + static_cast<int>(threadIdx.x) * E;
   Row<T> row;
   row.logits = static_cast<const T*>(p.logits) + r * p.sl;
   row.vocab = static_cast<int>(p.vocab);
@@ -906,13 +908,13 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     }
     at = winner<kSliceThreads / 64>(score, at, f32, u32);
   }
-  if (threadIdx.x == 0) static_cast<Slice*>(p.slices)[blockIdx.x] = Slice{m, m == -inf ? 0.f : sum, at};
+  if (threadIdx.x == 0) static_cast<Slice*>(p.slices)[group] = Slice{m, m == -inf ? 0.f : sum, at};
 }
 
 // A row's token from its slices' winners, one lane each.
 template <typename T, bool GREEDY>
 __global__ __launch_bounds__(64) void sample_join_kernel(const SampleParams p, int slices) {
-  const int64_t r = blockIdx.x;
+  const int64_t r = p.first + blockIdx.x;
   const int lane = threadIdx.x;
   const float inf = __builtin_inff();
   const Slice mine = lane < slices ? static_cast<const Slice*>(p.slices)[r * slices + lane] : Slice{-inf, 0.f, 0u};
@@ -951,20 +953,25 @@ __global__ __launch_bounds__(64) void sample_join_kernel(const SampleParams p, i
   }
 }
 
-template <typename T> void launch(const SampleParams& p, hipStream_t st) {
+template <typename T, bool GREEDY> void launch_slices(SampleParams p, int64_t slices, hipStream_t st) {
+  const int n = static_cast<int>(slices);
+  launch_all(p.rows * slices, kSliceThreads, [&](int64_t first, unsigned groups) {
+    p.first = first;
+    hipLaunchKernelGGL((sample_slice_kernel<T, GREEDY>), dim3(groups), dim3(kSliceThreads), 0, st, p, n);
+  });
+  launch_all(p.rows, 64, [&](int64_t first, unsigned groups) {
+    p.first = first;
+    hipLaunchKernelGGL((sample_join_kernel<T, GREEDY>), dim3(groups), dim3(64), 0, st, p, n);
+  });
+}
+
+template <typename T> void launch(SampleParams p, hipStream_t st) {
   const int64_t slices = sample_slices(p);
-  if (slices == 0) {
-    hipLaunchKernelGGL(sample_row_kernel<T>, dim3(static_cast<unsigned>(p.rows)), dim3(kThreads), 0, st, p);
-    return;
-  }
-  const dim3 grid(static_cast<unsigned>(p.rows * slices)), rows(static_cast<unsigned>(p.rows));
-  if (p.temperature > 0.f) {
-    hipLaunchKernelGGL((sample_slice_kernel<T, false>), grid, dim3(kSliceThreads), 0, st, p, static_cast<int>(slices));
-    hipLaunchKernelGGL((sample_join_kernel<T, false>), rows, dim3(64), 0, st, p, static_cast<int>(slices));
-  } else {
-    hipLaunchKernelGGL((sample_slice_kernel<T, true>), grid, dim3(kSliceThreads), 0, st, p, static_cast<int>(slices));
-    hipLaunchKernelGGL((sample_join_kernel<T, true>), rows, dim3(64), 0, st, p, static_cast<int>(slices));
-  }
+  if (slices > 0) return p.temperature > 0.f ? launch_slices<T, false>(p, slices, st) : launch_slices<T, true>(p, slices, st);
+  launch_all(p.rows, kThreads, [&](int64_t first, unsigned groups) {
+    p.first = first;
+    hipLaunchKernelGGL(sample_row_kernel<T>, dim3(groups), dim3(kThreads), 0, st, p);
+  });
 }
 
 }  // namespace
@@ -982,7 +989,7 @@ int64_t sample_slices(const SampleParams& p) {
 }
 size_t sample_workspace(const SampleParams& p) { return sizeof(Slice) * p.rows * sample_slices(p); }
 
-hipError_t sample_launch(const SampleParams& p, hipStream_t st) {
+hipError_t sample_launch(SampleParams p, hipStream_t st) {
   if (p.dtype == MCPU_F32) launch<float>(p, st);
   else if (p.dtype == MCPU_BF16) launch<bf16>(p, st);
   else launch<f16>(p, st);
