@@ -28,10 +28,11 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 }
 void* ws_ptr(const Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
 
+// Whether a call goes through its autograd function: for a backward, or with a
+// forward-mode tangent, which the function refuses (none has a rule for it).
 bool any_grad(std::initializer_list<optional<Tensor>> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
   for (const optional<Tensor>& t : tensors)
-    if (has(t) && t->requires_grad()) return true;
+    if (has(t) && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
   return false;
 }
 

@@ -62,6 +62,7 @@ def sample_fn(logits, noise=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     kept one with the largest w / noise, which draws from the kept in
     proportion to w; the same noise gives the same token. A row whose logits
     are all -inf or NaN gives token -1 and logprob -inf; NaN counts as -inf.
+    No gradient: the log-probability is cut from the logits' graph.
     """
     if logits.device.type != "cuda":
         raise ValueError(f"mamba_cpu (MI355X build) runs on ROCm GPU tensors, got device {logits.device}")
