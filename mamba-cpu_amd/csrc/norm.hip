@@ -252,26 +252,30 @@ __device__ __forceinline__ float load_z(const NormParams& p, int64_t row, int64_
 }
 
 template <typename T, typename R> __global__ __launch_bounds__(kThreads) void norm_wide_fwd_kernel(const NormParams p) {
-  __shared__ float slots[2][kThreads / 64];
+  __shared__ float slots[3][kThreads / 64];
   const int64_t row = p.first + blockIdx.x;
   float sum = 0.f;
   if (!p.rms)
     for (int64_t i = threadIdx.x; i < p.dim; i += kThreads) sum += load_z<T, R>(p, row, i);
   const float mean = p.rms ? 0.f : group_sum(sum, slots[0]) / p.dim;
-  float sq = 0.f;
+  // As above: what the mean's rounding left is taken out of what is left (off).
+  float sq = 0.f, rest = 0.f;
   for (int64_t i = threadIdx.x; i < p.dim; i += kThreads) {
     const float z = load_z<T, R>(p, row, i) - mean;
     sq = fmaf(z, z, sq);
+    rest += z;
   }
-  const float rstd = 1.0f / sqrtf(group_sum(sq, slots[1]) / p.dim + p.eps);
+  sq = group_sum(sq, slots[1]) / p.dim;
+  const float off = p.rms ? 0.f : group_sum(rest, slots[2]) / p.dim;
+  const float rstd = 1.0f / sqrtf(fmaf(-off, off, sq) + p.eps);
   for (int64_t i = threadIdx.x; i < p.dim; i += kThreads) {
     const float z = load_z<T, R>(p, row, i);
-    const float y = (z - mean) * rstd * p.weight[i] + (p.bias == nullptr ? 0.f : p.bias[i]);
+    const float y = (z - mean - off) * rstd * p.weight[i] + (p.bias == nullptr ? 0.f : p.bias[i]);
     st<T>(p.y, row * p.sy + i, y);
     if (p.res_out != nullptr) st<R>(p.res_out, row * p.dim + i, z);
   }
   if (threadIdx.x == 0) {
-    if (p.mean != nullptr) p.mean[row] = mean;
+    if (p.mean != nullptr) p.mean[row] = mean + off;
     if (p.rstd != nullptr) p.rstd[row] = rstd;
   }
 }
