@@ -49,7 +49,7 @@ def layer_norm_fn(x, weight, bias=None, residual=None, eps=1e-5, prenorm=False, 
     """
     if x.device.type != "cuda":
         raise ValueError(f"mamba_cpu (MI355X build) runs on ROCm GPU tensors, got device {x.device}")
-    in_dtype, res = x.dtype, residual
+    in_dtype, given, res = x.dtype, x, residual
     if in_dtype not in _X_DTYPES:
         x = x.float()
     if res is not None and res.dtype != x.dtype and res.dtype != torch.float32:
@@ -63,5 +63,5 @@ def layer_norm_fn(x, weight, bias=None, residual=None, eps=1e-5, prenorm=False, 
     if not prenorm:
         return y
     if not want:
-        return y, x
+        return y, x if residual_in_fp32 else given
     return y, z if residual is None else z.to(residual.dtype)
