@@ -162,8 +162,10 @@ __device__ __forceinline__ uint32_t starts(const GatedScanParams& p, const Place
 
 // P is 0 where a sequence starts among the steps, and only there: products of
 // decays are held above 0, so that a NaN or an infinity stays in the state of
-// its sequence however much decays, and never enters the next one's.
-constexpr float kFaint = 1.17549435e-38f;  // the smallest normal number
+// its sequence however much decays, and never enters the next one's. The smallest
+// they take is the smallest float32 number (a denormal; the kernels are built with
+// them), so that a state leaves a segment or chunk at most 2^-149 of itself too large.
+constexpr float kFaint = 0x1p-149f;
 __device__ __forceinline__ float after(float2 s, float h) { return s.x == 0.f ? s.y : fmaf(s.x, h, s.y); }
 __device__ __forceinline__ float join(float P, float Q) { return fmaxf(P * Q, fminf(fminf(P, Q), kFaint)); }
 
