@@ -57,9 +57,9 @@ def gated_linear_scan_fn(x, a_gate, x_gate, decay, initial_state=None, seq_idx=N
     x: (batch, seqlen, dim); a_gate, x_gate: like x, before their sigmoids
     decay: (dim,), before its softplus
     initial_state: optional (batch, dim), the state before the first step
-    seq_idx: optional (batch, seqlen) int ids of packed sequences: the state
-        does not cross a change of id; the initial state belongs to the first
-        id of each row
+    seq_idx: optional (batch, seqlen) int32 or int64 (compared in their low 32
+        bits) ids of packed sequences: the state does not cross a change of id;
+        the initial state belongs to the first id of each row
     c: the decay's factor, not negative
     Returns y like x, in x's dtype [, last_state: (batch, dim) float32].
 
@@ -108,6 +108,8 @@ def gated_linear_update(state, x, a_gate, x_gate, decay, c=8.0, state_batch_indi
         if (state_batch_indices.dtype not in (torch.int32, torch.int64)
                 or state_batch_indices.shape != (x.shape[0],)):
             raise ValueError(f"state_batch_indices must be an integer tensor of shape ({x.shape[0]},)")
+        if state_batch_indices.dtype == torch.int64:  # out of range stays out of range
+            state_batch_indices = state_batch_indices.clamp(-1, 2 ** 31 - 1)
         idx = state_batch_indices.to(device=x.device, dtype=torch.int32).contiguous()
     dt = _one_dtype(x, a_gate, x_gate)
     if dt == x.dtype:
