@@ -95,6 +95,9 @@ template <int WAVES = kWaves> __device__ __forceinline__ float group_max(float v
 template <int WAVES = kWaves> __device__ __forceinline__ float group_fsum(float v, float* slot) {
   return group_reduce<WAVES>(v, slot, [](float a, float b) { return a + b; });
 }
+__device__ __forceinline__ uint32_t group_usum(uint32_t v, uint32_t* slot) {
+  return group_reduce<kWaves>(v, slot, [](uint32_t a, uint32_t b) { return a + b; });
+}
 template <int WAVES = kWaves> __device__ __forceinline__ uint32_t group_min(uint32_t v, uint32_t* slot) {
   return group_reduce<WAVES>(v, slot, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
@@ -777,8 +780,9 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
       const bool in = static_cast<int>(threadIdx.x) < n;
       bool holds = few || least || row.vocab <= kThreads;
       if (!holds) {
-        const float w = in ? row.weight_fast(value_of(s.list[threadIdx.x] >> 32)) : 0.f;
-        holds = group_fsum(w, s.f32) > part * total * (2.0f - kNear);
+        // In integers: the list's order, not yet sorted, is another from call to call.
+        const uint32_t mass = in ? units<true>(row, value_of(s.list[threadIdx.x] >> 32), 0x1p31f / total) : 0;
+        holds = group_usum(mass, s.u32) > static_cast<uint32_t>(part * (2.0f - kNear) * 0x1p31f);
       }
       if (holds) {
         const uint64_t e = sorted_entry(s, n);
