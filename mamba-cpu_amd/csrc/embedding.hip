@@ -147,8 +147,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams p, int chunks, int tiles) {
   constexpr int kBatch = 16;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = static_cast<int>(p.first + blockIdx.x);
-  if (group < chunks * tiles) {
+  const uint32_t group = static_cast<uint32_t>(p.first) + blockIdx.x;
+  if (static_cast<int>(group) < chunks * tiles) {
     const int chunk = group / tiles, c0 = chunk * kEmbedChunk;
     const int rows = min(kEmbedChunk, p.start[p.vocab] - c0);
     const int64_t i = (group % tiles) * 1024ll + (w * 64 + lane) * 4;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void embedding_dw_kernel(const EmbeddingParams
     }
     return;
   }
-  const int64_t v0 = (group - chunks * tiles) * 16ll + w * 4;
+  const int64_t v0 = (static_cast<int64_t>(group) - chunks * tiles) * 16 + w * 4;
   const int64_t at = min(v0 + lane, p.vocab);
   const int starts = lane < 5 ? p.start[at] : 0;
   const float zero[4] = {};

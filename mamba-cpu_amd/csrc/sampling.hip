@@ -25,12 +25,12 @@
 //  - bins: counts or masses of kBins equal steps below M, and the sorted list of
 //    the one bin that holds the cut.
 //  - radix descent over the keys, 8 bits at a time, where a list overflows:
-//    masses of equal logits, or a cut far below M; and for top-p near 1.
+//    masses of equal logits, or a cut far below M.
 // Masses are added as integers: the sums are exact in any order, so LDS atomics
 // leave the result unchanged. Bins count in units of 2^-31 of the total, each
 // logit to the nearest: the cut is off by at most vocab / 2 units, which is allowed
-// up to 1/16 of what top-p cuts off (and 2^-13 of the total). Beyond that, the
-// radix descent counts in 64 bits. Where
+// up to 1/16 of what top-p cuts off (and 2^-13 of the total). Beyond that, for
+// top-p near 1, and in the radix descent, masses have 64 bits. Where
 // nothing is cut for any row, sample_slice_kernel takes rows in slices instead,
 // so that few rows fill the chip, and sample_join_kernel compares their winners.
 //
@@ -64,14 +64,17 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 struct Shared {
-  uint32_t bins[kBins];  // bins, and the radix descent's
+  union {
+    uint32_t bins[kBins];
+    uint64_t wide_bins[kBins];  // the radix descent's, too
+  };
   uint64_t list[kThreads];
   float tops[kThreads];  // each thread's largest logit
   uint32_t u32[kWaves];
   float f32[kWaves];
   uint32_t odd[kWaves];
-  uint32_t n, pick, left;
-  uint64_t entry;
+  uint32_t n, pick;
+  uint64_t left, entry;
 };
 
 // Reductions over the WAVES waves of a workgroup, in every thread, ending
@@ -323,41 +326,46 @@ __device__ __forceinline__ void append(Shared& s, float l, int i) {
 
 // ---- cuts -----------------------------------------------------------------------------------
 
-// What a logit counts for a cut: one token, or its mass in units of the total
-// (`unit` of them to a weight of 1, 2^31 to the whole).
-template <bool BY_MASS, typename R> __device__ __forceinline__ uint32_t units(const R& row, float l, float unit) {
-  return BY_MASS ? static_cast<uint32_t>(fmaf(row.weight_fast(l), unit, 0.5f)) : 1u;
+// What a logit counts for a cut: one token, or its mass, `unit` to a weight of 1.
+template <bool BY_MASS, typename U, typename R>
+__device__ __forceinline__ U units(const R& row, float l, float unit) {
+  return BY_MASS ? static_cast<U>(fmaf(row.weight_fast(l), unit, 0.5f)) : U{1};
+}
+// The unit of 64-bit masses: 2^(62 - bits of vocab), so that a row's sum fits 63 bits.
+template <typename R> __device__ __forceinline__ float wide_unit(const R& row) {
+  return ldexpf(1.0f, 30 + __builtin_clz(row.vocab));
+}
+// The fraction `part` of a mass: at least 1 unit, and not more than there is.
+__device__ __forceinline__ uint64_t fraction(float part, uint64_t all) {
+  const double want = ceil(static_cast<double>(part) * static_cast<double>(all));
+  return want < 1.0 ? 1 : min(static_cast<uint64_t>(want), all);
 }
 
 // The shortest prefix of `from` that holds what is wanted, the last token
 // counted if any of it is: BY_MASS the fraction `part` of its mass, else `count`
 // tokens (at least 1 and at most what `from` holds). By radix descent over the
-// keys. Masses are integers of 2^(62 - bits of vocab) to a weight of 1, so that a
-// row's sum fits 63 bits; what is wanted is taken from their own sum, so that it
-// is there to be found.
+// keys. What is wanted of a mass is taken from the sum of its units, so that it is
+// there to be found.
 template <bool BY_MASS, typename R>
 __device__ Cut radix_cut(const R& row, const Cut& from, uint32_t count, float part, Shared& s) {
-  auto* const bins = reinterpret_cast<unsigned long long*>(s.bins);
-  const float one = ldexpf(1.0f, 30 + __builtin_clz(row.vocab));
-  auto units = [&](float l) -> uint64_t { return BY_MASS ? static_cast<uint64_t>(row.weight_fast(l) * one) : 1u; };
+  const float unit = wide_unit(row);
   uint32_t prefix = 0, mask = 0;  // the key's bits found so far, and which they are
   uint64_t left = count;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) bins[threadIdx.x] = 0;
+    if (threadIdx.x < 256) s.wide_bins[threadIdx.x] = 0;
     __syncthreads();
     row.each([&](int i, float l) {
       const uint32_t k = key_of(l);
-      if ((k & mask) == prefix && from.has(l, i)) atomicAdd(&bins[(k >> shift) & 255], units(l));
+      if ((k & mask) == prefix && from.has(l, i)) atomicAdd(&s.wide_bins[(k >> shift) & 255], units<BY_MASS, uint64_t>(row, l, unit));
     });
     __syncthreads();
     // Thread t has bin 255 - t, of the largest keys first.
-    const uint64_t mine = threadIdx.x < 256 ? bins[255 - threadIdx.x] : 0;
+    const uint64_t mine = threadIdx.x < 256 ? s.wide_bins[255 - threadIdx.x] : 0;
     const uint64_t before = group_before(mine, s.list);
     if (BY_MASS && shift == 24) {
       if (threadIdx.x == kThreads - 1) s.entry = before + mine;  // the whole, at least the largest logit's
       __syncthreads();
-      const double want = ceil(static_cast<double>(part) * static_cast<double>(s.entry));
-      left = want < 1.0 ? 1 : min(static_cast<uint64_t>(want), s.entry);
+      left = fraction(part, s.entry);
       __syncthreads();
     }
     if (before < left && before + mine >= left) {
@@ -374,7 +382,7 @@ __device__ Cut radix_cut(const R& row, const Cut& from, uint32_t count, float pa
   // that is (they count the same), then where the last of them lies. A wave
   // looks at a run of the row.
   const float edge = value_of(prefix);
-  const uint64_t each = max(units(edge), uint64_t{1});
+  const uint64_t each = max(units<BY_MASS, uint64_t>(row, edge, unit), uint64_t{1});
   const uint32_t want = static_cast<uint32_t>((left + each - 1) / each);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int run = ((row.vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
@@ -407,27 +415,41 @@ __device__ Cut radix_cut(const R& row, const Cut& from, uint32_t count, float pa
 }
 
 // The same by bins of equal width below M: as far as the row reaches (`low`),
-// at most 24 T (where w is 4e-11); the last bin takes what lies beyond. `want` is
-// in units. False where that bin holds the cut, or the cut's bin too many logits.
-template <bool BY_MASS, typename R>
-__device__ __forceinline__ bool bins_cut(const R& row, float low, const Cut& from, uint32_t want, float unit, Shared& s,
-                                         Cut& cut) {
+// at most 24 T (where w is 4e-11); the last bin takes what lies beyond. False
+// where that bin holds the cut, or the cut's bin too many logits. With U of 32
+// bits, `want` of the units is looked for, else the fraction `part` of their sum.
+template <bool BY_MASS, typename U, typename R>
+__device__ __forceinline__ bool bins_cut(const R& row, float low, const Cut& from, U want, float part, float unit,
+                                         Shared& s, Cut& cut) {
+  U *bins, *slot;
+  if constexpr (sizeof(U) == 4) {
+    bins = s.bins;
+    slot = s.u32;
+  } else {
+    bins = s.wide_bins;
+    slot = s.list;
+  }
   const float scale = (kBins - 1) / fmaxf(fminf(24.0f * row.temperature, row.top - low), 1e-30f);
   auto bin_of = [&](float l) {
     return static_cast<int>(__builtin_amdgcn_fmed3f((l - row.ref) * -scale, 0.f, kBins - 1.0f));
   };
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) bins[i] = 0;
   __syncthreads();
   if (BY_MASS && from.edge == -__builtin_inff()) {  // everything; beyond the row's end the mass is 0
-    row.each([&](int, float l) { atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit)); });
+    row.each([&](int, float l) { atomicAdd(&bins[bin_of(l)], units<BY_MASS, U>(row, l, unit)); });
   } else {
     row.each([&](int i, float l) {
-      if (from.has(l, i)) atomicAdd(&s.bins[bin_of(l)], units<BY_MASS>(row, l, unit));
+      if (from.has(l, i)) atomicAdd(&bins[bin_of(l)], units<BY_MASS, U>(row, l, unit));
     });
   }
   __syncthreads();
-  const uint32_t b0 = s.bins[2 * threadIdx.x], b1 = s.bins[2 * threadIdx.x + 1];
-  const uint32_t before = group_before(b0 + b1, s.u32);
+  const U b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
+  const U before = group_before(b0 + b1, slot);
+  if constexpr (sizeof(U) == 8) {
+    if (threadIdx.x == kThreads - 1) s.entry = before + b0 + b1;
+    __syncthreads();
+    want = fraction(part, s.entry);
+  }
   if (threadIdx.x == 0) {
     s.pick = kBins - 1;  // rounding may leave the sum short of `want`
     s.n = 0;
@@ -440,7 +462,7 @@ __device__ __forceinline__ bool bins_cut(const R& row, float low, const Cut& fro
   }
   __syncthreads();
   const int bin = static_cast<int>(s.pick);
-  const uint32_t left = s.left;
+  const U left = static_cast<U>(s.left);
   if (bin < kBins - 1) {
     // Logits near the bin's range first (two comparisons), then the bin itself:
     // half a bin and four roundings of M wide of it, and bin 0 has no upper end.
@@ -464,8 +486,8 @@ __device__ __forceinline__ bool bins_cut(const R& row, float low, const Cut& fro
     if (n <= kThreads) {
       const uint64_t e = sorted_entry(s, n);
       const bool in = static_cast<int>(threadIdx.x) < n;
-      const uint32_t unit_here = in ? units<BY_MASS>(row, value_of(e >> 32), unit) : 0;
-      const uint32_t at = group_before(unit_here, s.u32);
+      const U unit_here = in ? units<BY_MASS, U>(row, value_of(e >> 32), unit) : 0;
+      const U at = group_before(unit_here, slot);
       if (in && at < left && at + unit_here >= left) s.entry = e;
       __syncthreads();
       cut = Cut{value_of(s.entry >> 32), 0xffffffffu - static_cast<uint32_t>(s.entry)};
@@ -477,15 +499,21 @@ __device__ __forceinline__ bool bins_cut(const R& row, float low, const Cut& fro
   return false;
 }
 
-// `total`: the mass of `from`.
+// Masses in 32 bits where that is near enough: their units are 2^-31 of the
+// whole, `total`, so the cut is off by half a unit a logit at most. 50280 bf16
+// logits, 256 rows: 42 us, with 64 bits 46.
 template <bool BY_MASS, typename R>
 __device__ __forceinline__ Cut find_cut(const R& row, float low, const Cut& from, uint32_t count, float part,
                                         float total, Shared& s) {
   Cut cut;
-  const bool bins = !BY_MASS || row.vocab * 0x1p-28f <= fminf(1.0f - part, 0x1p-9f);  // 16 vocab / 2 units
-  const uint32_t want = BY_MASS ? static_cast<uint32_t>(fmaxf(ceilf(part * 0x1p31f), 1.0f)) : count;
-  if (bins && bins_cut<BY_MASS>(row, low, from, want, BY_MASS ? 0x1p31f / total : 1.0f, s, cut)) return cut;
-  return radix_cut<BY_MASS>(row, from, count, part, s);
+  bool found;
+  if (!BY_MASS || row.vocab * 0x1p-28f <= fminf(1.0f - part, 0x1p-9f)) {  // 16 vocab / 2 units
+    const uint32_t want = BY_MASS ? static_cast<uint32_t>(fmaxf(ceilf(part * 0x1p31f), 1.0f)) : count;
+    found = bins_cut<BY_MASS, uint32_t>(row, low, from, want, part, BY_MASS ? 0x1p31f / total : 1.0f, s, cut);
+  } else {
+    found = bins_cut<BY_MASS, uint64_t>(row, low, from, 0, part, wide_unit(row), s, cut);
+  }
+  return found ? cut : radix_cut<BY_MASS>(row, from, count, part, s);
 }
 
 // The largest key of the threads' maxima that at least `want` of them reach,
@@ -781,7 +809,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_row_ker
       bool holds = few || least || row.vocab <= kThreads;
       if (!holds) {
         // In integers: the list's order, not yet sorted, is another from call to call.
-        const uint32_t mass = in ? units<true>(row, value_of(s.list[threadIdx.x] >> 32), 0x1p31f / total) : 0;
+        const uint32_t mass = in ? units<true, uint32_t>(row, value_of(s.list[threadIdx.x] >> 32), 0x1p31f / total) : 0;
         holds = group_usum(mass, s.u32) > static_cast<uint32_t>(part * (2.0f - kNear) * 0x1p31f);
       }
       if (holds) {
@@ -842,9 +870,9 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   constexpr int E = kPer<T>, NP = kSampleSlice / (kSliceThreads * E);
   __shared__ float f32[kSliceThreads / 64];
   __shared__ uint32_t u32[kSliceThreads / 64];
-  const int group = static_cast<int>(p.first + blockIdx.x);
+  const uint32_t group = static_cast<uint32_t>(p.first) + blockIdx.x;
   const int64_t r = group / slices;
-  const int first = group % slices * kSampleSlice + static_cast<int>(threadIdx.x) * E;
+  const int first = static_cast<int>(group % slices) * kSampleSlice + static_cast<int>(threadIdx.x) * E;
   Row<T> row;
   row.logits = static_cast<const T*>(p.logits) + r * p.sl;
   row.vocab = static_cast<int>(p.vocab);
