@@ -71,7 +71,7 @@ __device__ __forceinline__ float gate(float x, float& e) {
 __device__ __forceinline__ float rest(float e, float sigmoid) { return fminf(e, 3e38f) * sigmoid; }
 
 // q = 1 - exp(-2 s) for s >= 0, given a = exp(-s): below 2 s = 1/2 by a
-// polynomial of (1 - exp(-y)) / y, y = 2 s (degree 5, fitted to 1.3e-9; here in
+// polynomial of (1 - exp(-y)) / y, y = 2 s (degree 5, within 4.2e-9; here in
 // powers of s), above it by the difference, which loses little more than a bit.
 __device__ __forceinline__ float input_share(float s, float a) {
   float q = -64 * 0.001124026020988822f;

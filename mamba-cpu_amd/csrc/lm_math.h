@@ -18,14 +18,6 @@ __device__ __forceinline__ float exp_acc(float x) {
   return fmaf(e, lo * kLn2, e);
 }
 
-// sigmoid(x) and 1 - sigmoid(x) from one exponential, each to its own ulp.
-__device__ __forceinline__ float sigmoid_acc(float x, float& one_minus) {
-  const float e = exp_acc(-x);
-  const float s = fast_rcp(1.0f + e);
-  one_minus = e * s;
-  return s;
-}
-
 // softplus(x), stable at both ends: log(1 + e) by v_log_f32 of u = 1 + e as
 // rounded, times e / (u - 1), which takes the rounding back (Kahan's log1p); 20
 // instructions where expf and log1pf take 100.

@@ -17,7 +17,8 @@
 // or by the four waves of a workgroup. The backward makes one pass: a workgroup
 // takes every parts-th row, forms dz and adds to the parameters' gradients in
 // its registers; the parts are then added in order. Longer rows are read again
-// for each step by the norm_wide kernels.
+// for each step by the norm_wide kernels, an element a load: 4096 x 12288 bf16 take
+// 158 us forward and 152 + 71 backward, where their bytes take 39 and 59.
 //
 // Every sum is float32 in a fixed order. t is rounded before mean(t) is taken
 // from it (no contraction), so that what cancels cancels exactly.
