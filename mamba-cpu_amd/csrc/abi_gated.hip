@@ -191,6 +191,8 @@ extern "C" int mcpu_gated_step(const mcpu_gated_step_args* a, void* stream) {
   if (a->batch < 0 || a->dim < 0 || a->state_batch < 0) return fail(MCPU_ERR_INVALID, "%s: negative size", what);
   if (!valid_dtype(a->dtype)) return fail(MCPU_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
   if (!(a->c >= 0.f)) return fail(MCPU_ERR_INVALID, "%s: c must not be negative", what);
+  if (a->dim > 0 && a->batch > (int64_t{1} << 38) / a->dim)
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x dim too large", what);
   if (a->batch * a->dim > 0 && (a->x == nullptr || a->a_gate == nullptr || a->x_gate == nullptr ||
                                 a->decay == nullptr || a->y == nullptr ||
                                 (a->state == nullptr && a->state_batch > 0)))
@@ -199,7 +201,6 @@ extern "C" int mcpu_gated_step(const mcpu_gated_step_args* a, void* stream) {
     return fail(MCPU_ERR_INVALID, "%s: state has fewer rows than the batch", what);
   if (any_negative({a->state_stride, a->x_stride, a->a_stride, a->i_stride}, 2))
     return fail(MCPU_ERR_INVALID, "%s: negative stride", what);
-  if (a->batch * a->dim > (int64_t{1} << 38)) return fail(MCPU_ERR_UNSUPPORTED, "%s: batch x dim too large", what);
   if (int rc = mcpu_check_device()) return rc;
   if (a->batch == 0 || a->dim == 0) return MCPU_OK;
   GatedStepParams p;
