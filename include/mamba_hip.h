@@ -749,6 +749,61 @@ typedef struct mcpu_sample_args {
 size_t mcpu_sample_workspace_size(const mcpu_sample_args* a);
 int mcpu_sample(const mcpu_sample_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Losses of a language model's head.                                        */
+/* ------------------------------------------------------------------------ */
+
+/* With s_tv = hidden_t . weight_v, not kept, and c = 1 / temperature:
+ *   lse_t = log sum_v exp(c s_tv)
+ *   teacher NULL: cross entropy, k = 1 and temperature 1:
+ *     loss_t = lse_t - s_{t, ids_t}
+ *   else distillation from k entries of the teacher:
+ *     q_t = softmax(c teacher_t) over the entries whose id lies in [0, vocab)
+ *     loss_t = (sum_k q_k log q_k + lse_t - sum_k q_k c s_{t, ids_tk}) / c^2
+ * A row counts when its target lies in [0, vocab) and is not ignore_index, or
+ * when one of its entries has an id there and is not -inf. Others have loss and
+ * lse 0 and no gradient, and nothing in them reaches another row. The loss is
+ * per row, or the sum of all rows', or that over the number of rows that count
+ * (0 when none does). Backward, with g_t and e_t the gradients of loss_t and
+ * lse_t:
+ *   ds_tv = a_t exp(c s_tv - lse_t) - b_t sum_{k: ids_tk = v} q_tk
+ *     cross entropy: a = g + e, b = g;  distillation: a = b = g / c
+ *   dhidden = ds weight;  dweight = ds^T hidden
+ * hidden, weight and their gradients have `dtype`; rows of hidden and weight are
+ * contiguous and a row stride apart; the rest is contiguous. One block for both
+ * directions: the backward reads lse, picked, share and rows as the forward left
+ * them. No counterpart in the reference. */
+#define MCPU_REDUCE_NONE 0
+#define MCPU_REDUCE_SUM 1
+#define MCPU_REDUCE_MEAN 2
+typedef struct mcpu_linear_loss_args {
+  const void* hidden;       /* (tokens, dim) */
+  const void* weight;       /* (vocab, dim) */
+  const void* ids;          /* (tokens, k) int32, or int64 when ids64 */
+  const float* teacher;     /* (tokens, k), optional; not read by the backward */
+  int64_t tokens, vocab, dim, k;       /* k at most 1024 */
+  int64_t hidden_stride, weight_stride;  /* elements between rows */
+  int64_t ignore_index;     /* cross entropy */
+  float temperature;        /* above 0; 1 for cross entropy */
+  int32_t dtype;
+  int32_t ids64;
+  int32_t reduction;
+  float* loss;              /* (tokens), or (1) where reduced */
+  float* lse;               /* (tokens) */
+  float* picked;            /* (tokens, k): s at the ids */
+  float* share;             /* (tokens, k): q; required iff distillation */
+  int32_t* rows;            /* (tokens + 1): rows that count, the others, how many count */
+  const float* dloss;       /* backward: like loss; NULL: zero */
+  const float* dlse;        /* (tokens), optional, cross entropy */
+  void* dhidden;            /* (tokens, dim), optional */
+  void* dweight;            /* (vocab, dim), optional */
+} mcpu_linear_loss_args;
+
+size_t mcpu_linear_loss_fwd_workspace_size(const mcpu_linear_loss_args* a);
+int mcpu_linear_loss_fwd(const mcpu_linear_loss_args* a, void* workspace, size_t workspace_bytes, void* stream);
+size_t mcpu_linear_loss_bwd_workspace_size(const mcpu_linear_loss_args* a);
+int mcpu_linear_loss_bwd(const mcpu_linear_loss_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

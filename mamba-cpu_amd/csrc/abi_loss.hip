@@ -1,0 +1,176 @@
+// C-ABI entry points of the head's losses: argument checks, workspace layout,
+// launches.
+#include <cstring>
+
+#include "abi_util.h"
+#include "loss_params.h"
+
+namespace mcpu {
+namespace {
+
+int check_loss(const mcpu_linear_loss_args* a, const char* what) {
+  if (a == nullptr) return fail(MCPU_ERR_INVALID, "%s: null argument block", what);
+  if (a->tokens < 0 || a->vocab < 0 || a->dim < 0 || a->k < 0 || a->hidden_stride < 0 || a->weight_stride < 0)
+    return fail(MCPU_ERR_INVALID, "%s: negative size or stride", what);
+  if (!valid_dtype(a->dtype) || (a->ids64 != 0 && a->ids64 != 1))
+    return fail(MCPU_ERR_INVALID, "%s: bad dtype %d or ids64 %d", what, a->dtype, a->ids64);
+  if (a->reduction < MCPU_REDUCE_NONE || a->reduction > MCPU_REDUCE_MEAN)
+    return fail(MCPU_ERR_INVALID, "%s: bad reduction %d", what, a->reduction);
+  if (a->dim == 0) return fail(MCPU_ERR_INVALID, "%s: dim must be positive", what);
+  if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
+    return fail(MCPU_ERR_INVALID, "%s: temperature must be above 0", what);
+  const bool distil = a->teacher != nullptr || a->share != nullptr;
+  if (!distil && (a->k != 1 || a->temperature != 1.f))
+    return fail(MCPU_ERR_INVALID, "%s: cross entropy has one target a row and temperature 1", what);
+  if (distil && a->dlse != nullptr) return fail(MCPU_ERR_INVALID, "%s: distillation has no dlse", what);
+  if (a->tokens > (1 << 26) || a->vocab > (1 << 24) || a->dim > (1 << 20) || a->k > kLossMaxK)
+    return fail(MCPU_ERR_UNSUPPORTED, "%s: at most 2^26 tokens, 2^24 vocabulary rows, 2^20 columns and %lld entries",
+                what, static_cast<long long>(kLossMaxK));
+  if (a->tokens > 0 && (a->hidden == nullptr || (a->vocab > 0 && a->weight == nullptr) ||
+                        (a->k > 0 && (a->ids == nullptr || a->picked == nullptr)) || a->lse == nullptr ||
+                        a->rows == nullptr))
+    return fail(MCPU_ERR_INVALID, "%s: hidden, weight, ids, lse, picked and rows are required", what);
+  return MCPU_OK;
+}
+
+bool sixteen(const void* p, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
+}
+
+LossParams make_loss(const mcpu_linear_loss_args* a) {
+  LossParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.hidden = a->hidden;
+  p.weight = a->weight;
+  p.ids = a->ids;
+  p.teacher = a->teacher;
+  p.ids64 = a->ids64;
+  p.tokens = a->tokens;
+  p.vocab = a->vocab;
+  p.dim = a->dim;
+  p.k = a->k;
+  p.sh = a->hidden_stride;
+  p.sw = a->weight_stride;
+  p.ignore = a->ignore_index;
+  p.temperature = a->temperature;
+  p.dtype = a->dtype;
+  p.reduction = a->reduction;
+  p.loss = a->loss;
+  p.lse = a->lse;
+  p.picked = a->picked;
+  p.share = a->share;
+  p.rows = a->rows;
+  p.dloss = a->dloss;
+  p.dlse = a->dlse;
+  p.dhidden = a->dhidden;
+  p.dweight = a->dweight;
+  loss_plan(p);
+  return p;
+}
+
+// The products read 16-byte groups of whole depths: weight as it lies where it has them.
+bool weight_in_place(const mcpu_linear_loss_args* a) {
+  return a->dtype != MCPU_F32 && a->dim % kLossDepth == 0 && a->weight_stride <= (int64_t{1} << 20) &&
+         sixteen(a->weight, a->weight_stride);
+}
+
+// Takes parts of a workspace one after the other; without one it counts.
+struct Layout {
+  char* at;
+  size_t used = 0;
+  template <typename T> void take(T*& p, int64_t count, size_t each = sizeof(T)) {
+    p = at != nullptr ? reinterpret_cast<T*>(at + used) : nullptr;
+    used += align_up(static_cast<size_t>(count) * each);
+  }
+  void take(void*& p, int64_t count, size_t each) {
+    char* q;
+    take<char>(q, count, each);
+    p = q;
+  }
+};
+
+void lay_operands(const mcpu_linear_loss_args* a, LossParams& p, Layout& w) {
+  const int pieces = loss_pieces(a->dtype);
+  w.take(p.scal, 1);
+  w.take(p.hrows, pieces * p.tpad * p.dpad, 2);
+  if (!weight_in_place(a)) w.take(p.wrows, pieces * p.vocab * p.dpad, 2);
+}
+
+size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
+  Layout w{static_cast<char*>(workspace)};
+  lay_operands(a, p, w);
+  w.take(p.keep, p.tokens);
+  w.take(p.neg, p.tokens);
+  w.take(p.part, (p.vocab + kLossPart - 1) / kLossPart * p.tpad);
+  p.each = p.loss;
+  if (p.reduction != MCPU_REDUCE_NONE) w.take(p.each, p.tokens);
+  return w.used;
+}
+
+size_t lay_bwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
+  Layout w{static_cast<char*>(workspace)};
+  lay_operands(a, p, w);
+  w.take(p.coef, 3 * p.tpad);
+  w.take(p.grad, loss_pieces(a->dtype) * p.tpad * p.vpiece, 2);
+  if (p.dhidden != nullptr) w.take(p.acc, p.hsplit * p.tpad * p.dpad);
+  if (p.dweight != nullptr && p.wsplit > 1) w.take(p.dwpart, p.wsplit * p.vpiece * p.dpad);
+  return w.used;
+}
+
+}  // namespace
+}  // namespace mcpu
+
+using namespace mcpu;
+
+extern "C" size_t mcpu_linear_loss_fwd_workspace_size(const mcpu_linear_loss_args* a) {
+  if (check_loss(a, "linear_loss") != MCPU_OK) {
+    clear_error();
+    return 0;
+  }
+  if (a->tokens == 0 || a->vocab == 0) return 0;
+  LossParams p = make_loss(a);
+  return lay_fwd(a, p, nullptr);
+}
+
+extern "C" int mcpu_linear_loss_fwd(const mcpu_linear_loss_args* a, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+  const char* what = "linear_loss_fwd";
+  clear_error();
+  if (int rc = check_loss(a, what)) return rc;
+  if (a->tokens == 0 || a->vocab == 0)
+    return fail(MCPU_ERR_INVALID, "%s: no tokens or no vocabulary", what);
+  if (a->loss == nullptr || (a->teacher == nullptr) != (a->share == nullptr))
+    return fail(MCPU_ERR_INVALID, "%s: loss, and share with a teacher, are required", what);
+  if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_linear_loss_fwd_workspace_size(a))) return rc;
+  if (int rc = mcpu_check_device()) return rc;
+  LossParams p = make_loss(a);
+  lay_fwd(a, p, workspace);
+  return hip_status(loss_fwd_launch(p, static_cast<hipStream_t>(stream)), "linear_loss_fwd launch");
+}
+
+extern "C" size_t mcpu_linear_loss_bwd_workspace_size(const mcpu_linear_loss_args* a) {
+  if (check_loss(a, "linear_loss") != MCPU_OK) {
+    clear_error();
+    return 0;
+  }
+  if (a->tokens == 0 || a->vocab == 0) return 0;
+  LossParams p = make_loss(a);
+  return lay_bwd(a, p, nullptr);
+}
+
+extern "C" int mcpu_linear_loss_bwd(const mcpu_linear_loss_args* a, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+  const char* what = "linear_loss_bwd";
+  clear_error();
+  if (int rc = check_loss(a, what)) return rc;
+  if (a->tokens == 0 || a->vocab == 0)
+    return fail(MCPU_ERR_INVALID, "%s: no tokens or no vocabulary", what);
+  if (a->dloss == nullptr && a->reduction != MCPU_REDUCE_NONE)
+    return fail(MCPU_ERR_INVALID, "%s: dloss is required where the loss is reduced", what);
+  if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_linear_loss_bwd_workspace_size(a))) return rc;
+  if (int rc = mcpu_check_device()) return rc;
+  if (a->dhidden == nullptr && a->dweight == nullptr) return MCPU_OK;
+  LossParams p = make_loss(a);
+  lay_bwd(a, p, workspace);
+  return hip_status(loss_bwd_launch(p, static_cast<hipStream_t>(stream)), "linear_loss_bwd launch");
+}

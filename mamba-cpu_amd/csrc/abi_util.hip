@@ -70,6 +70,7 @@ extern "C" size_t mcpu_args_size(const char* name) {
   if (std::strcmp(name, "norm") == 0) return sizeof(mcpu_norm_args);
   if (std::strcmp(name, "embedding") == 0) return sizeof(mcpu_embedding_args);
   if (std::strcmp(name, "sample") == 0) return sizeof(mcpu_sample_args);
+  if (std::strcmp(name, "linear_loss") == 0) return sizeof(mcpu_linear_loss_args);
   return 0;
 }
 

@@ -1,0 +1,69 @@
+// Kernel parameter block of the head's losses, shared by the kernels and the
+// C-ABI layer that fills it.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "mamba_hip.h"
+
+namespace mcpu {
+
+// What one call passes between its kernels on the GPU.
+struct LossScalars {
+  int32_t kept;          // rows that count
+  uint32_t hmax, wmax;   // float32 operands: the largest finite magnitudes, as bits
+  float unit;            // backward: a power of two near the largest coefficient of a row
+};
+
+struct LossParams {
+  const void* hidden;    // (tokens, dim), row stride sh
+  const void* weight;    // (vocab, dim), row stride sw
+  const void* ids;       // (tokens, k) int32 or int64
+  const float* teacher;  // (tokens, k), or null: cross entropy
+  int ids64;
+  int64_t tokens, vocab, dim, k, sh, sw, ignore;
+  float temperature;
+  int dtype, reduction;
+  float* loss;    // (tokens), or (1) where reduced
+  float* each;    // (tokens): loss, or the terms of the reduced one
+  float* lse;     // (tokens)
+  float* picked;  // (tokens, k): the products of hidden with the ids' rows
+  float* share;   // (tokens, k): the teacher's distribution, or null
+  int32_t* rows;  // (tokens + 1): the rows that count in order, then the others; then how many count
+  // backward
+  const float* dloss;  // (tokens), or (1) where reduced
+  const float* dlse;   // (tokens), or null
+  void* dhidden;       // (tokens, dim) contiguous, or null
+  void* dweight;       // (vocab, dim) contiguous, or null
+  // workspace
+  LossScalars* scal;
+  uint8_t* keep;      // (tokens)
+  float* neg;         // (tokens): sum of q log q
+  float2* part;       // (vocab parts, padded tokens): base-2 maximum and sum of each part
+  float* coef;        // (3, padded tokens): softmax and target coefficients, base-2 log-sum-exp
+  void* hrows;        // (pieces, padded tokens, padded dim): hidden's rows that count
+  void* wrows;        // (pieces, vocab, padded dim), or null: weight is read in place
+  void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits
+  float* acc;         // (splits, padded tokens, padded dim): gradient of hidden
+  float* dwpart;      // (splits, vocab piece, padded dim), or null: gradient of weight in one go
+  int64_t tpad, dpad, vpiece;
+  int hsplit, wsplit;
+  int64_t first;      // this launch's first workgroup
+};
+
+constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a product
+constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
+constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
+constexpr int64_t kLossMaxK = 1024;
+
+// float32 operands are two f16 pieces.
+inline int loss_pieces(int dtype) { return dtype == MCPU_F32 ? 2 : 1; }
+// Sets the padded sizes, the vocabulary piece and the splits.
+void loss_plan(LossParams& p);
+hipError_t loss_fwd_launch(LossParams p, hipStream_t st);
+hipError_t loss_bwd_launch(LossParams p, hipStream_t st);
+
+}  // namespace mcpu

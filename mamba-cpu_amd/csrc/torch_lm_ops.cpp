@@ -15,26 +15,13 @@
 #include <tuple>
 
 #include "mamba_hip.h"
-#include "torch_util.h"
+#include "torch_lm_util.h"
 
 namespace mcpu_torch {
 namespace {
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-Tensor workspace(size_t bytes, const Tensor& like) {
-  return bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : Tensor();
-}
-void* ws_ptr(const Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
-
-// Whether a call goes through its autograd function: for a backward, or with a
-// forward-mode tangent, which the function refuses (none has a rule for it).
-bool any_grad(std::initializer_list<optional<Tensor>> tensors) {
-  for (const optional<Tensor>& t : tensors)
-    if (has(t) && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
-  return false;
-}
 
 // ---- gated linear recurrence -----------------------------------------------------
 
@@ -265,9 +252,7 @@ Tensor gated_step_inplace(Tensor& state, const Tensor& x, const Tensor& a_gate, 
 
 // ---- residual norm -----------------------------------------------------------------
 
-// Rows the kernels take as they are: contiguous elements, any distance.
-Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
-// The same of a tensor of any dimensions, rows along the last.
+// Rows along the last of any dimensions.
 Tensor as_rows(const Tensor& t) {
   const int64_t dim = t.size(-1);
   return rows_of(t.dim() == 2 ? t : t.reshape({dim > 0 ? t.numel() / dim : 0, dim}));

@@ -1,0 +1,217 @@
+// The torch operators of the head's losses, in C++ over the C ABI of
+// libmamba_hip.so, in the manner of torch_lm_ops.cpp.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/autograd.h>
+#include <torch/library.h>
+
+#include <cstring>
+#include <tuple>
+
+#include "mamba_hip.h"
+#include "torch_lm_util.h"
+
+namespace mcpu_torch {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+mcpu_linear_loss_args loss_args(const char* name, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
+                                int64_t ignore_index, double temperature, int64_t reduction) {
+  for (const Tensor& t : {hidden, weight, ids}) check_gpu(name, t);
+  TORCH_CHECK_VALUE(hidden.dim() == 2 && weight.dim() == 2 && hidden.size(1) == weight.size(1) &&
+                        x_dtype(hidden.scalar_type()) && weight.scalar_type() == hidden.scalar_type(),
+                    name, " expects hidden (tokens, dim) and weight (vocab, dim) of one type, float32, bfloat16 or "
+                    "float16, got ", hidden.sizes(), " ", hidden.scalar_type(), " and ", weight.sizes(), " ",
+                    weight.scalar_type());
+  TORCH_CHECK_VALUE((ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) && ids.dim() == 2 &&
+                        ids.size(0) == hidden.size(0) && ids.is_contiguous(),
+                    name, " expects contiguous ids (tokens, k) in int32 or int64");
+  for (const Tensor& t : {weight, ids})
+    TORCH_CHECK_VALUE(t.device() == hidden.device(), name, " expects its tensors on one device, got ", t.device(),
+                      " and ", hidden.device());
+  mcpu_linear_loss_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.hidden = hidden.data_ptr();
+  a.weight = weight.data_ptr();
+  a.ids = ids.data_ptr();
+  a.tokens = hidden.size(0);
+  a.vocab = weight.size(0);
+  a.dim = hidden.size(1);
+  a.k = ids.size(1);
+  a.hidden_stride = hidden.stride(0);
+  a.weight_stride = weight.stride(0);
+  a.ignore_index = ignore_index;
+  a.temperature = static_cast<float>(temperature);
+  a.dtype = dtype_tag(hidden.scalar_type());
+  a.ids64 = ids.scalar_type() == at::kLong ? 1 : 0;
+  a.reduction = static_cast<int32_t>(reduction);
+  return a;
+}
+
+const Tensor& check_like(const char* name, const char* what, const Tensor& t, at::ScalarType dtype,
+                         at::IntArrayRef sizes, const Tensor& with) {
+  TORCH_CHECK_VALUE(t.device() == with.device() && t.scalar_type() == dtype && t.sizes() == sizes && t.is_contiguous(),
+                    name, " expects ", what, " as a contiguous ", dtype, " tensor of ", sizes, " on ", with.device());
+  return t;
+}
+
+bool nothing_to_do(const mcpu_linear_loss_args& a) { return a.tokens == 0 || a.vocab == 0 || a.k == 0; }
+
+// loss, lse, the ids' products, the teacher's distribution (distillation), and the rows that count.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in,
+                                                                   const Tensor& ids, const optional<Tensor>& teacher,
+                                                                   int64_t ignore_index, double temperature,
+                                                                   int64_t reduction) {
+  const char* name = "mamba_cpu::linear_loss_fwd";
+  check_gpu(name, hidden_in);
+  c10::DeviceGuard guard(hidden_in.device());
+  TORCH_CHECK_VALUE(hidden_in.dim() == 2 && weight_in.dim() == 2, name, " expects hidden and weight of two dimensions");
+  const Tensor hidden = rows_of(hidden_in), weight = rows_of(weight_in);
+  mcpu_linear_loss_args a = loss_args(name, hidden, weight, ids, ignore_index, temperature, reduction);
+  const auto f32 = hidden.options().dtype(at::kFloat);
+  const int64_t tokens = a.tokens;
+  if (has(teacher)) a.teacher = static_cast<const float*>(
+      check_like(name, "the teacher's logits", *teacher, at::kFloat, ids.sizes(), hidden).data_ptr());
+  const at::IntArrayRef all(&tokens, 1), one;
+  Tensor loss = at::empty(reduction == MCPU_REDUCE_NONE ? all : one, f32), lse = at::empty({tokens}, f32);
+  Tensor picked = at::empty({tokens, a.k}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
+  Tensor rows = at::empty({tokens + 1}, hidden.options().dtype(at::kInt));
+  if (nothing_to_do(a)) {
+    for (const Tensor& t : {loss, lse, rows}) t.zero_();
+    return {loss, lse, picked, share, rows};
+  }
+  a.loss = static_cast<float*>(loss.data_ptr());
+  a.lse = static_cast<float*>(lse.data_ptr());
+  a.picked = static_cast<float*>(picked.data_ptr());
+  a.share = has(teacher) ? static_cast<float*>(share.data_ptr()) : nullptr;
+  a.rows = static_cast<int32_t*>(rows.data_ptr());
+  const size_t nws = mcpu_linear_loss_fwd_workspace_size(&a);
+  Tensor ws = workspace(nws, hidden);
+  check_rc(mcpu_linear_loss_fwd(&a, ws_ptr(ws), nws, stream_of(hidden)), name);
+  return {loss, lse, picked, share, rows};
+}
+
+// Gradients of hidden and weight, each where wanted.
+std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const optional<Tensor>& dlse,
+                                           const Tensor& hidden_in, const Tensor& weight_in, const Tensor& ids,
+                                           const Tensor& lse, const Tensor& picked, const Tensor& share,
+                                           const Tensor& rows, int64_t ignore_index, double temperature,
+                                           int64_t reduction, bool distil, bool want_hidden, bool want_weight) {
+  const char* name = "mamba_cpu::linear_loss_bwd";
+  check_gpu(name, hidden_in);
+  c10::DeviceGuard guard(hidden_in.device());
+  TORCH_CHECK_VALUE(hidden_in.dim() == 2 && weight_in.dim() == 2, name, " expects hidden and weight of two dimensions");
+  const Tensor hidden = rows_of(hidden_in), weight = rows_of(weight_in);
+  mcpu_linear_loss_args a = loss_args(name, hidden, weight, ids, ignore_index, temperature, reduction);
+  Tensor dh = at::empty({want_hidden ? a.tokens : 0, a.dim}, hidden.options());
+  Tensor dw = at::empty({want_weight ? a.vocab : 0, a.dim}, weight.options());
+  if (nothing_to_do(a)) {
+    for (const Tensor& t : {dh, dw}) t.zero_();
+    return {dh, dw};
+  }
+  const int64_t n = a.tokens, k = a.k, last = n + 1;
+  const int64_t all[2] = {n, k};
+  const at::IntArrayRef per(&n, 1), both(all, 2), one;
+  a.lse = static_cast<float*>(check_like(name, "lse", lse, at::kFloat, per, hidden).data_ptr());
+  a.picked = static_cast<float*>(check_like(name, "picked", picked, at::kFloat, both, hidden).data_ptr());
+  if (distil) a.share = static_cast<float*>(check_like(name, "share", share, at::kFloat, both, hidden).data_ptr());
+  a.rows = static_cast<int32_t*>(
+      check_like(name, "rows", rows, at::kInt, at::IntArrayRef(&last, 1), hidden).data_ptr());
+  Tensor g, e;
+  if (has(dloss)) {
+    g = dloss->to(at::kFloat).contiguous();
+    a.dloss = static_cast<const float*>(
+        check_like(name, "dloss", g, at::kFloat, reduction == MCPU_REDUCE_NONE ? per : one, hidden).data_ptr());
+  }
+  if (has(dlse)) {
+    e = dlse->to(at::kFloat).contiguous();
+    a.dlse = static_cast<const float*>(check_like(name, "dlse", e, at::kFloat, per, hidden).data_ptr());
+  }
+  if (want_hidden) a.dhidden = dh.data_ptr();
+  if (want_weight) a.dweight = dw.data_ptr();
+  const size_t nws = mcpu_linear_loss_bwd_workspace_size(&a);
+  Tensor ws = workspace(nws, hidden);
+  check_rc(mcpu_linear_loss_bwd(&a, ws_ptr(ws), nws, stream_of(hidden)), name);
+  return {dh, dw};
+}
+
+auto loss_fwd_below() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("mamba_cpu::linear_loss_fwd", "")
+                       .typed<decltype(linear_loss_fwd)>();
+  return op;
+}
+
+struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
+                               const optional<Tensor>& teacher, int64_t ignore_index, double temperature,
+                               int64_t reduction) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
+    const Tensor lse = std::get<1>(r), picked = std::get<2>(r), share = std::get<3>(r), rows = std::get<4>(r);
+    ctx->mark_non_differentiable(has(teacher) ? variable_list{lse, picked, share, rows}
+                                              : variable_list{picked, share, rows});
+    ctx->save_for_backward({hidden, weight, ids, lse, picked, share, rows});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["distil"] = has(teacher);
+    ctx->set_materialize_grads(false);
+    return {std::get<0>(r), lse, picked, share, rows};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    const bool want_hidden = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
+    optional<Tensor> g = opt(grads[0]);
+    if (!has(g) && reduction != MCPU_REDUCE_NONE) g = at::zeros({}, s[3].options());
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("mamba_cpu::linear_loss_bwd", "")
+                         .typed<decltype(linear_loss_bwd)>();
+    auto r = op.call(g, opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["ignore"].toInt(),
+                     ctx->saved_data["temperature"].toDouble(), reduction, ctx->saved_data["distil"].toBool(),
+                     want_hidden, want_weight);
+    return {want_hidden ? std::get<0>(r) : Tensor(), want_weight ? std::get<1>(r) : Tensor(),
+            Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(const Tensor& hidden, const Tensor& weight,
+                                                                        const Tensor& ids,
+                                                                        const optional<Tensor>& teacher,
+                                                                        int64_t ignore_index, double temperature,
+                                                                        int64_t reduction) {
+  TORCH_CHECK_VALUE(!any_grad({teacher}), "mamba_cpu::linear_loss_fwd has no gradient of the teacher's logits: detach "
+                    "them");
+  if (!any_grad({opt(hidden), opt(weight)})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
+  }
+  auto r = LinearLossFn::apply(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
+  return {r[0], r[1], r[2], r[3], r[4]};
+}
+
+}  // namespace
+}  // namespace mcpu_torch
+
+TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
+  m.def("linear_loss_fwd(Tensor hidden, Tensor weight, Tensor ids, Tensor? teacher, int ignore_index, "
+        "float temperature, int reduction) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_loss_bwd(Tensor? dloss, Tensor? dlse, Tensor hidden, Tensor weight, Tensor ids, Tensor lse, "
+        "Tensor picked, Tensor share, Tensor rows, int ignore_index, float temperature, int reduction, bool distil, "
+        "bool want_hidden, bool want_weight) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
+  using namespace mcpu_torch;
+  m.impl("linear_loss_fwd", &linear_loss_fwd);
+  m.impl("linear_loss_bwd", &linear_loss_bwd);
+}
+
+TORCH_LIBRARY_IMPL(mamba_cpu, Autograd, m) {
+  using namespace mcpu_torch;
+  m.impl("linear_loss_fwd", &linear_loss_autograd);
+}

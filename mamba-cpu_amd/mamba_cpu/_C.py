@@ -199,11 +199,21 @@ class SampleArgs(ctypes.Structure):
     ]
 
 
+class LinearLossArgs(ctypes.Structure):
+    _fields_ = [
+        ("hidden", _P), ("weight", _P), ("ids", _P), ("teacher", _P),
+        ("tokens", _I64), ("vocab", _I64), ("dim", _I64), ("k", _I64), ("hidden_stride", _I64),
+        ("weight_stride", _I64), ("ignore_index", _I64), ("temperature", ctypes.c_float), ("dtype", _I32),
+        ("ids64", _I32), ("reduction", _I32), ("loss", _P), ("lse", _P), ("picked", _P), ("share", _P),
+        ("rows", _P), ("dloss", _P), ("dlse", _P), ("dhidden", _P), ("dweight", _P),
+    ]
+
+
 _BLOCKS = (("scan", ScanArgs), ("conv", ConvArgs), ("conv_update", ConvUpdateArgs),
            ("state_update", StateUpdateArgs), ("ssd", SsdArgs), ("mixer_step", MixerStepArgs),
            ("norm_linear", NormLinearArgs), ("mamba2_step", Mamba2StepArgs),
            ("gated_scan", GatedScanArgs), ("gated_step", GatedStepArgs), ("norm", NormArgs),
-           ("embedding", EmbeddingArgs), ("sample", SampleArgs))
+           ("embedding", EmbeddingArgs), ("sample", SampleArgs), ("linear_loss", LinearLossArgs))
 _ARGP = {n: ctypes.POINTER(c) for n, c in _BLOCKS}
 
 lib.mcpu_last_error.restype = ctypes.c_char_p
@@ -282,6 +292,12 @@ lib.mcpu_sample_workspace_size.argtypes = [_ARGP["sample"]]
 lib.mcpu_sample_workspace_size.restype = ctypes.c_size_t
 lib.mcpu_sample.argtypes = [_ARGP["sample"], _P, ctypes.c_size_t, _P]
 lib.mcpu_sample.restype = ctypes.c_int
+
+for _name in ("fwd", "bwd"):
+    getattr(lib, f"mcpu_linear_loss_{_name}_workspace_size").argtypes = [_ARGP["linear_loss"]]
+    getattr(lib, f"mcpu_linear_loss_{_name}_workspace_size").restype = ctypes.c_size_t
+    getattr(lib, f"mcpu_linear_loss_{_name}").argtypes = [_ARGP["linear_loss"], _P, ctypes.c_size_t, _P]
+    getattr(lib, f"mcpu_linear_loss_{_name}").restype = ctypes.c_int
 
 for _name, _cls in _BLOCKS:
     _want = lib.mcpu_args_size(_name.encode())

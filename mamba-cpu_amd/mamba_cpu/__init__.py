@@ -17,6 +17,8 @@ from mamba_cpu.ops import (
     gated_linear_scan_fn,
     gated_linear_update,
     layer_norm_fn,
+    linear_cross_entropy_fn,
+    linear_distillation_fn,
     mamba_chunk_scan_combined,
     mamba_inner_fn,
     sample_fn,
@@ -35,6 +37,8 @@ __all__ = [
     "gated_linear_scan_fn",
     "gated_linear_update",
     "layer_norm_fn",
+    "linear_cross_entropy_fn",
+    "linear_distillation_fn",
     "mamba_chunk_scan_combined",
     "mamba_inner_fn",
     "sample_fn",
