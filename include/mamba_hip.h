@@ -771,7 +771,7 @@ int mcpu_sample(const mcpu_sample_args* a, void* workspace, size_t workspace_byt
  *   dhidden = ds weight;  dweight = ds^T hidden
  * hidden, weight and their gradients have `dtype`; rows of hidden and weight are
  * contiguous and a row stride apart; the rest is contiguous. One block for both
- * directions: the backward reads lse, picked, share and rows as the forward left
+ * directions: the backward reads picked, stat, share and rows as the forward left
  * them. No counterpart in the reference. */
 #define MCPU_REDUCE_NONE 0
 #define MCPU_REDUCE_SUM 1
@@ -789,8 +789,9 @@ typedef struct mcpu_linear_loss_args {
   int32_t ids64;
   int32_t reduction;
   float* loss;              /* (tokens), or (1) where reduced */
-  float* lse;               /* (tokens) */
-  float* picked;            /* (tokens, k): s at the ids */
+  float* lse;               /* (tokens); not read by the backward */
+  float* picked;            /* (tokens, k): s at the ids, left for the backward; likewise stat */
+  float* stat;              /* (4, tokens) */
   float* share;             /* (tokens, k): q; required iff distillation */
   int32_t* rows;            /* (tokens + 1): rows that count, the others, how many count */
   const float* dloss;       /* backward: like loss; NULL: zero */

@@ -27,9 +27,9 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
     return fail(MCPU_ERR_UNSUPPORTED, "%s: at most 2^26 tokens, 2^24 vocabulary rows, 2^20 columns and %lld entries",
                 what, static_cast<long long>(kLossMaxK));
   if (a->tokens > 0 && (a->hidden == nullptr || (a->vocab > 0 && a->weight == nullptr) ||
-                        (a->k > 0 && (a->ids == nullptr || a->picked == nullptr)) || a->lse == nullptr ||
-                        a->rows == nullptr))
-    return fail(MCPU_ERR_INVALID, "%s: hidden, weight, ids, lse, picked and rows are required", what);
+                        (a->k > 0 && (a->ids == nullptr || a->picked == nullptr)) ||
+                        a->stat == nullptr || a->rows == nullptr))
+    return fail(MCPU_ERR_INVALID, "%s: hidden, weight, ids, picked, stat and rows are required", what);
   return MCPU_OK;
 }
 
@@ -58,6 +58,7 @@ LossParams make_loss(const mcpu_linear_loss_args* a) {
   p.loss = a->loss;
   p.lse = a->lse;
   p.picked = a->picked;
+  p.stat = a->stat;
   p.share = a->share;
   p.rows = a->rows;
   p.dloss = a->dloss;
@@ -92,6 +93,7 @@ struct Layout {
 void lay_operands(const mcpu_linear_loss_args* a, LossParams& p, Layout& w) {
   const int pieces = loss_pieces(a->dtype);
   w.take(p.scal, 1);
+  if (a->teacher == nullptr && a->share == nullptr) w.take(p.target, p.tpad);
   w.take(p.hrows, pieces * p.tpad * p.dpad, 2);
   if (!weight_in_place(a)) w.take(p.wrows, pieces * p.vocab * p.dpad, 2);
 }
@@ -100,7 +102,7 @@ size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   Layout w{static_cast<char*>(workspace)};
   lay_operands(a, p, w);
   w.take(p.keep, p.tokens);
-  w.take(p.neg, p.tokens);
+  w.take(p.cross, p.tokens);
   w.take(p.part, (p.vocab + kLossPart - 1) / kLossPart * p.tpad);
   p.each = p.loss;
   if (p.reduction != MCPU_REDUCE_NONE) w.take(p.each, p.tokens);
@@ -139,8 +141,8 @@ extern "C" int mcpu_linear_loss_fwd(const mcpu_linear_loss_args* a, void* worksp
   if (int rc = check_loss(a, what)) return rc;
   if (a->tokens == 0 || a->vocab == 0)
     return fail(MCPU_ERR_INVALID, "%s: no tokens or no vocabulary", what);
-  if (a->loss == nullptr || (a->teacher == nullptr) != (a->share == nullptr))
-    return fail(MCPU_ERR_INVALID, "%s: loss, and share with a teacher, are required", what);
+  if (a->loss == nullptr || a->lse == nullptr || (a->teacher == nullptr) != (a->share == nullptr))
+    return fail(MCPU_ERR_INVALID, "%s: loss, lse, and share with a teacher, are required", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_linear_loss_fwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   LossParams p = make_loss(a);

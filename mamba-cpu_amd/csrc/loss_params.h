@@ -15,7 +15,7 @@ namespace mcpu {
 struct LossScalars {
   int32_t kept;          // rows that count
   uint32_t hmax, wmax;   // float32 operands: the largest finite magnitudes, as bits
-  float unit;            // backward: a power of two near the largest coefficient of a row
+  float unit;            // backward: the largest coefficient of a row
 };
 
 struct LossParams {
@@ -30,7 +30,8 @@ struct LossParams {
   float* loss;    // (tokens), or (1) where reduced
   float* each;    // (tokens): loss, or the terms of the reduced one
   float* lse;     // (tokens)
-  float* picked;  // (tokens, k): the products of hidden with the ids' rows
+  float* picked;  // (tokens, k): the products of hidden with the ids' rows; cross entropy: in the order of `rows`
+  float* stat;    // (4, tokens) in the order of `rows`: maximum, sum of exp(c (s - it)), a target's share of it, the others'
   float* share;   // (tokens, k): the teacher's distribution, or null
   int32_t* rows;  // (tokens + 1): the rows that count in order, then the others; then how many count
   // backward
@@ -41,9 +42,10 @@ struct LossParams {
   // workspace
   LossScalars* scal;
   uint8_t* keep;      // (tokens)
-  float* neg;         // (tokens): sum of q log q
-  float2* part;       // (vocab parts, padded tokens): base-2 maximum and sum of each part
-  float* coef;        // (3, padded tokens): softmax and target coefficients, base-2 log-sum-exp
+  int32_t* target;    // (padded tokens) in the order of `rows`, cross entropy; else null
+  float* cross;       // (tokens): sum of q (log q - c s)
+  float2* part;       // (vocab parts, padded tokens): maximum of each part and sum of exp(c (s - it))
+  float* coef;        // (3, padded tokens): factor of 2^(logit - maximum), the target's ds or the shares' factor, maximum
   void* hrows;        // (pieces, padded tokens, padded dim): hidden's rows that count
   void* wrows;        // (pieces, vocab, padded dim), or null: weight is read in place
   void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits

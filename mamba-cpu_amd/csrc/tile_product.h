@@ -103,18 +103,25 @@ template <bool TERM> __device__ __forceinline__ s16x8 tile_frag(const char* lds,
   }
 }
 
-// Accumulators of a wave: acc[i][j][e] is D at
+// Accumulators of a wave: v[j][i][e] is D at
 //   m = m0 + 128 (wave / 4) + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
 //   n = n0 + 64 (wave % 4) + 32 j + lane % 32.
 struct Acc {
-  f32x16 v[4][2];
+  f32x16 v[2][4];
 };
+
+// A workgroup's LDS: both operands' tiles, twice. Four arrays, not one, for the
+// compiler to see that what is read is not what the loads on their way write.
+#define MCPU_TILE_LDS(a0, b0, a1, b1)                              \
+  __shared__ __attribute__((aligned(1024))) char a0[kTileBytes]; \
+  __shared__ __attribute__((aligned(1024))) char b0[kTileBytes]; \
+  __shared__ __attribute__((aligned(1024))) char a1[kTileBytes]; \
+  __shared__ __attribute__((aligned(1024))) char b1[kTileBytes]
 
 // Depths [kt0, kt1) of the tile at (m0, n0), counted over all runs.
 template <typename T, bool TA, bool TB>
-__device__ __forceinline__ void tile_product(const ProductParams& p, int64_t m0, int64_t n0, int kt0, int kt1,
-                                             Acc& acc) {
-  __shared__ __attribute__((aligned(1024))) char a0[kTileBytes], b0[kTileBytes], a1[kTileBytes], b1[kTileBytes];
+__device__ __forceinline__ void tile_product(const ProductParams& p, int64_t m0, int64_t n0, int kt0, int kt1, char* a0,
+                                             char* b0, char* a1, char* b1, Acc& acc) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
   const int depths = static_cast<int>(p.depth / kLossDepth);
@@ -124,11 +131,11 @@ __device__ __forceinline__ void tile_product(const ProductParams& p, int64_t m0,
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc.v[i][j][e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc.v[j][i][e] = 0.f;
   if (kt0 >= kt1) return;
 
   auto load = [&](char* la, char* lb, int kt) {
-    const int run = kt / depths;
+    const int run = kt >= 2 * depths ? 2 : kt >= depths ? 1 : 0;
     const int64_t k0 = int64_t{kt - run * depths} * kLossDepth;
     tile_load<TA>(la, tile_rsrc<TA>(p.a, m0, k0, run == 2), lda2, wave, lane);
     tile_load<TB>(lb, tile_rsrc<TB>(p.b, n0, k0, run == 1), ldb2, wave, lane);
@@ -151,7 +158,7 @@ __device__ __forceinline__ void tile_product(const ProductParams& p, int64_t m0,
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc.v[i][j] = mma32<T>(a[i], b[j], acc.v[i][j]);
+        for (int j = 0; j < 2; ++j) acc.v[j][i] = mma32<T>(a[i], b[j], acc.v[j][i]);
     }
   };
   load(a0, b0, kt0);

@@ -59,8 +59,9 @@ const Tensor& check_like(const char* name, const char* what, const Tensor& t, at
 
 bool nothing_to_do(const mcpu_linear_loss_args& a) { return a.tokens == 0 || a.vocab == 0 || a.k == 0; }
 
-// loss, lse, the ids' products, the teacher's distribution (distillation), and the rows that count.
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in,
+// loss, lse, and for the backward the ids' products, the rows' statistics, the teacher's distribution
+// (distillation) and the rows that count.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in,
                                                                    const Tensor& ids, const optional<Tensor>& teacher,
                                                                    int64_t ignore_index, double temperature,
                                                                    int64_t reduction) {
@@ -76,27 +77,28 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const Tensor&
       check_like(name, "the teacher's logits", *teacher, at::kFloat, ids.sizes(), hidden).data_ptr());
   const at::IntArrayRef all(&tokens, 1), one;
   Tensor loss = at::empty(reduction == MCPU_REDUCE_NONE ? all : one, f32), lse = at::empty({tokens}, f32);
-  Tensor picked = at::empty({tokens, a.k}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
+  Tensor picked = at::empty({tokens, a.k}, f32), stat = at::empty({4, tokens}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
   Tensor rows = at::empty({tokens + 1}, hidden.options().dtype(at::kInt));
   if (nothing_to_do(a)) {
     for (const Tensor& t : {loss, lse, rows}) t.zero_();
-    return {loss, lse, picked, share, rows};
+    return {loss, lse, picked, stat, share, rows};
   }
   a.loss = static_cast<float*>(loss.data_ptr());
   a.lse = static_cast<float*>(lse.data_ptr());
   a.picked = static_cast<float*>(picked.data_ptr());
+  a.stat = static_cast<float*>(stat.data_ptr());
   a.share = has(teacher) ? static_cast<float*>(share.data_ptr()) : nullptr;
   a.rows = static_cast<int32_t*>(rows.data_ptr());
   const size_t nws = mcpu_linear_loss_fwd_workspace_size(&a);
   Tensor ws = workspace(nws, hidden);
   check_rc(mcpu_linear_loss_fwd(&a, ws_ptr(ws), nws, stream_of(hidden)), name);
-  return {loss, lse, picked, share, rows};
+  return {loss, lse, picked, stat, share, rows};
 }
 
 // Gradients of hidden and weight, each where wanted.
 std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const optional<Tensor>& dlse,
                                            const Tensor& hidden_in, const Tensor& weight_in, const Tensor& ids,
-                                           const Tensor& lse, const Tensor& picked, const Tensor& share,
+                                           const Tensor& picked, const Tensor& stat, const Tensor& share,
                                            const Tensor& rows, int64_t ignore_index, double temperature,
                                            int64_t reduction, bool distil, bool want_hidden, bool want_weight) {
   const char* name = "mamba_cpu::linear_loss_bwd";
@@ -112,9 +114,9 @@ std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const 
     return {dh, dw};
   }
   const int64_t n = a.tokens, k = a.k, last = n + 1;
-  const int64_t all[2] = {n, k};
-  const at::IntArrayRef per(&n, 1), both(all, 2), one;
-  a.lse = static_cast<float*>(check_like(name, "lse", lse, at::kFloat, per, hidden).data_ptr());
+  const int64_t all[2] = {n, k}, stats[2] = {4, n};
+  const at::IntArrayRef per(&n, 1), both(all, 2), four(stats, 2), one;
+  a.stat = static_cast<float*>(check_like(name, "stat", stat, at::kFloat, four, hidden).data_ptr());
   a.picked = static_cast<float*>(check_like(name, "picked", picked, at::kFloat, both, hidden).data_ptr());
   if (distil) a.share = static_cast<float*>(check_like(name, "share", share, at::kFloat, both, hidden).data_ptr());
   a.rows = static_cast<int32_t*>(
@@ -150,16 +152,17 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
                                int64_t reduction) {
     at::AutoDispatchBelowADInplaceOrView below;
     auto r = loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
-    const Tensor lse = std::get<1>(r), picked = std::get<2>(r), share = std::get<3>(r), rows = std::get<4>(r);
-    ctx->mark_non_differentiable(has(teacher) ? variable_list{lse, picked, share, rows}
-                                              : variable_list{picked, share, rows});
-    ctx->save_for_backward({hidden, weight, ids, lse, picked, share, rows});
+    const Tensor lse = std::get<1>(r), picked = std::get<2>(r), stat = std::get<3>(r), share = std::get<4>(r),
+                 rows = std::get<5>(r);
+    ctx->mark_non_differentiable(has(teacher) ? variable_list{lse, picked, stat, share, rows}
+                                              : variable_list{picked, stat, share, rows});
+    ctx->save_for_backward({hidden, weight, ids, picked, stat, share, rows});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["distil"] = has(teacher);
     ctx->set_materialize_grads(false);
-    return {std::get<0>(r), lse, picked, share, rows};
+    return {std::get<0>(r), lse, picked, stat, share, rows};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -179,7 +182,7 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(const Tensor& hidden, const Tensor& weight,
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(const Tensor& hidden, const Tensor& weight,
                                                                         const Tensor& ids,
                                                                         const optional<Tensor>& teacher,
                                                                         int64_t ignore_index, double temperature,
@@ -191,7 +194,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(const Te
     return loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
   }
   auto r = LinearLossFn::apply(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
-  return {r[0], r[1], r[2], r[3], r[4]};
+  return {r[0], r[1], r[2], r[3], r[4], r[5]};
 }
 
 }  // namespace
@@ -199,9 +202,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(const Te
 
 TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
   m.def("linear_loss_fwd(Tensor hidden, Tensor weight, Tensor ids, Tensor? teacher, int ignore_index, "
-        "float temperature, int reduction) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def("linear_loss_bwd(Tensor? dloss, Tensor? dlse, Tensor hidden, Tensor weight, Tensor ids, Tensor lse, "
-        "Tensor picked, Tensor share, Tensor rows, int ignore_index, float temperature, int reduction, bool distil, "
+        "float temperature, int reduction) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_loss_bwd(Tensor? dloss, Tensor? dlse, Tensor hidden, Tensor weight, Tensor ids, Tensor picked, "
+        "Tensor stat, Tensor share, Tensor rows, int ignore_index, float temperature, int reduction, bool distil, "
         "bool want_hidden, bool want_weight) -> (Tensor, Tensor)");
 }
 

@@ -204,8 +204,8 @@ class LinearLossArgs(ctypes.Structure):
         ("hidden", _P), ("weight", _P), ("ids", _P), ("teacher", _P),
         ("tokens", _I64), ("vocab", _I64), ("dim", _I64), ("k", _I64), ("hidden_stride", _I64),
         ("weight_stride", _I64), ("ignore_index", _I64), ("temperature", ctypes.c_float), ("dtype", _I32),
-        ("ids64", _I32), ("reduction", _I32), ("loss", _P), ("lse", _P), ("picked", _P), ("share", _P),
-        ("rows", _P), ("dloss", _P), ("dlse", _P), ("dhidden", _P), ("dweight", _P),
+        ("ids64", _I32), ("reduction", _I32), ("loss", _P), ("lse", _P), ("picked", _P), ("stat", _P),
+        ("share", _P), ("rows", _P), ("dloss", _P), ("dlse", _P), ("dhidden", _P), ("dweight", _P),
     ]
 
 

@@ -34,12 +34,13 @@ def _(hidden, weight, ids, teacher, ignore_index, temperature, reduction):
     tokens, k = ids.shape
     f32 = dict(dtype=torch.float32)
     return (hidden.new_empty(() if reduction else (tokens,), **f32), hidden.new_empty(tokens, **f32),
-            hidden.new_empty(tokens, k, **f32), hidden.new_empty(tokens if teacher is not None else 0, k, **f32),
+            hidden.new_empty(tokens, k, **f32), hidden.new_empty(4, tokens, **f32),
+            hidden.new_empty(tokens if teacher is not None else 0, k, **f32),
             hidden.new_empty(tokens + 1, dtype=torch.int32))
 
 
 @torch.library.register_fake("mamba_cpu::linear_loss_bwd")
-def _(dloss, dlse, hidden, weight, ids, lse, picked, share, rows, ignore_index, temperature, reduction, distil,
+def _(dloss, dlse, hidden, weight, ids, picked, stat, share, rows, ignore_index, temperature, reduction, distil,
       want_hidden, want_weight):
     return (hidden.new_empty(hidden.shape[0] if want_hidden else 0, hidden.shape[1]),
             weight.new_empty(weight.shape[0] if want_weight else 0, weight.shape[1]))
@@ -90,7 +91,7 @@ def linear_cross_entropy_fn(hidden, weight, targets, ignore_index=-100, reductio
     ids = _ids("targets", targets, hidden.shape[:-1], hidden.device).reshape(-1, 1)
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
-    loss, lse, _, _, _ = torch.ops.mamba_cpu.linear_loss_fwd(h, w, ids.contiguous(), None, int(ignore_index), 1.0,
+    loss, lse, *_ = torch.ops.mamba_cpu.linear_loss_fwd(h, w, ids.contiguous(), None, int(ignore_index), 1.0,
                                                              _REDUCTIONS[reduction])
     if reduction == "none":
         loss = loss.view(targets.shape)
@@ -124,7 +125,7 @@ def linear_distillation_fn(hidden, weight, teacher_ids, teacher_logits, temperat
     if teacher_logits.device != hidden.device:
         raise ValueError(f"teacher_logits must be on {hidden.device}, got {teacher_logits.device}")
     shape = (h.shape[0], ids.shape[-1])
-    loss, _, _, _, _ = torch.ops.mamba_cpu.linear_loss_fwd(
+    loss, *_ = torch.ops.mamba_cpu.linear_loss_fwd(
         h, w, ids.reshape(shape).contiguous(), teacher_logits.float().reshape(shape).contiguous(), -1,
         float(temperature), _REDUCTIONS[reduction])
     return loss.view(lead) if reduction == "none" else loss
