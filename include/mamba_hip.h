@@ -790,8 +790,8 @@ typedef struct mcpu_linear_loss_args {
   int32_t reduction;
   float* loss;              /* (tokens), or (1) where reduced */
   float* lse;               /* (tokens); not read by the backward */
-  float* picked;            /* (tokens, k): s at the ids, left for the backward; likewise stat */
-  float* stat;              /* (4, tokens) */
+  float* picked;            /* (tokens, k): s at the ids, left for the backward; required iff distillation */
+  float* stat;              /* (4, tokens), left for the backward */
   float* share;             /* (tokens, k): q; required iff distillation */
   int32_t* rows;            /* (tokens + 1): rows that count, the others, how many count */
   const float* dloss;       /* backward: like loss; NULL: zero */

@@ -8,6 +8,8 @@
 namespace mcpu {
 namespace {
 
+bool distil(const mcpu_linear_loss_args* a) { return a->teacher != nullptr || a->share != nullptr; }
+
 int check_loss(const mcpu_linear_loss_args* a, const char* what) {
   if (a == nullptr) return fail(MCPU_ERR_INVALID, "%s: null argument block", what);
   if (a->tokens < 0 || a->vocab < 0 || a->dim < 0 || a->k < 0 || a->hidden_stride < 0 || a->weight_stride < 0)
@@ -19,17 +21,16 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
   if (a->dim == 0) return fail(MCPU_ERR_INVALID, "%s: dim must be positive", what);
   if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
     return fail(MCPU_ERR_INVALID, "%s: temperature must be above 0", what);
-  const bool distil = a->teacher != nullptr || a->share != nullptr;
-  if (!distil && (a->k != 1 || a->temperature != 1.f))
+  if (!distil(a) && (a->k != 1 || a->temperature != 1.f))
     return fail(MCPU_ERR_INVALID, "%s: cross entropy has one target a row and temperature 1", what);
-  if (distil && a->dlse != nullptr) return fail(MCPU_ERR_INVALID, "%s: distillation has no dlse", what);
+  if (distil(a) && a->dlse != nullptr) return fail(MCPU_ERR_INVALID, "%s: distillation has no dlse", what);
   if (a->tokens > (1 << 26) || a->vocab > (1 << 24) || a->dim > (1 << 20) || a->k > kLossMaxK)
     return fail(MCPU_ERR_UNSUPPORTED, "%s: at most 2^26 tokens, 2^24 vocabulary rows, 2^20 columns and %lld entries",
                 what, static_cast<long long>(kLossMaxK));
   if (a->tokens > 0 && (a->hidden == nullptr || (a->vocab > 0 && a->weight == nullptr) ||
-                        (a->k > 0 && (a->ids == nullptr || a->picked == nullptr)) ||
+                        (a->k > 0 && (a->ids == nullptr || (distil(a) && a->picked == nullptr))) ||
                         a->stat == nullptr || a->rows == nullptr))
-    return fail(MCPU_ERR_INVALID, "%s: hidden, weight, ids, picked, stat and rows are required", what);
+    return fail(MCPU_ERR_INVALID, "%s: hidden, weight, ids, stat, rows and (distillation) picked are required", what);
   return MCPU_OK;
 }
 
@@ -93,26 +94,32 @@ struct Layout {
 void lay_operands(const mcpu_linear_loss_args* a, LossParams& p, Layout& w) {
   const int pieces = loss_pieces(a->dtype);
   w.take(p.scal, 1);
-  if (a->teacher == nullptr && a->share == nullptr) w.take(p.target, p.tpad);
+  if (!distil(a)) w.take(p.target, p.tpad);
   w.take(p.hrows, pieces * p.tpad * p.dpad, 2);
   if (!weight_in_place(a)) w.take(p.wrows, pieces * p.vocab * p.dpad, 2);
 }
 
 size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   Layout w{static_cast<char*>(workspace)};
-  lay_operands(a, p, w);
-  w.take(p.keep, p.tokens);
-  w.take(p.cross, p.tokens);
-  w.take(p.part, (p.vocab + kLossPart - 1) / kLossPart * p.tpad);
   p.each = p.loss;
   if (p.reduction != MCPU_REDUCE_NONE) w.take(p.each, p.tokens);
+  if (distil(a)) w.take(p.keep, p.tokens);
+  if (distil(a)) w.take(p.cross, p.tokens);
+  if (!distil(a)) w.take(p.picked, p.tpad);
+  if (p.tokens <= kLossFew) {
+    w.take(p.part, (p.vocab + 255) / 256 * kLossFew);
+    return w.used;
+  }
+  lay_operands(a, p, w);
+  w.take(p.part, (p.vocab + kLossPart - 1) / kLossPart * p.tpad);
   return w.used;
 }
 
 size_t lay_bwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   Layout w{static_cast<char*>(workspace)};
   lay_operands(a, p, w);
-  w.take(p.coef, 3 * p.tpad);
+  w.take(p.coef, 4 * p.tpad);
+  if (!distil(a)) w.take(p.hscaled, loss_pieces(a->dtype) * p.tpad * p.dpad, 2);
   w.take(p.grad, loss_pieces(a->dtype) * p.tpad * p.vpiece, 2);
   if (p.dhidden != nullptr) w.take(p.acc, p.hsplit * p.tpad * p.dpad);
   if (p.dweight != nullptr && p.wsplit > 1) w.take(p.dwpart, p.wsplit * p.vpiece * p.dpad);

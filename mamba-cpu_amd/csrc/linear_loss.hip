@@ -39,6 +39,11 @@ __device__ __forceinline__ int up_exponent(uint32_t most) {
   const int e = 13 - (static_cast<int>(most >> 23) - 127);
   return e > 120 ? 120 : e;
 }
+// The unit of a row that counts.
+__device__ __forceinline__ float unit_of(const LossParams& p, int64_t i) {
+  const float u = p.coef[3 * p.tpad + i];
+  return u > 0.f ? u : p.scal->unit;
+}
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
 
 // hi + lo of a scaled value; one that is not finite has no lo.
@@ -76,24 +81,24 @@ template <typename T> __device__ __forceinline__ float dot16(const T* h, const T
   return row_allreduce16(s);
 }
 
-// Distillation: a wave a token.
+// Distillation: a workgroup a token, 16 lanes a product.
 template <typename T> __global__ __launch_bounds__(256) void loss_teacher_kernel(const LossParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (t >= p.tokens) return;
+  __shared__ float parts[4];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t t = p.first + blockIdx.x;
   const int k = static_cast<int>(p.k);
   const float* teacher = p.teacher + t * k;
-  float* share = p.share + t * k;
   const float c = 1.f / p.temperature;
-  auto in = [&](int i) {
-    const int64_t id = id_at(p, t * k + i);
-    return id >= 0 && id < p.vocab;
-  };
   // An entry of -inf has no share; NaN has, and makes the row NaN.
+  auto has = [&](int i) {
+    const int64_t id = id_at(p, t * k + i);
+    return id >= 0 && id < p.vocab && !(teacher[i] == -INFINITY);
+  };
+  // Every wave by itself.
   float m = -INFINITY;
   bool any = false;
   for (int i = lane; i < k; i += 64)
-    if (in(i) && !(teacher[i] == -INFINITY)) {
+    if (has(i)) {
       any = true;
       m = fmaxf(m, teacher[i]);
     }
@@ -102,33 +107,34 @@ template <typename T> __global__ __launch_bounds__(256) void loss_teacher_kernel
   const bool keep = __any(any);
   float sum = 0.f;
   for (int i = lane; i < k; i += 64)
-    if (in(i) && !(teacher[i] == -INFINITY)) sum += exp_acc((teacher[i] - m) * c);
+    if (has(i)) sum += exp_acc((teacher[i] - m) * c);
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
   const float logsum = logf(sum), inv = 1.f / sum;
-  for (int i = lane; i < k; i += 64)
-    share[i] = in(i) && !(teacher[i] == -INFINITY) ? exp_acc((teacher[i] - m) * c) * inv : 0.f;
-  // The products, 16 lanes each, and sum q (log q - c s).
+  // The products, and sum q (log q - c s).
   const int j = lane & 15;
   float cross = 0.f;
-  for (int i = lane >> 4; i < k; i += 4) {
-    const bool have = in(i) && !(teacher[i] == -INFINITY);
-    float s = 0.f;
-    if (have)
+  for (int i = threadIdx.x >> 4; i < k; i += 16) {
+    float s = 0.f, q = 0.f;
+    if (has(i)) {
       s = dot16<T>(static_cast<const T*>(p.hidden) + t * p.sh,
                    static_cast<const T*>(p.weight) + id_at(p, t * k + i) * p.sw, p.dim, j);
-    if (j == 0) p.picked[t * k + i] = s;
-    if (have) {
-      const float x = (teacher[i] - m) * c, q = exp_acc(x) * inv;
+      const float x = (teacher[i] - m) * c;
+      q = exp_acc(x) * inv;
       if (!(q == 0.f)) cross = fmaf(q, (x - logsum) - c * s, cross);
+    }
+    if (j == 0) {
+      p.picked[t * k + i] = s;
+      p.share[t * k + i] = q;
     }
   }
   cross += __shfl_xor(cross, 16);
   cross += __shfl_xor(cross, 32);
-  if (lane == 0) {
-    p.keep[t] = keep;
-    p.cross[t] = cross;
-  }
+  if (lane == 0) parts[w] = cross;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  p.keep[t] = keep;
+  p.cross[t] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
 }
 
 __device__ __forceinline__ bool counts(const LossParams& p, int64_t t) {
@@ -207,7 +213,13 @@ __global__ __launch_bounds__(256) void loss_most_kernel(const LossParams p, bool
     const uint32_t o = __shfl_xor(most, s);
     most = o > most ? o : most;
   }
-  if ((threadIdx.x & 63) == 0 && most > 0) atomicMax(of_weight ? &p.scal->wmax : &p.scal->hmax, most);
+  // One atomic a workgroup: one a wave, 8192 to one address, took 80 us.
+  __shared__ uint32_t tops[4];
+  if (lane == 0) tops[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 4; ++i) most = tops[i] > most ? tops[i] : most;
+  if (most > 0) atomicMax(of_weight ? &p.scal->wmax : &p.scal->hmax, most);
 }
 
 // A row in the products' layout, zero behind its end: a wave a row, 64 elements at a time.
@@ -225,6 +237,8 @@ __device__ __forceinline__ void lay_row(const T* from, void* to, int64_t at, int
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[e] = hi[e], out[piece + e] = lo[e];
     } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= up;
       st4_elem<T>(static_cast<T*>(to) + at, i, v);
     }
   }
@@ -234,18 +248,22 @@ template <typename T> __global__ __launch_bounds__(256) void loss_gather_kernel(
   const int64_t i = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t kept = p.scal->kept;
   if (i >= (kept + kLossTile - 1) / kLossTile * kLossTile) return;
-  const float up = pow2(up_exponent(p.scal->hmax));
+  const float up = std::is_same_v<T, float> ? pow2(up_exponent(p.scal->hmax)) : 1.f;
   const int64_t t = i < kept ? p.rows[i] : 0;
   const T* from = i < kept ? static_cast<const T*>(p.hidden) + t * p.sh : nullptr;
   if (p.target != nullptr && (threadIdx.x & 63) == 0)
     p.target[i] = i < kept ? static_cast<int32_t>(id_at(p, t)) : -1;
   lay_row<T>(from, p.hrows, i * p.dpad, p.tpad * p.dpad, p.dim, p.dpad, up, threadIdx.x & 63);
+  // The backward's, in the largest unit.
+  if (p.hscaled != nullptr)
+    lay_row<T>(from, p.hscaled, i * p.dpad, p.tpad * p.dpad, p.dim, p.dpad,
+               up * (i < kept ? unit_of(p, i) / p.scal->unit : 0.f), threadIdx.x & 63);
 }
 
 template <typename T> __global__ __launch_bounds__(256) void loss_weight_kernel(const LossParams p) {
   const int64_t v = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (v >= p.vocab) return;
-  const float up = pow2(up_exponent(p.scal->wmax));
+  const float up = std::is_same_v<T, float> ? pow2(up_exponent(p.scal->wmax)) : 1.f;
   lay_row<T>(static_cast<const T*>(p.weight) + v * p.sw, p.wrows, v * p.dpad, p.vocab * p.dpad, p.dim, p.dpad, up,
              threadIdx.x & 63);
 }
@@ -264,8 +282,8 @@ template <typename T> __device__ __forceinline__ float logit_scale(const LossPar
   return kLog2e / p.temperature * logit_back<T>(p);
 }
 
-__device__ __forceinline__ Operand rows_operand(const LossParams& p) {
-  return {p.hrows, p.dpad, p.tpad * p.dpad, p.tpad * p.dpad};
+__device__ __forceinline__ Operand rows_operand(const LossParams& p, const void* rows) {
+  return {rows, p.dpad, p.tpad * p.dpad, p.tpad * p.dpad};
 }
 __device__ __forceinline__ Operand weight_operand(const LossParams& p, int64_t v0) {
   // In place, the rows end with dim = dpad elements.
@@ -311,7 +329,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_logits_kern
   const float c = logit_scale<T>(p), back = logit_back<T>(p);
   const int32_t target[2] = {p.target != nullptr ? p.target[t0] : -1, p.target != nullptr ? p.target[t0 + 32] : -1};
   constexpr int runs = kRuns<T>;
-  const ProductParams q = {weight_operand(p, 0), rows_operand(p), p.dpad, runs};
+  const ProductParams q = {weight_operand(p, 0), rows_operand(p, p.hrows), p.dpad, runs};
   MCPU_TILE_LDS(a0, b0, a1, b1);
   Acc acc;
   tile_product<Kept<T>, false, false>(q, mt * kLossTile, nt * kLossTile, 0,
@@ -361,19 +379,20 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
   if (!tile_of(blockIdx.x, p.vpiece / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = mt * kLossTile + (wave >> 2) * 128, t0 = nt * kLossTile + (wave & 3) * 64 + (lane & 31);
-  const float c = logit_scale<T>(p), up = kUp<E> / p.scal->unit;
+  const float c = logit_scale<T>(p);
   float a[2], b[2], m2[2];
   int32_t target[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t t = t0 + j * 32;
+    const float up = kUp<E> / unit_of(p, t);
     a[j] = p.coef[t] * up;
     b[j] = p.coef[p.tpad + t] * up;
     m2[j] = p.coef[2 * p.tpad + t];
     target[j] = p.target != nullptr ? p.target[t] : -1;
   }
   constexpr int runs = kRuns<T>;
-  const ProductParams q = {weight_operand(p, vp), rows_operand(p), p.dpad, runs};
+  const ProductParams q = {weight_operand(p, vp), rows_operand(p, p.hrows), p.dpad, runs};
   MCPU_TILE_LDS(a0, b0, a1, b1);
   Acc acc;
   tile_product<E, false, false>(q, mt * kLossTile, nt * kLossTile, 0, static_cast<int>(p.dpad / kLossDepth) * runs,
@@ -421,7 +440,11 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
   }
 }
 
-// Distillation: the ids' places of ds, a_t exp(c s - L) less all shares of that id. A wave a row.
+// Distillation: the ids' places of ds, a_t exp(c s - L) less all shares of that id. A
+// wave a row. In 16 bits that is formed anew, to be rounded once. float32 takes p
+// from the two pieces that are there: where p and its share are both near 1, their
+// difference is as good as p agrees with the row's sum, and that is of the same
+// product, while `picked` is a sum of its own.
 template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(const LossParams p, int64_t vp) {
   using E = Kept<T>;
   const int lane = threadIdx.x & 63;
@@ -429,21 +452,26 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
   if (i >= p.scal->kept) return;
   const int64_t t = p.rows[i];
   const int k = static_cast<int>(p.k);
-  const float up = kUp<E> / p.scal->unit, c = kLog2e / p.temperature;
+  const float up = kUp<E> / unit_of(p, i), c = kLog2e / p.temperature;
   const float a = p.coef[i] * up, b = p.coef[p.tpad + i] * up, m2 = p.coef[2 * p.tpad + i];
   for (int e = lane; e < k; e += 64) {
     const int64_t id = id_at(p, t * k + e);
     const int64_t v = id - vp;
     if (id < 0 || id >= p.vocab || v < 0 || v >= p.vpiece) continue;
     float q = 0.f;
-    for (int o = 0; o < k; ++o) q += id_at(p, t * k + o) == id ? p.share[t * k + o] : 0.f;
-    const float g = a * fast_exp2(fmaf(p.picked[t * k + e], c, -m2)) - b * q;
-    uint16_t* out = static_cast<uint16_t*>(p.grad) + i * p.vpiece + v;
-    *out = __builtin_bit_cast(uint16_t, from_f32<E>(g));
+    bool first = true;
+    for (int o = 0; o < k; ++o) {
+      const bool same = id_at(p, t * k + o) == id;
+      q += same ? p.share[t * k + o] : 0.f;
+      first = first && !(same && o < e);
+    }
+    if (!first || q == 0.f) continue;  // an id's first entry places it; entries left out may have no product
+    E* out = static_cast<E*>(p.grad) + i * p.vpiece + v;
     if constexpr (std::is_same_v<T, float>) {
-      f16 h, l;
-      split_f16(g, h, l);
-      out[p.tpad * p.vpiece] = __builtin_bit_cast(uint16_t, l);
+      E* low = out + p.tpad * p.vpiece;
+      split_f16((static_cast<float>(*out) + static_cast<float>(*low)) - b * q, *out, *low);
+    } else {
+      *out = from_f32<E>(a * fast_exp2(fmaf(p.picked[t * k + e], c, -m2)) - b * q);
     }
   }
 }
@@ -488,27 +516,34 @@ __global__ __launch_bounds__(512, 2) void loss_dhidden_kernel(const LossParams p
   }
 }
 
-// dhidden in its own type: the splits' sum; rows that do not count have none. A wave a row.
+// Sums of splits' results at four columns, eight loads on their way.
+__device__ __forceinline__ void sum_splits(const float* at, int64_t stride, int splits, float (&v)[4]) {
+  for (int s0 = 0; s0 < splits; s0 += 8) {
+    float4 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      x[u] = s0 + u < splits ? *reinterpret_cast<const float4*>(at + (s0 + u) * stride) : make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[0] += x[u].x, v[1] += x[u].y, v[2] += x[u].z, v[3] += x[u].w;
+  }
+}
+
+// dhidden in its own type: the splits' sum; rows that do not count have none. A wave 256 columns of a row.
 template <typename T> __global__ __launch_bounds__(256) void loss_dhidden_out_kernel(const LossParams p) {
   using E = Kept<T>;
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (i >= p.tokens) return;
+  const int64_t at = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t across = (p.dim + 255) / 256, i = at / across, d = (at - i * across) * 256 + (threadIdx.x & 63) * 4;
+  if (i >= p.tokens || d >= p.dim) return;
   const bool in = i < p.scal->kept;
-  float scale = p.scal->unit / kUp<E>;
-  if constexpr (std::is_same_v<T, float>) scale *= pow2(-up_exponent(p.scal->wmax));
-  T* out = static_cast<T*>(p.dhidden) + p.rows[i] * p.dim;
-  for (int64_t d = lane * 4; d < p.dim; d += 256) {
-    float v[4] = {};
-    if (in)
-      for (int s = 0; s < p.hsplit; ++s) {
-        const float4 o = *reinterpret_cast<const float4*>(p.acc + (s * p.tpad + i) * p.dpad + d);
-        v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
-      }
+  float v[4] = {};
+  if (in) {
+    float scale = unit_of(p, i) / kUp<E>;
+    if constexpr (std::is_same_v<T, float>) scale *= pow2(-up_exponent(p.scal->wmax));
+    sum_splits(p.acc + i * p.dpad + d, p.tpad * p.dpad, p.hsplit, v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = in ? v[e] * scale : 0.f;
-    st_upto4<T>(out, d, upto4(p.dim - d), v);
+    for (int e = 0; e < 4; ++e) v[e] *= scale;
   }
+  st_upto4<T>(static_cast<T*>(p.dhidden) + p.rows[i] * p.dim, d, upto4(p.dim - d), v);
 }
 
 // dweight of a piece: m along the dim, n along the vocabulary, terms along the tokens.
@@ -522,7 +557,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(const LossParams p
   const int split = static_cast<int>(ns - nt * p.wsplit);
   constexpr int runs = kRuns<T>;
   const int64_t depth = (int64_t{p.scal->kept} + kLossDepth - 1) / kLossDepth * kLossDepth;
-  const ProductParams q = {rows_operand(p), grad_operand(p), depth, runs};
+  const ProductParams q = {rows_operand(p, p.hscaled != nullptr ? p.hscaled : p.hrows), grad_operand(p), depth, runs};
   const int depths = static_cast<int>(depth / kLossDepth) * runs;
   MCPU_TILE_LDS(a0, b0, a1, b1);
   Acc acc;
@@ -555,23 +590,45 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(const LossParams p
   }
 }
 
-// dweight of a piece from its splits. A wave a row.
+// dweight of a piece from its splits. A wave 256 columns of a row.
 template <typename T> __global__ __launch_bounds__(256) void loss_dweight_out_kernel(const LossParams p, int64_t vp) {
-  const int lane = threadIdx.x & 63;
-  const int64_t vl = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (vl >= p.vpiece || vp + vl >= p.vocab) return;
-  T* out = static_cast<T*>(p.dweight) + (vp + vl) * p.dim;
-  for (int64_t d = lane * 4; d < p.dim; d += 256) {
-    float v[4] = {};
-    for (int s = 0; s < p.wsplit; ++s) {
-      const float4 o = *reinterpret_cast<const float4*>(p.dwpart + (s * p.vpiece + vl) * p.dpad + d);
-      v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
-    }
-    st_upto4<T>(out, d, upto4(p.dim - d), v);
-  }
+  const int64_t at = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t across = (p.dim + 255) / 256, vl = at / across;
+  const int64_t d = (at - vl * across) * 256 + (threadIdx.x & 63) * 4;
+  if (vl >= p.vpiece || vp + vl >= p.vocab || d >= p.dim) return;
+  float v[4] = {};
+  sum_splits(p.dwpart + vl * p.dpad + d, p.vpiece * p.dpad, p.wsplit, v);
+  st_upto4<T>(static_cast<T*>(p.dweight) + (vp + vl) * p.dim, d, upto4(p.dim - d), v);
 }
 
 // ---- the loss of a row, and of all ------------------------------------------------------------
+
+// The loss of row t, the i-th that counts, from the maximum of its logits and the sum relative to it; cross
+// entropy: of all but the target's, which comes by itself.
+__device__ __forceinline__ void finish_row(const LossParams& p, int64_t t, int64_t i, float top, float sum,
+                                           float own) {
+  const float c = kLog2e / p.temperature;
+  float* stat = p.stat + i;
+  if (p.teacher == nullptr) {
+    // The target joins the others: relative to their maximum, as long as that is in float32's range.
+    const float d = own - top;
+    const bool far = !(d <= 40.f);
+    const float mine = far ? 1.f : fast_exp2(d * c), others = far ? sum * fast_exp2(-d * c) : sum;
+    const float all = mine + others;
+    // log(all / mine), by log1p where the target is the largest.
+    const float r = others / mine, u = 1.f + r;
+    p.each[t] = d >= 0.f ? (u == 1.f ? r : logf(u) * (r / (u - 1.f))) : logf(all) - d;
+    stat[2 * p.tokens] = mine / all;
+    stat[3 * p.tokens] = others / all;
+    top = far ? own : top;
+    sum = all;
+  }
+  const float lse = top / p.temperature + logf(sum);
+  p.lse[t] = lse;
+  stat[0] = top;
+  stat[p.tokens] = sum;
+  if (p.teacher != nullptr) p.each[t] = (p.cross[t] + lse) * p.temperature * p.temperature;
+}
 
 // 32 tokens a workgroup: eight threads a token join the parts, one takes the loss.
 __global__ __launch_bounds__(256) void loss_join_kernel(const LossParams p) {
@@ -614,27 +671,282 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const LossParams p) {
   const float sub = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
   for (int q = 0; q < 8; ++q) sum = fmaf(ss[q][x], fast_exp2((ms[q][x] - sub) * c), sum);
-  float* stat = p.stat + i;
-  if (p.teacher == nullptr) {
-    // The target joins the others: relative to their maximum, as long as that is in float32's range.
-    const float own = p.picked[i], d = own - top;
-    const bool far = !(d <= 40.f);
-    const float mine = far ? 1.f : fast_exp2(d * c), others = far ? sum * fast_exp2(-d * c) : sum;
-    const float all = mine + others;
-    // log(all / mine), by log1p where the target is the largest.
-    const float r = others / mine, u = 1.f + r;
-    p.each[t] = d >= 0.f ? (u == 1.f ? r : logf(u) * (r / (u - 1.f))) : logf(all) - d;
-    stat[2 * p.tokens] = mine / all;
-    stat[3 * p.tokens] = others / all;
-    top = far ? own : top;
-    sum = all;
-  }
-  const float lse = top / p.temperature + logf(sum);
-  p.lse[t] = lse;
-  stat[0] = top;
-  stat[p.tokens] = sum;
-  if (p.teacher != nullptr) p.each[t] = (p.cross[t] + lse) * p.temperature * p.temperature;
+  finish_row(p, t, i, top, sum, p.teacher == nullptr ? p.picked[i] : 0.f);
 }
+
+// ---- few tokens ------------------------------------------------------------------------------------
+
+// Up to 64 tokens: the weight streams past them once, straight into the operands'
+// registers, 32 vocabulary rows a wave and every wave by itself, so that what
+// bounds it is HBM. Terms are taken in the order the loads bring them, the same for
+// both operands: lane l has row l % 16 and the 16 bytes at l / 16 of each 64.
+// float32 goes through v_mfma_f32_16x16x4_f32, four to a load.
+typedef uint32_t u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T> constexpr int kChunk = 16 / static_cast<int>(sizeof(T));
+
+template <typename T> __device__ __forceinline__ u32x4 chunk_at(const T* row, int64_t k) {
+  return *reinterpret_cast<const u32x4_e2*>(row + k);
+}
+// A chunk of which the row may have less, or nothing.
+template <typename T> __device__ __forceinline__ u32x4 chunk_left(const T* row, int64_t k, int64_t dim) {
+  if (k + kChunk<T> <= dim) return chunk_at<T>(row, k);
+  T v[kChunk<T>];
+#pragma unroll
+  for (int e = 0; e < kChunk<T>; ++e) v[e] = k + e < dim ? row[k + e] : T{};
+  return __builtin_bit_cast(u32x4, v);
+}
+template <typename T> __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (std::is_same_v<T, bf16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  } else if constexpr (std::is_same_v<T, f16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  } else {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// The products of NF x 16 rows of hidden, h, and a wave's 32 rows of weight from v0 on:
+// s[i][j][e] is of vocabulary row v0 + 16 i + 4 (lane / 16) + e and token 16 j + lane % 16.
+// Forward and backward form them alike, to the bit.
+template <typename T, int NF>
+__device__ __forceinline__ void few_products(const LossParams& p, const T* const (&h)[NF], int64_t v0, int lane,
+                                             f32x4 (&s)[2][NF]) {
+  const int64_t k0 = (lane >> 4) * kChunk<T>;
+  const T* w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t v = v0 + 16 * i + (lane & 15);  // a row that is not there is read as the last
+    w[i] = static_cast<const T*>(p.weight) + (v < p.vocab ? v : p.vocab - 1) * p.sw;
+  }
+  // Two sums of every other load's products: half the roundings in a row.
+  f32x4 acc[2][2][NF];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) acc[u][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kStep = 4 * kChunk<T>, kTurn = 4;  // terms of a load, loads of a turn
+  const int64_t whole = p.dim / (kStep * kTurn) * (kStep * kTurn);
+  u32x4 a[2][kTurn][2], b[2][kTurn][NF];  // this turn's and the next's
+  auto load = [&](int to, int64_t k) {
+#pragma unroll
+    for (int u = 0; u < kTurn; ++u) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) a[to][u][i] = chunk_at<T>(w[i], k + k0 + u * kStep);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) b[to][u][j] = chunk_at<T>(h[j], k + k0 + u * kStep);
+    }
+  };
+  auto turn = [&](int of) {
+#pragma unroll
+    for (int u = 0; u < kTurn; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[u & 1][i][j] = mma16<T>(a[of][u][i], b[of][u][j], acc[u & 1][i][j]);
+  };
+  int64_t k = 0;
+  if (whole > 0) load(0, 0);
+  for (; k + 2 * kStep * kTurn <= whole; k += 2 * kStep * kTurn) {
+    load(1, k + kStep * kTurn);
+    turn(0);
+    load(0, k + 2 * kStep * kTurn < whole ? k + 2 * kStep * kTurn : k);
+    turn(1);
+  }
+  if (k < whole) turn(0);
+  for (k = whole; k < p.dim; k += kStep) {
+    u32x4 x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = chunk_left<T>(w[i], k + k0, p.dim);
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const u32x4 y = chunk_left<T>(h[j], k + k0, p.dim);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[0][i][j] = mma16<T>(x[i], y, acc[0][i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][j][e] = acc[0][i][j][e] + acc[1][i][j][e];
+}
+
+// NF x 16 tokens; 256 vocabulary rows a workgroup, and of them one maximum and sum a token.
+template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_kernel(const LossParams p) {
+  __shared__ float2 parts[8][NF * 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t v0 = blockIdx.x * int64_t{256} + wave * 32;
+  const T* h[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const int64_t t = 16 * j + (lane & 15);  // a token that is not there is read as the last
+    h[j] = static_cast<const T*>(p.hidden) + (t < p.tokens ? t : p.tokens - 1) * p.sh;
+  }
+  f32x4 acc[2][NF];
+  few_products<T, NF>(p, h, v0, lane, acc);
+  const float c = kLog2e / p.temperature;
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const int64_t t = 16 * j + (lane & 15);
+    const int64_t target = p.teacher == nullptr && t < p.tokens && counts(p, t) ? id_at(p, t) : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t v = v0 + 16 * i + 4 * (lane >> 4) + e;
+        if (v == target) p.picked[t] = acc[i][j][e];
+        if (v == target || v >= p.vocab) acc[i][j][e] = -INFINITY;
+        m = fmaxf(m, acc[i][j][e]);
+      }
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float sub = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += fast_exp2((acc[i][j][e] - sub) * c);
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (lane < 16) parts[wave][16 * j + lane] = make_float2(m, s);
+  }
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t >= NF * 16 || t >= p.tokens) return;
+  float m = parts[0][t].x, s = 0.f;
+  for (int q = 1; q < 8; ++q) m = fmaxf(m, parts[q][t].x);
+  const float sub = m == -INFINITY ? 0.f : m;
+  for (int q = 0; q < 8; ++q) s = fmaf(parts[q][t].y, fast_exp2((parts[q][t].x - sub) * c), s);
+  p.part[int64_t{blockIdx.x} * kLossFew + t] = make_float2(m, s);
+}
+
+// ds of up to 64 tokens that count, as loss_grad_kernel; rows behind them up to 64 are zero.
+template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
+  using E = Kept<T>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t vl = blockIdx.x * int64_t{256} + wave * 32, v0 = vp + vl;
+  const int kept = p.scal->kept;
+  f32x4 acc[2][NF];
+  const T* h[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const int i = 16 * j + (lane & 15);
+    h[j] = static_cast<const T*>(p.hidden) + p.rows[kept == 0 ? 0 : i < kept ? i : kept - 1] * p.sh;
+  }
+  few_products<T, NF>(p, h, v0, lane, acc);
+  const float c = kLog2e / p.temperature;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int t = 16 * j + (lane & 15);
+    const bool in = j < NF && t < kept;
+    const float up = in ? kUp<E> / unit_of(p, t) : 0.f;
+    const float a = in ? p.coef[t] * up : 0.f, b = in ? p.coef[p.tpad + t] * up : 0.f;
+    const float m2 = in ? p.coef[2 * p.tpad + t] : 0.f;
+    const int64_t target = in && p.target != nullptr ? p.target[t] : -1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = 16 * i + 4 * (lane >> 4);
+      float x[4] = {};
+      if (in) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t v = v0 + at + e;
+          x[e] = v >= p.vocab ? 0.f : v == target ? b : a * fast_exp2(fmaf(acc[i][j < NF ? j : 0][e], c, -m2));
+        }
+      }
+      E* out = static_cast<E*>(p.grad) + t * p.vpiece + vl + at;
+      st4_elem<E>(out, 0, x);
+      if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f16 hi, lo;
+          split_f16(x[e], hi, lo);
+          x[e] = static_cast<float>(lo);
+        }
+        st4_elem<E>(out, p.tpad * p.vpiece, x);
+      }
+    }
+  }
+}
+
+// As f<16-token groups>() for up to 64 tokens.
+template <typename F> void for_few(int64_t tokens, F&& f) {
+  if (tokens <= 16)
+    f(std::integral_constant<int, 1>{});
+  else if (tokens <= 32)
+    f(std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 4>{});
+}
+
+// The rows that count, their losses and all rows' of up to 64 tokens: one workgroup, 16 threads a token.
+__global__ __launch_bounds__(1024) void loss_few_join_kernel(const LossParams p) {
+  const int t = threadIdx.x >> 4, j = threadIdx.x & 15, n = static_cast<int>(p.tokens);
+  __shared__ float losses[64];
+  __shared__ unsigned long long mask;
+  if (threadIdx.x < 64) {
+    const unsigned long long m = __ballot(threadIdx.x < n && counts(p, threadIdx.x));
+    if (threadIdx.x == 0) mask = m;
+  }
+  __syncthreads();
+  const bool keep = mask >> t & 1;
+  const int kept = __popcll(mask), before = __popcll(mask & ((1ull << t) - 1));
+  const int64_t parts = (p.vocab + 255) / 256;
+  const float c = kLog2e / p.temperature;
+  float m = -INFINITY, s = 0.f;
+  if (keep)
+    for (int64_t q0 = j; q0 < parts; q0 += 128) {
+      float2 x[8];
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        x[u] = q0 + 16 * u < parts ? p.part[(q0 + 16 * u) * kLossFew + t] : make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, x[u].x);
+      }
+      const float sub = top == -INFINITY ? 0.f : top;
+      s *= fast_exp2((m - sub) * c);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s = fmaf(x[u].y, fast_exp2((x[u].x - sub) * c), s);
+      m = top;
+    }
+  float top = m;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  s *= fast_exp2((m - (top == -INFINITY ? 0.f : top)) * c);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+  if (j == 0) {
+    if (keep) {
+      finish_row(p, t, before, top, s, p.teacher == nullptr ? p.picked[t] : 0.f);
+    } else if (t < n) {
+      p.lse[t] = 0.f;
+      p.each[t] = 0.f;
+    }
+    if (t < n) p.rows[keep ? before : kept + t - before] = t;
+    losses[t] = t < n ? p.each[t] : 0.f;
+    if (t == 0) p.rows[n] = kept;
+  }
+  if (p.reduction == MCPU_REDUCE_NONE) return;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  float sum = losses[threadIdx.x];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  if (threadIdx.x == 0)
+    p.loss[0] = p.reduction == MCPU_REDUCE_MEAN ? sum / static_cast<float>(kept > 0 ? kept : 1) : sum;
+}
+
+// ---- all rows ------------------------------------------------------------------------------------
 
 // The sum or mean of the rows' losses, one workgroup, in a fixed order.
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossParams p) {
@@ -656,9 +968,11 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossParams p) {
   p.loss[0] = p.reduction == MCPU_REDUCE_MEAN ? s / static_cast<float>(kept > 0 ? kept : 1) : s;
 }
 
-// Coefficients of the rows that count, and the unit their gradients are kept in: the
-// largest coefficient itself, so that where all are alike, as under a mean, a
-// target's ds of nearly -unit is not rounded the same way in every row. One workgroup.
+// Coefficients of the rows that count, and the unit each one's ds is kept in. In
+// 16 bits a rounding of the target's ds, the row's largest, would be in all of
+// the row's gradient alike; so the unit is that ds itself (exactly 1 then), and
+// dweight takes the units from hidden's rows, scaled by unit / the largest unit.
+// Distillation: one unit, the largest coefficient. One workgroup.
 __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   __shared__ float tops[16];
   const int32_t kept = p.rows[p.tokens];
@@ -686,12 +1000,14 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
       const float a = g[u] + e[u];
       // exp(c (s - maximum)) as 2^(c s - m2), with the rounding of m2 in the factor.
       const float m2 = stat[0][u] * c, off = fmaf(stat[0][u], c, -m2);
-      p.coef[i] = a / stat[1][u] * fmaf(-kLn2, off, 1.f);
-      // Cross entropy: the target's ds, a p - g = (a - g) p - g (1 - p).
-      p.coef[p.tpad + i] = p.share != nullptr ? g[u] : e[u] * stat[2][u] - g[u] * stat[3][u];
-      p.coef[2 * p.tpad + i] = m2;
-      const float top = fmaxf(__builtin_fabsf(a), __builtin_fabsf(g[u]));
+      // Cross entropy: the target's ds, a p - g = (a - g) p - g (1 - p); no other is above a (1 - p).
+      const float own = p.share != nullptr ? g[u] : e[u] * stat[2][u] - g[u] * stat[3][u];
+      const float top = fmaxf(__builtin_fabsf(own), __builtin_fabsf(a) * (p.share != nullptr ? 1.f : stat[3][u]));
       if (top < INFINITY) most = fmaxf(most, top);
+      p.coef[i] = a / stat[1][u] * fmaf(-kLn2, off, 1.f);
+      p.coef[p.tpad + i] = own;
+      p.coef[2 * p.tpad + i] = m2;
+      p.coef[3 * p.tpad + i] = p.share == nullptr && top > 0x1p-100f && top < INFINITY ? top : 0.f;
     }
   }
 #pragma unroll
@@ -717,8 +1033,8 @@ void run(K kernel, LossParams p, int64_t groups, int threads, hipStream_t st, A.
 
 template <typename T> void lay_operands(const LossParams& p, hipStream_t st) {
   if constexpr (std::is_same_v<T, float>) {
-    run(loss_most_kernel, p, std::min<int64_t>((p.tokens + 3) / 4, 2048), 256, st, false);
-    run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 3) / 4, 2048), 256, st, true);
+    run(loss_most_kernel, p, std::min<int64_t>((p.tokens + 3) / 4, 512), 256, st, false);
+    run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 3) / 4, 1024), 256, st, true);
   }
   run(loss_gather_kernel<T>, p, p.tpad / 4, 256, st);
   if (p.wrows != nullptr) run(loss_weight_kernel<T>, p, (p.vocab + 3) / 4, 256, st);
@@ -726,7 +1042,14 @@ template <typename T> void lay_operands(const LossParams& p, hipStream_t st) {
 
 template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   if (p.teacher != nullptr)
-    run(loss_teacher_kernel<T>, p, (p.tokens + 3) / 4, 256, st);
+    run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
+  if (p.tokens <= kLossFew) {
+    for_few(p.tokens, [&](auto nf) {
+      run(loss_few_kernel<T, decltype(nf)::value>, p, (p.vocab + 255) / 256, 512, st);
+    });
+    run(loss_few_join_kernel, p, 1, 1024, st);
+    return hipGetLastError();
+  }
   run(loss_rows_kernel, p, 1, 1024, st);
   lay_operands<T>(p, st);
   const int64_t vt = (p.vocab + kLossTile - 1) / kLossTile, tt = p.tpad / kLossTile;
@@ -741,15 +1064,20 @@ template <typename T> hipError_t bwd(const LossParams& p, hipStream_t st) {
   lay_operands<T>(p, st);
   const int64_t tt = p.tpad / kLossTile, vt = p.vpiece / kLossTile, dt = (p.dpad + kLossTile - 1) / kLossTile;
   for (int64_t vp = 0; vp < p.vocab; vp += p.vpiece) {
-    run(loss_grad_kernel<T>, p, vt * tt, 512, st, vp);
+    if (p.tokens <= kLossFew)
+      for_few(p.tokens, [&](auto nf) {
+        run(loss_few_grad_kernel<T, decltype(nf)::value>, p, vt, 512, st, vp);
+      });
+    else
+      run(loss_grad_kernel<T>, p, vt * tt, 512, st, vp);
     if (p.share != nullptr) run(loss_place_kernel<T>, p, (p.tokens + 3) / 4, 256, st, vp);
     if (p.dhidden != nullptr) run(loss_dhidden_kernel<T>, p, dt * tt * p.hsplit, 512, st, vp, vp > 0);
     if (p.dweight != nullptr) {
       run(loss_dweight_kernel<T>, p, dt * vt * p.wsplit, 512, st, vp);
-      if (p.dwpart != nullptr) run(loss_dweight_out_kernel<T>, p, vt * kLossTile / 4, 256, st, vp);
+      if (p.dwpart != nullptr) run(loss_dweight_out_kernel<T>, p, (p.vpiece * ((p.dim + 255) / 256) + 3) / 4, 256, st, vp);
     }
   }
-  if (p.dhidden != nullptr) run(loss_dhidden_out_kernel<T>, p, (p.tokens + 3) / 4, 256, st);
+  if (p.dhidden != nullptr) run(loss_dhidden_out_kernel<T>, p, (p.tokens * ((p.dim + 255) / 256) + 3) / 4, 256, st);
   return hipGetLastError();
 }
 

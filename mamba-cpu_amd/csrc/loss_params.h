@@ -15,7 +15,7 @@ namespace mcpu {
 struct LossScalars {
   int32_t kept;          // rows that count
   uint32_t hmax, wmax;   // float32 operands: the largest finite magnitudes, as bits
-  float unit;            // backward: the largest coefficient of a row
+  float unit;            // backward: the largest unit of a row's ds
 };
 
 struct LossParams {
@@ -30,7 +30,8 @@ struct LossParams {
   float* loss;    // (tokens), or (1) where reduced
   float* each;    // (tokens): loss, or the terms of the reduced one
   float* lse;     // (tokens)
-  float* picked;  // (tokens, k): the products of hidden with the ids' rows; cross entropy: in the order of `rows`
+  float* picked;  // distillation: (tokens, k), the products of hidden with the ids' rows; else workspace, (padded
+                  // tokens), the targets' in the order of `rows` (few tokens: as they come)
   float* stat;    // (4, tokens) in the order of `rows`: maximum, sum of exp(c (s - it)), a target's share of it, the others'
   float* share;   // (tokens, k): the teacher's distribution, or null
   int32_t* rows;  // (tokens + 1): the rows that count in order, then the others; then how many count
@@ -45,8 +46,10 @@ struct LossParams {
   int32_t* target;    // (padded tokens) in the order of `rows`, cross entropy; else null
   float* cross;       // (tokens): sum of q (log q - c s)
   float2* part;       // (vocab parts, padded tokens): maximum of each part and sum of exp(c (s - it))
-  float* coef;        // (3, padded tokens): factor of 2^(logit - maximum), the target's ds or the shares' factor, maximum
+  float* coef;        // (4, padded tokens): factor of 2^(logit - maximum), the target's ds or the shares' factor,
+                      // the maximum, the unit of ds (0: the largest)
   void* hrows;        // (pieces, padded tokens, padded dim): hidden's rows that count
+  void* hscaled;      // hrows in the largest unit, or null: hrows has it (distillation)
   void* wrows;        // (pieces, vocab, padded dim), or null: weight is read in place
   void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits
   float* acc;         // (splits, padded tokens, padded dim): gradient of hidden
@@ -59,6 +62,7 @@ struct LossParams {
 constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a product
 constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
 constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
+constexpr int kLossFew = 64;      // most tokens of a forward that streams the weight past them
 constexpr int64_t kLossMaxK = 1024;
 
 // float32 operands are two f16 pieces.

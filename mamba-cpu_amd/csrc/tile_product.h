@@ -17,8 +17,9 @@
 //   by term  512 bytes a term, chunk c of term k at c ^ (2 (k % 4))
 //
 // float32 operands come as two f16 pieces, value = hi + lo, scaled to the f16
-// range by a power of two; their product is hi hi + hi lo + lo hi, three runs over
-// the same terms. What is left out is below 2^-22 of the factors.
+// range by a power of two; their product is hi lo + lo hi + hi hi, three runs over
+// the same terms, the small ones first, while a sum's roundings are small too. What
+// is left out is below 2^-22 of the factors.
 #pragma once
 
 #include "loss_params.h"
@@ -26,6 +27,7 @@
 
 namespace mcpu {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -137,8 +139,8 @@ __device__ __forceinline__ void tile_product(const ProductParams& p, int64_t m0,
   auto load = [&](char* la, char* lb, int kt) {
     const int run = kt >= 2 * depths ? 2 : kt >= depths ? 1 : 0;
     const int64_t k0 = int64_t{kt - run * depths} * kLossDepth;
-    tile_load<TA>(la, tile_rsrc<TA>(p.a, m0, k0, run == 2), lda2, wave, lane);
-    tile_load<TB>(lb, tile_rsrc<TB>(p.b, n0, k0, run == 1), ldb2, wave, lane);
+    tile_load<TA>(la, tile_rsrc<TA>(p.a, m0, k0, p.runs > 1 && run == 1), lda2, wave, lane);
+    tile_load<TB>(lb, tile_rsrc<TB>(p.b, n0, k0, p.runs > 1 && run == 0), ldb2, wave, lane);
   };
   auto step = [&](const char* la, const char* lb, char* na, char* nb, int kt) {
     // This wave's loads have arrived, then every wave's; and no wave reads the other buffer any more.

@@ -77,7 +77,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const
       check_like(name, "the teacher's logits", *teacher, at::kFloat, ids.sizes(), hidden).data_ptr());
   const at::IntArrayRef all(&tokens, 1), one;
   Tensor loss = at::empty(reduction == MCPU_REDUCE_NONE ? all : one, f32), lse = at::empty({tokens}, f32);
-  Tensor picked = at::empty({tokens, a.k}, f32), stat = at::empty({4, tokens}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
+  Tensor picked = at::empty({has(teacher) ? tokens : 0, a.k}, f32), stat = at::empty({4, tokens}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
   Tensor rows = at::empty({tokens + 1}, hidden.options().dtype(at::kInt));
   if (nothing_to_do(a)) {
     for (const Tensor& t : {loss, lse, rows}) t.zero_();
@@ -85,7 +85,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const
   }
   a.loss = static_cast<float*>(loss.data_ptr());
   a.lse = static_cast<float*>(lse.data_ptr());
-  a.picked = static_cast<float*>(picked.data_ptr());
+  a.picked = has(teacher) ? static_cast<float*>(picked.data_ptr()) : nullptr;
   a.stat = static_cast<float*>(stat.data_ptr());
   a.share = has(teacher) ? static_cast<float*>(share.data_ptr()) : nullptr;
   a.rows = static_cast<int32_t*>(rows.data_ptr());
@@ -117,7 +117,7 @@ std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const 
   const int64_t all[2] = {n, k}, stats[2] = {4, n};
   const at::IntArrayRef per(&n, 1), both(all, 2), four(stats, 2), one;
   a.stat = static_cast<float*>(check_like(name, "stat", stat, at::kFloat, four, hidden).data_ptr());
-  a.picked = static_cast<float*>(check_like(name, "picked", picked, at::kFloat, both, hidden).data_ptr());
+  if (distil) a.picked = static_cast<float*>(check_like(name, "picked", picked, at::kFloat, both, hidden).data_ptr());
   if (distil) a.share = static_cast<float*>(check_like(name, "share", share, at::kFloat, both, hidden).data_ptr());
   a.rows = static_cast<int32_t*>(
       check_like(name, "rows", rows, at::kInt, at::IntArrayRef(&last, 1), hidden).data_ptr());

@@ -34,7 +34,7 @@ def _(hidden, weight, ids, teacher, ignore_index, temperature, reduction):
     tokens, k = ids.shape
     f32 = dict(dtype=torch.float32)
     return (hidden.new_empty(() if reduction else (tokens,), **f32), hidden.new_empty(tokens, **f32),
-            hidden.new_empty(tokens, k, **f32), hidden.new_empty(4, tokens, **f32),
+            hidden.new_empty(tokens if teacher is not None else 0, k, **f32), hidden.new_empty(4, tokens, **f32),
             hidden.new_empty(tokens if teacher is not None else 0, k, **f32),
             hidden.new_empty(tokens + 1, dtype=torch.int32))
 

@@ -126,7 +126,8 @@ def verify_ce(dtype, h, w, ids, reduction="none", g=None, dlse=None, ignore_inde
 
 
 SIZES = [(1, 2, 1), (1, 300, 8), (2, 128, 64), (5, 129, 65), (64, 257, 200), (255, 200, 77), (256, 256, 64),
-         (257, 513, 128), (300, 1000, 192), (513, 70, 320), (40, 3001, 33)]
+         (257, 513, 128), (300, 1000, 192), (513, 70, 320), (40, 3001, 33),
+         (16, 260, 129), (17, 31, 1000), (32, 511, 512), (65, 130, 520)]
 
 
 @pytest.mark.gpu
