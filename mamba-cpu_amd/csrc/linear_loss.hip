@@ -376,7 +376,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
   using E = Kept<T>;
   const int64_t kept = p.scal->kept;
   int64_t mt, nt;
-  if (!tile_of(blockIdx.x, p.vpiece / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
+  if (!tile_of(blockIdx.x, p.vrows / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = mt * kLossTile + (wave >> 2) * 128, t0 = nt * kLossTile + (wave & 3) * 64 + (lane & 31);
   const float c = logit_scale<T>(p);
@@ -487,8 +487,8 @@ __global__ __launch_bounds__(512, 2) void loss_dhidden_kernel(const LossParams p
   const int64_t nt = ns / p.hsplit;
   const int split = static_cast<int>(ns - nt * p.hsplit);
   constexpr int runs = kRuns<T>;
-  const ProductParams q = {weight_operand(p, vp), grad_operand(p), p.vpiece, runs};
-  const int depths = static_cast<int>(p.vpiece / kLossDepth) * runs;
+  const ProductParams q = {weight_operand(p, vp), grad_operand(p), p.vrows, runs};
+  const int depths = static_cast<int>(p.vrows / kLossDepth) * runs;
   MCPU_TILE_LDS(a0, b0, a1, b1);
   Acc acc;
   tile_product<E, true, false>(q, mt * kLossTile, nt * kLossTile, static_cast<int>(int64_t{depths} * split / p.hsplit),
@@ -552,7 +552,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(const LossParams p
   using E = Kept<T>;
   const int64_t mts = (p.dpad + kLossTile - 1) / kLossTile;
   int64_t mt, ns;
-  if (!tile_of(blockIdx.x, mts, p.vpiece / kLossTile * p.wsplit, mt, ns)) return;
+  if (!tile_of(blockIdx.x, mts, p.vrows / kLossTile * p.wsplit, mt, ns)) return;
   const int64_t nt = ns / p.wsplit;
   const int split = static_cast<int>(ns - nt * p.wsplit);
   constexpr int runs = kRuns<T>;
@@ -595,7 +595,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_dweight_out_ke
   const int64_t at = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t across = (p.dim + 255) / 256, vl = at / across;
   const int64_t d = (at - vl * across) * 256 + (threadIdx.x & 63) * 4;
-  if (vl >= p.vpiece || vp + vl >= p.vocab || d >= p.dim) return;
+  if (vl >= p.vrows || vp + vl >= p.vocab || d >= p.dim) return;
   float v[4] = {};
   sum_splits(p.dwpart + vl * p.dpad + d, p.vpiece * p.dpad, p.wsplit, v);
   st_upto4<T>(static_cast<T*>(p.dweight) + (vp + vl) * p.dim, d, upto4(p.dim - d), v);
@@ -1059,11 +1059,14 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <typename T> hipError_t bwd(const LossParams& p, hipStream_t st) {
+template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
   run(loss_coef_kernel, p, 1, 1024, st);
   lay_operands<T>(p, st);
-  const int64_t tt = p.tpad / kLossTile, vt = p.vpiece / kLossTile, dt = (p.dpad + kLossTile - 1) / kLossTile;
+  const int64_t tt = p.tpad / kLossTile, dt = (p.dpad + kLossTile - 1) / kLossTile;
+  float* const dwpart = p.dwpart;
   for (int64_t vp = 0; vp < p.vocab; vp += p.vpiece) {
+    p.vrows = loss_piece_rows(p, vp);
+    const int64_t vt = p.vrows / kLossTile;
     if (p.tokens <= kLossFew)
       for_few(p.tokens, [&](auto nf) {
         run(loss_few_grad_kernel<T, decltype(nf)::value>, p, vt, 512, st, vp);
@@ -1073,8 +1076,10 @@ template <typename T> hipError_t bwd(const LossParams& p, hipStream_t st) {
     if (p.share != nullptr) run(loss_place_kernel<T>, p, (p.tokens + 3) / 4, 256, st, vp);
     if (p.dhidden != nullptr) run(loss_dhidden_kernel<T>, p, dt * tt * p.hsplit, 512, st, vp, vp > 0);
     if (p.dweight != nullptr) {
+      p.wsplit = loss_wsplit(p, vp);
+      p.dwpart = p.wsplit > 1 ? dwpart : nullptr;
       run(loss_dweight_kernel<T>, p, dt * vt * p.wsplit, 512, st, vp);
-      if (p.dwpart != nullptr) run(loss_dweight_out_kernel<T>, p, (p.vpiece * ((p.dim + 255) / 256) + 3) / 4, 256, st, vp);
+      if (p.wsplit > 1) run(loss_dweight_out_kernel<T>, p, (p.vrows * ((p.dim + 255) / 256) + 3) / 4, 256, st, vp);
     }
   }
   if (p.dhidden != nullptr) run(loss_dhidden_out_kernel<T>, p, (p.tokens * ((p.dim + 255) / 256) + 3) / 4, 256, st);
@@ -1083,30 +1088,64 @@ template <typename T> hipError_t bwd(const LossParams& p, hipStream_t st) {
 
 }  // namespace
 
-// Splits of a product's terms, for `tiles` results of 256 KiB over `depths` each: what 256 workgroups at a
-// time take, at 4.6 TFLOP/s each, and 4 TB/s for the splits' results, written and read.
-static int splits_for(int64_t tiles, int64_t depths) {
+// Microseconds of a product of `tiles` results of 256 KiB over `depths` each in
+// `splits`: 256 workgroups at a time, at 4.7 TFLOP/s each with 6 us around a tile,
+// and 4 TB/s for float32 results, written and read, where there are any.
+static double product_us(int64_t tiles, int64_t depths, int splits, bool apart) {
+  const double rounds = static_cast<double>((tiles * splits + 255) / 256);
+  return rounds * (static_cast<double>((depths + splits - 1) / splits) * 1.8 + 6) +
+         (apart || splits > 1 ? static_cast<double>(tiles * splits) * 0.131 : 0);
+}
+static int splits_for(int64_t tiles, int64_t depths, bool apart) {
   int best = 1;
-  double least = 0;
-  for (int s = 1; s <= 64 && (s == 1 || depths / s >= 8); ++s) {
-    const double rounds = static_cast<double>((tiles * s + 255) / 256), each = static_cast<double>(depths) / s;
-    const double us = rounds * (each * 1.8 + 6) + (s > 1 ? tiles * s * 0.131 : 0);
-    if (s == 1 || us < 0.97 * least) best = s, least = us;
-  }
+  for (int s : {2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64})
+    if (depths / s >= 4 && product_us(tiles, depths, s, apart) < 0.97 * product_us(tiles, depths, best, apart)) best = s;
   return best;
 }
 
+// The vocabulary piece: ds of one is at most 1 GiB, and of the sizes below that
+// give whole rounds of dweight's tiles, or equal pieces, the one that takes least.
+// Workspace, not time, grows with it otherwise.
 void loss_plan(LossParams& p) {
-  const int pieces = loss_pieces(p.dtype);
-  auto up = [](int64_t n, int64_t to) { return (n + to - 1) / to * to; };
-  p.tpad = up(p.tokens, kLossTile);
-  p.dpad = up(p.dim, kLossDepth);
-  const int64_t most = std::max<int64_t>(1, (int64_t{1} << 29) / pieces / p.tpad / kLossTile) * kLossTile;
-  const int64_t count = (p.vocab + most - 1) / most;
-  p.vpiece = up((p.vocab + count - 1) / count, kLossTile);
+  const int pieces = loss_pieces(p.dtype), runs = pieces == 2 ? 3 : 1;
+  auto up = [](int64_t n, int64_t to) { return (n + to - 1) / to; };
+  p.tpad = up(p.tokens, kLossTile) * kLossTile;
+  p.dpad = up(p.dim, kLossDepth) * kLossDepth;
+  const int64_t all = up(p.vocab, kLossTile), tt = p.tpad / kLossTile, dt = up(p.dpad, kLossTile);
+  const int64_t most = std::max<int64_t>(1, std::min(all, (int64_t{1} << 29) / pieces / p.tpad / kLossTile));
+  const int64_t per = kLossTile / kLossDepth;  // depths of a tile's rows
+  auto hsplit = [&](int64_t vt) { return splits_for(dt * tt, vt * per * runs, true); };
+  auto piece = [&](int64_t n, int h) {
+    const int w = splits_for(dt * n, tt * per * runs, false);
+    return product_us(n * tt, p.dpad / kLossDepth * runs, 1, false) + product_us(dt * tt, n * per * runs, h, true) +
+           product_us(dt * n, tt * per * runs, w, false) + 10;
+  };
+  auto cost = [&](int64_t vt) {
+    const int h = hsplit(vt);
+    const int64_t left = all % vt;
+    return static_cast<double>(all / vt) * piece(vt, h) + (left > 0 ? piece(left, h) : 0);
+  };
+  int64_t best = up(all, up(all, most));  // equal pieces
+  double least = cost(best);
+  for (int64_t rounds = 1; rounds <= 8; ++rounds) {
+    const int64_t vt = 256 * rounds / dt;
+    if (vt < 1 || vt > most) continue;
+    const double us = cost(vt);
+    if (us < 0.99 * least) least = us, best = vt;
+  }
+  p.vpiece = best * kLossTile;
+  p.hsplit = hsplit(best);
+  p.wsplit = std::max(loss_wsplit(p, 0), loss_wsplit(p, (all - 1) / best * p.vpiece));
+}
+
+int64_t loss_piece_rows(const LossParams& p, int64_t vp) {
+  const int64_t left = (p.vocab - vp + kLossTile - 1) / kLossTile * kLossTile;
+  return std::min(left, p.vpiece);
+}
+int loss_wsplit(const LossParams& p, int64_t vp) {
   const int64_t dt = (p.dpad + kLossTile - 1) / kLossTile;
-  p.hsplit = splits_for(dt * (p.tpad / kLossTile), p.vpiece / kLossDepth * (pieces == 2 ? 3 : 1));
-  p.wsplit = splits_for(dt * (p.vpiece / kLossTile), p.tpad / kLossDepth * (pieces == 2 ? 3 : 1));
+  return splits_for(dt * (loss_piece_rows(p, vp) / kLossTile), p.tpad / kLossDepth * (loss_pieces(p.dtype) == 2 ? 3 : 1),
+                    false);
 }
 
 hipError_t loss_fwd_launch(LossParams p, hipStream_t st) {

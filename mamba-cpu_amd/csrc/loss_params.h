@@ -55,6 +55,7 @@ struct LossParams {
   float* acc;         // (splits, padded tokens, padded dim): gradient of hidden
   float* dwpart;      // (splits, vocab piece, padded dim), or null: gradient of weight in one go
   int64_t tpad, dpad, vpiece;
+  int64_t vrows;      // of this piece, a multiple of 256, at most vpiece
   int hsplit, wsplit;
   int64_t first;      // this launch's first workgroup
 };
@@ -67,8 +68,11 @@ constexpr int64_t kLossMaxK = 1024;
 
 // float32 operands are two f16 pieces.
 inline int loss_pieces(int dtype) { return dtype == MCPU_F32 ? 2 : 1; }
-// Sets the padded sizes, the vocabulary piece and the splits.
+// Sets the padded sizes, the vocabulary piece and the splits (wsplit: the most of any piece); what a piece
+// that begins at vp has of them.
 void loss_plan(LossParams& p);
+int64_t loss_piece_rows(const LossParams& p, int64_t vp);
+int loss_wsplit(const LossParams& p, int64_t vp);
 hipError_t loss_fwd_launch(LossParams p, hipStream_t st);
 hipError_t loss_bwd_launch(LossParams p, hipStream_t st);
 
