@@ -121,7 +121,7 @@ size_t lay_bwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   w.take(p.coef, 4 * p.tpad);
   if (!distil(a)) w.take(p.hscaled, loss_pieces(a->dtype) * p.tpad * p.dpad, 2);
   w.take(p.grad, loss_pieces(a->dtype) * p.tpad * p.vpiece, 2);
-  if (p.dhidden != nullptr) w.take(p.acc, p.hsplit * p.tpad * p.dpad);
+  if (p.dhidden != nullptr) w.take(p.acc, p.htiles * kLossTile * kLossTile);
   if (p.dweight != nullptr && p.wsplit > 1) w.take(p.dwpart, p.wsplit * p.vpiece * p.dpad);
   return w.used;
 }

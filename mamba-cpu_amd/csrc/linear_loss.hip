@@ -33,6 +33,25 @@ __device__ __forceinline__ int64_t id_at(const LossParams& p, int64_t i) {
   return p.ids64 ? static_cast<const int64_t*>(p.ids)[i] : static_cast<const int32_t*>(p.ids)[i];
 }
 
+// Microseconds of a product of `tiles` results of 256 KiB over `depths` each in
+// `splits`: 256 workgroups at a time, at 4.7 TFLOP/s each with 6 us around a tile,
+// and 4 TB/s for float32 results, written and read, where there are any.
+__host__ __device__ inline float product_us(int64_t tiles, int64_t depths, int splits, bool apart) {
+  const float rounds = static_cast<float>((tiles * splits + 255) / 256);
+  return rounds * (static_cast<float>((depths + splits - 1) / splits) * 1.8f + 6.f) +
+         (apart || splits > 1 ? static_cast<float>(tiles * splits) * 0.131f : 0.f);
+}
+__host__ __device__ inline int splits_for(int64_t tiles, int64_t depths, bool apart) {
+  constexpr int kTry[] = {2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
+  int best = 1;
+  float least = product_us(tiles, depths, 1, apart);
+  for (int s : kTry) {
+    const float us = product_us(tiles, depths, s, apart);
+    if (depths / s >= 4 && tiles * s <= kLossSplitTiles && us < 0.97f * least) best = s, least = us;
+  }
+  return best;
+}
+
 // The power of two that brings a largest magnitude (as bits) to [2^13, 2^14), and its inverse.
 __device__ __forceinline__ int up_exponent(uint32_t most) {
   if (most == 0) return 0;
@@ -82,10 +101,9 @@ template <typename T> __device__ __forceinline__ float dot16(const T* h, const T
 }
 
 // Distillation: a workgroup a token, 16 lanes a product.
-template <typename T> __global__ __launch_bounds__(256) void loss_teacher_kernel(const LossParams p) {
-  __shared__ float parts[4];
+template <typename T, int THREADS> __device__ __forceinline__ void teacher_row(const LossParams& p, int64_t t) {
+  __shared__ float parts[THREADS / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t t = p.first + blockIdx.x;
   const int k = static_cast<int>(p.k);
   const float* teacher = p.teacher + t * k;
   const float c = 1.f / p.temperature;
@@ -114,7 +132,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_teacher_kernel
   // The products, and sum q (log q - c s).
   const int j = lane & 15;
   float cross = 0.f;
-  for (int i = threadIdx.x >> 4; i < k; i += 16) {
+  for (int i = threadIdx.x >> 4; i < k; i += THREADS / 16) {
     float s = 0.f, q = 0.f;
     if (has(i)) {
       s = dot16<T>(static_cast<const T*>(p.hidden) + t * p.sh,
@@ -133,8 +151,12 @@ template <typename T> __global__ __launch_bounds__(256) void loss_teacher_kernel
   if (lane == 0) parts[w] = cross;
   __syncthreads();
   if (threadIdx.x != 0) return;
+  for (int i = 1; i < THREADS / 64; ++i) cross += parts[i];
   p.keep[t] = keep;
-  p.cross[t] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
+  p.cross[t] = cross;
+}
+template <typename T> __global__ __launch_bounds__(256) void loss_teacher_kernel(const LossParams p) {
+  teacher_row<T, 256>(p, p.first + blockIdx.x);
 }
 
 __device__ __forceinline__ bool counts(const LossParams& p, int64_t t) {
@@ -143,38 +165,46 @@ __device__ __forceinline__ bool counts(const LossParams& p, int64_t t) {
   return id >= 0 && id < p.vocab && id != p.ignore;
 }
 
-// The rows that count, in order, then the others; one workgroup, 16 rows a thread at a time.
+// The rows that count, in order, then the others; one workgroup, 16 runs of 1024 rows at a time.
 __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossParams p) {
-  __shared__ int32_t sums[16];
+  __shared__ int32_t before[16][17];  // of a run's waves, then of all before them
+  __shared__ int32_t runs[17];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int64_t kept = 0;
   for (int64_t t0 = 0; t0 < p.tokens; t0 += 16384) {
-    const int64_t lo = t0 + threadIdx.x * 16;
-    uint32_t mask = 0;
+    uint32_t flags = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (lo + i < p.tokens) mask |= static_cast<uint32_t>(counts(p, lo + i)) << i;
-    const int32_t n = __popc(mask);
-    int32_t before = n;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int32_t o = __shfl_up(before, s);
-      if (lane >= s) before += o;
-    }
-    if (lane == 63) sums[w] = before;
-    __syncthreads();
-    int32_t base = 0, all = 0;
     for (int i = 0; i < 16; ++i) {
-      base += i < w ? sums[i] : 0;
-      all += sums[i];
+      const int64_t t = t0 + i * 1024 + threadIdx.x;
+      if (t < p.tokens) flags |= static_cast<uint32_t>(counts(p, t)) << i;
+    }
+    unsigned long long mask[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      mask[i] = __ballot(flags >> i & 1);
+      if (lane == 0) before[i][w] = __popcll(mask[i]);
     }
     __syncthreads();
-    int64_t at = kept + base + before - n;
-    int64_t other = p.tokens - 1 - (lo - at);  // from the end
+    if (threadIdx.x < 16) {  // a run each
+      int32_t sum = 0;
+      for (int q = 0; q < 16; ++q) {
+        const int32_t n = before[threadIdx.x][q];
+        before[threadIdx.x][q] = sum;
+        sum += n;
+      }
+      runs[threadIdx.x] = sum;
+    }
+    __syncthreads();
+    int64_t at = kept;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (lo + i < p.tokens) p.rows[mask >> i & 1 ? at++ : other--] = static_cast<int32_t>(lo + i);
-    kept += all;
+    for (int i = 0; i < 16; ++i) {
+      const int64_t t = t0 + i * 1024 + threadIdx.x;
+      const int64_t mine = at + before[i][w] + __popcll(mask[i] & ((1ull << lane) - 1));  // that count before t
+      if (t < p.tokens) p.rows[flags >> i & 1 ? mine : p.tokens - 1 - (t - mine)] = static_cast<int32_t>(t);
+      at += runs[i];
+    }
+    kept = at;
+    __syncthreads();
   }
   if (threadIdx.x == 0) {
     p.rows[p.tokens] = static_cast<int32_t>(kept);
@@ -482,22 +512,23 @@ __global__ __launch_bounds__(512, 2) void loss_dhidden_kernel(const LossParams p
   using E = Kept<T>;
   const int64_t kept = p.scal->kept;
   const int64_t mts = (p.dpad + kLossTile - 1) / kLossTile, nts = (kept + kLossTile - 1) / kLossTile;
+  const int splits = p.scal->hsplit;
   int64_t mt, ns;
-  if (!tile_of(blockIdx.x, mts, nts * p.hsplit, mt, ns)) return;
-  const int64_t nt = ns / p.hsplit;
-  const int split = static_cast<int>(ns - nt * p.hsplit);
+  if (!tile_of(blockIdx.x, mts, nts * splits, mt, ns)) return;
+  const int64_t nt = ns / splits;
+  const int split = static_cast<int>(ns - nt * splits);
   constexpr int runs = kRuns<T>;
   const ProductParams q = {weight_operand(p, vp), grad_operand(p), p.vrows, runs};
   const int depths = static_cast<int>(p.vrows / kLossDepth) * runs;
   MCPU_TILE_LDS(a0, b0, a1, b1);
   Acc acc;
-  tile_product<E, true, false>(q, mt * kLossTile, nt * kLossTile, static_cast<int>(int64_t{depths} * split / p.hsplit),
-                               static_cast<int>(int64_t{depths} * (split + 1) / p.hsplit), a0, b0, a1, b1, acc);
+  tile_product<E, true, false>(q, mt * kLossTile, nt * kLossTile, static_cast<int>(int64_t{depths} * split / splits),
+                               static_cast<int>(int64_t{depths} * (split + 1) / splits), a0, b0, a1, b1, acc);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t t = nt * kLossTile + (wave & 3) * 64 + j * 32 + (lane & 31);
-    float* out = p.acc + (split * p.tpad + t) * p.dpad;
+    float* out = p.acc + (split * nts * kLossTile + t) * p.dpad;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -539,7 +570,8 @@ template <typename T> __global__ __launch_bounds__(256) void loss_dhidden_out_ke
   if (in) {
     float scale = unit_of(p, i) / kUp<E>;
     if constexpr (std::is_same_v<T, float>) scale *= pow2(-up_exponent(p.scal->wmax));
-    sum_splits(p.acc + i * p.dpad + d, p.tpad * p.dpad, p.hsplit, v);
+    const int64_t rows = (int64_t{p.scal->kept} + kLossTile - 1) / kLossTile * kLossTile;
+    sum_splits(p.acc + i * p.dpad + d, rows * p.dpad, p.scal->hsplit, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= scale;
   }
@@ -711,12 +743,19 @@ template <typename T> __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f
   }
 }
 
-// The products of NF x 16 rows of hidden, h, and a wave's 32 rows of weight from v0 on:
-// s[i][j][e] is of vocabulary row v0 + 16 i + 4 (lane / 16) + e and token 16 j + lane % 16.
-// Forward and backward form them alike, to the bit.
-template <typename T, int NF>
-__device__ __forceinline__ void few_products(const LossParams& p, const T* const (&h)[NF], int64_t v0, int lane,
-                                             f32x4 (&s)[2][NF]) {
+// The products of NF x 16 rows of hidden and a wave's 32 rows of weight from v0 on:
+// s[i][j][e] is of vocabulary row v0 + 16 i + 4 (lane / 16) + e and token 16 j + lane % 16;
+// row(t) is where token t's row of hidden begins. Forward and backward form them alike,
+// to the bit.
+// Up to 16 tokens hidden is read like weight, by every wave. More go through LDS, 256
+// bytes of a row at a time: read by every wave they are twice the weight's bytes for
+// 64 tokens, and a load of 64 lanes in as many lines is what the cache serves slowest (93
+// against 54 us, 33 x 50280 x 2560 bf16). Chunks of a row are where c ^ (row % 16) puts them.
+template <typename T, int NF, typename Row>
+__device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int64_t v0, f32x4 (&s)[2][NF]) {
+  constexpr bool kShared = NF > 1;
+  __shared__ u32x4 shared[kShared ? 2 : 1][kShared ? NF * 256 : 1];
+  const int lane = threadIdx.x & 63;
   const int64_t k0 = (lane >> 4) * kChunk<T>;
   const T* w[2];
 #pragma unroll
@@ -724,6 +763,14 @@ __device__ __forceinline__ void few_products(const LossParams& p, const T* const
     const int64_t v = v0 + 16 * i + (lane & 15);  // a row that is not there is read as the last
     w[i] = static_cast<const T*>(p.weight) + (v < p.vocab ? v : p.vocab - 1) * p.sw;
   }
+  const T* h[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) h[j] = row(16 * j + (lane & 15));
+  // What a thread brings to LDS of each 256 bytes: chunk threadIdx % 16 of rows threadIdx / 16 and, 32 apart, on.
+  constexpr int kBring = kShared ? NF / 2 : 1;
+  const T* from[kBring];
+#pragma unroll
+  for (int i = 0; i < kBring; ++i) from[i] = row((threadIdx.x >> 4) + 32 * i) + (threadIdx.x & 15) * kChunk<T>;
   // Two sums of every other load's products: half the roundings in a row.
   f32x4 acc[2][2][NF];
 #pragma unroll
@@ -734,31 +781,59 @@ __device__ __forceinline__ void few_products(const LossParams& p, const T* const
       for (int j = 0; j < NF; ++j) acc[u][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int kStep = 4 * kChunk<T>, kTurn = 4;  // terms of a load, loads of a turn
   const int64_t whole = p.dim / (kStep * kTurn) * (kStep * kTurn);
-  u32x4 a[2][kTurn][2], b[2][kTurn][NF];  // this turn's and the next's
+  u32x4 a[2][kTurn][2], b[2][kTurn][kShared ? 1 : NF], bring[kBring];  // this turn's and the next's
   auto load = [&](int to, int64_t k) {
+    if constexpr (kShared) {
+#pragma unroll
+      for (int i = 0; i < kBring; ++i) bring[i] = chunk_at<T>(from[i], k);
+    }
 #pragma unroll
     for (int u = 0; u < kTurn; ++u) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) a[to][u][i] = chunk_at<T>(w[i], k + k0 + u * kStep);
+      if constexpr (!kShared) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) b[to][u][j] = chunk_at<T>(h[j], k + k0 + u * kStep);
+        for (int j = 0; j < NF; ++j) b[to][u][j] = chunk_at<T>(h[j], k + k0 + u * kStep);
+      }
+    }
+  };
+  auto store = [&](int to) {
+    if constexpr (kShared) {
+#pragma unroll
+      for (int i = 0; i < kBring; ++i) {
+        const int r = (threadIdx.x >> 4) + 32 * i;
+        shared[to][r * 16 + ((threadIdx.x & 15) ^ (r & 15))] = bring[i];
+      }
+      __syncthreads();
     }
   };
   auto turn = [&](int of) {
 #pragma unroll
     for (int u = 0; u < kTurn; ++u)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < NF; ++j) {
+        u32x4 y;
+        if constexpr (kShared)
+          y = shared[of][(16 * j + (lane & 15)) * 16 + ((u * 4 + (lane >> 4)) ^ (lane & 15))];
+        else
+          y = b[of][u][j];
 #pragma unroll
-        for (int j = 0; j < NF; ++j) acc[u & 1][i][j] = mma16<T>(a[of][u][i], b[of][u][j], acc[u & 1][i][j]);
+        for (int i = 0; i < 2; ++i) acc[u & 1][i][j] = mma16<T>(a[of][u][i], y, acc[u & 1][i][j]);
+      }
   };
   int64_t k = 0;
-  if (whole > 0) load(0, 0);
+  if (whole > 0) {
+    load(0, 0);
+    store(0);
+  }
+  // A buffer is written while the other is read; who writes it next has passed the barrier between.
   for (; k + 2 * kStep * kTurn <= whole; k += 2 * kStep * kTurn) {
     load(1, k + kStep * kTurn);
     turn(0);
+    store(1);
     load(0, k + 2 * kStep * kTurn < whole ? k + 2 * kStep * kTurn : k);
     turn(1);
+    store(0);
   }
   if (k < whole) turn(0);
   for (k = whole; k < p.dim; k += kStep) {
@@ -780,19 +855,19 @@ __device__ __forceinline__ void few_products(const LossParams& p, const T* const
       for (int e = 0; e < 4; ++e) s[i][j][e] = acc[0][i][j][e] + acc[1][i][j][e];
 }
 
-// NF x 16 tokens; 256 vocabulary rows a workgroup, and of them one maximum and sum a token.
+// NF x 16 tokens; 256 vocabulary rows a workgroup, and of them one maximum and sum a token. Distillation: one more
+// workgroup a token, first, for the teacher's part, which would take 10 us before or after.
 template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_kernel(const LossParams p) {
+  const int64_t teachers = p.teacher != nullptr ? p.tokens : 0;
+  if (blockIdx.x < teachers) return teacher_row<T, 512>(p, blockIdx.x);
+  const int64_t group = blockIdx.x - teachers;
   __shared__ float2 parts[8][NF * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t v0 = blockIdx.x * int64_t{256} + wave * 32;
-  const T* h[NF];
-#pragma unroll
-  for (int j = 0; j < NF; ++j) {
-    const int64_t t = 16 * j + (lane & 15);  // a token that is not there is read as the last
-    h[j] = static_cast<const T*>(p.hidden) + (t < p.tokens ? t : p.tokens - 1) * p.sh;
-  }
+  const int64_t v0 = group * 256 + wave * 32;
   f32x4 acc[2][NF];
-  few_products<T, NF>(p, h, v0, lane, acc);
+  few_products<T, NF>(p, [&](int64_t t) {  // a token that is not there is read as the last
+    return static_cast<const T*>(p.hidden) + (t < p.tokens ? t : p.tokens - 1) * p.sh;
+  }, v0, acc);
   const float c = kLog2e / p.temperature;
 #pragma unroll
   for (int j = 0; j < NF; ++j) {
@@ -827,7 +902,7 @@ template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_ke
   for (int q = 1; q < 8; ++q) m = fmaxf(m, parts[q][t].x);
   const float sub = m == -INFINITY ? 0.f : m;
   for (int q = 0; q < 8; ++q) s = fmaf(parts[q][t].y, fast_exp2((parts[q][t].x - sub) * c), s);
-  p.part[int64_t{blockIdx.x} * kLossFew + t] = make_float2(m, s);
+  p.part[group * kLossFew + t] = make_float2(m, s);
 }
 
 // ds of up to 64 tokens that count, as loss_grad_kernel; rows behind them up to 64 are zero.
@@ -837,13 +912,9 @@ template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_gr
   const int64_t vl = blockIdx.x * int64_t{256} + wave * 32, v0 = vp + vl;
   const int kept = p.scal->kept;
   f32x4 acc[2][NF];
-  const T* h[NF];
-#pragma unroll
-  for (int j = 0; j < NF; ++j) {
-    const int i = 16 * j + (lane & 15);
-    h[j] = static_cast<const T*>(p.hidden) + p.rows[kept == 0 ? 0 : i < kept ? i : kept - 1] * p.sh;
-  }
-  few_products<T, NF>(p, h, v0, lane, acc);
+  few_products<T, NF>(p, [&](int i) {
+    return static_cast<const T*>(p.hidden) + p.rows[kept == 0 ? 0 : i < kept ? i : kept - 1] * p.sh;
+  }, v0, acc);
   const float c = kLog2e / p.temperature;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -1017,6 +1088,9 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   if (threadIdx.x != 0) return;
   for (int i = 1; i < 16; ++i) most = fmaxf(most, tops[i]);
   p.scal->kept = kept;
+  // By the rows that count, which the host does not know.
+  p.scal->hsplit = splits_for((p.dpad + kLossTile - 1) / kLossTile * ((kept + kLossTile - 1) / kLossTile),
+                              p.vpiece / kLossDepth * (p.dtype == MCPU_F32 ? 3 : 1), true);
   p.scal->hmax = p.scal->wmax = 0;
   p.scal->unit = most == 0.f ? 1.f : fmaxf(most, 0x1p-100f);
 }
@@ -1041,15 +1115,15 @@ template <typename T> void lay_operands(const LossParams& p, hipStream_t st) {
 }
 
 template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
-  if (p.teacher != nullptr)
-    run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
   if (p.tokens <= kLossFew) {
     for_few(p.tokens, [&](auto nf) {
-      run(loss_few_kernel<T, decltype(nf)::value>, p, (p.vocab + 255) / 256, 512, st);
+      run(loss_few_kernel<T, decltype(nf)::value>, p, (p.vocab + 255) / 256 + (p.teacher != nullptr ? p.tokens : 0), 512,
+          st);
     });
     run(loss_few_join_kernel, p, 1, 1024, st);
     return hipGetLastError();
   }
+  if (p.teacher != nullptr) run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
   run(loss_rows_kernel, p, 1, 1024, st);
   lay_operands<T>(p, st);
   const int64_t vt = (p.vocab + kLossTile - 1) / kLossTile, tt = p.tpad / kLossTile;
@@ -1074,7 +1148,7 @@ template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
     else
       run(loss_grad_kernel<T>, p, vt * tt, 512, st, vp);
     if (p.share != nullptr) run(loss_place_kernel<T>, p, (p.tokens + 3) / 4, 256, st, vp);
-    if (p.dhidden != nullptr) run(loss_dhidden_kernel<T>, p, dt * tt * p.hsplit, 512, st, vp, vp > 0);
+    if (p.dhidden != nullptr) run(loss_dhidden_kernel<T>, p, p.htiles, 512, st, vp, vp > 0);
     if (p.dweight != nullptr) {
       p.wsplit = loss_wsplit(p, vp);
       p.dwpart = p.wsplit > 1 ? dwpart : nullptr;
@@ -1087,21 +1161,6 @@ template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
 }
 
 }  // namespace
-
-// Microseconds of a product of `tiles` results of 256 KiB over `depths` each in
-// `splits`: 256 workgroups at a time, at 4.7 TFLOP/s each with 6 us around a tile,
-// and 4 TB/s for float32 results, written and read, where there are any.
-static double product_us(int64_t tiles, int64_t depths, int splits, bool apart) {
-  const double rounds = static_cast<double>((tiles * splits + 255) / 256);
-  return rounds * (static_cast<double>((depths + splits - 1) / splits) * 1.8 + 6) +
-         (apart || splits > 1 ? static_cast<double>(tiles * splits) * 0.131 : 0);
-}
-static int splits_for(int64_t tiles, int64_t depths, bool apart) {
-  int best = 1;
-  for (int s : {2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64})
-    if (depths / s >= 4 && product_us(tiles, depths, s, apart) < 0.97 * product_us(tiles, depths, best, apart)) best = s;
-  return best;
-}
 
 // The vocabulary piece: ds of one is at most 1 GiB, and of the sizes below that
 // give whole rounds of dweight's tiles, or equal pieces, the one that takes least.
@@ -1123,18 +1182,18 @@ void loss_plan(LossParams& p) {
   auto cost = [&](int64_t vt) {
     const int h = hsplit(vt);
     const int64_t left = all % vt;
-    return static_cast<double>(all / vt) * piece(vt, h) + (left > 0 ? piece(left, h) : 0);
+    return static_cast<float>(all / vt) * piece(vt, h) + (left > 0 ? piece(left, h) : 0.f);
   };
   int64_t best = up(all, up(all, most));  // equal pieces
-  double least = cost(best);
+  float least = cost(best);
   for (int64_t rounds = 1; rounds <= 8; ++rounds) {
     const int64_t vt = 256 * rounds / dt;
     if (vt < 1 || vt > most) continue;
-    const double us = cost(vt);
-    if (us < 0.99 * least) least = us, best = vt;
+    const float us = cost(vt);
+    if (us < 0.99f * least) least = us, best = vt;
   }
   p.vpiece = best * kLossTile;
-  p.hsplit = hsplit(best);
+  p.htiles = std::max(dt * tt, std::min<int64_t>(kLossSplitTiles, 64 * dt * tt));
   p.wsplit = std::max(loss_wsplit(p, 0), loss_wsplit(p, (all - 1) / best * p.vpiece));
 }
 

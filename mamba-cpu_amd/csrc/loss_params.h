@@ -15,6 +15,7 @@ namespace mcpu {
 struct LossScalars {
   int32_t kept;          // rows that count
   uint32_t hmax, wmax;   // float32 operands: the largest finite magnitudes, as bits
+  int32_t hsplit;        // backward: splits of dhidden's products
   float unit;            // backward: the largest unit of a row's ds
 };
 
@@ -52,11 +53,12 @@ struct LossParams {
   void* hscaled;      // hrows in the largest unit, or null: hrows has it (distillation)
   void* wrows;        // (pieces, vocab, padded dim), or null: weight is read in place
   void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits
-  float* acc;         // (splits, padded tokens, padded dim): gradient of hidden
+  float* acc;         // (splits, rows that count, padded, padded dim): gradient of hidden
   float* dwpart;      // (splits, vocab piece, padded dim), or null: gradient of weight in one go
   int64_t tpad, dpad, vpiece;
   int64_t vrows;      // of this piece, a multiple of 256, at most vpiece
-  int hsplit, wsplit;
+  int64_t htiles;     // most tiles of 256 x 256 of dhidden's products, splits counted
+  int wsplit;
   int64_t first;      // this launch's first workgroup
 };
 
@@ -64,6 +66,7 @@ constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a 
 constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
 constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
 constexpr int kLossFew = 64;      // most tokens of a forward that streams the weight past them
+constexpr int64_t kLossSplitTiles = 768;  // most results of a split product, of 256 KiB each
 constexpr int64_t kLossMaxK = 1024;
 
 // float32 operands are two f16 pieces.
