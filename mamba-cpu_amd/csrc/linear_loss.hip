@@ -484,18 +484,28 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
   const int k = static_cast<int>(p.k);
   const float up = kUp<E> / unit_of(p, i), c = kLog2e / p.temperature;
   const float a = p.coef[i] * up, b = p.coef[p.tpad + i] * up, m2 = p.coef[2 * p.tpad + i];
-  for (int e = lane; e < k; e += 64) {
-    const int64_t id = id_at(p, t * k + e);
+  for (int e0 = 0; e0 < k; e0 += 64) {
+    const int e = e0 + lane;
+    const int64_t id = e < k ? id_at(p, t * k + e) : -1;
     const int64_t v = id - vp;
-    if (id < 0 || id >= p.vocab || v < 0 || v >= p.vpiece) continue;
+    const bool here = id >= 0 && id < p.vocab && v >= 0 && v < p.vpiece;
+    if (!__any(here)) continue;
+    // All entries of that id, 64 at a time from the lanes that hold them.
     float q = 0.f;
     bool first = true;
-    for (int o = 0; o < k; ++o) {
-      const bool same = id_at(p, t * k + o) == id;
-      q += same ? p.share[t * k + o] : 0.f;
-      first = first && !(same && o < e);
+    for (int o0 = 0; o0 < k; o0 += 64) {
+      const int mine = o0 + lane;
+      const int32_t other = mine < k ? static_cast<int32_t>(id_at(p, t * k + mine)) : -1;
+      const float share = mine < k ? p.share[t * k + mine] : 0.f;
+      const int n = k - o0 < 64 ? k - o0 : 64;
+      for (int o = 0; o < n; ++o) {
+        const bool same = __builtin_amdgcn_readlane(other, o) == static_cast<int32_t>(id);
+        const float more = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, share), o));
+        q += same ? more : 0.f;
+        first = first && !(same && o0 + o < e);
+      }
     }
-    if (!first || q == 0.f) continue;  // an id's first entry places it; entries left out may have no product
+    if (!here || !first || q == 0.f) continue;  // an id's first entry places it; entries left out may have no product
     E* out = static_cast<E*>(p.grad) + i * p.vpiece + v;
     if constexpr (std::is_same_v<T, float>) {
       E* low = out + p.tpad * p.vpiece;

@@ -3,7 +3,7 @@ training, prompts (whole or in pieces), packed sequences, and sampled decoding
 with each token's step replayed from a HIP graph.
 
     model = RecurrentLM(vocab_size=50280, d_model=768, n_layer=24).cuda()
-    loss = torch.nn.functional.cross_entropy(model(ids[:, :-1]).flatten(0, 1), ids[:, 1:].flatten())
+    loss = model.loss(ids[:, :-1], ids[:, 1:])
     tokens = generate(model, prompt, max_new_tokens=128, temperature=0.8, top_p=0.95)
 
 A block is RMS norm -> in_proj (to u and a gate z) -> causal conv1d with silu
@@ -15,8 +15,9 @@ layers and with one dense matrix for the gates. The reference has no such model.
 
 Per call the token embedding is embedding_fn, the norms (with the residual
 sum) layer_norm_fn, the recurrence gated_linear_scan_fn or, for one token,
-gated_linear_update, and the choice of a token sample_fn; the products are the
-library's.
+gated_linear_update, and the choice of a token sample_fn; the losses are
+linear_cross_entropy_fn and linear_distillation_fn over the embedding's weight, so
+that training keeps no logits; the blocks' products are the library's.
 """
 
 import math
@@ -31,6 +32,8 @@ from mamba_cpu.ops import (
     gated_linear_scan_fn,
     gated_linear_update,
     layer_norm_fn,
+    linear_cross_entropy_fn,
+    linear_distillation_fn,
     sample_fn,
 )
 from mamba_cpu.ops.sampling import setting_rows
@@ -98,7 +101,22 @@ class RecurrentLM(nn.Module):
         return layer_norm_fn(hidden, self.norm_weight, residual=residual, eps=self.eps, is_rms_norm=True)
 
     def forward(self, ids, seq_idx=None):
-        return self._run(ids, lambda i, block, x: block(x, seq_idx=seq_idx)) @ self.embedding.t()
+        return self._hidden(ids, seq_idx) @ self.embedding.t()
+
+    def _hidden(self, ids, seq_idx=None):
+        return self._run(ids, lambda i, block, x: block(x, seq_idx=seq_idx))
+
+    def loss(self, ids, targets, seq_idx=None, ignore_index=-100, reduction="mean"):
+        """Cross entropy of targets (batch, seqlen) against forward(ids)'s logits, which are not formed as a whole
+        (linear_cross_entropy_fn). With "none" and no gradient: minus the targets' log-probabilities."""
+        return linear_cross_entropy_fn(self._hidden(ids, seq_idx), self.embedding, targets, ignore_index=ignore_index,
+                                       reduction=reduction)
+
+    def distillation_loss(self, ids, teacher_ids, teacher_logits, temperature=1.0, seq_idx=None, reduction="mean"):
+        """Divergence of forward(ids)'s logits from a teacher's top ones, (batch, seqlen, k) each
+        (linear_distillation_fn)."""
+        return linear_distillation_fn(self._hidden(ids, seq_idx), self.embedding, teacher_ids, teacher_logits,
+                                      temperature=temperature, reduction=reduction)
 
     def new_cache(self, batch):
         """Per block the conv window and the state, as before the first token."""

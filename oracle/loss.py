@@ -40,6 +40,11 @@ def rows(hidden, weight, ids, teacher=None, temperature=1.0, ignore_index=-100):
         s = w @ h[i] / temperature
         m = s.max()
         lse[i] = m + np.log(np.exp(s - m).sum())
+        if teacher is None:  # log(1 + sum over the others of exp(s - s_target)), whose digits lse - s_target loses
+            with np.errstate(over="ignore"):
+                others = np.delete(np.exp(s - s[at[i, 0]]), at[i, 0]).sum()
+            loss[i] = np.log1p(others) if others < 1e300 else lse[i] - s[at[i, 0]]
+            continue
         for k, share in enumerate(q[i]):
             if share != 0:
                 loss[i] += share * (np.log(share) + lse[i] - s[at[i, k]])
@@ -57,7 +62,12 @@ def logits_grad(hidden, weight, ids, dloss, dlse=None, teacher=None, temperature
     for i in np.flatnonzero(keep):
         p = np.exp(w @ h[i] / temperature - lse[i])
         g = temperature * float(dloss[i])
-        ds[i] = (g + (0.0 if dlse is None else float(dlse[i]))) * p
+        e = 0.0 if dlse is None else float(dlse[i])
+        ds[i] = (g + e) * p
+        if teacher is None:  # p - 1 is minus the others' sum
+            y = at[i, 0]
+            ds[i, y] = e * p[y] - g * np.delete(p, y).sum()
+            continue
         for k, share in enumerate(q[i]):
             if share != 0:
                 ds[i, at[i, k]] -= g * share

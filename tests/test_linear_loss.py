@@ -14,7 +14,8 @@ Tolerances, with u = eps / 2 of float32 (2^-24) and S = max_tv sum_d |h_td w_vd|
 - ds: its rounding to the kept type (bf16 2^-8, f16 2^-11, float32 2^-21), and
   the relative error of p, which is that of its exponent, twice lse's;
 - gradients: |ds| |operand| summed, times ds' error and n u for a sum of n
-  float32 terms, and the result's own rounding; f16 adds its smallest step.
+  float32 terms, and the result's own rounding; dweight takes hidden's rows times
+  their unit, rounded to the kept type once more; f16 adds its smallest step.
 """
 
 import numpy as np
@@ -79,6 +80,7 @@ def check_grads(dtype, h, w, ds, ltol, dh, dw):
     mag = mag + 2 * float(np.max(ltol, initial=0)) / e * top * (mag > 0)
     floor = 2.0 ** -24 if dtype == "f16" else 0.0
     low = 2.0 ** -36 * np.abs(ds).max(initial=0) if dtype != "bf16" else 0.0
+    low += 2.0 ** -100  # ds below that is kept beside the largest, which leaves float32's and f16's range
     want_h, want_w = O.grads(finite(h), w, ds)
     if dh is not None:
         check("dhidden", dh, want_h,
@@ -86,7 +88,7 @@ def check_grads(dtype, h, w, ds, ltol, dh, dw):
     if dw is not None:
         live = (ds != 0).any(1)[:, None]
         check("dweight", dw, want_w,
-              (e + ds.shape[0] * U) * (mag.T @ (hd * live)) + low * (hd * live).sum(0) + OUT[dtype] * np.abs(want_w)
+              (e + KEPT[dtype] + ds.shape[0] * U) * (mag.T @ (hd * live)) + low * (hd * live).sum(0) + OUT[dtype] * np.abs(want_w)
               + floor)
 
 
