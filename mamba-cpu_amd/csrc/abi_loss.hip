@@ -21,7 +21,7 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
   if (a->dim == 0) return fail(MCPU_ERR_INVALID, "%s: dim must be positive", what);
   if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
     return fail(MCPU_ERR_INVALID, "%s: temperature must be above 0", what);
-  if (!distil(a) && (a->k != 1 || a->temperature != 1.f))
+  if (!distil(a) && a->k > 0 && (a->k != 1 || a->temperature != 1.f))
     return fail(MCPU_ERR_INVALID, "%s: cross entropy has one target a row and temperature 1", what);
   if (distil(a) && a->dlse != nullptr) return fail(MCPU_ERR_INVALID, "%s: distillation has no dlse", what);
   if (a->tokens > (1 << 26) || a->vocab > (1 << 24) || a->dim > (1 << 20) || a->k > kLossMaxK)
@@ -33,6 +33,9 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
     return fail(MCPU_ERR_INVALID, "%s: hidden, weight, ids, stat, rows and (distillation) picked are required", what);
   return MCPU_OK;
 }
+
+// Nothing to take a loss of: no rows, no vocabulary or no entries.
+bool nothing(const mcpu_linear_loss_args* a) { return a->tokens == 0 || a->vocab == 0 || a->k == 0; }
 
 bool sixteen(const void* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
@@ -136,7 +139,7 @@ extern "C" size_t mcpu_linear_loss_fwd_workspace_size(const mcpu_linear_loss_arg
     clear_error();
     return 0;
   }
-  if (a->tokens == 0 || a->vocab == 0) return 0;
+  if (nothing(a)) return 0;
   LossParams p = make_loss(a);
   return lay_fwd(a, p, nullptr);
 }
@@ -146,15 +149,22 @@ extern "C" int mcpu_linear_loss_fwd(const mcpu_linear_loss_args* a, void* worksp
   const char* what = "linear_loss_fwd";
   clear_error();
   if (int rc = check_loss(a, what)) return rc;
-  if (a->tokens == 0 || a->vocab == 0)
-    return fail(MCPU_ERR_INVALID, "%s: no tokens or no vocabulary", what);
-  if (a->loss == nullptr || a->lse == nullptr || (a->teacher == nullptr) != (a->share == nullptr))
+  const int64_t losses = a->reduction == MCPU_REDUCE_NONE ? a->tokens : 1;
+  if ((a->loss == nullptr && losses > 0) || (a->tokens > 0 && a->lse == nullptr) ||
+      (!nothing(a) && (a->teacher == nullptr) != (a->share == nullptr)))
     return fail(MCPU_ERR_INVALID, "%s: loss, lse, and share with a teacher, are required", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_linear_loss_fwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (nothing(a)) {  // no row counts
+    hipError_t e = loss_zero(a->loss, 4 * losses, st);
+    if (e == hipSuccess) e = loss_zero(a->lse, 4 * a->tokens, st);
+    if (e == hipSuccess) e = loss_zero(a->rows, a->rows != nullptr ? 4 * (a->tokens + 1) : 0, st);
+    return hip_status(e, "linear_loss_fwd launch");
+  }
   LossParams p = make_loss(a);
   lay_fwd(a, p, workspace);
-  return hip_status(loss_fwd_launch(p, static_cast<hipStream_t>(stream)), "linear_loss_fwd launch");
+  return hip_status(loss_fwd_launch(p, st), "linear_loss_fwd launch");
 }
 
 extern "C" size_t mcpu_linear_loss_bwd_workspace_size(const mcpu_linear_loss_args* a) {
@@ -162,7 +172,7 @@ extern "C" size_t mcpu_linear_loss_bwd_workspace_size(const mcpu_linear_loss_arg
     clear_error();
     return 0;
   }
-  if (a->tokens == 0 || a->vocab == 0) return 0;
+  if (nothing(a)) return 0;
   LossParams p = make_loss(a);
   return lay_bwd(a, p, nullptr);
 }
@@ -172,14 +182,19 @@ extern "C" int mcpu_linear_loss_bwd(const mcpu_linear_loss_args* a, void* worksp
   const char* what = "linear_loss_bwd";
   clear_error();
   if (int rc = check_loss(a, what)) return rc;
-  if (a->tokens == 0 || a->vocab == 0)
-    return fail(MCPU_ERR_INVALID, "%s: no tokens or no vocabulary", what);
   if (a->dloss == nullptr && a->reduction != MCPU_REDUCE_NONE)
     return fail(MCPU_ERR_INVALID, "%s: dloss is required where the loss is reduced", what);
   if (int rc = check_workspace(what, workspace, workspace_bytes, mcpu_linear_loss_bwd_workspace_size(a))) return rc;
   if (int rc = mcpu_check_device()) return rc;
   if (a->dhidden == nullptr && a->dweight == nullptr) return MCPU_OK;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (nothing(a)) {
+    const int64_t row = a->dim * dtype_size(a->dtype);
+    hipError_t e = loss_zero(a->dhidden, a->dhidden != nullptr ? a->tokens * row : 0, st);
+    if (e == hipSuccess) e = loss_zero(a->dweight, a->dweight != nullptr ? a->vocab * row : 0, st);
+    return hip_status(e, "linear_loss_bwd launch");
+  }
   LossParams p = make_loss(a);
   lay_bwd(a, p, workspace);
-  return hip_status(loss_bwd_launch(p, static_cast<hipStream_t>(stream)), "linear_loss_bwd launch");
+  return hip_status(loss_bwd_launch(p, st), "linear_loss_bwd launch");
 }

@@ -36,18 +36,21 @@ __device__ __forceinline__ int64_t id_at(const LossParams& p, int64_t i) {
 // Microseconds of a product of `tiles` results of 256 KiB over `depths` each in
 // `splits`: 256 workgroups at a time, at 4.7 TFLOP/s each with 6 us around a tile,
 // and 4 TB/s for float32 results, written and read, where there are any.
-__host__ __device__ inline float product_us(int64_t tiles, int64_t depths, int splits, bool apart) {
+template <typename I> __host__ __device__ inline float product_us(I tiles, I depths, I splits, bool apart) {
   const float rounds = static_cast<float>((tiles * splits + 255) / 256);
   return rounds * (static_cast<float>((depths + splits - 1) / splits) * 1.8f + 6.f) +
          (apart || splits > 1 ? static_cast<float>(tiles * splits) * 0.131f : 0.f);
 }
 __host__ __device__ inline int splits_for(int64_t tiles, int64_t depths, bool apart) {
   constexpr int kTry[] = {2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
+  if (tiles < 1 || tiles > kLossSplitTiles / 2) return 1;
+  // In 32 bits, which the sizes left fit: the GPU divides 64 by a routine.
+  const int t = static_cast<int>(tiles), d = static_cast<int>(depths);
   int best = 1;
-  float least = product_us(tiles, depths, 1, apart);
+  float least = product_us(t, d, 1, apart);
   for (int s : kTry) {
-    const float us = product_us(tiles, depths, s, apart);
-    if (depths / s >= 4 && tiles * s <= kLossSplitTiles && us < 0.97f * least) best = s, least = us;
+    const float us = product_us(t, d, s, apart);
+    if (d / s >= 4 && t * s <= kLossSplitTiles && us < 0.97f * least) best = s, least = us;
   }
   return best;
 }
@@ -1105,6 +1108,11 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   p.scal->unit = most == 0.f ? 1.f : fmaxf(most, 0x1p-100f);
 }
 
+// Results of calls without rows, vocabulary or entries.
+__global__ __launch_bounds__(256) void loss_zero_kernel(uint8_t* at, int64_t bytes) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < bytes; i += 256ll * gridDim.x) at[i] = 0;
+}
+
 // ---- launches -----------------------------------------------------------------------------------
 
 template <typename K, typename... A>
@@ -1186,8 +1194,9 @@ void loss_plan(LossParams& p) {
   auto hsplit = [&](int64_t vt) { return splits_for(dt * tt, vt * per * runs, true); };
   auto piece = [&](int64_t n, int h) {
     const int w = splits_for(dt * n, tt * per * runs, false);
-    return product_us(n * tt, p.dpad / kLossDepth * runs, 1, false) + product_us(dt * tt, n * per * runs, h, true) +
-           product_us(dt * n, tt * per * runs, w, false) + 10;
+    return product_us<int64_t>(n * tt, p.dpad / kLossDepth * runs, 1, false) +
+           product_us<int64_t>(dt * tt, n * per * runs, h, true) +
+           product_us<int64_t>(dt * n, tt * per * runs, w, false) + 10;
   };
   auto cost = [&](int64_t vt) {
     const int h = hsplit(vt);
@@ -1215,6 +1224,13 @@ int loss_wsplit(const LossParams& p, int64_t vp) {
   const int64_t dt = (p.dpad + kLossTile - 1) / kLossTile;
   return splits_for(dt * (loss_piece_rows(p, vp) / kLossTile), p.tpad / kLossDepth * (loss_pieces(p.dtype) == 2 ? 3 : 1),
                     false);
+}
+
+hipError_t loss_zero(void* at, int64_t bytes, hipStream_t st) {
+  if (bytes <= 0) return hipSuccess;
+  hipLaunchKernelGGL(loss_zero_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((bytes + 255) / 256, 4096))),
+                     dim3(256), 0, st, static_cast<uint8_t*>(at), bytes);
+  return hipGetLastError();
 }
 
 hipError_t loss_fwd_launch(LossParams p, hipStream_t st) {

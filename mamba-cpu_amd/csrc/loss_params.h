@@ -66,7 +66,7 @@ constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a 
 constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
 constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
 constexpr int kLossFew = 64;      // most tokens of a forward that streams the weight past them
-constexpr int64_t kLossSplitTiles = 768;  // most results of a split product, of 256 KiB each
+constexpr int64_t kLossSplitTiles = 1536;  // most results of a split product, of 256 KiB each
 constexpr int64_t kLossMaxK = 1024;
 
 // float32 operands are two f16 pieces.
@@ -76,6 +76,7 @@ inline int loss_pieces(int dtype) { return dtype == MCPU_F32 ? 2 : 1; }
 void loss_plan(LossParams& p);
 int64_t loss_piece_rows(const LossParams& p, int64_t vp);
 int loss_wsplit(const LossParams& p, int64_t vp);
+hipError_t loss_zero(void* at, int64_t bytes, hipStream_t st);
 hipError_t loss_fwd_launch(LossParams p, hipStream_t st);
 hipError_t loss_bwd_launch(LossParams p, hipStream_t st);
 

