@@ -355,7 +355,7 @@ __device__ __forceinline__ int rows_left(const LossParams& p, int64_t v0, int la
 template <typename T> __global__ __launch_bounds__(512, 2) void loss_logits_kernel(const LossParams p) {
   const int64_t kept = p.scal->kept;
   int64_t mt, nt;
-  if (!tile_of(blockIdx.x, (p.vocab + kLossTile - 1) / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
+  if (!tile_of(p.first + blockIdx.x, (p.vocab + kLossTile - 1) / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = mt * kLossTile + (wave >> 2) * kLossPart, t0 = nt * kLossTile + (wave & 3) * 64 + (lane & 31);
   // What the epilogue needs is on its way before the product.
@@ -409,7 +409,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
   using E = Kept<T>;
   const int64_t kept = p.scal->kept;
   int64_t mt, nt;
-  if (!tile_of(blockIdx.x, p.vrows / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
+  if (!tile_of(p.first + blockIdx.x, p.vrows / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = mt * kLossTile + (wave >> 2) * 128, t0 = nt * kLossTile + (wave & 3) * 64 + (lane & 31);
   const float c = logit_scale<T>(p);
@@ -473,6 +473,12 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
   }
 }
 
+// An entry's id, or -1 where it lies outside the vocabulary or there is none.
+__device__ __forceinline__ int32_t in_vocab(const LossParams& p, int64_t i, bool any) {
+  const int64_t id = any ? id_at(p, i) : -1;
+  return id >= 0 && id < p.vocab ? static_cast<int32_t>(id) : -1;
+}
+
 // Distillation: the ids' places of ds, a_t exp(c s - L) less all shares of that id. A
 // wave a row. In 16 bits that is formed anew, to be rounded once. float32 takes p
 // from the two pieces that are there: where p and its share are both near 1, their
@@ -489,20 +495,20 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
   const float a = p.coef[i] * up, b = p.coef[p.tpad + i] * up, m2 = p.coef[2 * p.tpad + i];
   for (int e0 = 0; e0 < k; e0 += 64) {
     const int e = e0 + lane;
-    const int64_t id = e < k ? id_at(p, t * k + e) : -1;
+    const int32_t id = in_vocab(p, t * k + e, e < k);
     const int64_t v = id - vp;
-    const bool here = id >= 0 && id < p.vocab && v >= 0 && v < p.vpiece;
+    const bool here = id >= 0 && v >= 0 && v < p.vrows;
     if (!__any(here)) continue;
     // All entries of that id, 64 at a time from the lanes that hold them.
     float q = 0.f;
     bool first = true;
     for (int o0 = 0; o0 < k; o0 += 64) {
       const int mine = o0 + lane;
-      const int32_t other = mine < k ? static_cast<int32_t>(id_at(p, t * k + mine)) : -1;
+      const int32_t other = in_vocab(p, t * k + mine, mine < k);
       const float share = mine < k ? p.share[t * k + mine] : 0.f;
       const int n = k - o0 < 64 ? k - o0 : 64;
       for (int o = 0; o < n; ++o) {
-        const bool same = __builtin_amdgcn_readlane(other, o) == static_cast<int32_t>(id);
+        const bool same = __builtin_amdgcn_readlane(other, o) == id;
         const float more = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, share), o));
         q += same ? more : 0.f;
         first = first && !(same && o0 + o < e);
@@ -527,7 +533,7 @@ __global__ __launch_bounds__(512, 2) void loss_dhidden_kernel(const LossParams p
   const int64_t mts = (p.dpad + kLossTile - 1) / kLossTile, nts = (kept + kLossTile - 1) / kLossTile;
   const int splits = p.scal->hsplit;
   int64_t mt, ns;
-  if (!tile_of(blockIdx.x, mts, nts * splits, mt, ns)) return;
+  if (!tile_of(p.first + blockIdx.x, mts, nts * splits, mt, ns)) return;
   const int64_t nt = ns / splits;
   const int split = static_cast<int>(ns - nt * splits);
   constexpr int runs = kRuns<T>;
@@ -597,7 +603,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(const LossParams p
   using E = Kept<T>;
   const int64_t mts = (p.dpad + kLossTile - 1) / kLossTile;
   int64_t mt, ns;
-  if (!tile_of(blockIdx.x, mts, p.vrows / kLossTile * p.wsplit, mt, ns)) return;
+  if (!tile_of(p.first + blockIdx.x, mts, p.vrows / kLossTile * p.wsplit, mt, ns)) return;
   const int64_t nt = ns / p.wsplit;
   const int split = static_cast<int>(ns - nt * p.wsplit);
   constexpr int runs = kRuns<T>;
@@ -872,8 +878,8 @@ __device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int
 // workgroup a token, first, for the teacher's part, which would take 10 us before or after.
 template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_kernel(const LossParams p) {
   const int64_t teachers = p.teacher != nullptr ? p.tokens : 0;
-  if (blockIdx.x < teachers) return teacher_row<T, 512>(p, blockIdx.x);
-  const int64_t group = blockIdx.x - teachers;
+  const int64_t at = p.first + blockIdx.x, group = at - teachers;
+  if (group < 0) return teacher_row<T, 512>(p, at);
   __shared__ float2 parts[8][NF * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = group * 256 + wave * 32;
@@ -922,7 +928,7 @@ template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_ke
 template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
   using E = Kept<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t vl = blockIdx.x * int64_t{256} + wave * 32, v0 = vp + vl;
+  const int64_t vl = (p.first + blockIdx.x) * 256 + wave * 32, v0 = vp + vl;
   const int kept = p.scal->kept;
   f32x4 acc[2][NF];
   few_products<T, NF>(p, [&](int i) {
@@ -1058,13 +1064,13 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossParams p) {
 // dweight takes the units from hidden's rows, scaled by unit / the largest unit.
 // Distillation: one unit, the largest coefficient. One workgroup.
 __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
-  __shared__ float tops[16];
+  __shared__ float tops[16], largest[16];
   const int32_t kept = p.rows[p.tokens];
   const float share = p.reduction == MCPU_REDUCE_MEAN ? 1.f / static_cast<float>(kept > 0 ? kept : 1) : 1.f;
   const float c = kLog2e / p.temperature;
   const bool each = p.reduction == MCPU_REDUCE_NONE;
   const float all = each ? 0.f : p.dloss[0] * share;
-  float most = 0.f;
+  float most = 0.f, factor = 0.f;  // the largest unit, and the largest softmax coefficient
   for (int64_t i0 = threadIdx.x; i0 < kept; i0 += 1024 * 8) {
     float g[8], e[8], stat[4][8];
 #pragma unroll
@@ -1088,18 +1094,25 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
       const float own = p.share != nullptr ? g[u] : e[u] * stat[2][u] - g[u] * stat[3][u];
       const float top = fmaxf(__builtin_fabsf(own), __builtin_fabsf(a) * (p.share != nullptr ? 1.f : stat[3][u]));
       if (top < INFINITY) most = fmaxf(most, top);
+      if (__builtin_fabsf(a) < INFINITY) factor = fmaxf(factor, __builtin_fabsf(a));
       p.coef[i] = a / stat[1][u] * fmaf(-kLn2, off, 1.f);
       p.coef[p.tpad + i] = own;
       p.coef[2 * p.tpad + i] = m2;
-      p.coef[3 * p.tpad + i] = p.share == nullptr && top > 0x1p-100f && top < INFINITY ? top : 0.f;
+      // Not where a / unit would leave float32's range: the others' share is below 2^-90, a loss of 0 but for that.
+      const bool fits = top > 0x1p-100f && top > __builtin_fabsf(a) * 0x1p-90f && top < INFINITY;
+      p.coef[3 * p.tpad + i] = p.share == nullptr && fits ? top : 0.f;
     }
   }
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) most = fmaxf(most, __shfl_xor(most, s));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = most;
+  for (int s = 1; s < 64; s <<= 1) {
+    most = fmaxf(most, __shfl_xor(most, s));
+    factor = fmaxf(factor, __shfl_xor(factor, s));
+  }
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = most, largest[threadIdx.x >> 6] = factor;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int i = 1; i < 16; ++i) most = fmaxf(most, tops[i]);
+  for (int i = 1; i < 16; ++i) most = fmaxf(most, tops[i]), factor = fmaxf(factor, largest[i]);
+  most = fmaxf(most, factor * 0x1p-90f);
   p.scal->kept = kept;
   // By the rows that count, which the host does not know.
   p.scal->hsplit = splits_for((p.dpad + kLossTile - 1) / kLossTile * ((kept + kLossTile - 1) / kLossTile),
@@ -1123,13 +1136,13 @@ void run(K kernel, LossParams p, int64_t groups, int threads, hipStream_t st, A.
   });
 }
 
-template <typename T> void lay_operands(const LossParams& p, hipStream_t st) {
+template <typename T> void lay_operands(const LossParams& p, bool weight, hipStream_t st) {
   if constexpr (std::is_same_v<T, float>) {
     run(loss_most_kernel, p, std::min<int64_t>((p.tokens + 3) / 4, 512), 256, st, false);
-    run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 3) / 4, 1024), 256, st, true);
+    if (weight) run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 3) / 4, 1024), 256, st, true);
   }
   run(loss_gather_kernel<T>, p, p.tpad / 4, 256, st);
-  if (p.wrows != nullptr) run(loss_weight_kernel<T>, p, (p.vocab + 3) / 4, 256, st);
+  if (weight && p.wrows != nullptr) run(loss_weight_kernel<T>, p, (p.vocab + 3) / 4, 256, st);
 }
 
 template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
@@ -1143,7 +1156,7 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   }
   if (p.teacher != nullptr) run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
   run(loss_rows_kernel, p, 1, 1024, st);
-  lay_operands<T>(p, st);
+  lay_operands<T>(p, true, st);
   const int64_t vt = (p.vocab + kLossTile - 1) / kLossTile, tt = p.tpad / kLossTile;
   run(loss_logits_kernel<T>, p, vt * tt, 512, st);
   run(loss_join_kernel, p, (p.tokens + 31) / 32, 256, st);
@@ -1153,7 +1166,8 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
 
 template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
   run(loss_coef_kernel, p, 1, 1024, st);
-  lay_operands<T>(p, st);
+  // Of few tokens ds is formed from weight as it lies.
+  lay_operands<T>(p, p.tokens > kLossFew || p.dhidden != nullptr, st);
   const int64_t tt = p.tpad / kLossTile, dt = (p.dpad + kLossTile - 1) / kLossTile;
   float* const dwpart = p.dwpart;
   for (int64_t vp = 0; vp < p.vocab; vp += p.vpiece) {

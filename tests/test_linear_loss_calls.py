@@ -376,6 +376,71 @@ def test_infinite_gradients_come_through(t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t", [40, 100])
+@pytest.mark.parametrize("some", [True, False])
+def test_targets_far_above_under_a_loss_scale(dtype, t, some):
+    """Targets 60 to 100 above all others, under a loss scale of 2^16: ds down to the end of float32's range, with and
+    without a row of ordinary size beside."""
+    w = torch.eye(260, 64, dtype=torch.float64)
+    ids = torch.arange(t) % 64
+    h = torch.zeros(t, 64, dtype=torch.float64)
+    h[torch.arange(t), ids] = torch.linspace(60, 100, t, dtype=torch.float64)
+    if some:
+        h[5] = 0
+    h, w = h.to({"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]), w.to(
+        {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype])
+    loss, lse, dh, dw = run_ce(dtype, h, w, ids, "none", 2.0 ** 16)
+    want, want_lse, _ = O.rows(h, w, ids)
+    check("loss", loss, want, 2.0 ** -16 * (1 + want))
+    ds = O.logits_grad(h, w, ids, np.full(t, 2.0 ** 16))
+    want_h, want_w = O.grads(h, w, ds)
+    # One rounding of ds and one of the result, and f16's smallest steps: of ds beside the largest, of the result.
+    u, low = 3 * OUT[dtype] + 2.0 ** -14, 2.0 ** -36 * 2.0 ** 16 + 2.0 ** -24 if some or dtype == "f16" else 2.0 ** -70
+    check("dhidden", dh, want_h, u * np.abs(ds) @ np.abs(w.double().numpy()) + low)
+    check("dweight", dw, want_w, u * np.abs(ds).T @ np.abs(h.double().numpy()) + 100 * low)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [20, 70])
+def test_ids_past_32_bits_are_no_other_ids(t):
+    """An id of 2^32 + v is outside the vocabulary, and is not v, whichever comes first."""
+    h, w, _, g = inputs("bf16", t, 300, 64)
+    ids, tl = teacher(t, 300, 6, g)
+    wild = torch.cat([ids[:, :2] + 2 ** 32, ids, ids[:, 3:4] - 2 ** 32, torch.full_like(ids[:, :1], 2 ** 62)], 1)
+    wide = torch.cat([torch.zeros(t, 2), tl, torch.full((t, 2), 9.0)], 1)
+    outs = []
+    for i, l in ((ids, tl), (wild, wide)):
+        hg, wg = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        loss = mamba_cpu.linear_distillation_fn(hg, wg, i.to(DEV), l.to(DEV), reduction="none")
+        outs.append((loss, *torch.autograd.grad(loss.sum(), [hg, wg])))
+    for a, b in zip(*outs):
+        assert torch.allclose(a, b, rtol=2.0 ** -7, atol=1e-6)
+    ce = [mamba_cpu.linear_cross_entropy_fn(h.to(DEV), w.to(DEV), i.to(DEV), reduction="none")
+          for i in (ids[:, 0], ids[:, 0] + 2 ** 32)]
+    assert (ce[0] > 0).all() and torch.count_nonzero(ce[1]) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("t", [20, 70, 300])
+def test_what_lies_around_the_operands(dtype, t):
+    """Operands in the middle of memory that holds NaN, where weight is read in place: nothing of it is read into a
+    result."""
+    key = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}[dtype]
+    h, w, ids, _ = inputs(key, t, 300, 64)
+    want = run_ce(key, h, w, ids, "none", 1.0)
+    hs = torch.full((t + 40, 192), float("nan"), dtype=dtype, device=DEV)
+    ws = torch.full((1000, 192), float("nan"), dtype=dtype, device=DEV)
+    hs[8:t + 8, 64:128], ws[200:500, 64:128] = h.to(DEV), w.to(DEV)
+    hv, wv = hs[8:t + 8, 64:128].detach().requires_grad_(), ws[200:500, 64:128].detach().requires_grad_()
+    loss, lse = mamba_cpu.linear_cross_entropy_fn(hv, wv, ids.to(DEV), reduction="none", return_lse=True)
+    dh, dw = torch.autograd.grad(loss.sum(), [hv, wv])
+    for a, b in zip((loss, lse, dh, dw), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_loss_scaled_float16():
     """Gradients of 2^-14 a token under a scale of 2^14 and without: the same but for float16's smallest step."""
     h, w, ids, _ = inputs("f16", 200, 300, 64)
