@@ -794,12 +794,17 @@ typedef struct mcpu_linear_loss_args {
   float* stat;              /* (4, tokens), left for the backward */
   float* share;             /* (tokens, k): q; required iff distillation */
   int32_t* rows;            /* (tokens + 1): rows that count, the others, how many count */
+  void* laid;               /* mcpu_linear_loss_laid_size bytes, 256-byte aligned, optional: weight as the
+                               products read it, left by the forward and read by the backward, which
+                               forms it again without */
   const float* dloss;       /* backward: like loss; NULL: zero */
   const float* dlse;        /* (tokens), optional, cross entropy */
   void* dhidden;            /* (tokens, dim), optional */
   void* dweight;            /* (vocab, dim), optional */
 } mcpu_linear_loss_args;
 
+/* 0 where weight is read in place (16-bit, whole groups of 64 columns, 16-byte aligned) or tokens are few. */
+size_t mcpu_linear_loss_laid_size(const mcpu_linear_loss_args* a);
 size_t mcpu_linear_loss_fwd_workspace_size(const mcpu_linear_loss_args* a);
 int mcpu_linear_loss_fwd(const mcpu_linear_loss_args* a, void* workspace, size_t workspace_bytes, void* stream);
 size_t mcpu_linear_loss_bwd_workspace_size(const mcpu_linear_loss_args* a);

@@ -94,12 +94,25 @@ struct Layout {
   }
 };
 
+// Weight as a forward of more than a few tokens lays it out, behind its largest magnitude; none where it is read in
+// place.
+size_t laid_bytes(const mcpu_linear_loss_args* a, const LossParams& p) {
+  if (weight_in_place(a) || p.tokens <= kLossFew) return 0;
+  return 256 + align_up(static_cast<size_t>(loss_pieces(a->dtype) * p.vocab * p.dpad) * 2);
+}
+
 void lay_operands(const mcpu_linear_loss_args* a, LossParams& p, Layout& w) {
   const int pieces = loss_pieces(a->dtype);
   w.take(p.scal, 1);
   if (!distil(a)) w.take(p.target, p.tpad);
   w.take(p.hrows, pieces * p.tpad * p.dpad, 2);
-  if (!weight_in_place(a)) w.take(p.wrows, pieces * p.vocab * p.dpad, 2);
+  if (weight_in_place(a)) return;
+  if (a->laid != nullptr && laid_bytes(a, p) > 0) {
+    p.laid = static_cast<uint32_t*>(a->laid);
+    p.wrows = static_cast<char*>(a->laid) + 256;
+  } else {
+    w.take(p.wrows, pieces * p.vocab * p.dpad, 2);
+  }
 }
 
 size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
@@ -133,6 +146,14 @@ size_t lay_bwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
 }  // namespace mcpu
 
 using namespace mcpu;
+
+extern "C" size_t mcpu_linear_loss_laid_size(const mcpu_linear_loss_args* a) {
+  if (check_loss(a, "linear_loss") != MCPU_OK) {
+    clear_error();
+    return 0;
+  }
+  return nothing(a) ? 0 : laid_bytes(a, make_loss(a));
+}
 
 extern "C" size_t mcpu_linear_loss_fwd_workspace_size(const mcpu_linear_loss_args* a) {
   if (check_loss(a, "linear_loss") != MCPU_OK) {

@@ -41,16 +41,18 @@ template <typename I> __host__ __device__ inline float product_us(I tiles, I dep
   return rounds * (static_cast<float>((depths + splits - 1) / splits) * 1.8f + 6.f) +
          (apart || splits > 1 ? static_cast<float>(tiles * splits) * 0.131f : 0.f);
 }
+// Splits that fill one to eight rounds of 256, or none, whichever takes least.
 __host__ __device__ inline int splits_for(int64_t tiles, int64_t depths, bool apart) {
-  constexpr int kTry[] = {2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
   if (tiles < 1 || tiles > kLossSplitTiles / 2) return 1;
   // In 32 bits, which the sizes left fit: the GPU divides 64 by a routine.
   const int t = static_cast<int>(tiles), d = static_cast<int>(depths);
   int best = 1;
   float least = product_us(t, d, 1, apart);
-  for (int s : kTry) {
+  for (int rounds = 1; rounds <= 8; ++rounds) {
+    const int s = 256 * rounds / t < kLossMostSplits ? 256 * rounds / t : kLossMostSplits;
+    if (s < 2 || d / s < 4 || t * s > kLossSplitTiles) continue;
     const float us = product_us(t, d, s, apart);
-    if (d / s >= 4 && t * s <= kLossSplitTiles && us < 0.97f * least) best = s, least = us;
+    if (us < 0.97f * least) best = s, least = us;
   }
   return best;
 }
@@ -296,6 +298,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_gather_kernel(
 template <typename T> __global__ __launch_bounds__(256) void loss_weight_kernel(const LossParams p) {
   const int64_t v = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (v >= p.vocab) return;
+  if (p.laid != nullptr && v == 0 && (threadIdx.x & 63) == 0) *p.laid = p.scal->wmax;
   const float up = std::is_same_v<T, float> ? pow2(up_exponent(p.scal->wmax)) : 1.f;
   lay_row<T>(static_cast<const T*>(p.weight) + v * p.sw, p.wrows, v * p.dpad, p.vocab * p.dpad, p.dim, p.dpad, up,
              threadIdx.x & 63);
@@ -1117,7 +1120,8 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   // By the rows that count, which the host does not know.
   p.scal->hsplit = splits_for((p.dpad + kLossTile - 1) / kLossTile * ((kept + kLossTile - 1) / kLossTile),
                               p.vpiece / kLossDepth * (p.dtype == MCPU_F32 ? 3 : 1), true);
-  p.scal->hmax = p.scal->wmax = 0;
+  p.scal->hmax = 0;
+  p.scal->wmax = p.laid != nullptr ? *p.laid : 0;
   p.scal->unit = most == 0.f ? 1.f : fmaxf(most, 0x1p-100f);
 }
 
@@ -1167,7 +1171,7 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
 template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
   run(loss_coef_kernel, p, 1, 1024, st);
   // Of few tokens ds is formed from weight as it lies.
-  lay_operands<T>(p, p.tokens > kLossFew || p.dhidden != nullptr, st);
+  lay_operands<T>(p, p.laid == nullptr && (p.tokens > kLossFew || p.dhidden != nullptr), st);
   const int64_t tt = p.tpad / kLossTile, dt = (p.dpad + kLossTile - 1) / kLossTile;
   float* const dwpart = p.dwpart;
   for (int64_t vp = 0; vp < p.vocab; vp += p.vpiece) {
@@ -1226,7 +1230,7 @@ void loss_plan(LossParams& p) {
     if (us < 0.99f * least) least = us, best = vt;
   }
   p.vpiece = best * kLossTile;
-  p.htiles = std::max(dt * tt, std::min<int64_t>(kLossSplitTiles, 64 * dt * tt));
+  p.htiles = std::max(dt * tt, std::min<int64_t>(kLossSplitTiles, kLossMostSplits * dt * tt));
   p.wsplit = std::max(loss_wsplit(p, 0), loss_wsplit(p, (all - 1) / best * p.vpiece));
 }
 

@@ -36,6 +36,7 @@ struct LossParams {
   float* stat;    // (4, tokens) in the order of `rows`: maximum, sum of exp(c (s - it)), a target's share of it, the others'
   float* share;   // (tokens, k): the teacher's distribution, or null
   int32_t* rows;  // (tokens + 1): the rows that count in order, then the others; then how many count
+  uint32_t* laid;      // float32: wmax beside wrows, where both are kept for the backward; or null
   // backward
   const float* dloss;  // (tokens), or (1) where reduced
   const float* dlse;   // (tokens), or null
@@ -66,6 +67,7 @@ constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a 
 constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
 constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
 constexpr int kLossFew = 64;      // most tokens of a forward that streams the weight past them
+constexpr int kLossMostSplits = 64;
 constexpr int64_t kLossSplitTiles = 1536;  // most results of a split product, of 256 KiB each
 constexpr int64_t kLossMaxK = 1024;
 

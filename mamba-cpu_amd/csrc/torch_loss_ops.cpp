@@ -58,11 +58,11 @@ const Tensor& check_like(const char* name, const char* what, const Tensor& t, at
 }
 
 // loss, lse, and for the backward the ids' products, the rows' statistics, the teacher's distribution
-// (distillation) and the rows that count.
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in,
-                                                                   const Tensor& ids, const optional<Tensor>& teacher,
-                                                                   int64_t ignore_index, double temperature,
-                                                                   int64_t reduction) {
+// (distillation), the rows that count and, where saved, weight as the products read it.
+using Losses = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+Losses linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in, const Tensor& ids,
+                       const optional<Tensor>& teacher, int64_t ignore_index, double temperature, int64_t reduction,
+                       bool save) {
   const char* name = "mamba_cpu::linear_loss_fwd";
   check_gpu(name, hidden_in);
   c10::DeviceGuard guard(hidden_in.device());
@@ -83,17 +83,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_fwd(const
   a.stat = static_cast<float*>(stat.data_ptr());
   a.share = has(teacher) ? static_cast<float*>(share.data_ptr()) : nullptr;
   a.rows = static_cast<int32_t*>(rows.data_ptr());
+  const size_t kept = save ? mcpu_linear_loss_laid_size(&a) : 0;
+  Tensor laid = at::empty({static_cast<int64_t>(kept)}, hidden.options().dtype(at::kByte));
+  if (kept > 0) a.laid = laid.data_ptr();
   const size_t nws = mcpu_linear_loss_fwd_workspace_size(&a);
   Tensor ws = workspace(nws, hidden);
   check_rc(mcpu_linear_loss_fwd(&a, ws_ptr(ws), nws, stream_of(hidden)), name);
-  return {loss, lse, picked, stat, share, rows};
+  return {loss, lse, picked, stat, share, rows, laid};
 }
 
 // Gradients of hidden and weight, each where wanted.
 std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const optional<Tensor>& dlse,
                                            const Tensor& hidden_in, const Tensor& weight_in, const Tensor& ids,
                                            const Tensor& picked, const Tensor& stat, const Tensor& share,
-                                           const Tensor& rows, int64_t ignore_index, double temperature,
+                                           const Tensor& rows, const Tensor& laid, int64_t ignore_index, double temperature,
                                            int64_t reduction, bool distil, bool want_hidden, bool want_weight) {
   const char* name = "mamba_cpu::linear_loss_bwd";
   check_gpu(name, hidden_in);
@@ -111,6 +114,12 @@ std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const 
   if (distil) a.share = static_cast<float*>(check_like(name, "share", share, at::kFloat, both, hidden).data_ptr());
   a.rows = static_cast<int32_t*>(
       check_like(name, "rows", rows, at::kInt, at::IntArrayRef(&last, 1), hidden).data_ptr());
+  const size_t kept = mcpu_linear_loss_laid_size(&a);
+  if (laid.numel() > 0) {
+    TORCH_CHECK_VALUE(static_cast<size_t>(laid.numel()) == kept && laid.scalar_type() == at::kByte && laid.is_contiguous() &&
+                          laid.device() == hidden.device(), name, " expects the laid out weight that the forward left");
+    a.laid = laid.data_ptr();
+  }
   Tensor g, e;
   if (has(dloss)) {
     g = dloss->to(at::kFloat).contiguous();
@@ -139,20 +148,20 @@ auto loss_fwd_below() {
 struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
                                const optional<Tensor>& teacher, int64_t ignore_index, double temperature,
-                               int64_t reduction) {
+                               int64_t reduction, bool save) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto r = loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
+    auto r = loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction, save);
     const Tensor lse = std::get<1>(r), picked = std::get<2>(r), stat = std::get<3>(r), share = std::get<4>(r),
-                 rows = std::get<5>(r);
-    ctx->mark_non_differentiable(has(teacher) ? variable_list{lse, picked, stat, share, rows}
-                                              : variable_list{picked, stat, share, rows});
-    ctx->save_for_backward({hidden, weight, ids, picked, stat, share, rows});
+                 rows = std::get<5>(r), laid = std::get<6>(r);
+    ctx->mark_non_differentiable(has(teacher) ? variable_list{lse, picked, stat, share, rows, laid}
+                                              : variable_list{picked, stat, share, rows, laid});
+    ctx->save_for_backward({hidden, weight, ids, picked, stat, share, rows, laid});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["distil"] = has(teacher);
     ctx->set_materialize_grads(false);
-    return {std::get<0>(r), lse, picked, stat, share, rows};
+    return {std::get<0>(r), lse, picked, stat, share, rows, laid};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -164,27 +173,25 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("mamba_cpu::linear_loss_bwd", "")
                          .typed<decltype(linear_loss_bwd)>();
-    auto r = op.call(g, opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["ignore"].toInt(),
+    auto r = op.call(g, opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["ignore"].toInt(),
                      ctx->saved_data["temperature"].toDouble(), reduction, ctx->saved_data["distil"].toBool(),
                      want_hidden, want_weight);
     return {want_hidden ? std::get<0>(r) : Tensor(), want_weight ? std::get<1>(r) : Tensor(),
-            Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+            Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(const Tensor& hidden, const Tensor& weight,
-                                                                        const Tensor& ids,
-                                                                        const optional<Tensor>& teacher,
-                                                                        int64_t ignore_index, double temperature,
-                                                                        int64_t reduction) {
+Losses linear_loss_autograd(const Tensor& hidden, const Tensor& weight, const Tensor& ids,
+                            const optional<Tensor>& teacher, int64_t ignore_index, double temperature,
+                            int64_t reduction, bool save) {
   TORCH_CHECK_VALUE(!any_grad({teacher}), "mamba_cpu::linear_loss_fwd has no gradient of the teacher's logits: detach "
                     "them");
   if (!any_grad({opt(hidden), opt(weight)})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
+    return loss_fwd_below().call(hidden, weight, ids, teacher, ignore_index, temperature, reduction, save);
   }
-  auto r = LinearLossFn::apply(hidden, weight, ids, teacher, ignore_index, temperature, reduction);
-  return {r[0], r[1], r[2], r[3], r[4], r[5]};
+  auto r = LinearLossFn::apply(hidden, weight, ids, teacher, ignore_index, temperature, reduction, save);
+  return {r[0], r[1], r[2], r[3], r[4], r[5], r[6]};
 }
 
 }  // namespace
@@ -192,9 +199,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_loss_autograd(
 
 TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
   m.def("linear_loss_fwd(Tensor hidden, Tensor weight, Tensor ids, Tensor? teacher, int ignore_index, "
-        "float temperature, int reduction) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "float temperature, int reduction, bool save) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("linear_loss_bwd(Tensor? dloss, Tensor? dlse, Tensor hidden, Tensor weight, Tensor ids, Tensor picked, "
-        "Tensor stat, Tensor share, Tensor rows, int ignore_index, float temperature, int reduction, bool distil, "
+        "Tensor stat, Tensor share, Tensor rows, Tensor laid, int ignore_index, float temperature, int reduction, bool distil, "
         "bool want_hidden, bool want_weight) -> (Tensor, Tensor)");
 }
 

@@ -205,7 +205,7 @@ class LinearLossArgs(ctypes.Structure):
         ("tokens", _I64), ("vocab", _I64), ("dim", _I64), ("k", _I64), ("hidden_stride", _I64),
         ("weight_stride", _I64), ("ignore_index", _I64), ("temperature", ctypes.c_float), ("dtype", _I32),
         ("ids64", _I32), ("reduction", _I32), ("loss", _P), ("lse", _P), ("picked", _P), ("stat", _P),
-        ("share", _P), ("rows", _P), ("dloss", _P), ("dlse", _P), ("dhidden", _P), ("dweight", _P),
+        ("share", _P), ("rows", _P), ("laid", _P), ("dloss", _P), ("dlse", _P), ("dhidden", _P), ("dweight", _P),
     ]
 
 
@@ -298,6 +298,8 @@ for _name in ("fwd", "bwd"):
     getattr(lib, f"mcpu_linear_loss_{_name}_workspace_size").restype = ctypes.c_size_t
     getattr(lib, f"mcpu_linear_loss_{_name}").argtypes = [_ARGP["linear_loss"], _P, ctypes.c_size_t, _P]
     getattr(lib, f"mcpu_linear_loss_{_name}").restype = ctypes.c_int
+lib.mcpu_linear_loss_laid_size.argtypes = [_ARGP["linear_loss"]]
+lib.mcpu_linear_loss_laid_size.restype = ctypes.c_size_t
 
 for _name, _cls in _BLOCKS:
     _want = lib.mcpu_args_size(_name.encode())

@@ -29,18 +29,31 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 # its shape functions for FakeTensor tracing.
 
 
+def _laid_size(hidden, weight, save):
+    """Bytes of weight in the products' layout, where it is kept for the backward and is not read in place (an
+    unaligned first element aside, which a traced tensor does not tell)."""
+    (tokens, dim), vocab = hidden.shape, weight.shape[0]
+    wide = hidden.dtype == torch.float32
+    stride = weight.stride(0) if weight.stride(1) == 1 or dim <= 1 else dim
+    if not save or tokens <= 64 or vocab == 0 or (
+            not wide and dim % 64 == 0 and stride % 8 == 0 and stride <= 2 ** 20):
+        return 0
+    return 256 + (vocab * -(-dim // 64) * 64 * (4 if wide else 2) + 255) // 256 * 256
+
+
 @torch.library.register_fake("mamba_cpu::linear_loss_fwd")
-def _(hidden, weight, ids, teacher, ignore_index, temperature, reduction):
+def _(hidden, weight, ids, teacher, ignore_index, temperature, reduction, save):
     tokens, k = ids.shape
     f32 = dict(dtype=torch.float32)
     return (hidden.new_empty(() if reduction else (tokens,), **f32), hidden.new_empty(tokens, **f32),
             hidden.new_empty(tokens if teacher is not None else 0, k, **f32), hidden.new_empty(4, tokens, **f32),
             hidden.new_empty(tokens if teacher is not None else 0, k, **f32),
-            hidden.new_empty(tokens + 1, dtype=torch.int32))
+            hidden.new_empty(tokens + 1, dtype=torch.int32),
+            hidden.new_empty(_laid_size(hidden, weight, save), dtype=torch.uint8))
 
 
 @torch.library.register_fake("mamba_cpu::linear_loss_bwd")
-def _(dloss, dlse, hidden, weight, ids, picked, stat, share, rows, ignore_index, temperature, reduction, distil,
+def _(dloss, dlse, hidden, weight, ids, picked, stat, share, rows, laid, ignore_index, temperature, reduction, distil,
       want_hidden, want_weight):
     return (hidden.new_empty(hidden.shape[0] if want_hidden else 0, hidden.shape[1]),
             weight.new_empty(weight.shape[0] if want_weight else 0, weight.shape[1]))
@@ -60,6 +73,11 @@ def _operands(hidden, weight, reduction):
     dt = hidden.dtype if hidden.dtype in _DTYPES and weight.dtype == hidden.dtype else torch.float32
     tokens = hidden.numel() // hidden.shape[-1]
     return hidden.to(dt).reshape(tokens, hidden.shape[-1]), weight.to(dt)
+
+
+def _saved(hidden, weight):
+    """Whether a backward may follow, for which the forward then keeps the weight as it laid it out."""
+    return torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
 
 
 def _ids(name, ids, shape, device):
@@ -92,7 +110,7 @@ def linear_cross_entropy_fn(hidden, weight, targets, ignore_index=-100, reductio
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
     loss, lse, *_ = torch.ops.mamba_cpu.linear_loss_fwd(h, w, ids.contiguous(), None, int(ignore_index), 1.0,
-                                                             _REDUCTIONS[reduction])
+                                                       _REDUCTIONS[reduction], _saved(h, w))
     if reduction == "none":
         loss = loss.view(targets.shape)
     return (loss, lse.view(targets.shape)) if return_lse else loss
@@ -127,5 +145,5 @@ def linear_distillation_fn(hidden, weight, teacher_ids, teacher_logits, temperat
     shape = (h.shape[0], ids.shape[-1])
     loss, *_ = torch.ops.mamba_cpu.linear_loss_fwd(
         h, w, ids.reshape(shape).contiguous(), teacher_logits.float().reshape(shape).contiguous(), -1,
-        float(temperature), _REDUCTIONS[reduction])
+        float(temperature), _REDUCTIONS[reduction], _saved(h, w))
     return loss.view(lead) if reduction == "none" else loss

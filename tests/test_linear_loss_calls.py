@@ -118,7 +118,7 @@ def test_shape_functions_follow_the_operators():
         assert kd.shape == (3, 5)
         dh, dw = torch.ops.mamba_cpu.linear_loss_bwd(
             None, None, h.view(15, 8), w, ids.view(15, 1), kd.new_empty(0, 1), kd.new_empty(4, 15),
-            kd.new_empty(0, 1), ids.new_empty(16, dtype=torch.int32), -100, 1.0, 0, False, True, True)
+            kd.new_empty(0, 1), ids.new_empty(16, dtype=torch.int32), kd.new_empty(0, dtype=torch.uint8), -100, 1.0, 0, False, True, True)
         assert dh.shape == (15, 8) and dw.shape == (11, 8) and dh.dtype == dw.dtype == torch.bfloat16
 
 
