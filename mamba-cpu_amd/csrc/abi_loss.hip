@@ -37,8 +37,9 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
 // Nothing to take a loss of: no rows, no vocabulary or no entries.
 bool nothing(const mcpu_linear_loss_args* a) { return a->tokens == 0 || a->vocab == 0 || a->k == 0; }
 
-bool sixteen(const void* p, int64_t stride) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
+// Rows that begin at multiples of 16 bytes.
+bool aligned_rows(const void* p, int64_t stride, int dtype) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * dtype_size(dtype) % 16 == 0;
 }
 
 LossParams make_loss(const mcpu_linear_loss_args* a) {
@@ -69,6 +70,8 @@ LossParams make_loss(const mcpu_linear_loss_args* a) {
   p.dlse = a->dlse;
   p.dhidden = a->dhidden;
   p.dweight = a->dweight;
+  p.few_lds = aligned_rows(a->hidden, a->hidden_stride, a->dtype) &&
+              aligned_rows(a->weight, a->weight_stride, a->dtype);
   loss_plan(p);
   return p;
 }
@@ -76,7 +79,7 @@ LossParams make_loss(const mcpu_linear_loss_args* a) {
 // The products read 16-byte groups of whole depths: weight as it lies where it has them.
 bool weight_in_place(const mcpu_linear_loss_args* a) {
   return a->dtype != MCPU_F32 && a->dim % kLossDepth == 0 && a->weight_stride <= (int64_t{1} << 20) &&
-         sixteen(a->weight, a->weight_stride);
+         aligned_rows(a->weight, a->weight_stride, a->dtype);
 }
 
 // Takes parts of a workspace one after the other; without one it counts.
@@ -123,7 +126,7 @@ size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   if (distil(a)) w.take(p.cross, p.tokens);
   if (!distil(a)) w.take(p.picked, p.tpad);
   if (p.tokens <= kLossFew) {
-    w.take(p.part, (p.vocab + 255) / 256 * kLossFew);
+    w.take(p.part, (p.vocab + kFewPart - 1) / kFewPart * kLossFew);
     return w.used;
   }
   lay_operands(a, p, w);

@@ -48,9 +48,10 @@ __host__ __device__ inline int splits_for(int64_t tiles, int64_t depths, bool ap
   const int t = static_cast<int>(tiles), d = static_cast<int>(depths);
   int best = 1;
   float least = product_us(t, d, 1, apart);
+  const int most = d / 4 < kLossMostSplits ? d / 4 : kLossMostSplits;
   for (int rounds = 1; rounds <= 8; ++rounds) {
-    const int s = 256 * rounds / t < kLossMostSplits ? 256 * rounds / t : kLossMostSplits;
-    if (s < 2 || d / s < 4 || t * s > kLossSplitTiles) continue;
+    const int s = 256 * rounds / t < most ? 256 * rounds / t : most;
+    if (s < 2 || t * s > kLossSplitTiles) continue;
     const float us = product_us(t, d, s, apart);
     if (us < 0.97f * least) best = s, least = us;
   }
@@ -730,11 +731,10 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const LossParams p) {
 
 // ---- few tokens ------------------------------------------------------------------------------------
 
-// Up to 64 tokens: the weight streams past them once, straight into the operands'
-// registers, 32 vocabulary rows a wave and every wave by itself, so that what
-// bounds it is HBM. Terms are taken in the order the loads bring them, the same for
-// both operands: lane l has row l % 16 and the 16 bytes at l / 16 of each 64.
-// float32 goes through v_mfma_f32_16x16x4_f32, four to a load.
+// Up to 64 tokens: the weight streams past them once, 32 vocabulary rows a wave and
+// 128 a workgroup, so that what bounds it is HBM. A lane's part of an operand is row
+// l % 16 and the 16 bytes at l / 16 of each 64, the same terms for both operands.
+// float32 goes through v_mfma_f32_16x16x4_f32, four to 16 bytes.
 typedef uint32_t u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
 
 template <typename T> constexpr int kChunk = 16 / static_cast<int>(sizeof(T));
@@ -765,34 +765,97 @@ template <typename T> __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f
   }
 }
 
+// A stage of LDS: 128 bytes of each row of the workgroup's 128 of weight and NF x 16 of
+// hidden. Three, 72 KiB at most, leave room for two workgroups on a CU; a fourth,
+// where it leaves one, is 6 % slower, else as fast.
+template <int NF> constexpr int kStageBytes = (128 + NF * 16) * 128;
+
+// Products of whole groups of 128 bytes, where rows are 16-byte aligned: loads write
+// straight into LDS, eight lanes a row of 128 bytes, in the order that spreads a read
+// over the banks (chunk c of row r at c ^ (r % 8)). Straight into the operands'
+// registers a load touches 16 rows, and the cache takes 50 cycles for it: 49 against
+// 15 us with 3 tokens, 688 x 2560 bf16, and 70 against 59, 16 x 50280 x 2560 (257 MB).
+template <typename T, int NF, typename Row>
+__device__ __forceinline__ int64_t few_products_lds(const LossParams& p, Row&& row, int64_t v0,
+                                                    f32x4 (&acc)[2][2][NF]) {
+  constexpr int kHidden = NF == 4 ? 2 : 1, kLoads = 4 + kHidden;
+  constexpr int kTerms = 128 / static_cast<int>(sizeof(T));
+  __shared__ __attribute__((aligned(1024))) char s0[kStageBytes<NF>];
+  __shared__ __attribute__((aligned(1024))) char s1[kStageBytes<NF>];
+  __shared__ __attribute__((aligned(1024))) char s2[kStageBytes<NF>];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = static_cast<int>(p.dim / kTerms);
+  if (groups == 0) return 0;
+  // A lane's 16 bytes of eight rows a load: four loads of the wave's own rows of
+  // weight, and its share of hidden's (of 16 tokens, waves 2 and 3 bring what 0 and 1 do).
+  const int r8 = lane >> 3, swap = ((lane & 7) ^ r8) * (16 / static_cast<int>(sizeof(T)));
+  const T* from[kLoads];
+  int to[kLoads];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t v = v0 + 8 * i + r8;  // a row that is not there is read as the last
+    from[i] = static_cast<const T*>(p.weight) + (v < p.vocab ? v : p.vocab - 1) * p.sw + swap;
+    to[i] = (wave * 32 + 8 * i) * 128;
+  }
+#pragma unroll
+  for (int i = 0; i < kHidden; ++i) {
+    const int t8 = NF == 1 ? wave & 1 : wave * kHidden + i;
+    from[4 + i] = row(8 * t8 + r8) + swap;
+    to[4 + i] = (128 + 8 * t8) * 128;
+  }
+  using lds_ptr = __attribute__((address_space(3))) void*;
+  using global_ptr = const __attribute__((address_space(1))) void*;
+  auto load = [&](char* stage, int group) {
+    const int64_t at = int64_t{group < groups ? group : groups - 1} * kTerms;  // behind the end: once more, unused
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds((global_ptr)(from[i] + at), (lds_ptr)(stage + to[i]), 16, 0, 0);
+  };
+  auto step = [&](const char* stage, char* next, int group) {
+    // The loads of this group have arrived, those of the next need not have; and no wave reads `next` any more.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | kLoads);  // vmcnt(kLoads) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load(next, group + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    const int r = lane & 15;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = ((u * 4 + (lane >> 4)) ^ (r & 7)) * 16;
+      u32x4 a[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) a[i] = *reinterpret_cast<const u32x4*>(stage + (wave * 32 + 16 * i + r) * 128 + at);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        const u32x4 b = *reinterpret_cast<const u32x4*>(stage + (128 + 16 * j + r) * 128 + at);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[u][i][j] = mma16<T>(a[i], b, acc[u][i][j]);
+      }
+    }
+  };
+  load(s0, 0);
+  load(s1, 1);
+  int g = 0;
+  for (; g + 3 <= groups; g += 3) {
+    step(s0, s2, g);
+    step(s1, s0, g + 1);
+    step(s2, s1, g + 2);
+  }
+  if (g < groups) step(s0, s2, g);
+  if (g + 1 < groups) step(s1, s0, g + 1);
+  __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is on its way into LDS any more
+  return int64_t{groups} * kTerms;
+}
+
 // The products of NF x 16 rows of hidden and a wave's 32 rows of weight from v0 on:
 // s[i][j][e] is of vocabulary row v0 + 16 i + 4 (lane / 16) + e and token 16 j + lane % 16;
 // row(t) is where token t's row of hidden begins. Forward and backward form them alike,
 // to the bit.
-// Up to 16 tokens hidden is read like weight, by every wave. More go through LDS, 256
-// bytes of a row at a time: read by every wave they are twice the weight's bytes for
-// 64 tokens, and a load of 64 lanes in as many lines is what the cache serves slowest (93
-// against 54 us, 33 x 50280 x 2560 bf16). Chunks of a row are where c ^ (row % 16) puts them.
 template <typename T, int NF, typename Row>
 __device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int64_t v0, f32x4 (&s)[2][NF]) {
-  constexpr bool kShared = NF > 1;
-  __shared__ u32x4 shared[kShared ? 2 : 1][kShared ? NF * 256 : 1];
   const int lane = threadIdx.x & 63;
   const int64_t k0 = (lane >> 4) * kChunk<T>;
-  const T* w[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t v = v0 + 16 * i + (lane & 15);  // a row that is not there is read as the last
-    w[i] = static_cast<const T*>(p.weight) + (v < p.vocab ? v : p.vocab - 1) * p.sw;
-  }
-  const T* h[NF];
-#pragma unroll
-  for (int j = 0; j < NF; ++j) h[j] = row(16 * j + (lane & 15));
-  // What a thread brings to LDS of each 256 bytes: chunk threadIdx % 16 of rows threadIdx / 16 and, 32 apart, on.
-  constexpr int kBring = kShared ? NF / 2 : 1;
-  const T* from[kBring];
-#pragma unroll
-  for (int i = 0; i < kBring; ++i) from[i] = row((threadIdx.x >> 4) + 32 * i) + (threadIdx.x & 15) * kChunk<T>;
   // Two sums of every other load's products: half the roundings in a row.
   f32x4 acc[2][2][NF];
 #pragma unroll
@@ -801,64 +864,34 @@ __device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < NF; ++j) acc[u][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int kStep = 4 * kChunk<T>, kTurn = 4;  // terms of a load, loads of a turn
-  const int64_t whole = p.dim / (kStep * kTurn) * (kStep * kTurn);
-  u32x4 a[2][kTurn][2], b[2][kTurn][kShared ? 1 : NF], bring[kBring];  // this turn's and the next's
-  auto load = [&](int to, int64_t k) {
-    if constexpr (kShared) {
+  int64_t k = p.few_lds ? few_products_lds<T, NF>(p, row, v0, acc) : 0;
+  // Rows that are not aligned, and what is left of those that are: into registers, two loads a turn.
+  const T *w[2], *h[NF];
 #pragma unroll
-      for (int i = 0; i < kBring; ++i) bring[i] = chunk_at<T>(from[i], k);
-    }
-#pragma unroll
-    for (int u = 0; u < kTurn; ++u) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) a[to][u][i] = chunk_at<T>(w[i], k + k0 + u * kStep);
-      if constexpr (!kShared) {
-#pragma unroll
-        for (int j = 0; j < NF; ++j) b[to][u][j] = chunk_at<T>(h[j], k + k0 + u * kStep);
-      }
-    }
-  };
-  auto store = [&](int to) {
-    if constexpr (kShared) {
-#pragma unroll
-      for (int i = 0; i < kBring; ++i) {
-        const int r = (threadIdx.x >> 4) + 32 * i;
-        shared[to][r * 16 + ((threadIdx.x & 15) ^ (r & 15))] = bring[i];
-      }
-      __syncthreads();
-    }
-  };
-  auto turn = [&](int of) {
-#pragma unroll
-    for (int u = 0; u < kTurn; ++u)
-#pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        u32x4 y;
-        if constexpr (kShared)
-          y = shared[of][(16 * j + (lane & 15)) * 16 + ((u * 4 + (lane >> 4)) ^ (lane & 15))];
-        else
-          y = b[of][u][j];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) acc[u & 1][i][j] = mma16<T>(a[of][u][i], y, acc[u & 1][i][j]);
-      }
-  };
-  int64_t k = 0;
-  if (whole > 0) {
-    load(0, 0);
-    store(0);
+  for (int i = 0; i < 2; ++i) {
+    const int64_t v = v0 + 16 * i + (lane & 15);  // a row that is not there is read as the last
+    w[i] = static_cast<const T*>(p.weight) + (v < p.vocab ? v : p.vocab - 1) * p.sw;
   }
-  // A buffer is written while the other is read; who writes it next has passed the barrier between.
-  for (; k + 2 * kStep * kTurn <= whole; k += 2 * kStep * kTurn) {
-    load(1, k + kStep * kTurn);
-    turn(0);
-    store(1);
-    load(0, k + 2 * kStep * kTurn < whole ? k + 2 * kStep * kTurn : k);
-    turn(1);
-    store(0);
+#pragma unroll
+  for (int j = 0; j < NF; ++j) h[j] = row(16 * j + (lane & 15));
+  constexpr int kStep = 4 * kChunk<T>;  // terms of a load
+  for (; k + 2 * kStep <= p.dim; k += 2 * kStep) {
+    u32x4 a[2][2], b[2][NF];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) a[u][i] = chunk_at<T>(w[i], k + k0 + u * kStep);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) b[u][j] = chunk_at<T>(h[j], k + k0 + u * kStep);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[u][i][j] = mma16<T>(a[u][i], b[u][j], acc[u][i][j]);
   }
-  if (k < whole) turn(0);
-  for (k = whole; k < p.dim; k += kStep) {
+  for (; k < p.dim; k += kStep) {
     u32x4 x[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) x[i] = chunk_left<T>(w[i], k + k0, p.dim);
@@ -877,15 +910,15 @@ __device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int
       for (int e = 0; e < 4; ++e) s[i][j][e] = acc[0][i][j][e] + acc[1][i][j][e];
 }
 
-// NF x 16 tokens; 256 vocabulary rows a workgroup, and of them one maximum and sum a token. Distillation: one more
+// NF x 16 tokens; 128 vocabulary rows a workgroup, and of them one maximum and sum a token. Distillation: one more
 // workgroup a token, first, for the teacher's part, which would take 10 us before or after.
-template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_kernel(const LossParams p) {
+template <typename T, int NF> __global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
   const int64_t teachers = p.teacher != nullptr ? p.tokens : 0;
   const int64_t at = p.first + blockIdx.x, group = at - teachers;
-  if (group < 0) return teacher_row<T, 512>(p, at);
-  __shared__ float2 parts[8][NF * 16];
+  if (group < 0) return teacher_row<T, 256>(p, at);
+  __shared__ float2 parts[4][NF * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t v0 = group * 256 + wave * 32;
+  const int64_t v0 = group * kFewPart + wave * 32;
   f32x4 acc[2][NF];
   few_products<T, NF>(p, [&](int64_t t) {  // a token that is not there is read as the last
     return static_cast<const T*>(p.hidden) + (t < p.tokens ? t : p.tokens - 1) * p.sh;
@@ -921,17 +954,17 @@ template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_ke
   const int t = threadIdx.x;
   if (t >= NF * 16 || t >= p.tokens) return;
   float m = parts[0][t].x, s = 0.f;
-  for (int q = 1; q < 8; ++q) m = fmaxf(m, parts[q][t].x);
+  for (int q = 1; q < 4; ++q) m = fmaxf(m, parts[q][t].x);
   const float sub = m == -INFINITY ? 0.f : m;
-  for (int q = 0; q < 8; ++q) s = fmaf(parts[q][t].y, fast_exp2((parts[q][t].x - sub) * c), s);
+  for (int q = 0; q < 4; ++q) s = fmaf(parts[q][t].y, fast_exp2((parts[q][t].x - sub) * c), s);
   p.part[group * kLossFew + t] = make_float2(m, s);
 }
 
 // ds of up to 64 tokens that count, as loss_grad_kernel; rows behind them up to 64 are zero.
-template <typename T, int NF> __global__ __launch_bounds__(512) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
+template <typename T, int NF> __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
   using E = Kept<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t vl = (p.first + blockIdx.x) * 256 + wave * 32, v0 = vp + vl;
+  const int64_t vl = (p.first + blockIdx.x) * kFewPart + wave * 32, v0 = vp + vl;
   const int kept = p.scal->kept;
   f32x4 acc[2][NF];
   few_products<T, NF>(p, [&](int i) {
@@ -994,7 +1027,7 @@ __global__ __launch_bounds__(1024) void loss_few_join_kernel(const LossParams p)
   __syncthreads();
   const bool keep = mask >> t & 1;
   const int kept = __popcll(mask), before = __popcll(mask & ((1ull << t) - 1));
-  const int64_t parts = (p.vocab + 255) / 256;
+  const int64_t parts = (p.vocab + kFewPart - 1) / kFewPart;
   const float c = kLog2e / p.temperature;
   float m = -INFINITY, s = 0.f;
   if (keep)
@@ -1152,8 +1185,8 @@ template <typename T> void lay_operands(const LossParams& p, bool weight, hipStr
 template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   if (p.tokens <= kLossFew) {
     for_few(p.tokens, [&](auto nf) {
-      run(loss_few_kernel<T, decltype(nf)::value>, p, (p.vocab + 255) / 256 + (p.teacher != nullptr ? p.tokens : 0), 512,
-          st);
+      run(loss_few_kernel<T, decltype(nf)::value>, p,
+          (p.vocab + kFewPart - 1) / kFewPart + (p.teacher != nullptr ? p.tokens : 0), 256, st);
     });
     run(loss_few_join_kernel, p, 1, 1024, st);
     return hipGetLastError();
@@ -1179,7 +1212,7 @@ template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
     const int64_t vt = p.vrows / kLossTile;
     if (p.tokens <= kLossFew)
       for_few(p.tokens, [&](auto nf) {
-        run(loss_few_grad_kernel<T, decltype(nf)::value>, p, vt, 512, st, vp);
+        run(loss_few_grad_kernel<T, decltype(nf)::value>, p, p.vrows / kFewPart, 256, st, vp);
       });
     else
       run(loss_grad_kernel<T>, p, vt * tt, 512, st, vp);
