@@ -97,10 +97,9 @@ struct Layout {
   }
 };
 
-// Weight as a forward of more than a few tokens lays it out, behind its largest magnitude; none where it is read in
-// place.
+// Weight as the forward lays it out, behind its largest magnitude; none where it is read in place.
 size_t laid_bytes(const mcpu_linear_loss_args* a, const LossParams& p) {
-  if (weight_in_place(a) || p.tokens <= kLossFew) return 0;
+  if (weight_in_place(a) || p.blocks) return 0;
   return 256 + align_up(static_cast<size_t>(loss_pieces(a->dtype) * p.vocab * p.dpad) * 2);
 }
 
@@ -129,7 +128,10 @@ size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
     w.take(p.part, (p.vocab + kFewPart - 1) / kFewPart * kLossFew);
     return w.used;
   }
-  lay_operands(a, p, w);
+  if (p.blocks)
+    w.take(p.scal, 1);
+  else
+    lay_operands(a, p, w);
   w.take(p.part, (p.vocab + kLossPart - 1) / kLossPart * p.tpad);
   return w.used;
 }

@@ -910,24 +910,34 @@ __device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int
       for (int e = 0; e < 4; ++e) s[i][j][e] = acc[0][i][j][e] + acc[1][i][j][e];
 }
 
-// NF x 16 tokens; 128 vocabulary rows a workgroup, and of them one maximum and sum a token. Distillation: one more
-// workgroup a token, first, for the teacher's part, which would take 10 us before or after.
-template <typename T, int NF> __global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
-  const int64_t teachers = p.teacher != nullptr ? p.tokens : 0;
-  const int64_t at = p.first + blockIdx.x, group = at - teachers;
-  if (group < 0) return teacher_row<T, 256>(p, at);
+// NF x 16 tokens and 128 vocabulary rows a workgroup, and of these one maximum and sum a token.
+// Up to 64 tokens in all (not ROWS), as they come; distillation: one more workgroup a
+// token, first, for the teacher's part, which would take 10 us before or after.
+// ROWS: 64 of the rows that count a workgroup, as loss_logits_kernel takes and leaves
+// them, where its tiles are too few to fill the GPU.
+template <typename T, int NF, bool ROWS>
+__global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
+  const int64_t teachers = !ROWS && p.teacher != nullptr ? p.tokens : 0;
+  const int64_t at = p.first + blockIdx.x - teachers;
+  if (at < 0) return teacher_row<T, 256>(p, at + teachers);
+  const int64_t groups = (p.vocab + kFewPart - 1) / kFewPart;
+  const int64_t group = ROWS ? at % groups : at, t0 = ROWS ? at / groups * kLossFew : 0;
+  const int64_t tokens = ROWS ? p.scal->kept : p.tokens;
+  if (t0 >= tokens) return;
   __shared__ float2 parts[4][NF * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = group * kFewPart + wave * 32;
+  auto row = [&](int64_t t) { return ROWS ? int64_t{p.rows[t]} : t; };
   f32x4 acc[2][NF];
-  few_products<T, NF>(p, [&](int64_t t) {  // a token that is not there is read as the last
-    return static_cast<const T*>(p.hidden) + (t < p.tokens ? t : p.tokens - 1) * p.sh;
+  few_products<T, NF>(p, [&](int64_t i) {  // a token that is not there is read as the last
+    return static_cast<const T*>(p.hidden) + row(t0 + i < tokens ? t0 + i : tokens - 1) * p.sh;
   }, v0, acc);
   const float c = kLog2e / p.temperature;
 #pragma unroll
   for (int j = 0; j < NF; ++j) {
-    const int64_t t = 16 * j + (lane & 15);
-    const int64_t target = p.teacher == nullptr && t < p.tokens && counts(p, t) ? id_at(p, t) : -1;
+    const int64_t t = t0 + 16 * j + (lane & 15);
+    const bool aim = p.teacher == nullptr && t < tokens && (ROWS || counts(p, t));
+    const int64_t target = aim ? id_at(p, row(t)) : -1;
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -951,29 +961,31 @@ template <typename T, int NF> __global__ __launch_bounds__(256, 2) void loss_few
     if (lane < 16) parts[wave][16 * j + lane] = make_float2(m, s);
   }
   __syncthreads();
-  const int t = threadIdx.x;
-  if (t >= NF * 16 || t >= p.tokens) return;
-  float m = parts[0][t].x, s = 0.f;
-  for (int q = 1; q < 4; ++q) m = fmaxf(m, parts[q][t].x);
+  const int i = threadIdx.x;
+  if (i >= NF * 16 || t0 + i >= tokens) return;
+  float m = parts[0][i].x, s = 0.f;
+  for (int q = 1; q < 4; ++q) m = fmaxf(m, parts[q][i].x);
   const float sub = m == -INFINITY ? 0.f : m;
-  for (int q = 0; q < 4; ++q) s = fmaf(parts[q][t].y, fast_exp2((parts[q][t].x - sub) * c), s);
-  p.part[group * kLossFew + t] = make_float2(m, s);
+  for (int q = 0; q < 4; ++q) s = fmaf(parts[q][i].y, fast_exp2((parts[q][i].x - sub) * c), s);
+  p.part[group * (ROWS ? p.tpad : kLossFew) + t0 + i] = make_float2(m, s);
 }
 
-// ds of up to 64 tokens that count, as loss_grad_kernel; rows behind them up to 64 are zero.
+// ds of 64 of the rows that count a workgroup, as loss_grad_kernel; rows behind the last, up to whole 64, are zero.
 template <typename T, int NF> __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
   using E = Kept<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t vl = (p.first + blockIdx.x) * kFewPart + wave * 32, v0 = vp + vl;
-  const int kept = p.scal->kept;
+  const int64_t at = p.first + blockIdx.x, groups = p.vrows / kFewPart, t0 = at / groups * kLossFew;
+  const int64_t vl = at % groups * kFewPart + wave * 32, v0 = vp + vl;
+  const int64_t kept = p.scal->kept;
+  if (t0 >= kept) return;
   f32x4 acc[2][NF];
-  few_products<T, NF>(p, [&](int i) {
-    return static_cast<const T*>(p.hidden) + p.rows[kept == 0 ? 0 : i < kept ? i : kept - 1] * p.sh;
+  few_products<T, NF>(p, [&](int64_t i) {
+    return static_cast<const T*>(p.hidden) + p.rows[t0 + i < kept ? t0 + i : kept - 1] * p.sh;
   }, v0, acc);
   const float c = kLog2e / p.temperature;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int t = 16 * j + (lane & 15);
+    const int64_t t = t0 + 16 * j + (lane & 15);
     const bool in = j < NF && t < kept;
     const float up = in ? kUp<E> / unit_of(p, t) : 0.f;
     const float a = in ? p.coef[t] * up : 0.f, b = in ? p.coef[p.tpad + t] * up : 0.f;
@@ -1185,7 +1197,7 @@ template <typename T> void lay_operands(const LossParams& p, bool weight, hipStr
 template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   if (p.tokens <= kLossFew) {
     for_few(p.tokens, [&](auto nf) {
-      run(loss_few_kernel<T, decltype(nf)::value>, p,
+      run(loss_few_kernel<T, decltype(nf)::value, false>, p,
           (p.vocab + kFewPart - 1) / kFewPart + (p.teacher != nullptr ? p.tokens : 0), 256, st);
     });
     run(loss_few_join_kernel, p, 1, 1024, st);
@@ -1193,9 +1205,13 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   }
   if (p.teacher != nullptr) run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
   run(loss_rows_kernel, p, 1, 1024, st);
-  lay_operands<T>(p, true, st);
-  const int64_t vt = (p.vocab + kLossTile - 1) / kLossTile, tt = p.tpad / kLossTile;
-  run(loss_logits_kernel<T>, p, vt * tt, 512, st);
+  if (p.blocks) {
+    run(loss_few_kernel<T, 4, true>, p, (p.vocab + kFewPart - 1) / kFewPart * ((p.tokens + kLossFew - 1) / kLossFew), 256,
+        st);
+  } else {
+    lay_operands<T>(p, true, st);
+    run(loss_logits_kernel<T>, p, (p.vocab + kLossTile - 1) / kLossTile * (p.tpad / kLossTile), 512, st);
+  }
   run(loss_join_kernel, p, (p.tokens + 31) / 32, 256, st);
   if (p.reduction != MCPU_REDUCE_NONE) run(loss_sum_kernel, p, 1, 1024, st);
   return hipGetLastError();
@@ -1203,16 +1219,17 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
 
 template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
   run(loss_coef_kernel, p, 1, 1024, st);
-  // Of few tokens ds is formed from weight as it lies.
-  lay_operands<T>(p, p.laid == nullptr && (p.tokens > kLossFew || p.dhidden != nullptr), st);
+  // Blocks of 64 tokens read weight as it lies.
+  lay_operands<T>(p, p.laid == nullptr && (!p.blocks || p.dhidden != nullptr), st);
   const int64_t tt = p.tpad / kLossTile, dt = (p.dpad + kLossTile - 1) / kLossTile;
   float* const dwpart = p.dwpart;
   for (int64_t vp = 0; vp < p.vocab; vp += p.vpiece) {
     p.vrows = loss_piece_rows(p, vp);
     const int64_t vt = p.vrows / kLossTile;
-    if (p.tokens <= kLossFew)
+    if (p.blocks)
       for_few(p.tokens, [&](auto nf) {
-        run(loss_few_grad_kernel<T, decltype(nf)::value>, p, p.vrows / kFewPart, 256, st, vp);
+        run(loss_few_grad_kernel<T, decltype(nf)::value>, p,
+            p.vrows / kFewPart * ((p.tokens + kLossFew - 1) / kLossFew), 256, st, vp);
       });
     else
       run(loss_grad_kernel<T>, p, vt * tt, 512, st, vp);
@@ -1231,7 +1248,7 @@ template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
 
 }  // namespace
 
-// The vocabulary piece: ds of one is at most 1 GiB, and of the sizes below that
+// The way, the vocabulary piece and the splits. The piece: its ds is at most 1 GiB, and of the sizes below that
 // give whole rounds of dweight's tiles, or equal pieces, the one that takes least.
 // Workspace, not time, grows with it otherwise.
 void loss_plan(LossParams& p) {
@@ -1263,6 +1280,11 @@ void loss_plan(LossParams& p) {
     if (us < 0.99f * least) least = us, best = vt;
   }
   p.vpiece = best * kLossTile;
+  // Blocks where all of them are on the GPU at once, two a CU: tiles of 256 x 256 would
+  // be on an eighth of it to a quarter. Forward and backward, us: 512 x 4096 x 2560 bf16
+  // 74 and 133 in tiles, 31 and 97 in blocks; 1024 x 8192 x 2560, twice what fits, 75 and
+  // 194, 67 and 196; 256 x 50280 x 768 44 and 135, 71 and 175.
+  p.blocks = p.tokens <= kLossFew || up(p.vocab, kFewPart) * up(p.tokens, kLossFew) <= kFewBlocks;
   p.htiles = std::max(dt * tt, std::min<int64_t>(kLossSplitTiles, kLossMostSplits * dt * tt));
   p.wsplit = std::max(loss_wsplit(p, 0), loss_wsplit(p, (all - 1) / best * p.vpiece));
 }

@@ -60,6 +60,7 @@ struct LossParams {
   int64_t vrows;      // of this piece, a multiple of 256, at most vpiece
   int64_t htiles;     // most tiles of 256 x 256 of dhidden's products, splits counted
   int wsplit;
+  int blocks;         // logits by blocks of 64 tokens and 128 vocabulary rows
   int few_lds;        // hidden's and weight's rows are 16-byte aligned
   int64_t first;      // this launch's first workgroup
 };
@@ -68,7 +69,9 @@ constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a 
 constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
 constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
 constexpr int kLossFew = 64;      // most tokens of a forward that streams the weight past them
-constexpr int kFewPart = 128;      // vocabulary rows of one maximum and sum there
+constexpr int kFewPart = 128;      // vocabulary rows of one maximum and sum of a block of 64 tokens: kLossPart
+static_assert(kLossPart == 128, "both ways leave the parts that one pass joins");
+constexpr int kFewBlocks = 512;    // most blocks of 64 tokens and 128 rows taken instead of tiles of 256 x 256
 constexpr int kLossMostSplits = 64;
 constexpr int64_t kLossSplitTiles = 1536;  // most results of a split product, of 256 KiB each
 constexpr int64_t kLossMaxK = 1024;

@@ -35,7 +35,8 @@ def _laid_size(hidden, weight, save):
     (tokens, dim), vocab = hidden.shape, weight.shape[0]
     wide = hidden.dtype == torch.float32
     stride = weight.stride(0) if weight.stride(1) == 1 or dim <= 1 else dim
-    if not save or tokens <= 64 or vocab == 0 or (
+    blocks = tokens <= 64 or -(-vocab // 128) * -(-tokens // 64) <= 512  # read in place too
+    if not save or blocks or (
             not wide and dim % 64 == 0 and stride % 8 == 0 and stride <= 2 ** 20):
         return 0
     return 256 + (vocab * -(-dim // 64) * 64 * (4 if wide else 2) + 255) // 256 * 256

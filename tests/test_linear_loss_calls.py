@@ -17,7 +17,7 @@ import torch
 import mamba_cpu
 from conftest import ROOT
 from oracle import loss as O
-from test_linear_loss import KEPT, OUT, U, check, inputs, logit_err, lse_tol, run_ce, teacher, verify_ce, verify_kd
+from test_linear_loss import KEPT, OUT, U, WAYS, check, inputs, logit_err, lse_tol, run_ce, teacher, verify_ce, verify_kd
 
 DEV = "cuda"
 
@@ -142,13 +142,13 @@ def test_forward_mode_raises(which):
 # ---- streams and graphs ----
 
 
-def _draw(seed, t=300, dtype=torch.bfloat16):
+def _draw(seed, t=300, dtype=torch.bfloat16, v=14000):
     g = torch.Generator(device=DEV).manual_seed(seed)
     h = torch.randn(t, 192, device=DEV, generator=g).to(dtype)
-    w = (torch.randn(700, 192, device=DEV, generator=g) / 14).to(dtype)
-    ids = torch.randint(700, (t,), device=DEV, generator=g)
+    w = (torch.randn(v, 192, device=DEV, generator=g) / 14).to(dtype)
+    ids = torch.randint(v, (t,), device=DEV, generator=g)
     ids[torch.rand(t, device=DEV, generator=g) < 0.1 * (seed % 7)] = -100  # another number of rows each time
-    top = torch.randint(-1, 700, (t, 6), device=DEV, generator=g)
+    top = torch.randint(-1, v, (t, 6), device=DEV, generator=g)
     return {"h": h, "w": w, "ids": ids, "top": top, "tl": torch.randn(t, 6, device=DEV, generator=g)}
 
 
@@ -163,9 +163,10 @@ def _step(d):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t,dtype", [(300, torch.bfloat16), (300, torch.float32), (20, torch.bfloat16)])
-def test_calls_replay_from_a_graph(t, dtype):
-    static = _draw(0, t, dtype)
+@pytest.mark.parametrize("t,v,dtype", [(300, 14000, torch.bfloat16), (300, 14000, torch.float32),
+                                       (20, 700, torch.bfloat16), (100, 700, torch.float32)])
+def test_calls_replay_from_a_graph(t, v, dtype):
+    static = _draw(0, t, dtype, v)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -177,12 +178,12 @@ def test_calls_replay_from_a_graph(t, dtype):
         outs = _step(static)
     torch.cuda.synchronize()
     for seed in (1, 2, 3, 4, 8):
-        for k, v in _draw(seed, t, dtype).items():
-            static[k].copy_(v)
+        for k, x in _draw(seed, t, dtype, v).items():
+            static[k].copy_(x)
         graph.replay()
         got = [x.clone() for x in outs]
         torch.cuda.synchronize()
-        want = _step(_draw(seed, t, dtype))
+        want = _step(_draw(seed, t, dtype, v))
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), seed
@@ -259,7 +260,7 @@ def test_vocabulary_in_pieces(dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [9, 80])
+@pytest.mark.parametrize("t", [9, 80])  # blocks, tiles
 def test_weight_past_4_gib(t):
     """2^31 elements and more of weight: the last rows' logits and gradients are as those of the rows by themselves."""
     d = 2048
@@ -290,13 +291,15 @@ def test_weight_past_4_gib(t):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [20, 70])
-def test_rows_far_apart(t):
-    """hidden's rows 2^26 elements apart, weight's 2^21: offsets past 32 bits, and rows the products cannot step over."""
-    h, w, ids, _ = inputs("bf16", t, 300, 64)
+@pytest.mark.parametrize("t,v", [(20, 300), (70, 300), (300, 14000)])
+def test_rows_far_apart(t, v):
+    """hidden's rows 2^26 (2^24) elements apart, weight's 2^21 (2^18): offsets past 32 bits, and rows the products
+    cannot step over."""
+    h, w, ids, _ = inputs("bf16", t, v, 64)
     want = run_ce("bf16", h, w, ids, "none", 1.0)
-    hs = torch.empty(t * 2 ** 26, device=DEV, dtype=torch.bfloat16).view(t, 2 ** 26)[:, :64]
-    ws = torch.empty(300 * 2 ** 21, device=DEV, dtype=torch.bfloat16).view(300, 2 ** 21)[:, :64]
+    far_h, far_w = (2 ** 26, 2 ** 21) if t < 100 else (2 ** 24, 2 ** 18)
+    hs = torch.empty(t * far_h, device=DEV, dtype=torch.bfloat16).view(t, far_h)[:, :64]
+    ws = torch.empty(v * far_w, device=DEV, dtype=torch.bfloat16).view(v, far_w)[:, :64]
     hs.copy_(h), ws.copy_(w)
     hs, ws = hs.detach().requires_grad_(), ws.detach().requires_grad_()
     loss, lse = mamba_cpu.linear_cross_entropy_fn(hs, ws, ids.to(DEV), reduction="none", return_lse=True)
@@ -306,10 +309,10 @@ def test_rows_far_apart(t):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [30, 90])
-def test_broadcast_hidden(t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_broadcast_hidden(t, v):
     """One row for all tokens, expanded: its gradient is the sum of theirs."""
-    h, w, ids, _ = inputs("f32", t, 300, 64)
+    h, w, ids, _ = inputs("f32", t, v, 64)
     one = h[:1].to(DEV).requires_grad_()
     wg = w.to(DEV)
     mamba_cpu.linear_cross_entropy_fn(one.expand(t, 64), wg, ids.to(DEV), reduction="sum").backward()
@@ -322,10 +325,10 @@ def test_broadcast_hidden(t):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t", [40, 100])
-def test_extreme_logits(dtype, t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_extreme_logits(dtype, t, v):
     """Logits of hundreds, targets far above all others (a loss of 0) and far below (a loss as large as the gap)."""
-    h, w, ids, g = inputs(dtype, t, 260, 64)
+    h, w, ids, g = inputs(dtype, t, v, 64)
     h = h * 64
     best = (h.double() @ w.double().t()).argmax(1)
     ids = torch.where(torch.arange(t) % 2 == 0, best, ids)
@@ -333,10 +336,10 @@ def test_extreme_logits(dtype, t):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [40, 100])
-def test_a_small_loss_keeps_its_digits(t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_a_small_loss_keeps_its_digits(t, v):
     """Targets 12 above the others: a loss of about 2e-3 or less, to the relative error of its own exponent."""
-    h, w, ids, _ = inputs("f32", t, 260, 64, seed=3)
+    h, w, ids, _ = inputs("f32", t, v, 64, seed=3)
     w = w / w.norm(dim=1, keepdim=True)
     h = 18 * w[ids] + 0.05 * h
     loss, _, _, _ = run_ce("f32", h, w, ids, "none", 1.0)
@@ -347,42 +350,42 @@ def test_a_small_loss_keeps_its_digits(t):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [40, 100])
-def test_float32_rows_of_unequal_size(t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_float32_rows_of_unequal_size(t, v):
     """Rows of hidden and weight over six powers of ten: float32 operands are scaled by their largest value."""
-    h, w, ids, g = inputs("f32", t, 260, 64)
+    h, w, ids, g = inputs("f32", t, v, 64)
     h = h * 10.0 ** (-6 * torch.rand(t, 1, generator=g))
-    w = w * 10.0 ** (-6 * torch.rand(260, 1, generator=g))
+    w = w * 10.0 ** (-6 * torch.rand(v, 1, generator=g))
     verify_ce("f32", h, w, ids, "none", g)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t", [40, 100])
-def test_constant_and_zero_operands(dtype, t):
-    h, w, ids, g = inputs(dtype, t, 260, 64)
+@pytest.mark.parametrize("t,v", WAYS)
+def test_constant_and_zero_operands(dtype, t, v):
+    h, w, ids, g = inputs(dtype, t, v, 64)
     verify_ce(dtype, torch.zeros_like(h), w, ids, "none", g)
     verify_ce(dtype, h, torch.zeros_like(w), ids, "none", g)
-    verify_kd(dtype, torch.zeros_like(h), w, *teacher(t, 260, 5, g), 1.0, "none", g)
+    verify_kd(dtype, torch.zeros_like(h), w, *teacher(t, v, 5, g), 1.0, "none", g)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [40, 100])
-def test_infinite_gradients_come_through(t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_infinite_gradients_come_through(t, v):
     """A loss scale that overflowed: inf or NaN out, for the scaler to see."""
-    h, w, ids, _ = inputs("f16", t, 260, 64)
+    h, w, ids, _ = inputs("f16", t, v, 64)
     _, _, dh, dw = run_ce("f16", h, w, ids, "mean", float("inf"))
     assert not torch.isfinite(dh).all(1).any() and not torch.isfinite(dw).all()
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t", [40, 100])
+@pytest.mark.parametrize("t,v", WAYS)
 @pytest.mark.parametrize("some", [True, False])
-def test_targets_far_above_under_a_loss_scale(dtype, t, some):
+def test_targets_far_above_under_a_loss_scale(dtype, t, v, some):
     """Targets 60 to 100 above all others, under a loss scale of 2^16: ds down to the end of float32's range, with and
     without a row of ordinary size beside."""
-    w = torch.eye(260, 64, dtype=torch.float64)
+    w = torch.eye(v, 64, dtype=torch.float64)
     ids = torch.arange(t) % 64
     h = torch.zeros(t, 64, dtype=torch.float64)
     h[torch.arange(t), ids] = torch.linspace(60, 100, t, dtype=torch.float64)
@@ -402,11 +405,11 @@ def test_targets_far_above_under_a_loss_scale(dtype, t, some):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t", [20, 70])
-def test_ids_past_32_bits_are_no_other_ids(t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_ids_past_32_bits_are_no_other_ids(t, v):
     """An id of 2^32 + v is outside the vocabulary, and is not v, whichever comes first."""
-    h, w, _, g = inputs("bf16", t, 300, 64)
-    ids, tl = teacher(t, 300, 6, g)
+    h, w, _, g = inputs("bf16", t, v, 64)
+    ids, tl = teacher(t, v, 6, g)
     wild = torch.cat([ids[:, :2] + 2 ** 32, ids, ids[:, 3:4] - 2 ** 32, torch.full_like(ids[:, :1], 2 ** 62)], 1)
     wide = torch.cat([torch.zeros(t, 2), tl, torch.full((t, 2), 9.0)], 1)
     outs = []
@@ -423,17 +426,17 @@ def test_ids_past_32_bits_are_no_other_ids(t):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("t", [20, 70, 300])
-def test_what_lies_around_the_operands(dtype, t):
+@pytest.mark.parametrize("t,v", WAYS)
+def test_what_lies_around_the_operands(dtype, t, v):
     """Operands in the middle of memory that holds NaN, where weight is read in place: nothing of it is read into a
     result."""
     key = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}[dtype]
-    h, w, ids, _ = inputs(key, t, 300, 64)
+    h, w, ids, _ = inputs(key, t, v, 64)
     want = run_ce(key, h, w, ids, "none", 1.0)
     hs = torch.full((t + 40, 192), float("nan"), dtype=dtype, device=DEV)
-    ws = torch.full((1000, 192), float("nan"), dtype=dtype, device=DEV)
-    hs[8:t + 8, 64:128], ws[200:500, 64:128] = h.to(DEV), w.to(DEV)
-    hv, wv = hs[8:t + 8, 64:128].detach().requires_grad_(), ws[200:500, 64:128].detach().requires_grad_()
+    ws = torch.full((v + 700, 192), float("nan"), dtype=dtype, device=DEV)
+    hs[8:t + 8, 64:128], ws[200:v + 200, 64:128] = h.to(DEV), w.to(DEV)
+    hv, wv = hs[8:t + 8, 64:128].detach().requires_grad_(), ws[200:v + 200, 64:128].detach().requires_grad_()
     loss, lse = mamba_cpu.linear_cross_entropy_fn(hv, wv, ids.to(DEV), reduction="none", return_lse=True)
     dh, dw = torch.autograd.grad(loss.sum(), [hv, wv])
     for a, b in zip((loss, lse, dh, dw), want):
@@ -441,9 +444,10 @@ def test_what_lies_around_the_operands(dtype, t):
 
 
 @pytest.mark.gpu
-def test_loss_scaled_float16():
+@pytest.mark.parametrize("t,v", WAYS)
+def test_loss_scaled_float16(t, v):
     """Gradients of 2^-14 a token under a scale of 2^14 and without: the same but for float16's smallest step."""
-    h, w, ids, _ = inputs("f16", 200, 300, 64)
+    h, w, ids, _ = inputs("f16", t, v, 64)
     _, _, dh, dw = run_ce("f16", h, w, ids, "sum", 1.0)
     _, _, sh, sw = run_ce("f16", h, w, ids, "sum", 2.0 ** -10)
     for a, b in ((dh, sh), (dw, sw)):
