@@ -685,31 +685,35 @@ __device__ __forceinline__ void finish_row(const LossParams& p, int64_t t, int64
   if (p.teacher != nullptr) p.each[t] = (p.cross[t] + lse) * p.temperature * p.temperature;
 }
 
-// 32 tokens a workgroup: eight threads a token join the parts, one takes the loss.
-__global__ __launch_bounds__(256) void loss_join_kernel(const LossParams p) {
-  __shared__ float ms[8][33], ss[8][33];
+// A thread's parts of one token, `step` apart: their maximum m and the sum s relative to it, eight loads on their way.
+__device__ __forceinline__ void join_parts(const float2* part, int64_t stride, int64_t first, int step, int64_t parts,
+                                           float c, float& m, float& s) {
+  for (int64_t q0 = first; q0 < parts; q0 += step * 8) {
+    float2 x[8];
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      x[u] = q0 + u * step < parts ? part[(q0 + u * step) * stride] : make_float2(-INFINITY, 0.f);
+      top = fmaxf(top, x[u].x);
+    }
+    const float sub = top == -INFINITY ? 0.f : top;
+    s *= fast_exp2((m - sub) * c);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s = fmaf(x[u].y, fast_exp2((x[u].x - sub) * c), s);
+    m = top;
+  }
+}
+
+// 32 tokens a workgroup: 32 threads a token join the parts, one takes the loss.
+__global__ __launch_bounds__(1024) void loss_join_kernel(const LossParams p) {
+  __shared__ float ms[32][33], ss[32][33];
   const int64_t kept = p.scal->kept;
   const int64_t i = (p.first + blockIdx.x) * 32 + (threadIdx.x & 31);
   const int slice = threadIdx.x >> 5;
   const int64_t parts = (p.vocab + kLossPart - 1) / kLossPart;
   const float c = kLog2e / p.temperature;
   float m = -INFINITY, s = 0.f;
-  if (i < kept) {
-    for (int64_t q0 = slice; q0 < parts; q0 += 64) {
-      float2 x[8];
-      float top = m;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        x[u] = q0 + u * 8 < parts ? p.part[(q0 + u * 8) * p.tpad + i] : make_float2(-INFINITY, 0.f);
-        top = fmaxf(top, x[u].x);
-      }
-      const float sub = top == -INFINITY ? 0.f : top;
-      s *= fast_exp2((m - sub) * c);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s = fmaf(x[u].y, fast_exp2((x[u].x - sub) * c), s);
-      m = top;
-    }
-  }
+  if (i < kept) join_parts(p.part + i, p.tpad, slice, 32, parts, c, m, s);
   ms[slice][threadIdx.x & 31] = m;
   ss[slice][threadIdx.x & 31] = s;
   __syncthreads();
@@ -722,10 +726,10 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const LossParams p) {
   }
   const int x = threadIdx.x;
   float top = ms[0][x];
-  for (int q = 1; q < 8; ++q) top = fmaxf(top, ms[q][x]);
+  for (int q = 1; q < 32; ++q) top = fmaxf(top, ms[q][x]);
   const float sub = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  for (int q = 0; q < 8; ++q) sum = fmaf(ss[q][x], fast_exp2((ms[q][x] - sub) * c), sum);
+  for (int q = 0; q < 32; ++q) sum = fmaf(ss[q][x], fast_exp2((ms[q][x] - sub) * c), sum);
   finish_row(p, t, i, top, sum, p.teacher == nullptr ? p.picked[i] : 0.f);
 }
 
@@ -967,7 +971,7 @@ __global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
   for (int q = 1; q < 4; ++q) m = fmaxf(m, parts[q][i].x);
   const float sub = m == -INFINITY ? 0.f : m;
   for (int q = 0; q < 4; ++q) s = fmaf(parts[q][i].y, fast_exp2((parts[q][i].x - sub) * c), s);
-  p.part[group * (ROWS ? p.tpad : kLossFew) + t0 + i] = make_float2(m, s);
+  p.part[group * (ROWS ? p.tpad : NF * 16) + t0 + i] = make_float2(m, s);
 }
 
 // ds of 64 of the rows that count a workgroup, as loss_grad_kernel; rows behind the last, up to whole 64, are zero.
@@ -1027,52 +1031,55 @@ template <typename F> void for_few(int64_t tokens, F&& f) {
     f(std::integral_constant<int, 4>{});
 }
 
-// The rows that count, their losses and all rows' of up to 64 tokens: one workgroup, 16 threads a token.
-__global__ __launch_bounds__(1024) void loss_few_join_kernel(const LossParams p) {
-  const int t = threadIdx.x >> 4, j = threadIdx.x & 15, n = static_cast<int>(p.tokens);
+// The rows that count, their losses and all rows' of up to NF x 16 tokens: one workgroup. A wave reads 512 bytes of
+// parts at a time, a token to every NF x 16 lanes: 7.3 us for 33 tokens and 393 parts, 9.6 with 32 bytes of a
+// token to each 16 threads.
+template <int NF> __global__ __launch_bounds__(1024) void loss_few_join_kernel(const LossParams p) {
+  constexpr int kWide = NF * 16, kSlices = 1024 / kWide;
+  const int n = static_cast<int>(p.tokens);
+  __shared__ float2 sums[kSlices][kWide + 1];
   __shared__ float losses[64];
   __shared__ unsigned long long mask;
   if (threadIdx.x < 64) {
     const unsigned long long m = __ballot(threadIdx.x < n && counts(p, threadIdx.x));
     if (threadIdx.x == 0) mask = m;
+    losses[threadIdx.x] = 0.f;
   }
-  __syncthreads();
-  const bool keep = mask >> t & 1;
-  const int kept = __popcll(mask), before = __popcll(mask & ((1ull << t) - 1));
   const int64_t parts = (p.vocab + kFewPart - 1) / kFewPart;
   const float c = kLog2e / p.temperature;
-  float m = -INFINITY, s = 0.f;
-  if (keep)
-    for (int64_t q0 = j; q0 < parts; q0 += 128) {
-      float2 x[8];
-      float top = m;
+  {
+    const int t = threadIdx.x % kWide, slice = threadIdx.x / kWide;
+    float m = -INFINITY, s = 0.f;
+    if (t < n) join_parts(p.part + t, kWide, slice, kSlices, parts, c, m, s);
+    sums[slice][t] = make_float2(m, s);
+  }
+  __syncthreads();
+  // 16 threads a token.
+  const int t = threadIdx.x >> 4, j = threadIdx.x & 15;
+  const bool keep = mask >> t & 1;
+  const int kept = __popcll(mask), before = __popcll(mask & ((1ull << t) - 1));
+  if (t < n) {
+    float m = -INFINITY, s = 0.f;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        x[u] = q0 + 16 * u < parts ? p.part[(q0 + 16 * u) * kLossFew + t] : make_float2(-INFINITY, 0.f);
-        top = fmaxf(top, x[u].x);
+    for (int q = j; q < kSlices; q += 16) m = fmaxf(m, sums[q][t].x);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float sub = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int q = j; q < kSlices; q += 16) s = fmaf(sums[q][t].y, fast_exp2((sums[q][t].x - sub) * c), s);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+    if (j == 0) {
+      if (keep) {
+        finish_row(p, t, before, m, s, p.teacher == nullptr ? p.picked[t] : 0.f);
+      } else {
+        p.lse[t] = 0.f;
+        p.each[t] = 0.f;
       }
-      const float sub = top == -INFINITY ? 0.f : top;
-      s *= fast_exp2((m - sub) * c);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s = fmaf(x[u].y, fast_exp2((x[u].x - sub) * c), s);
-      m = top;
+      p.rows[keep ? before : kept + t - before] = t;
+      losses[t] = p.each[t];
+      if (t == 0) p.rows[n] = kept;
     }
-  float top = m;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  s *= fast_exp2((m - (top == -INFINITY ? 0.f : top)) * c);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-  if (j == 0) {
-    if (keep) {
-      finish_row(p, t, before, top, s, p.teacher == nullptr ? p.picked[t] : 0.f);
-    } else if (t < n) {
-      p.lse[t] = 0.f;
-      p.each[t] = 0.f;
-    }
-    if (t < n) p.rows[keep ? before : kept + t - before] = t;
-    losses[t] = t < n ? p.each[t] : 0.f;
-    if (t == 0) p.rows[n] = kept;
   }
   if (p.reduction == MCPU_REDUCE_NONE) return;
   __syncthreads();
@@ -1199,8 +1206,8 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
     for_few(p.tokens, [&](auto nf) {
       run(loss_few_kernel<T, decltype(nf)::value, false>, p,
           (p.vocab + kFewPart - 1) / kFewPart + (p.teacher != nullptr ? p.tokens : 0), 256, st);
+      run(loss_few_join_kernel<decltype(nf)::value>, p, 1, 1024, st);
     });
-    run(loss_few_join_kernel, p, 1, 1024, st);
     return hipGetLastError();
   }
   if (p.teacher != nullptr) run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
@@ -1212,7 +1219,7 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
     lay_operands<T>(p, true, st);
     run(loss_logits_kernel<T>, p, (p.vocab + kLossTile - 1) / kLossTile * (p.tpad / kLossTile), 512, st);
   }
-  run(loss_join_kernel, p, (p.tokens + 31) / 32, 256, st);
+  run(loss_join_kernel, p, (p.tokens + 31) / 32, 1024, st);
   if (p.reduction != MCPU_REDUCE_NONE) run(loss_sum_kernel, p, 1, 1024, st);
   return hipGetLastError();
 }
