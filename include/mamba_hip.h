@@ -803,7 +803,8 @@ typedef struct mcpu_linear_loss_args {
   void* dweight;            /* (vocab, dim), optional */
 } mcpu_linear_loss_args;
 
-/* 0 where weight is read in place (16-bit, whole groups of 64 columns, 16-byte aligned) or tokens are few. */
+/* 0 where weight is read in place: 16-bit, whole groups of 64 columns, rows 16-byte aligned and at most 2^20
+ * elements apart; or up to 64 tokens, or 512 blocks of 64 tokens and 128 vocabulary rows. */
 size_t mcpu_linear_loss_laid_size(const mcpu_linear_loss_args* a);
 size_t mcpu_linear_loss_fwd_workspace_size(const mcpu_linear_loss_args* a);
 int mcpu_linear_loss_fwd(const mcpu_linear_loss_args* a, void* workspace, size_t workspace_bytes, void* stream);

@@ -125,7 +125,7 @@ size_t lay_fwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   if (distil(a)) w.take(p.cross, p.tokens);
   if (!distil(a)) w.take(p.picked, p.tpad);
   if (p.tokens <= kLossFew) {
-    w.take(p.part, (p.vocab + kFewPart - 1) / kFewPart * kLossFew);
+    w.take(p.part, (p.vocab + kLossPart - 1) / kLossPart * kLossFew);
     return w.used;
   }
   if (p.blocks)

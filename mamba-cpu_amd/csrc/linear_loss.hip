@@ -9,16 +9,25 @@
 //   a = g + e, b = g (cross entropy, q = 1);  a = b = g / c (distillation)
 //   dhidden = ds weight,  dweight = ds^T hidden.
 //
-// Forward: rows that count are gathered, then one product whose epilogue keeps
-// a maximum and a sum of 128 vocabulary rows per token, then one pass that joins
-// these. A target's logit is taken from the product; the products of hidden with a
-// teacher's ids are formed by themselves.
+// Forward: one product of the rows that count, whose epilogue keeps a maximum and a
+// sum of 128 vocabulary rows per token, then one pass that joins these. A target's
+// logit is taken from the product, and out of its sums: a loss near 0 then has its
+// digits. The products of hidden with a teacher's ids are formed by themselves.
 // Backward: a piece of the vocabulary at a time, the product again, now with ds in
 // 16 bits as its result (float32: two f16 pieces), the ids' places put right, and
 // the two products of the gradients over it. Rows that do not count take part in
 // no product, so nothing in them, NaN included, reaches another row.
 //
-// Everything is summed in float32 in an order that depends on the sizes alone.
+// Three ways to the logits, by how many tiles there are:
+//   tiles of 256 x 256     bound by the matrix cores at the clock that power leaves
+//                          them: 16384 x 50280 x 768 bf16 1.13-1.25 ms, 1010-1120 TFLOP/s
+//   blocks of 64 x 128     up to 512 of them, where tiles would not fill the GPU
+//   up to 64 tokens        the same kernel on the rows as they come and one more that does the
+//                          rest: bound by reading weight, 4.4 TB/s
+// loss_plan has the rule and both sides. The gradients' products are tiles always.
+//
+// Everything is summed in float32, in an order that depends on the sizes and on the
+// number of rows that count alone: no atomics add.
 #include "launch.h"
 #include "lm_math.h"
 #include "tile_product.h"
@@ -359,7 +368,8 @@ __device__ __forceinline__ int rows_left(const LossParams& p, int64_t v0, int la
 template <typename T> __global__ __launch_bounds__(512, 2) void loss_logits_kernel(const LossParams p) {
   const int64_t kept = p.scal->kept;
   int64_t mt, nt;
-  if (!tile_of(p.first + blockIdx.x, (p.vocab + kLossTile - 1) / kLossTile, (kept + kLossTile - 1) / kLossTile, mt, nt)) return;
+  const int64_t mts = (p.vocab + kLossTile - 1) / kLossTile, nts = (kept + kLossTile - 1) / kLossTile;
+  if (!tile_of(p.first + blockIdx.x, mts, nts, mt, nt)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t v0 = mt * kLossTile + (wave >> 2) * kLossPart, t0 = nt * kLossTile + (wave & 3) * 64 + (lane & 31);
   // What the epilogue needs is on its way before the product.
@@ -733,10 +743,10 @@ __global__ __launch_bounds__(1024) void loss_join_kernel(const LossParams p) {
   finish_row(p, t, i, top, sum, p.teacher == nullptr ? p.picked[i] : 0.f);
 }
 
-// ---- few tokens ------------------------------------------------------------------------------------
+// ---- few tokens, and blocks --------------------------------------------------------------------------
 
-// Up to 64 tokens: the weight streams past them once, 32 vocabulary rows a wave and
-// 128 a workgroup, so that what bounds it is HBM. A lane's part of an operand is row
+// Up to 64 tokens a workgroup, past which 128 vocabulary rows stream, 32 a wave. With
+// 64 in all every row is read once, and what bounds it is HBM. A lane's part of an operand is row
 // l % 16 and the 16 bytes at l / 16 of each 64, the same terms for both operands.
 // float32 goes through v_mfma_f32_16x16x4_f32, four to 16 bytes.
 typedef uint32_t u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -924,13 +934,13 @@ __global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
   const int64_t teachers = !ROWS && p.teacher != nullptr ? p.tokens : 0;
   const int64_t at = p.first + blockIdx.x - teachers;
   if (at < 0) return teacher_row<T, 256>(p, at + teachers);
-  const int64_t groups = (p.vocab + kFewPart - 1) / kFewPart;
+  const int64_t groups = (p.vocab + kLossPart - 1) / kLossPart;
   const int64_t group = ROWS ? at % groups : at, t0 = ROWS ? at / groups * kLossFew : 0;
   const int64_t tokens = ROWS ? p.scal->kept : p.tokens;
   if (t0 >= tokens) return;
   __shared__ float2 parts[4][NF * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t v0 = group * kFewPart + wave * 32;
+  const int64_t v0 = group * kLossPart + wave * 32;
   auto row = [&](int64_t t) { return ROWS ? int64_t{p.rows[t]} : t; };
   f32x4 acc[2][NF];
   few_products<T, NF>(p, [&](int64_t i) {  // a token that is not there is read as the last
@@ -975,11 +985,12 @@ __global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
 }
 
 // ds of 64 of the rows that count a workgroup, as loss_grad_kernel; rows behind the last, up to whole 64, are zero.
-template <typename T, int NF> __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
+template <typename T, int NF>
+__global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams p, int64_t vp) {
   using E = Kept<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t at = p.first + blockIdx.x, groups = p.vrows / kFewPart, t0 = at / groups * kLossFew;
-  const int64_t vl = at % groups * kFewPart + wave * 32, v0 = vp + vl;
+  const int64_t at = p.first + blockIdx.x, groups = p.vrows / kLossPart, t0 = at / groups * kLossFew;
+  const int64_t vl = at % groups * kLossPart + wave * 32, v0 = vp + vl;
   const int64_t kept = p.scal->kept;
   if (t0 >= kept) return;
   f32x4 acc[2][NF];
@@ -1045,7 +1056,7 @@ template <int NF> __global__ __launch_bounds__(1024) void loss_few_join_kernel(c
     if (threadIdx.x == 0) mask = m;
     losses[threadIdx.x] = 0.f;
   }
-  const int64_t parts = (p.vocab + kFewPart - 1) / kFewPart;
+  const int64_t parts = (p.vocab + kLossPart - 1) / kLossPart;
   const float c = kLog2e / p.temperature;
   {
     const int t = threadIdx.x % kWide, slice = threadIdx.x / kWide;
@@ -1205,7 +1216,7 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   if (p.tokens <= kLossFew) {
     for_few(p.tokens, [&](auto nf) {
       run(loss_few_kernel<T, decltype(nf)::value, false>, p,
-          (p.vocab + kFewPart - 1) / kFewPart + (p.teacher != nullptr ? p.tokens : 0), 256, st);
+          (p.vocab + kLossPart - 1) / kLossPart + (p.teacher != nullptr ? p.tokens : 0), 256, st);
       run(loss_few_join_kernel<decltype(nf)::value>, p, 1, 1024, st);
     });
     return hipGetLastError();
@@ -1213,8 +1224,8 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
   if (p.teacher != nullptr) run(loss_teacher_kernel<T>, p, p.tokens, 256, st);
   run(loss_rows_kernel, p, 1, 1024, st);
   if (p.blocks) {
-    run(loss_few_kernel<T, 4, true>, p, (p.vocab + kFewPart - 1) / kFewPart * ((p.tokens + kLossFew - 1) / kLossFew), 256,
-        st);
+    run(loss_few_kernel<T, 4, true>, p,
+        (p.vocab + kLossPart - 1) / kLossPart * ((p.tokens + kLossFew - 1) / kLossFew), 256, st);
   } else {
     lay_operands<T>(p, true, st);
     run(loss_logits_kernel<T>, p, (p.vocab + kLossTile - 1) / kLossTile * (p.tpad / kLossTile), 512, st);
@@ -1236,7 +1247,7 @@ template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
     if (p.blocks)
       for_few(p.tokens, [&](auto nf) {
         run(loss_few_grad_kernel<T, decltype(nf)::value>, p,
-            p.vrows / kFewPart * ((p.tokens + kLossFew - 1) / kLossFew), 256, st, vp);
+            p.vrows / kLossPart * ((p.tokens + kLossFew - 1) / kLossFew), 256, st, vp);
       });
     else
       run(loss_grad_kernel<T>, p, vt * tt, 512, st, vp);
@@ -1291,7 +1302,7 @@ void loss_plan(LossParams& p) {
   // be on an eighth of it to a quarter. Forward and backward, us: 512 x 4096 x 2560 bf16
   // 74 and 133 in tiles, 31 and 97 in blocks; 1024 x 8192 x 2560, twice what fits, 75 and
   // 194, 67 and 196; 256 x 50280 x 768 44 and 135, 71 and 175.
-  p.blocks = p.tokens <= kLossFew || up(p.vocab, kFewPart) * up(p.tokens, kLossFew) <= kFewBlocks;
+  p.blocks = p.tokens <= kLossFew || up(p.vocab, kLossPart) * up(p.tokens, kLossFew) <= kLossBlocks;
   p.htiles = std::max(dt * tt, std::min<int64_t>(kLossSplitTiles, kLossMostSplits * dt * tt));
   p.wsplit = std::max(loss_wsplit(p, 0), loss_wsplit(p, (all - 1) / best * p.vpiece));
 }
@@ -1302,8 +1313,8 @@ int64_t loss_piece_rows(const LossParams& p, int64_t vp) {
 }
 int loss_wsplit(const LossParams& p, int64_t vp) {
   const int64_t dt = (p.dpad + kLossTile - 1) / kLossTile;
-  return splits_for(dt * (loss_piece_rows(p, vp) / kLossTile), p.tpad / kLossDepth * (loss_pieces(p.dtype) == 2 ? 3 : 1),
-                    false);
+  return splits_for(dt * (loss_piece_rows(p, vp) / kLossTile),
+                    p.tpad / kLossDepth * (loss_pieces(p.dtype) == 2 ? 3 : 1), false);
 }
 
 hipError_t loss_zero(void* at, int64_t bytes, hipStream_t st) {

@@ -33,7 +33,8 @@ struct LossParams {
   float* lse;     // (tokens)
   float* picked;  // distillation: (tokens, k), the products of hidden with the ids' rows; else workspace, (padded
                   // tokens), the targets' in the order of `rows` (few tokens: as they come)
-  float* stat;    // (4, tokens) in the order of `rows`: maximum, sum of exp(c (s - it)), a target's share of it, the others'
+  float* stat;    // (4, tokens) in the order of `rows`: maximum, sum of exp(c (s - it)), a target's share of it,
+                  // the others'
   float* share;   // (tokens, k): the teacher's distribution, or null
   int32_t* rows;  // (tokens + 1): the rows that count in order, then the others; then how many count
   uint32_t* laid;      // float32: wmax beside wrows, where both are kept for the backward; or null
@@ -47,12 +48,13 @@ struct LossParams {
   uint8_t* keep;      // (tokens)
   int32_t* target;    // (padded tokens) in the order of `rows`, cross entropy; else null
   float* cross;       // (tokens): sum of q (log q - c s)
-  float2* part;       // (vocab parts, padded tokens): maximum of each part and sum of exp(c (s - it))
+  float2* part;       // (vocab parts, padded tokens; few tokens: whole 16, 32 or 64): maximum of each part and
+                      // sum of exp(c (s - it))
   float* coef;        // (4, padded tokens): factor of 2^(logit - maximum), the target's ds or the shares' factor,
                       // the maximum, the unit of ds (0: the largest)
   void* hrows;        // (pieces, padded tokens, padded dim): hidden's rows that count
   void* hscaled;      // hrows in the largest unit, or null: hrows has it (distillation)
-  void* wrows;        // (pieces, vocab, padded dim), or null: weight is read in place
+  void* wrows;        // (pieces, vocab, padded dim), which may be of `laid`, or null: weight is read in place
   void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits
   float* acc;         // (splits, rows that count, padded, padded dim): gradient of hidden
   float* dwpart;      // (splits, vocab piece, padded dim), or null: gradient of weight in one go
@@ -67,11 +69,9 @@ struct LossParams {
 
 constexpr int kLossTile = 256;   // rows and columns of a workgroup's tile of a product
 constexpr int kLossDepth = 64;   // terms of a tile that are in LDS at once
-constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum
-constexpr int kLossFew = 64;      // most tokens of a forward that streams the weight past them
-constexpr int kFewPart = 128;      // vocabulary rows of one maximum and sum of a block of 64 tokens: kLossPart
-static_assert(kLossPart == 128, "both ways leave the parts that one pass joins");
-constexpr int kFewBlocks = 512;    // most blocks of 64 tokens and 128 rows taken instead of tiles of 256 x 256
+constexpr int kLossPart = 128;   // vocabulary rows of one maximum and sum, and of a block
+constexpr int kLossFew = 64;     // tokens of a block; up to so many in all, the weight streams past them
+constexpr int kLossBlocks = 512;  // most blocks taken instead of tiles
 constexpr int kLossMostSplits = 64;
 constexpr int64_t kLossSplitTiles = 1536;  // most results of a split product, of 256 KiB each
 constexpr int64_t kLossMaxK = 1024;

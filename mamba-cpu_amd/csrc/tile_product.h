@@ -65,7 +65,8 @@ constexpr int kTileBytes = kLossTile * kLossDepth * 2;
 // Where an operand's tile of one depth begins, as a buffer that ends with the piece;
 // behind the last depth (not `any`) an empty one, whose loads leave zeros.
 template <bool TERM>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const Operand& o, int64_t row0, int64_t k0, bool second, bool any) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const Operand& o, int64_t row0, int64_t k0, bool second,
+                                                            bool any) {
   const int64_t at = TERM ? k0 * o.ld + row0 : row0 * o.ld + k0;
   const char* base = static_cast<const char*>(o.base) + 2 * (at + (second ? o.piece : 0));
   int64_t left = 2 * (o.span - at);

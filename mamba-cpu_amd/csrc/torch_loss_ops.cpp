@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/autograd.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
 #include <cstring>
@@ -75,7 +76,8 @@ Losses linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in, const T
       check_like(name, "the teacher's logits", *teacher, at::kFloat, ids.sizes(), hidden).data_ptr());
   const at::IntArrayRef all(&tokens, 1), one;
   Tensor loss = at::empty(reduction == MCPU_REDUCE_NONE ? all : one, f32), lse = at::empty({tokens}, f32);
-  Tensor picked = at::empty({has(teacher) ? tokens : 0, a.k}, f32), stat = at::empty({4, tokens}, f32), share = at::empty({has(teacher) ? tokens : 0, a.k}, f32);
+  Tensor picked = at::empty({has(teacher) ? tokens : 0, a.k}, f32), share = at::empty_like(picked);
+  Tensor stat = at::empty({4, tokens}, f32);
   Tensor rows = at::empty({tokens + 1}, hidden.options().dtype(at::kInt));
   a.loss = static_cast<float*>(loss.data_ptr());
   a.lse = static_cast<float*>(lse.data_ptr());
@@ -96,8 +98,9 @@ Losses linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in, const T
 std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const optional<Tensor>& dlse,
                                            const Tensor& hidden_in, const Tensor& weight_in, const Tensor& ids,
                                            const Tensor& picked, const Tensor& stat, const Tensor& share,
-                                           const Tensor& rows, const Tensor& laid, int64_t ignore_index, double temperature,
-                                           int64_t reduction, bool distil, bool want_hidden, bool want_weight) {
+                                           const Tensor& rows, const Tensor& laid, int64_t ignore_index,
+                                           double temperature, int64_t reduction, bool distil, bool want_hidden,
+                                           bool want_weight) {
   const char* name = "mamba_cpu::linear_loss_bwd";
   check_gpu(name, hidden_in);
   c10::DeviceGuard guard(hidden_in.device());
@@ -116,8 +119,9 @@ std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const 
       check_like(name, "rows", rows, at::kInt, at::IntArrayRef(&last, 1), hidden).data_ptr());
   const size_t kept = mcpu_linear_loss_laid_size(&a);
   if (laid.numel() > 0) {
-    TORCH_CHECK_VALUE(static_cast<size_t>(laid.numel()) == kept && laid.scalar_type() == at::kByte && laid.is_contiguous() &&
-                          laid.device() == hidden.device(), name, " expects the laid out weight that the forward left");
+    TORCH_CHECK_VALUE(static_cast<size_t>(laid.numel()) == kept && laid.scalar_type() == at::kByte &&
+                          laid.is_contiguous() && laid.device() == hidden.device(),
+                      name, " expects the laid out weight that the forward left");
     a.laid = laid.data_ptr();
   }
   Tensor g, e;
@@ -173,9 +177,9 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("mamba_cpu::linear_loss_bwd", "")
                          .typed<decltype(linear_loss_bwd)>();
-    auto r = op.call(g, opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["ignore"].toInt(),
-                     ctx->saved_data["temperature"].toDouble(), reduction, ctx->saved_data["distil"].toBool(),
-                     want_hidden, want_weight);
+    auto r = op.call(g, opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7],
+                     ctx->saved_data["ignore"].toInt(), ctx->saved_data["temperature"].toDouble(), reduction,
+                     ctx->saved_data["distil"].toBool(), want_hidden, want_weight);
     return {want_hidden ? std::get<0>(r) : Tensor(), want_weight ? std::get<1>(r) : Tensor(),
             Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -201,8 +205,8 @@ TORCH_LIBRARY_FRAGMENT(mamba_cpu, m) {
   m.def("linear_loss_fwd(Tensor hidden, Tensor weight, Tensor ids, Tensor? teacher, int ignore_index, "
         "float temperature, int reduction, bool save) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("linear_loss_bwd(Tensor? dloss, Tensor? dlse, Tensor hidden, Tensor weight, Tensor ids, Tensor picked, "
-        "Tensor stat, Tensor share, Tensor rows, Tensor laid, int ignore_index, float temperature, int reduction, bool distil, "
-        "bool want_hidden, bool want_weight) -> (Tensor, Tensor)");
+        "Tensor stat, Tensor share, Tensor rows, Tensor laid, int ignore_index, float temperature, int reduction, "
+        "bool distil, bool want_hidden, bool want_weight) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
@@ -214,4 +218,6 @@ TORCH_LIBRARY_IMPL(mamba_cpu, CUDA, m) {
 TORCH_LIBRARY_IMPL(mamba_cpu, Autograd, m) {
   using namespace mcpu_torch;
   m.impl("linear_loss_fwd", &linear_loss_autograd);
+  // A gradient of the gradient raises.
+  m.impl("linear_loss_bwd", torch::autograd::autogradNotImplementedFallback());
 }

@@ -88,8 +88,8 @@ def check_grads(dtype, h, w, ds, ltol, dh, dw):
     if dw is not None:
         live = (ds != 0).any(1)[:, None]
         check("dweight", dw, want_w,
-              (e + KEPT[dtype] + ds.shape[0] * U) * (mag.T @ (hd * live)) + low * (hd * live).sum(0) + OUT[dtype] * np.abs(want_w)
-              + floor)
+              (e + KEPT[dtype] + ds.shape[0] * U) * (mag.T @ (hd * live)) + low * (hd * live).sum(0)
+              + OUT[dtype] * np.abs(want_w) + floor)
 
 
 def run_ce(dtype, h, w, ids, reduction, dloss, dlse=None, ignore_index=-100):
@@ -130,10 +130,10 @@ def verify_ce(dtype, h, w, ids, reduction="none", g=None, dlse=None, ignore_inde
 # The ways through the kernels, by tokens and vocabulary: up to 64 tokens; blocks of 64 tokens and 128 rows up to 512 of
 # them; tiles of 256 x 256. WAYS has one of each.
 WAYS = [(40, 260), (100, 260), (1100, 4000)]
-SIZES = [(1, 2, 1), (1, 300, 8), (2, 128, 64), (5, 129, 65), (64, 257, 200), (255, 200, 77), (256, 256, 64),
-         (257, 513, 128), (300, 1000, 192), (513, 70, 320), (40, 3001, 33), (700, 6600, 72), (129, 33000, 64),
-         (1030, 4200, 33), (520, 8192, 256),
-         (16, 260, 129), (17, 31, 1000), (32, 511, 512), (65, 130, 520)]
+SIZES = [(1, 1, 8), (66, 1, 70), (1, 2, 1), (1, 300, 8), (2, 128, 64), (5, 129, 65), (64, 257, 200), (255, 200, 77),
+         (256, 256, 64), (257, 513, 128), (300, 1000, 192), (513, 70, 320), (40, 3001, 33), (700, 6600, 72),
+         (129, 33000, 64), (1030, 4200, 33), (520, 8192, 256), (16, 260, 129), (17, 31, 1000), (32, 511, 512),
+         (65, 130, 520)]
 
 
 @pytest.mark.gpu

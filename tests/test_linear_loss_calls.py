@@ -17,7 +17,8 @@ import torch
 import mamba_cpu
 from conftest import ROOT
 from oracle import loss as O
-from test_linear_loss import KEPT, OUT, U, WAYS, check, inputs, logit_err, lse_tol, run_ce, teacher, verify_ce, verify_kd
+from test_linear_loss import (KEPT, OUT, U, WAYS, check, inputs, logit_err, lse_tol, run_ce, teacher, verify_ce,
+                              verify_kd)
 
 DEV = "cuda"
 
@@ -61,7 +62,8 @@ def _block(**kw):
     (dict(temperature=2.0), False), (dict(k=2), False), (dict(share=4096, dlse=4096), False),
     (dict(tokens=2 ** 26 + 1), True), (dict(vocab=2 ** 24 + 1), True), (dict(dim=2 ** 20 + 1), True),
     (dict(share=4096, teacher=4096, k=1025), True), (dict(hidden=0), False), (dict(weight=0), False),
-    (dict(ids=0), False), (dict(stat=0), False), (dict(rows=0), False), (dict(share=4096, teacher=4096, picked=0), False)])
+    (dict(ids=0), False), (dict(stat=0), False), (dict(rows=0), False),
+    (dict(share=4096, teacher=4096, picked=0), False)])
 def test_bad_blocks_are_refused_before_a_device_is_touched(kw, unsupported):
     from mamba_cpu import _C
 
@@ -118,7 +120,8 @@ def test_shape_functions_follow_the_operators():
         assert kd.shape == (3, 5)
         dh, dw = torch.ops.mamba_cpu.linear_loss_bwd(
             None, None, h.view(15, 8), w, ids.view(15, 1), kd.new_empty(0, 1), kd.new_empty(4, 15),
-            kd.new_empty(0, 1), ids.new_empty(16, dtype=torch.int32), kd.new_empty(0, dtype=torch.uint8), -100, 1.0, 0, False, True, True)
+            kd.new_empty(0, 1), ids.new_empty(16, dtype=torch.int32), kd.new_empty(0, dtype=torch.uint8), -100, 1.0, 0,
+            False, True, True)
         assert dh.shape == (15, 8) and dw.shape == (11, 8) and dh.dtype == dw.dtype == torch.bfloat16
 
 
@@ -137,6 +140,21 @@ def test_forward_mode_raises(which):
         if which != "teacher":
             with pytest.raises((RuntimeError, NotImplementedError)):
                 mamba_cpu.linear_cross_entropy_fn(t["hidden"], t["weight"], ids[:, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["ce", "kd"])
+def test_a_second_gradient_is_refused(op):
+    h, w, ids, g = inputs("f32", 20, 50, 32)
+    hh, ww = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    if op == "ce":
+        loss = mamba_cpu.linear_cross_entropy_fn(hh, ww, ids.to(DEV))
+    else:
+        loss = mamba_cpu.linear_distillation_fn(hh, ww, *(x.to(DEV) for x in teacher(20, 50, 4, g)))
+    dh, dw = torch.autograd.grad(loss, [hh, ww], create_graph=True)
+    for d in (dh, dw):
+        with pytest.raises(RuntimeError, match="not implemented"):
+            torch.autograd.grad(d.sum(), [hh], retain_graph=True)
 
 
 # ---- streams and graphs ----
