@@ -9,11 +9,17 @@ Per token, with s = hidden @ weight.T formed in float32:
     distillation    q = softmax(teacher / T) over the teacher's entries,
                     loss = T^2 sum_k q_k (log q_k - log softmax(s / T)_id_k)
 
-Products are of hidden and weight as given, summed in float32 (float32 operands:
-as two float16 pieces each, which keep 22 bits of a value and 2^-38 of the
-tensor's largest). The logits' gradients are rounded once to the operands' type
-(float32: to 22 bits) before the products over them; the results' sums are
-float32, rounded once, in an order that does not change from call to call.
+Products are of hidden and weight as given, summed in float32 (many tokens of
+float32: as two float16 pieces each, which keep 22 bits of a value and 2^-38 of
+the tensor's largest). hidden and weight of different types, or of others than
+float32, bfloat16 and float16, go as float32. The logits' gradients are rounded once
+to the operands' type (float32: to 22 bits) before the products over them; the
+results' sums are float32, rounded once, in an order that does not change from
+call to call.
+
+Between forward and backward a call keeps a few numbers a token and, where the
+kernels do not read weight as it lies (float32, or 16 bits with a number of columns
+that is no multiple of 64 or rows that are not 16-byte aligned), a copy of it.
 """
 
 import torch
