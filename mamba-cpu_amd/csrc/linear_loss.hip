@@ -792,7 +792,7 @@ template <int NF> constexpr int kStageBytes = (128 + NF * 16) * 128;
 template <typename T, int NF, typename Row>
 __device__ __forceinline__ int64_t few_products_lds(const LossParams& p, Row&& row, int64_t v0,
                                                     f32x4 (&acc)[2][2][NF]) {
-  constexpr int kHidden = NF == 4 ? 2 : 1, kLoads = 4 + kHidden;
+  constexpr int kHidden = NF > 2 ? 2 : 1, kLoads = 4 + kHidden;
   constexpr int kTerms = 128 / static_cast<int>(sizeof(T));
   __shared__ __attribute__((aligned(1024))) char s0[kStageBytes<NF>];
   __shared__ __attribute__((aligned(1024))) char s1[kStageBytes<NF>];
@@ -801,7 +801,7 @@ __device__ __forceinline__ int64_t few_products_lds(const LossParams& p, Row&& r
   const int groups = static_cast<int>(p.dim / kTerms);
   if (groups == 0) return 0;
   // A lane's 16 bytes of eight rows a load: four loads of the wave's own rows of
-  // weight, and its share of hidden's (of 16 tokens, waves 2 and 3 bring what 0 and 1 do).
+  // weight, and its share of hidden's (of 16 tokens, and of the last 16 of 48, waves 2 and 3 bring what 0 and 1 do).
   const int r8 = lane >> 3, swap = ((lane & 7) ^ r8) * (16 / static_cast<int>(sizeof(T)));
   const T* from[kLoads];
   int to[kLoads];
@@ -813,7 +813,7 @@ __device__ __forceinline__ int64_t few_products_lds(const LossParams& p, Row&& r
   }
 #pragma unroll
   for (int i = 0; i < kHidden; ++i) {
-    const int t8 = NF == 1 ? wave & 1 : wave * kHidden + i;
+    const int t8 = NF == 1 ? wave & 1 : NF == 3 && i == 1 ? 4 + (wave & 1) : wave + 4 * i;
     from[4 + i] = row(8 * t8 + r8) + swap;
     to[4 + i] = (128 + 8 * t8) * 128;
   }
@@ -924,6 +924,9 @@ __device__ __forceinline__ void few_products(const LossParams& p, Row&& row, int
       for (int e = 0; e < 4; ++e) s[i][j][e] = acc[0][i][j][e] + acc[1][i][j][e];
 }
 
+// Tokens that a row of parts of NF groups has room for: 16, 32 or 64.
+constexpr int few_wide(int groups) { return groups > 2 ? 64 : groups * 16; }
+
 // NF x 16 tokens and 128 vocabulary rows a workgroup, and of these one maximum and sum a token.
 // Up to 64 tokens in all (not ROWS), as they come; distillation: one more workgroup a
 // token, first, for the teacher's part, which would take 10 us before or after.
@@ -981,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void loss_few_kernel(const LossParams p) {
   for (int q = 1; q < 4; ++q) m = fmaxf(m, parts[q][i].x);
   const float sub = m == -INFINITY ? 0.f : m;
   for (int q = 0; q < 4; ++q) s = fmaf(parts[q][i].y, fast_exp2((parts[q][i].x - sub) * c), s);
-  p.part[group * (ROWS ? p.tpad : NF * 16) + t0 + i] = make_float2(m, s);
+  p.part[group * (ROWS ? p.tpad : few_wide(NF)) + t0 + i] = make_float2(m, s);
 }
 
 // ds of 64 of the rows that count a workgroup, as loss_grad_kernel; rows behind the last, up to whole 64, are zero.
@@ -1032,21 +1035,24 @@ __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams 
   }
 }
 
-// As f<16-token groups>() for up to 64 tokens.
+// As f<16-token groups>() for up to 64 tokens. 33 tokens as three groups, not four: 148 against 185 us for
+// 50280 x 2560 float32, 64 against 65.5 in bf16.
 template <typename F> void for_few(int64_t tokens, F&& f) {
   if (tokens <= 16)
     f(std::integral_constant<int, 1>{});
   else if (tokens <= 32)
     f(std::integral_constant<int, 2>{});
+  else if (tokens <= 48)
+    f(std::integral_constant<int, 3>{});
   else
     f(std::integral_constant<int, 4>{});
 }
 
-// The rows that count, their losses and all rows' of up to NF x 16 tokens: one workgroup. A wave reads 512 bytes of
-// parts at a time, a token to every NF x 16 lanes: 7.3 us for 33 tokens and 393 parts, 9.6 with 32 bytes of a
+// The rows that count, their losses and all rows' of up to kWide tokens: one workgroup. A wave reads 512 bytes of
+// parts at a time, a token to every kWide lanes: 7.3 us for 33 tokens and 393 parts, 9.6 with 32 bytes of a
 // token to each 16 threads.
-template <int NF> __global__ __launch_bounds__(1024) void loss_few_join_kernel(const LossParams p) {
-  constexpr int kWide = NF * 16, kSlices = 1024 / kWide;
+template <int kWide> __global__ __launch_bounds__(1024) void loss_few_join_kernel(const LossParams p) {
+  constexpr int kSlices = 1024 / kWide;
   const int n = static_cast<int>(p.tokens);
   __shared__ float2 sums[kSlices][kWide + 1];
   __shared__ float losses[64];
@@ -1217,7 +1223,7 @@ template <typename T> hipError_t fwd(const LossParams& p, hipStream_t st) {
     for_few(p.tokens, [&](auto nf) {
       run(loss_few_kernel<T, decltype(nf)::value, false>, p,
           (p.vocab + kLossPart - 1) / kLossPart + (p.teacher != nullptr ? p.tokens : 0), 256, st);
-      run(loss_few_join_kernel<decltype(nf)::value>, p, 1, 1024, st);
+      run(loss_few_join_kernel<few_wide(decltype(nf)::value)>, p, 1, 1024, st);
     });
     return hipGetLastError();
   }
@@ -1268,7 +1274,7 @@ template <typename T> hipError_t bwd(LossParams p, hipStream_t st) {
 
 // The way, the vocabulary piece and the splits. The piece: its ds is at most 1 GiB, and of the sizes below that
 // give whole rounds of dweight's tiles, or equal pieces, the one that takes least.
-// Workspace, not time, grows with it otherwise.
+// Twice as much would gain 1 % (16384 x 50280 x 768) to 3 % (32768), at 2560 columns nothing.
 void loss_plan(LossParams& p) {
   const int pieces = loss_pieces(p.dtype), runs = pieces == 2 ? 3 : 1;
   auto up = [](int64_t n, int64_t to) { return (n + to - 1) / to; };

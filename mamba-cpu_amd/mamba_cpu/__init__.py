@@ -7,7 +7,8 @@ Mamba-1 mixer over them (transformers' training path). `mamba_cpu.hf.patch_trans
 routes Hugging Face Mamba / FalconMamba / Jamba / Mamba-2 models on the GPU to them.
 
 Beside the scans: the gated linear recurrence (`gated_linear_scan_fn`, `gated_linear_update`),
-`layer_norm_fn`, `embedding_fn` and `sample_fn`, which `mamba_cpu.recurrent_lm` puts together.
+`layer_norm_fn`, `embedding_fn`, `sample_fn` and the losses of a head without its logits
+(`linear_cross_entropy_fn`, `linear_distillation_fn`), which `mamba_cpu.recurrent_lm` puts together.
 """
 
 from mamba_cpu.ops import (

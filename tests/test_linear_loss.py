@@ -133,7 +133,7 @@ WAYS = [(40, 260), (100, 260), (1100, 4000)]
 SIZES = [(1, 1, 8), (66, 1, 70), (1, 2, 1), (1, 300, 8), (2, 128, 64), (5, 129, 65), (64, 257, 200), (255, 200, 77),
          (256, 256, 64), (257, 513, 128), (300, 1000, 192), (513, 70, 320), (40, 3001, 33), (700, 6600, 72),
          (129, 33000, 64), (1030, 4200, 33), (520, 8192, 256), (16, 260, 129), (17, 31, 1000), (32, 511, 512),
-         (65, 130, 520)]
+         (33, 1000, 264), (48, 300, 130), (65, 130, 520)]
 
 
 @pytest.mark.gpu
