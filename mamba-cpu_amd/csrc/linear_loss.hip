@@ -230,27 +230,37 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossParams p) {
 
 // ---- operands ----------------------------------------------------------------------------
 
-// The largest finite magnitude of `rows` float32 rows.
-__global__ __launch_bounds__(256) void loss_most_kernel(const LossParams p, bool of_weight) {
+// The largest finite magnitude of float32 rows: two rows a wave at a time, 1024 elements of each on their way. 256
+// workgroups of 16 waves, for one atomic each: one a wave, 8192 to one address, took 80 us.
+__global__ __launch_bounds__(1024) void loss_most_kernel(const LossParams p, bool of_weight) {
   const int64_t rows = of_weight ? p.vocab : p.scal->kept;
   const int lane = threadIdx.x & 63;
+  const int64_t waves = gridDim.x * 16ll;
   uint32_t most = 0;
-  // A wave a row, 1024 elements on their way at a time.
-  for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4) {
-    const float* row = of_weight ? static_cast<const float*>(p.weight) + r * p.sw
-                                 : static_cast<const float*>(p.hidden) + p.rows[r] * p.sh;
+  for (int64_t r = blockIdx.x * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += 2 * waves) {
+    const float* row[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int64_t at = r + w * waves < rows ? r + w * waves : r;
+      row[w] = of_weight ? static_cast<const float*>(p.weight) + at * p.sw
+                         : static_cast<const float*>(p.hidden) + p.rows[at] * p.sh;
+    }
     for (int64_t i0 = lane * 4; i0 < p.dim; i0 += 1024) {
-      float v[4][4] = {};
+      float v[2][4][4] = {};
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (i0 + u * 256 < p.dim) ld_upto4<float>(row, i0 + u * 256, upto4(p.dim - i0 - u * 256), v[u]);
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u)
+          if (i0 + u * 256 < p.dim) ld_upto4<float>(row[w], i0 + u * 256, upto4(p.dim - i0 - u * 256), v[w][u]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t b = __builtin_bit_cast(uint32_t, v[u][e]) & 0x7fffffffu;
-          most = b < 0x7f800000u && b > most ? b : most;
-        }
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, v[w][u][e]) & 0x7fffffffu;
+            most = b < 0x7f800000u && b > most ? b : most;
+          }
     }
   }
 #pragma unroll
@@ -258,12 +268,11 @@ __global__ __launch_bounds__(256) void loss_most_kernel(const LossParams p, bool
     const uint32_t o = __shfl_xor(most, s);
     most = o > most ? o : most;
   }
-  // One atomic a workgroup: one a wave, 8192 to one address, took 80 us.
-  __shared__ uint32_t tops[4];
+  __shared__ uint32_t tops[16];
   if (lane == 0) tops[threadIdx.x >> 6] = most;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int i = 1; i < 4; ++i) most = tops[i] > most ? tops[i] : most;
+  for (int i = 1; i < 16; ++i) most = tops[i] > most ? tops[i] : most;
   if (most > 0) atomicMax(of_weight ? &p.scal->wmax : &p.scal->hmax, most);
 }
 
@@ -1142,6 +1151,10 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   const float c = kLog2e / p.temperature;
   const bool each = p.reduction == MCPU_REDUCE_NONE;
   const float all = each ? 0.f : p.dloss[0] * share;
+  // By the rows that count, which the host does not know; beside the others' loads.
+  if (threadIdx.x == 1023)
+    p.scal->hsplit = splits_for((p.dpad + kLossTile - 1) / kLossTile * ((kept + kLossTile - 1) / kLossTile),
+                                p.vpiece / kLossDepth * (p.dtype == MCPU_F32 ? 3 : 1), true);
   float most = 0.f, factor = 0.f;  // the largest unit, and the largest softmax coefficient
   for (int64_t i0 = threadIdx.x; i0 < kept; i0 += 1024 * 8) {
     float g[8], e[8], stat[4][8];
@@ -1186,9 +1199,6 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   for (int i = 1; i < 16; ++i) most = fmaxf(most, tops[i]), factor = fmaxf(factor, largest[i]);
   most = fmaxf(most, factor * 0x1p-90f);
   p.scal->kept = kept;
-  // By the rows that count, which the host does not know.
-  p.scal->hsplit = splits_for((p.dpad + kLossTile - 1) / kLossTile * ((kept + kLossTile - 1) / kLossTile),
-                              p.vpiece / kLossDepth * (p.dtype == MCPU_F32 ? 3 : 1), true);
   p.scal->hmax = 0;
   p.scal->wmax = p.laid != nullptr ? *p.laid : 0;
   p.scal->unit = most == 0.f ? 1.f : fmaxf(most, 0x1p-100f);
@@ -1211,8 +1221,8 @@ void run(K kernel, LossParams p, int64_t groups, int threads, hipStream_t st, A.
 
 template <typename T> void lay_operands(const LossParams& p, bool weight, hipStream_t st) {
   if constexpr (std::is_same_v<T, float>) {
-    run(loss_most_kernel, p, std::min<int64_t>((p.tokens + 3) / 4, 512), 256, st, false);
-    if (weight) run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 3) / 4, 1024), 256, st, true);
+    run(loss_most_kernel, p, std::min<int64_t>((p.tokens + 15) / 16, 256), 1024, st, false);
+    if (weight) run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 15) / 16, 256), 1024, st, true);
   }
   run(loss_gather_kernel<T>, p, p.tpad / 4, 256, st);
   if (weight && p.wrows != nullptr) run(loss_weight_kernel<T>, p, (p.vocab + 3) / 4, 256, st);
