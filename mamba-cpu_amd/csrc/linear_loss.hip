@@ -523,6 +523,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
     const bool here = id >= 0 && v >= 0 && v < p.vrows;
     if (!__any(here)) continue;
     // All entries of that id, 64 at a time from the lanes that hold them.
+    const float own = e < k ? p.share[t * k + e] : 0.f;
     float q = 0.f;
     bool first = true;
     for (int o0 = 0; o0 < k; o0 += 64) {
@@ -534,10 +535,10 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
         const bool same = __builtin_amdgcn_readlane(other, o) == id;
         const float more = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, share), o));
         q += same ? more : 0.f;
-        first = first && !(same && o0 + o < e);
+        first = first && !(same && more != 0.f && o0 + o < e);
       }
     }
-    if (!here || !first || q == 0.f) continue;  // an id's first entry places it; entries left out may have no product
+    if (!here || !first || own == 0.f) continue;  // an id's first entry with a share places it: it has a product
     E* out = static_cast<E*>(p.grad) + i * p.vpiece + v;
     if constexpr (std::is_same_v<T, float>) {
       E* low = out + p.tpad * p.vpiece;
