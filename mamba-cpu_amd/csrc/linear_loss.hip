@@ -35,8 +35,13 @@
 namespace mcpu {
 namespace {
 
-// ds is kept as ds / unit times this: f16 then resolves 2^-37 of the largest coefficient.
+// ds is kept as ds / unit times this: f16's steps are then 2^-37 of the unit.
 template <typename E> constexpr float kUp = std::is_same_v<E, bf16> ? 1.f : 8192.f;
+// f16 pieces: the least unit of a row beside the largest. dweight's product takes unit / the largest from hidden's
+// rows, whose largest magnitude is 2^13 or more: with 2^-16 of it left, their elements down to 2^-11 of the largest keep
+// all bits of an f16. What is below goes to ds, whose largest of a row falls from 2^13 on. All of it to hidden, unscaled,
+// left 4 bits of an element near 1 at a unit of 2^-20 and nothing at 2^-26; all of it to ds would do that to dhidden.
+constexpr float kLeastUnit = 0x1p-16f;
 
 __device__ __forceinline__ int64_t id_at(const LossParams& p, int64_t i) {
   return p.ids64 ? static_cast<const int64_t*>(p.ids)[i] : static_cast<const int32_t*>(p.ids)[i];
@@ -73,10 +78,13 @@ __device__ __forceinline__ int up_exponent(uint32_t most) {
   const int e = 13 - (static_cast<int>(most >> 23) - 127);
   return e > 120 ? 120 : e;
 }
-// The unit of a row that counts.
-__device__ __forceinline__ float unit_of(const LossParams& p, int64_t i) {
-  const float u = p.coef[3 * p.tpad + i];
-  return u > 0.f ? u : p.scal->unit;
+// The unit of a row that counts. One below the least becomes that by a power of two: its target's ds stays exact.
+template <typename E> __device__ __forceinline__ float unit_of(const LossParams& p, int64_t i) {
+  const float u = p.coef[3 * p.tpad + i], most = p.scal->unit;
+  if (!(u > 0.f)) return most;
+  if (std::is_same_v<E, bf16> || u >= most * kLeastUnit) return u;
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, u) & 0x7fffffu) |
+                                       (__builtin_bit_cast(uint32_t, most * kLeastUnit) & 0x7f800000u));
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
 
@@ -230,20 +238,20 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossParams p) {
 
 // ---- operands ----------------------------------------------------------------------------
 
-// The largest finite magnitude of float32 rows: two rows a wave at a time, 1024 elements of each on their way. 256
+// The largest finite magnitude of rows: two rows a wave at a time, 1024 elements of each on their way. 256
 // workgroups of 16 waves, for one atomic each: one a wave, 8192 to one address, took 80 us.
-__global__ __launch_bounds__(1024) void loss_most_kernel(const LossParams p, bool of_weight) {
+template <typename T> __global__ __launch_bounds__(1024) void loss_most_kernel(const LossParams p, bool of_weight) {
   const int64_t rows = of_weight ? p.vocab : p.scal->kept;
   const int lane = threadIdx.x & 63;
   const int64_t waves = gridDim.x * 16ll;
   uint32_t most = 0;
   for (int64_t r = blockIdx.x * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += 2 * waves) {
-    const float* row[2];
+    const T* row[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const int64_t at = r + w * waves < rows ? r + w * waves : r;
-      row[w] = of_weight ? static_cast<const float*>(p.weight) + at * p.sw
-                         : static_cast<const float*>(p.hidden) + p.rows[at] * p.sh;
+      row[w] = of_weight ? static_cast<const T*>(p.weight) + at * p.sw
+                         : static_cast<const T*>(p.hidden) + p.rows[at] * p.sh;
     }
     for (int64_t i0 = lane * 4; i0 < p.dim; i0 += 1024) {
       float v[2][4][4] = {};
@@ -251,7 +259,7 @@ __global__ __launch_bounds__(1024) void loss_most_kernel(const LossParams p, boo
       for (int w = 0; w < 2; ++w)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (i0 + u * 256 < p.dim) ld_upto4<float>(row[w], i0 + u * 256, upto4(p.dim - i0 - u * 256), v[w][u]);
+          if (i0 + u * 256 < p.dim) ld_upto4<T>(row[w], i0 + u * 256, upto4(p.dim - i0 - u * 256), v[w][u]);
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -274,6 +282,17 @@ __global__ __launch_bounds__(1024) void loss_most_kernel(const LossParams p, boo
   if (threadIdx.x != 0) return;
   for (int i = 1; i < 16; ++i) most = tops[i] > most ? tops[i] : most;
   if (most > 0) atomicMax(of_weight ? &p.scal->wmax : &p.scal->hmax, most);
+}
+
+template <typename T> using Kept = std::conditional_t<std::is_same_v<T, float>, f16, T>;
+
+// What hidden's rows of dweight's product are scaled by: its largest magnitude to [2^13, 2^14). bf16 has float32's range.
+template <typename T> __device__ __forceinline__ int dweight_exponent(const LossParams& p) {
+  if (std::is_same_v<T, float> || (std::is_same_v<T, f16> && p.hscaled != nullptr)) return up_exponent(p.scal->hmax);
+  return 0;
+}
+template <typename T> __device__ __forceinline__ float dweight_up(const LossParams& p) {
+  return pow2(dweight_exponent<T>(p));
 }
 
 // A row in the products' layout, zero behind its end: a wave a row, 64 elements at a time.
@@ -311,7 +330,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_gather_kernel(
   // The backward's, in the largest unit.
   if (p.hscaled != nullptr)
     lay_row<T>(from, p.hscaled, i * p.dpad, p.tpad * p.dpad, p.dim, p.dpad,
-               up * (i < kept ? unit_of(p, i) / p.scal->unit : 0.f), threadIdx.x & 63);
+               dweight_up<T>(p) * (i < kept ? unit_of<Kept<T>>(p, i) / p.scal->unit : 0.f), threadIdx.x & 63);
 }
 
 template <typename T> __global__ __launch_bounds__(256) void loss_weight_kernel(const LossParams p) {
@@ -325,7 +344,6 @@ template <typename T> __global__ __launch_bounds__(256) void loss_weight_kernel(
 
 // ---- the products ---------------------------------------------------------------------------
 
-template <typename T> using Kept = std::conditional_t<std::is_same_v<T, float>, f16, T>;
 template <typename T> constexpr int kRuns = std::is_same_v<T, float> ? 3 : 1;
 
 // What takes the scaling of float32 operands back, and log2(e) c with it.
@@ -441,7 +459,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t t = t0 + j * 32;
-    const float up = kUp<E> / unit_of(p, t);
+    const float up = kUp<E> / unit_of<E>(p, t);
     a[j] = p.coef[t] * up;
     b[j] = p.coef[p.tpad + t] * up;
     m2[j] = p.coef[2 * p.tpad + t];
@@ -514,7 +532,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
   if (i >= p.scal->kept) return;
   const int64_t t = p.rows[i];
   const int k = static_cast<int>(p.k);
-  const float up = kUp<E> / unit_of(p, i), c = kLog2e / p.temperature;
+  const float up = kUp<E> / unit_of<E>(p, i), c = kLog2e / p.temperature;
   const float a = p.coef[i] * up, b = p.coef[p.tpad + i] * up, m2 = p.coef[2 * p.tpad + i];
   for (int e0 = 0; e0 < k; e0 += 64) {
     const int e = e0 + lane;
@@ -611,7 +629,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_dhidden_out_ke
   const bool in = i < p.scal->kept;
   float v[4] = {};
   if (in) {
-    float scale = unit_of(p, i) / kUp<E>;
+    float scale = unit_of<E>(p, i) / kUp<E>;
     if constexpr (std::is_same_v<T, float>) scale *= pow2(-up_exponent(p.scal->wmax));
     const int64_t rows = (int64_t{p.scal->kept} + kLossTile - 1) / kLossTile * kLossTile;
     sum_splits(p.acc + i * p.dpad + d, rows * p.dpad, p.scal->hsplit, v);
@@ -640,8 +658,7 @@ __global__ __launch_bounds__(512, 2) void loss_dweight_kernel(const LossParams p
                               static_cast<int>(int64_t{depths} * split / p.wsplit),
                               static_cast<int>(int64_t{depths} * (split + 1) / p.wsplit), a0, b0, a1, b1, acc);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float scale = p.scal->unit / kUp<E>;
-  if constexpr (std::is_same_v<T, float>) scale *= pow2(-up_exponent(p.scal->hmax));
+  const float scale = p.scal->unit / kUp<E> * pow2(-dweight_exponent<T>(p));
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t vl = nt * kLossTile + (wave & 3) * 64 + j * 32 + (lane & 31);
@@ -1015,7 +1032,7 @@ __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams 
   for (int j = 0; j < 4; ++j) {
     const int64_t t = t0 + 16 * j + (lane & 15);
     const bool in = j < NF && t < kept;
-    const float up = in ? kUp<E> / unit_of(p, t) : 0.f;
+    const float up = in ? kUp<E> / unit_of<E>(p, t) : 0.f;
     const float a = in ? p.coef[t] * up : 0.f, b = in ? p.coef[p.tpad + t] * up : 0.f;
     const float m2 = in ? p.coef[2 * p.tpad + t] : 0.f;
     const int64_t target = in && p.target != nullptr ? p.target[t] : -1;
@@ -1222,8 +1239,10 @@ void run(K kernel, LossParams p, int64_t groups, int threads, hipStream_t st, A.
 
 template <typename T> void lay_operands(const LossParams& p, bool weight, hipStream_t st) {
   if constexpr (std::is_same_v<T, float>) {
-    run(loss_most_kernel, p, std::min<int64_t>((p.tokens + 15) / 16, 256), 1024, st, false);
-    if (weight) run(loss_most_kernel, p, std::min<int64_t>((p.vocab + 15) / 16, 256), 1024, st, true);
+    run(loss_most_kernel<T>, p, std::min<int64_t>((p.tokens + 15) / 16, 256), 1024, st, false);
+    if (weight) run(loss_most_kernel<T>, p, std::min<int64_t>((p.vocab + 15) / 16, 256), 1024, st, true);
+  } else if (std::is_same_v<T, f16> && p.hscaled != nullptr && p.dweight != nullptr) {
+    run(loss_most_kernel<T>, p, std::min<int64_t>((p.tokens + 15) / 16, 256), 1024, st, false);
   }
   run(loss_gather_kernel<T>, p, p.tpad / 4, 256, st);
   if (weight && p.wrows != nullptr) run(loss_weight_kernel<T>, p, (p.vocab + 3) / 4, 256, st);

@@ -14,7 +14,7 @@ namespace mcpu {
 // What one call passes between its kernels on the GPU.
 struct LossScalars {
   int32_t kept;          // rows that count
-  uint32_t hmax, wmax;   // float32 operands: the largest finite magnitudes, as bits
+  uint32_t hmax, wmax;   // the largest finite magnitudes, as bits: float32 operands; hidden in f16 for dweight
   int32_t hsplit;        // backward: splits of dhidden's products
   float unit;            // backward: the largest unit of a row's ds
 };
@@ -53,7 +53,7 @@ struct LossParams {
   float* coef;        // (4, padded tokens): factor of 2^(logit - maximum), the target's ds or the shares' factor,
                       // the maximum, the unit of ds (0: the largest)
   void* hrows;        // (pieces, padded tokens, padded dim): hidden's rows that count
-  void* hscaled;      // hrows in the largest unit, or null: hrows has it (distillation)
+  void* hscaled;      // hidden's rows in the largest unit, or null: hrows has it (distillation)
   void* wrows;        // (pieces, vocab, padded dim), which may be of `laid`, or null: weight is read in place
   void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits
   float* acc;         // (splits, rows that count, padded, padded dim): gradient of hidden
