@@ -140,7 +140,9 @@ size_t lay_bwd(const mcpu_linear_loss_args* a, LossParams& p, void* workspace) {
   Layout w{static_cast<char*>(workspace)};
   lay_operands(a, p, w);
   w.take(p.coef, 4 * p.tpad);
-  if (!distil(a)) w.take(p.hscaled, loss_pieces(a->dtype) * p.tpad * p.dpad, 2);
+  // Distillation: rows have units of their own in f16 pieces, where each has a gradient of its own.
+  if (!distil(a) || (a->reduction == MCPU_REDUCE_NONE && a->dtype != MCPU_BF16))
+    w.take(p.hscaled, loss_pieces(a->dtype) * p.tpad * p.dpad, 2);
   w.take(p.grad, loss_pieces(a->dtype) * p.tpad * p.vpiece, 2);
   if (p.dhidden != nullptr) w.take(p.acc, p.htiles * kLossTile * kLossTile);
   if (p.dweight != nullptr && p.wsplit > 1) w.take(p.dwpart, p.wsplit * p.vpiece * p.dpad);

@@ -78,13 +78,17 @@ __device__ __forceinline__ int up_exponent(uint32_t most) {
   const int e = 13 - (static_cast<int>(most >> 23) - 127);
   return e > 120 ? 120 : e;
 }
+// The largest power of two that is not above x.
+__device__ __forceinline__ float power_below(float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0x7f800000u);
+}
 // The unit of a row that counts. One below the least becomes that by a power of two: its target's ds stays exact.
 template <typename E> __device__ __forceinline__ float unit_of(const LossParams& p, int64_t i) {
   const float u = p.coef[3 * p.tpad + i], most = p.scal->unit;
   if (!(u > 0.f)) return most;
   if (std::is_same_v<E, bf16> || u >= most * kLeastUnit) return u;
   return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, u) & 0x7fffffu) |
-                                       (__builtin_bit_cast(uint32_t, most * kLeastUnit) & 0x7f800000u));
+                                       __builtin_bit_cast(uint32_t, power_below(most * kLeastUnit)));
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
 
@@ -1161,7 +1165,9 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossParams p) {
 // 16 bits a rounding of the target's ds, the row's largest, would be in all of
 // the row's gradient alike; so the unit is that ds itself (exactly 1 then), and
 // dweight takes the units from hidden's rows, scaled by unit / the largest unit.
-// Distillation: one unit, the largest coefficient. One workgroup.
+// Distillation has no one largest: one unit, the largest coefficient; f16 pieces
+// with a gradient for each row: that row's coefficient, down to a power of two, which
+// rounds nothing of hidden. One workgroup.
 __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   __shared__ float tops[16], largest[16];
   const int32_t kept = p.rows[p.tokens];
@@ -1203,7 +1209,7 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
       p.coef[2 * p.tpad + i] = m2;
       // Not where a / unit would leave float32's range: the others' share is below 2^-90, a loss of 0 but for that.
       const bool fits = top > 0x1p-100f && top > __builtin_fabsf(a) * 0x1p-90f && top < INFINITY;
-      p.coef[3 * p.tpad + i] = p.share == nullptr && fits ? top : 0.f;
+      p.coef[3 * p.tpad + i] = fits && p.hscaled != nullptr ? (p.share == nullptr ? top : power_below(top)) : 0.f;
     }
   }
 #pragma unroll
@@ -1219,7 +1225,8 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
   p.scal->kept = kept;
   p.scal->hmax = 0;
   p.scal->wmax = p.laid != nullptr ? *p.laid : 0;
-  p.scal->unit = most == 0.f ? 1.f : fmaxf(most, 0x1p-100f);
+  most = most == 0.f ? 1.f : fmaxf(most, 0x1p-100f);
+  p.scal->unit = p.share != nullptr && p.hscaled != nullptr ? power_below(most) : most;
 }
 
 // Results of calls without rows, vocabulary or entries.

@@ -53,7 +53,8 @@ struct LossParams {
   float* coef;        // (4, padded tokens): factor of 2^(logit - maximum), the target's ds or the shares' factor,
                       // the maximum, the unit of ds (0: the largest)
   void* hrows;        // (pieces, padded tokens, padded dim): hidden's rows that count
-  void* hscaled;      // hidden's rows in the largest unit, or null: hrows has it (distillation)
+  void* hscaled;      // hidden's rows in the largest unit, or null: one unit for all (distillation, but for rows'
+                      // gradients in f16 pieces)
   void* wrows;        // (pieces, vocab, padded dim), which may be of `laid`, or null: weight is read in place
   void* grad;         // (pieces, padded tokens, vocab piece): gradients of the logits
   float* acc;         // (splits, rows that count, padded, padded dim): gradient of hidden

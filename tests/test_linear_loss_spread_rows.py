@@ -16,17 +16,20 @@ import numpy as np
 import pytest
 import torch
 
+import mamba_cpu
 from oracle import loss as O
-from test_linear_loss import DTYPES, KEPT, OUT, U, WAYS, check, lse_tol, run_ce
+from test_linear_loss import DEV, DTYPES, KEPT, OUT, U, WAYS, check, inputs, lse_tol, run_ce, teacher
 
 
-def held_to_its_size(dtype, h, w, ds, unit, ltol, dh, dw):
+def held_to_its_size(dtype, h, w, ds, unit, ltol, dh, dw, shares=0.0):
+    """shares: what ds has of its row's target distribution, taken from the probabilities, whose error is of their own
+    size."""
     hd, wd = np.abs(h.double().numpy()), np.abs(w.double().numpy())
     e = KEPT[dtype] + 2 * float(np.max(ltol))
     r = (unit / unit.max())[:, None]
     low = 2.0 ** -37 * unit[:, None] / np.minimum(1, 2.0 ** 16 * r) if dtype != "bf16" else np.zeros_like(r)
     floor = 2.0 ** -24 if dtype == "f16" else 0.0
-    mag = np.abs(ds)
+    mag = np.abs(ds) + shares
     want_h, want_w = O.grads(h, w, ds)
     assert dtype != "f16" or max(np.abs(want_h).max(), np.abs(want_w).max()) < 60000  # no overflow of the results
     check("dhidden", dh, want_h,
@@ -83,3 +86,22 @@ def test_weights_of_tokens_over_six_powers_of_ten(dtype, t, v):
     dloss = 2.0 ** 10 * 10.0 ** (-6 * (torch.arange(t) % 32) / 31)
     dloss[0] = 2.0 ** 14
     verify(dtype, h, w, ids, dloss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,v", WAYS)
+def test_distilled_tokens_of_weights_over_eight_powers_of_ten(dtype, t, v):
+    h, w, _, g = inputs(dtype, t, v, 64)
+    ids, tl = teacher(t, v, 8, g)
+    dloss = 2.0 ** 11 * 10.0 ** (-8 * torch.linspace(0, 1, t)) * (1 - 2 * (torch.arange(t) % 2))
+    hg, wg = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    loss = mamba_cpu.linear_distillation_fn(hg, wg, ids.to(DEV), tl.to(DEV), temperature=1.5, reduction="none")
+    dh, dw = torch.autograd.grad(loss, [hg, wg], dloss.to(DEV))
+    _, lse, _ = O.rows(h, w, ids, tl, 1.5)
+    ds = O.logits_grad(h, w, ids, dloss.double().numpy(), teacher=tl, temperature=1.5)
+    unit = 1.5 * np.abs(dloss.double().numpy())
+    q, _ = O.shares(ids, v, tl, 1.5)
+    shares = np.zeros_like(ds)
+    np.put_along_axis(shares, ids.numpy(), q * unit[:, None], 1)
+    held_to_its_size(dtype, h, w, ds, unit, lse_tol(dtype, h, w, lse, 1.5) + 2 * U * np.abs(lse) + 8 * U, dh, dw, shares)
