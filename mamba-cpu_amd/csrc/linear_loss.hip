@@ -15,8 +15,10 @@
 // digits. The products of hidden with a teacher's ids are formed by themselves.
 // Backward: a piece of the vocabulary at a time, the product again, now with ds in
 // 16 bits as its result (float32: two f16 pieces), the ids' places put right, and
-// the two products of the gradients over it. Rows that do not count take part in
-// no product, so nothing in them, NaN included, reaches another row.
+// the two products of the gradients over it. dweight's reads hidden's rows times their
+// ds's unit over the largest, rounded once more to the kept type (loss_coef_kernel has
+// why, kLeastUnit how far). Rows that do not count take part in no product, so nothing in
+// them, NaN included, reaches another row.
 //
 // Three ways to the logits, by how many tiles there are:
 //   tiles of 256 x 256     bound by the matrix cores at the clock that power leaves

@@ -9,13 +9,21 @@ Per token, with s = hidden @ weight.T formed in float32:
     distillation    q = softmax(teacher / T) over the teacher's entries,
                     loss = T^2 sum_k q_k (log q_k - log softmax(s / T)_id_k)
 
-Products are of hidden and weight as given, summed in float32 (many tokens of
+Logits are of hidden and weight as given, summed in float32 (many tokens of
 float32: as two float16 pieces each, which keep 22 bits of a value and 2^-38 of
 the tensor's largest). hidden and weight of different types, or of others than
-float32, bfloat16 and float16, go as float32. The logits' gradients are rounded once
-to the operands' type (float32: to 22 bits) before the products over them; the
-results' sums are float32, rounded once, in an order that does not change from
-call to call.
+float32, bfloat16 and float16, go as float32.
+
+The gradients are products over the logits' gradients ds, rounded once to the
+operands' type (float32: to 22 bits, two float16 pieces). A row of ds is kept in a
+unit of its own: its target's ds, or with a distillation loss for each row that
+row's gradient (bfloat16, and reduced distillation losses, one for all). dweight
+takes unit / largest unit from hidden's rows, which cross entropy then rounds once
+more to that type. In float16 pieces this holds for rows far below the largest:
+down to 2^-16 of it their ds has steps of 2^-37 of its unit, and hidden's elements all
+their bits down to 2^-11 of hidden's largest (float32: next to the largest); below,
+ds's steps grow as the row gets smaller. The results' sums are float32, rounded
+once, in an order that does not change from call to call.
 
 Between forward and backward a call keeps a few numbers a token and, where the
 kernels do not read weight as it lies (float32, or 16 bits with a number of columns
