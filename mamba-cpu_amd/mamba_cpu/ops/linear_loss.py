@@ -43,14 +43,14 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 # its shape functions for FakeTensor tracing.
 
 
-def _laid_size(hidden, weight, save):
+def _laid_size(hidden, weight, k, save):
     """Bytes of weight in the products' layout, where it is kept for the backward and is not read in place (an
     unaligned first element aside, which a traced tensor does not tell)."""
     (tokens, dim), vocab = hidden.shape, weight.shape[0]
     wide = hidden.dtype == torch.float32
     stride = weight.stride(0) if weight.stride(1) == 1 or dim <= 1 else dim
     blocks = tokens <= 64 or -(-vocab // 128) * -(-tokens // 64) <= 512  # read in place too
-    if not save or blocks or (
+    if not save or blocks or k == 0 or (
             not wide and dim % 64 == 0 and stride % 8 == 0 and stride <= 2 ** 20):
         return 0
     return 256 + (vocab * -(-dim // 64) * 64 * (4 if wide else 2) + 255) // 256 * 256
@@ -64,7 +64,7 @@ def _(hidden, weight, ids, teacher, ignore_index, temperature, reduction, save):
             hidden.new_empty(tokens if teacher is not None else 0, k, **f32), hidden.new_empty(4, tokens, **f32),
             hidden.new_empty(tokens if teacher is not None else 0, k, **f32),
             hidden.new_empty(tokens + 1, dtype=torch.int32),
-            hidden.new_empty(_laid_size(hidden, weight, save), dtype=torch.uint8))
+            hidden.new_empty(_laid_size(hidden, weight, k, save), dtype=torch.uint8))
 
 
 @torch.library.register_fake("mamba_cpu::linear_loss_bwd")
