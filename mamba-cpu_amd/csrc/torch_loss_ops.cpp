@@ -58,6 +58,13 @@ const Tensor& check_like(const char* name, const char* what, const Tensor& t, at
   return t;
 }
 
+// Bytes of weight kept for the backward: not by its address, which a traced tensor does not tell. Where that alone
+// keeps weight from being read in place, the backward lays it out once more.
+int64_t kept_bytes(mcpu_linear_loss_args a) {
+  a.weight = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(a.weight) & ~uintptr_t{255});
+  return static_cast<int64_t>(mcpu_linear_loss_laid_size(&a));
+}
+
 // loss, lse, and for the backward the ids' products, the rows' statistics, the teacher's distribution
 // (distillation), the rows that count and, where saved, weight as the products read it.
 using Losses = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
@@ -85,8 +92,8 @@ Losses linear_loss_fwd(const Tensor& hidden_in, const Tensor& weight_in, const T
   a.stat = static_cast<float*>(stat.data_ptr());
   a.share = has(teacher) ? static_cast<float*>(share.data_ptr()) : nullptr;
   a.rows = static_cast<int32_t*>(rows.data_ptr());
-  const size_t kept = save ? mcpu_linear_loss_laid_size(&a) : 0;
-  Tensor laid = at::empty({static_cast<int64_t>(kept)}, hidden.options().dtype(at::kByte));
+  const int64_t kept = save ? kept_bytes(a) : 0;
+  Tensor laid = at::empty({kept}, hidden.options().dtype(at::kByte));
   if (kept > 0) a.laid = laid.data_ptr();
   const size_t nws = mcpu_linear_loss_fwd_workspace_size(&a);
   Tensor ws = workspace(nws, hidden);

@@ -27,7 +27,7 @@ once, in an order that does not change from call to call.
 
 Between forward and backward a call keeps a few numbers a token and, where the
 kernels do not read weight as it lies (float32, or 16 bits with a number of columns
-that is no multiple of 64 or rows that are not 16-byte aligned), a copy of it.
+that is no multiple of 64 or rows that are no multiple of 16 bytes apart), a copy of it.
 """
 
 import torch
@@ -44,8 +44,8 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def _laid_size(hidden, weight, k, save):
-    """Bytes of weight in the products' layout, where it is kept for the backward and is not read in place (an
-    unaligned first element aside, which a traced tensor does not tell)."""
+    """Bytes of weight in the products' layout, where it is kept for the backward and would not be read in place from
+    an aligned first element on."""
     (tokens, dim), vocab = hidden.shape, weight.shape[0]
     wide = hidden.dtype == torch.float32
     stride = weight.stride(0) if weight.stride(1) == 1 or dim <= 1 else dim

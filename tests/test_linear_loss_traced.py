@@ -43,6 +43,17 @@ def test_the_kept_weight_has_the_size_that_is_traced():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("first,stride", [(0, 64), (1, 72), (8, 72), (0, 67)])
+def test_operator_returns_what_is_traced(dtype, first, stride):
+    t, v = 1100, 4000
+    h, _, ids, _ = inputs(dtype, t, v, 64)
+    w = torch.zeros(v * stride + first, device=DEV, dtype=DTYPES[dtype])[first:].view(v, stride)[:, :64]
+    outs = torch.ops.mamba_cpu.linear_loss_fwd(h.to(DEV), w, ids[:, None].to(DEV), None, -100, 1.0, 0, True)
+    assert [tuple(x.shape) for x in outs] == traced_sizes(t, v, 64, 1, stride, DTYPES[dtype], False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("op", ["ce", "kd"])
 @pytest.mark.parametrize("t,v,d", [(20, 60, 64), (1100, 4000, 72)])
 def test_operator_checks(dtype, op, t, v, d):
