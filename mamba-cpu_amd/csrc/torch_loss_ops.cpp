@@ -125,7 +125,8 @@ std::tuple<Tensor, Tensor> linear_loss_bwd(const optional<Tensor>& dloss, const 
   a.rows = static_cast<int32_t*>(
       check_like(name, "rows", rows, at::kInt, at::IntArrayRef(&last, 1), hidden).data_ptr());
   const size_t kept = mcpu_linear_loss_laid_size(&a);
-  if (laid.numel() > 0) {
+  // Not where weight is read in place, as of a saved weight that came back in another layout.
+  if (laid.numel() > 0 && kept > 0) {
     TORCH_CHECK_VALUE(static_cast<size_t>(laid.numel()) == kept && laid.scalar_type() == at::kByte &&
                           laid.is_contiguous() && laid.device() == hidden.device(),
                       name, " expects the laid out weight that the forward left");
