@@ -21,7 +21,8 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
   if (a->dim == 0) return fail(MCPU_ERR_INVALID, "%s: dim must be positive", what);
   if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
     return fail(MCPU_ERR_INVALID, "%s: temperature must be above 0", what);
-  if (!distil(a) && a->k > 0 && (a->k != 1 || a->temperature != 1.f))
+  // Without tokens a teacher's logits have no address to tell by.
+  if (!distil(a) && a->tokens > 0 && a->k > 0 && (a->k != 1 || a->temperature != 1.f))
     return fail(MCPU_ERR_INVALID, "%s: cross entropy has one target a row and temperature 1", what);
   if (distil(a) && a->dlse != nullptr) return fail(MCPU_ERR_INVALID, "%s: distillation has no dlse", what);
   if (a->tokens > (1 << 26) || a->vocab > (1 << 24) || a->dim > (1 << 20) || a->k > kLossMaxK)
