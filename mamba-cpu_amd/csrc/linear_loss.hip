@@ -716,6 +716,7 @@ __device__ __forceinline__ void finish_row(const LossParams& p, int64_t t, int64
     // log(all / mine), by log1p where the target is the largest.
     const float r = others / mine, u = 1.f + r;
     p.each[t] = d >= 0.f ? (u == 1.f ? r : logf(u) * (r / (u - 1.f))) : logf(all) - d;
+    if (own == INFINITY) p.each[t] = NAN;  // lse - s of an overflowed target, as its gradient
     stat[2 * p.tokens] = mine / all;
     stat[3 * p.tokens] = others / all;
     top = far ? own : top;
