@@ -80,6 +80,11 @@ __device__ __forceinline__ int up_exponent(uint32_t most) {
   const int e = 13 - (static_cast<int>(most >> 23) - 127);
   return e > 120 ? 120 : e;
 }
+// exp(c (x - m)) is 2^(c x - m2), one multiply-add, with m2 = c m as rounded and its rounding (2^-9 at most) taken out
+// of the sum. From here on that rounding is no small correction: such rows take the difference first.
+constexpr float kFar = 0x1p16f;
+__device__ __forceinline__ bool is_far(float m2) { return __builtin_fabsf(m2) >= kFar; }
+
 // The largest power of two that is not above x.
 __device__ __forceinline__ float power_below(float x) {
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0x7f800000u);
@@ -439,14 +444,23 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_logits_kern
       for (int e = 0; e < 16; ++e) m = fmaxf(m, acc.v[j][i][e]);
     m = fmaxf(m, __shfl_xor(m, 32));
     // Relative to m * c as rounded, one multiply-add an element; then its rounding is taken out.
-    const float m2 = m == -INFINITY ? 0.f : m * c, off = m == -INFINITY ? 0.f : fmaf(m, c, -m2);
+    const float m2 = m == -INFINITY ? 0.f : m * c;
     float s = 0.f;
+    if (__any(is_far(m2))) {
+      const float sub = m == -INFINITY ? 0.f : m;
+      each_row(acc.v[j], [&](float x, int) {
+        s += fast_exp2((x - sub) * c);
+        return x;
+      });
+      s += __shfl_xor(s, 32);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s += fast_exp2(fmaf(acc.v[j][i][e], c, -m2));
-    s += __shfl_xor(s, 32);
-    s = fmaf(s, -kLn2 * off, s);
+        for (int e = 0; e < 16; ++e) s += fast_exp2(fmaf(acc.v[j][i][e], c, -m2));
+      s += __shfl_xor(s, 32);
+      s = fmaf(s, -kLn2 * (m == -INFINITY ? 0.f : fmaf(m, c, -m2)), s);
+    }
     if (lane < 32 && v0 < p.vocab) p.part[(v0 / kLossPart) * p.tpad + t] = make_float2(m * back, s);
   }
 }
@@ -481,7 +495,14 @@ template <typename T> __global__ __launch_bounds__(512, 2) void loss_grad_kernel
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t t = t0 + j * 32;
-    each_row(acc.v[j], [&](float x, int) { return a[j] * fast_exp2(fmaf(x, c, -m2[j])); });
+    if (__any(is_far(m2[j]))) {
+      const float back = logit_back<T>(p), c0 = kLog2e / p.temperature, top = t < kept ? p.stat[t] : 0.f;
+      each_row(acc.v[j], [&](float x, int) {
+        return a[j] * fast_exp2(is_far(m2[j]) ? (x * back - top) * c0 : fmaf(x, c, -m2[j]));
+      });
+    } else {
+      each_row(acc.v[j], [&](float x, int) { return a[j] * fast_exp2(fmaf(x, c, -m2[j])); });
+    }
     const int at = target_row(target[j], vp + v0, lane);
     if (__any(at >= 0)) each_row(acc.v[j], [&](float x, int row) { return row == at ? b[j] : x; });
     if (edge) {
@@ -527,7 +548,8 @@ __device__ __forceinline__ int32_t in_vocab(const LossParams& p, int64_t i, bool
 }
 
 // Distillation: the ids' places of ds, a_t exp(c s - L) less all shares of that id. A
-// wave a row. In 16 bits that is formed anew, to be rounded once. float32 takes p
+// wave a row. In 16 bits that is formed anew, to be rounded once, but in far rows, where the
+// two products' roundings would part `picked` from the row's sum. float32 takes p
 // from the two pieces that are there: where p and its share are both near 1, their
 // difference is as good as p agrees with the row's sum, and that is of the same
 // product, while `picked` is a sum of its own.
@@ -568,7 +590,8 @@ template <typename T> __global__ __launch_bounds__(256) void loss_place_kernel(c
       E* low = out + p.tpad * p.vpiece;
       split_f16((static_cast<float>(*out) + static_cast<float>(*low)) - b * q, *out, *low);
     } else {
-      *out = from_f32<E>(a * fast_exp2(fmaf(p.picked[t * k + e], c, -m2)) - b * q);
+      const float of_v = is_far(m2) ? to_f32(*out) : a * fast_exp2(fmaf(p.picked[t * k + e], c, -m2));
+      *out = from_f32<E>(of_v - b * q);
     }
   }
 }
@@ -1041,7 +1064,7 @@ __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams 
     const bool in = j < NF && t < kept;
     const float up = in ? kUp<E> / unit_of<E>(p, t) : 0.f;
     const float a = in ? p.coef[t] * up : 0.f, b = in ? p.coef[p.tpad + t] * up : 0.f;
-    const float m2 = in ? p.coef[2 * p.tpad + t] : 0.f;
+    const float m2 = in ? p.coef[2 * p.tpad + t] : 0.f, top = in ? p.stat[t] : 0.f;
     const int64_t target = in && p.target != nullptr ? p.target[t] : -1;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -1051,7 +1074,8 @@ __global__ __launch_bounds__(256, 2) void loss_few_grad_kernel(const LossParams 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int64_t v = v0 + at + e;
-          x[e] = v >= p.vocab ? 0.f : v == target ? b : a * fast_exp2(fmaf(acc[i][j < NF ? j : 0][e], c, -m2));
+          const float s = acc[i][j < NF ? j : 0][e], power = is_far(m2) ? (s - top) * c : fmaf(s, c, -m2);
+          x[e] = v >= p.vocab ? 0.f : v == target ? b : a * fast_exp2(power);
         }
       }
       E* out = static_cast<E*>(p.grad) + t * p.vpiece + vl + at;
@@ -1201,7 +1225,7 @@ __global__ __launch_bounds__(1024) void loss_coef_kernel(const LossParams p) {
       g[u] *= p.temperature;  // 1 for cross entropy
       const float a = g[u] + e[u];
       // exp(c (s - maximum)) as 2^(c s - m2), with the rounding of m2 in the factor.
-      const float m2 = stat[0][u] * c, off = fmaf(stat[0][u], c, -m2);
+      const float m2 = stat[0][u] * c, off = is_far(m2) ? 0.f : fmaf(stat[0][u], c, -m2);
       // Cross entropy: the target's ds, a p - g = (a - g) p - g (1 - p); no other is above a (1 - p).
       const float own = p.share != nullptr ? g[u] : e[u] * stat[2][u] - g[u] * stat[3][u];
       const float top = fmaxf(__builtin_fabsf(own), __builtin_fabsf(a) * (p.share != nullptr ? 1.f : stat[3][u]));
