@@ -784,7 +784,7 @@ typedef struct mcpu_linear_loss_args {
   int64_t tokens, vocab, dim, k;       /* k at most 1024 */
   int64_t hidden_stride, weight_stride;  /* elements between rows */
   int64_t ignore_index;     /* cross entropy */
-  float temperature;        /* above 0; 1 for cross entropy */
+  float temperature;        /* 2^-60 to 2^60; 1 for cross entropy */
   int32_t dtype;
   int32_t ids64;
   int32_t reduction;

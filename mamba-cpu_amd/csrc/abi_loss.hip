@@ -19,8 +19,9 @@ int check_loss(const mcpu_linear_loss_args* a, const char* what) {
   if (a->reduction < MCPU_REDUCE_NONE || a->reduction > MCPU_REDUCE_MEAN)
     return fail(MCPU_ERR_INVALID, "%s: bad reduction %d", what, a->reduction);
   if (a->dim == 0) return fail(MCPU_ERR_INVALID, "%s: dim must be positive", what);
-  if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
-    return fail(MCPU_ERR_INVALID, "%s: temperature must be above 0", what);
+  // So that float32 has its inverse times a logit, and its square times a divergence.
+  if (!(a->temperature >= 0x1p-60f) || !(a->temperature <= 0x1p60f))
+    return fail(MCPU_ERR_INVALID, "%s: temperature must lie in 2^-60 to 2^60", what);
   // Without tokens a teacher's logits have no address to tell by.
   if (!distil(a) && a->tokens > 0 && a->k > 0 && (a->k != 1 || a->temperature != 1.f))
     return fail(MCPU_ERR_INVALID, "%s: cross entropy has one target a row and temperature 1", what);

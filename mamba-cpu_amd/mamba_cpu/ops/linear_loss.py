@@ -138,7 +138,7 @@ def linear_distillation_fn(hidden, weight, teacher_ids, teacher_logits, temperat
         teacher_logits: (..., k), their logits or log-probabilities; k at most 1024.
         An id outside [0, vocab) or a logit of -inf leaves its entry out; an id
         given twice has both entries' shares.
-    temperature: above 0, divides both sides' logits
+    temperature: divides both sides' logits, 2^-60 to 2^60
     reduction: as linear_cross_entropy_fn's; tokens without entries are left out
     Returns loss: () or, for "none", hidden's shape without its last, float32:
     temperature^2 times the divergence of softmax(s / temperature) over the whole
@@ -147,8 +147,8 @@ def linear_distillation_fn(hidden, weight, teacher_ids, teacher_logits, temperat
     Differentiable in hidden and weight (once); teacher_logits must not require
     a gradient.
     """
-    if not 0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be above 0, got {temperature}")
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+        raise ValueError(f"temperature must lie in 2^-60 to 2^60, got {temperature}")
     h, w = _operands(hidden, weight, reduction)
     lead = hidden.shape[:-1]
     ids = _ids("teacher_ids", teacher_ids, lead, hidden.device)
