@@ -734,12 +734,13 @@ __device__ __forceinline__ void finish_row(const LossParams& p, int64_t t, int64
     // The target joins the others: relative to their maximum, as long as that is in float32's range.
     const float d = own - top;
     const bool far = !(d <= 40.f);
-    const float mine = far ? 1.f : fast_exp2(d * c), others = far ? sum * fast_exp2(-d * c) : sum;
+    // An overflowed target: lse - s is inf - inf, and the gradient NaN likewise.
+    const float mine = own == INFINITY ? NAN : far ? 1.f : fast_exp2(d * c);
+    const float others = far ? sum * fast_exp2(-d * c) : sum;
     const float all = mine + others;
     // log(all / mine), by log1p where the target is the largest.
     const float r = others / mine, u = 1.f + r;
     p.each[t] = d >= 0.f ? (u == 1.f ? r : logf(u) * (r / (u - 1.f))) : logf(all) - d;
-    if (own == INFINITY) p.each[t] = NAN;  // lse - s of an overflowed target, as its gradient
     stat[2 * p.tokens] = mine / all;
     stat[3 * p.tokens] = others / all;
     top = far ? own : top;
