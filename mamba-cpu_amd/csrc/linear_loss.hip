@@ -40,9 +40,10 @@ namespace {
 // ds is kept as ds / unit times this: f16's steps are then 2^-37 of the unit.
 template <typename E> constexpr float kUp = std::is_same_v<E, bf16> ? 1.f : 8192.f;
 // f16 pieces: the least unit of a row beside the largest. dweight's product takes unit / the largest from hidden's
-// rows, whose largest magnitude is 2^13 or more: with 2^-16 of it left, their elements down to 2^-11 of the largest keep
-// all bits of an f16. What is below goes to ds, whose largest of a row falls from 2^13 on. All of it to hidden, unscaled,
-// left 4 bits of an element near 1 at a unit of 2^-20 and nothing at 2^-26; all of it to ds would do that to dhidden.
+// rows, whose largest magnitude is 2^13 or more: with 2^-16 of it left, their elements down to 2^-11 of the largest
+// keep all bits of an f16. What is below goes to ds, whose largest of a row falls from 2^13 on. All of it to hidden,
+// unscaled, left 4 bits of an element near 1 at a unit of 2^-20 and nothing at 2^-26; all of it to ds would do that
+// to dhidden.
 constexpr float kLeastUnit = 0x1p-16f;
 
 __device__ __forceinline__ int64_t id_at(const LossParams& p, int64_t i) {
@@ -250,7 +251,8 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossParams p) {
 // ---- operands ----------------------------------------------------------------------------
 
 // The largest finite magnitude of rows: two rows a wave at a time, 1024 elements of each on their way. 256
-// workgroups of 16 waves, for one atomic each: one a wave, 8192 to one address, took 80 us.
+// workgroups of 16 waves, for one atomic each: one a wave, 8192 to one address, took 80 us. 8.5 us for hidden of
+// 1021 x 1001 in f16.
 template <typename T> __global__ __launch_bounds__(1024) void loss_most_kernel(const LossParams p, bool of_weight) {
   const int64_t rows = of_weight ? p.vocab : p.scal->kept;
   const int lane = threadIdx.x & 63;

@@ -1,5 +1,5 @@
-"""A single confident token, scored: a loss of about 0.01 has float32's digits, though lse - s_target in float32, with lse
-near 16, has none behind the fourth.
+"""A single confident token, scored: a loss of about 0.01 has float32's digits, though lse - s_target in float32, with
+lse near 16, has none behind the fourth.
 
 Operands are multiples of 2^-3 and 2^-5, so that every logit is a multiple of 2^-8 below 2^8 and exact in float32 in any
 order of its sum. What is left: arguments of exp2 up to 2^5, each rounded by at most 2^-20 (a logit's difference, its

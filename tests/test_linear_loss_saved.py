@@ -1,5 +1,5 @@
-"""Hooks on the tensors that the head's losses save for their backward: operands come back contiguous and aligned, whatever
-they were in the forward."""
+"""Hooks on the tensors that the head's losses save for their backward: operands come back contiguous and aligned,
+whatever they were in the forward."""
 
 import pytest
 import torch

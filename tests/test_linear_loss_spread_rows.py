@@ -41,10 +41,10 @@ def held_to_its_size(dtype, h, w, ds, unit, ltol, dh, dw, shares=0.0):
 
 
 def confident(t, v, beyond):
-    """Token 0's target is 60 below word 41. The others' targets are words 0 to 31, above all others by as much as leaves
-    those about exp(-beyond[word]) together; the words behind its own have next to nothing of a token, so that each
-    word's gradient is of its own tokens' size. No row of weight has anything in columns 48 to 63: there hidden is 0.5 to
-    2, to no word's favour."""
+    """Token 0's target is 60 below word 41. The others' targets are words 0 to 31, above all others by as much as
+    leaves those about exp(-beyond[word]) together; the words behind its own have next to nothing of a token, so that
+    each word's gradient is of its own tokens' size. No row of weight has anything in columns 48 to 63: there hidden is
+    0.5 to 2, to no word's favour."""
     g = torch.Generator().manual_seed(1)
     w = torch.zeros(v, 64)
     w[:32, :32] = torch.eye(32)
@@ -104,4 +104,5 @@ def test_distilled_tokens_of_weights_over_eight_powers_of_ten(dtype, t, v):
     q, _ = O.shares(ids, v, tl, 1.5)
     shares = np.zeros_like(ds)
     np.put_along_axis(shares, ids.numpy(), q * unit[:, None], 1)
-    held_to_its_size(dtype, h, w, ds, unit, lse_tol(dtype, h, w, lse, 1.5) + 2 * U * np.abs(lse) + 8 * U, dh, dw, shares)
+    ltol = lse_tol(dtype, h, w, lse, 1.5) + 2 * U * np.abs(lse) + 8 * U
+    held_to_its_size(dtype, h, w, ds, unit, ltol, dh, dw, shares)
